@@ -342,6 +342,62 @@ int tllm_mxfp4_dequant_bf16(const void* blocks, const void* scales, void* out, i
 /* Diagnostic: threads of the largest launch that it makes; a grid holds fewer than 2^32. */
 int64_t tllm_mxfp4_launch_threads(int64_t n_blocks);
 
+/* ---- MXFP4 products and the experts --------------------------------------------------------------------------------
+ * An MXFP4 matrix [rows, K] is blocks [rows][K / 32][16] bytes (32 e2m1 codes each, the low nibble first) and scales
+ * [rows][K / 32] (e8m0, bias 127): the layout of a checkpoint's `.blocks` / `.scales`. A scale byte of 255 makes its block
+ * NaN, as the format has it; other values are those that tllm_mxfp4_dequant_bf16 gives. */
+enum { TLLM_BF16 = 0, TLLM_F16 = 1, TLLM_F32 = 2 };
+
+/* x [rows, cols] of type x_type, x_row_stride values from row to row -> MXFP4. The 32 values of a block share
+ * 2^max(floor(log2 max|x|) - 2, -127) and go to the nearest e2m1 value, ties to the even code, at most 6; a block with a NaN or
+ * an infinity gets the scale byte 255. cols a multiple of 32, rows of x and blocks 16-byte aligned. No counterpart in the
+ * reference, whose quantisation lives in the checkpoint's making. */
+int tllm_mxfp4_quantize(const void* x, int x_type, int64_t x_row_stride, void* blocks, void* scales, int64_t rows, int64_t cols,
+                        void* stream);
+
+/* out[r, n] = sum_k x[r, k] W[n, k] + bias[n] with W MXFP4 [out_dim, in_dim] (fp32 accumulate, one RNE to bf16). x is bf16
+ * with x_row_stride values from row to row, or, with x_scales not NULL, dense MXFP4 blocks. bias bf16 [out_dim] or NULL. in_dim a
+ * multiple of 32, rows of x and W's blocks 16-byte aligned, x within 4 GiB. Any number of rows. */
+int tllm_mxfp4_linear_bf16(const void* x, const void* x_scales, int64_t x_row_stride, const void* w_blocks, const void* w_scales,
+                           const void* bias, void* out, int64_t out_row_stride, int64_t rows, int64_t in_dim, int64_t out_dim,
+                           void* stream);
+
+/* Routing of tokens to experts (the router behind MLPBlock's gate, model.py:751-757: torch.topk + softmax over the chosen,
+ * which is score softmax, one group, renormalize 1). logits [tokens, n_experts] bf16 or fp32; bias fp32 [n_experts] or NULL.
+ *   s = softmax(logits) (sigmoid == 0) or 1 / (1 + exp(-logits));  c = s + bias (without a bias: ordered as the logits)
+ *   n_groups > 1: equal runs of experts; a group is worth the sum of its two largest c (s without a bias), topk_groups stay
+ *   experts[t, :top]: the largest c, descending, the lowest index where equal; weights[t, :] = s there, divided by their sum
+ *   with renormalize, times scale
+ * and the plan of the experts' products: order [tokens * top], the pairs t * top + j sorted by expert (by number within one),
+ * and offsets [n_experts + 1], each expert's first place there. A NaN logit or bias counts as -infinity, an expert of
+ * -infinity has a weight of 0. Up to 512 experts, 64 groups, top 32; tokens * top < 2^31. workspace: device memory of
+ * tllm_moe_route_workspace_bytes() bytes, 4-byte aligned (0 bytes for few tokens). tokens == 0 fills offsets with 0. */
+int64_t tllm_moe_route_workspace_bytes(int64_t tokens, int n_experts);
+int tllm_moe_route(const void* logits, int logits_is_f32, int64_t logits_row_stride, const float* bias, int sigmoid, int n_groups,
+                   int topk_groups, int renormalize, float scale, int32_t* experts, float* weights, int32_t* order,
+                   int32_t* offsets, void* workspace, int64_t workspace_bytes, int64_t tokens, int n_experts, int top, void* stream);
+
+/* The experts' first product with its SwiGLU, a row per pair in the order of tllm_moe_route's plan:
+ *   h[s, :] = swiglu(x[order[s] / top, :] . W[e]^T + bias[e])     e: the expert whose offsets hold s
+ * x [tokens, hidden] bf16, W MXFP4 [n_experts, 2 * inner, hidden] with gate and linear rows in turn, bias bf16 [n_experts,
+ * 2 * inner] or NULL, h [tokens * top, inner] bf16; SwiGLU as tllm_swiglu_bf16, on the fp32 sums. Replaces the gathered
+ * mlp1 matmul and swiglu of MLPBlock (model.py:751-757, moe.py:25-33). */
+int tllm_moe_mlp1_bf16(const void* x, int64_t x_row_stride, const int32_t* order, const int32_t* offsets, const void* w_blocks,
+                       const void* w_scales, const void* bias, void* h, int64_t h_row_stride, int64_t tokens, int n_experts, int top,
+                       int64_t hidden, int64_t inner, float alpha, float limit, int has_limit, void* stream);
+
+/* The experts' second product, weighted and summed over a token's experts:
+ *   out[t, :] = residual[t, :] + sum_j weights[t, j] (h[s(t, j), :] . W[e]^T + bias[e])     s: the place of pair t * top + j
+ * h [tokens * top, inner] bf16 in the plan's order, W MXFP4 [n_experts, hidden, inner], residual bf16 or NULL; out bf16, may be
+ * the residual buffer. fp32 throughout, one RNE on store, the same order of sums every time. workspace: device memory,
+ * 16-byte aligned, of tllm_moe_mlp2_workspace_bytes() bytes. Replaces the scattered mlp2 matmul and the residual add of
+ * MLPBlock (model.py:751-757). */
+int64_t tllm_moe_mlp2_workspace_bytes(int64_t tokens, int top, int64_t hidden);
+int tllm_moe_mlp2_bf16(const void* h, int64_t h_row_stride, const int32_t* order, const int32_t* offsets, const float* weights,
+                       const void* w_blocks, const void* w_scales, const void* bias, const void* residual, int64_t res_row_stride,
+                       void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, int64_t tokens, int n_experts,
+                       int top, int64_t inner, int64_t hidden, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

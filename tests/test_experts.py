@@ -1,0 +1,540 @@
+"""MXFP4 quantisation and products, routing to experts and the experts' two products against their definitions in float64 on the
+CPU. Tolerances: products of bf16 (or MXFP4) values are exact in fp32, so a sum of K of them is off by at most K 2^-23 of the sum of
+their magnitudes however it is ordered, and a bf16 result by 2^-8 of itself (half a place, doubled for the binade's edge)."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import tritonllm_amd as T
+from tritonllm_amd import _lib
+
+gpu = pytest.mark.gpu
+FP4 = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64)
+ALPHA, LIMIT = 1.702, 7.0
+
+
+def values(blocks, scales):
+    """MXFP4 in float64; a scale byte of 255 is NaN."""
+    v = torch.stack((FP4[(blocks & 15).long()], FP4[(blocks >> 4).long()]), -1).flatten(-2)
+    p = torch.ldexp(torch.ones((), dtype=torch.float64), scales.long() - 127)
+    return (v * torch.where(scales == 255, math.nan, p)[..., None]).flatten(-2)
+
+
+def random_mx(g, *shape, lo=118, hi=123):
+    *rows, k = shape
+    return (torch.randint(0, 256, (*rows, k // 32, 16), generator=g, dtype=torch.uint8),
+            torch.randint(lo, hi, (*rows, k // 32), generator=g, dtype=torch.uint8))
+
+
+def cuda(*ts):
+    return [t if t is None else t.cuda() for t in ts]
+
+
+def check_product(got, want, magnitude, k, what=""):
+    """got bf16 / want float64 / the sum of the products' magnitudes"""
+    got = got.double().cpu()
+    assert got.shape == want.shape
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan), what
+    off = (got - want).abs()
+    ok = nan | (off <= 2.0**-8 * want.abs() + k * 2.0**-23 * magnitude) | (got == want)
+    assert ok.all(), f"{what}: {(~ok).sum()} of {ok.numel()} off, the worst {off[~ok].max()}"
+
+
+# ---- quantisation -----------------------------------------------------------------------------------------------------------
+def quantize_ref(x):
+    """codes and scale bytes by search: every level's distance, the even code where two are as near"""
+    v = x.double().unflatten(-1, (-1, 32))
+    bad = ~v.isfinite().all(-1)
+    top = torch.where(bad[..., None], 0.0, v).abs().amax(-1)
+    e = torch.where(top > 0, torch.frexp(top).exponent.double() - 1, -1000.0).clamp(min=-125) - 2
+    a = (torch.where(bad[..., None], 0.0, v) * torch.exp2(-e)[..., None]).abs()
+    d = (a[..., None].clamp(max=6) - FP4[:8]).abs() + torch.tensor([0, 1, 0, 1, 0, 1, 0, 1]) * 1e-9      # (odd codes lose ties)
+    code = d.argmin(-1) + 8 * torch.signbit(v)
+    code[bad] = 0
+    scale = torch.where(bad, 255, (e + 127).long()).to(torch.uint8)
+    code = code.to(torch.uint8)
+    return code[..., 0::2] | (code[..., 1::2] << 4), scale
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(32,), (1, 64), (3, 96), (17, 2880), (2, 5, 160), (257, 4096)])
+def test_quantize(dtype, shape):
+    g = torch.Generator().manual_seed(len(shape) * 100 + shape[-1])
+    x = torch.randn(shape, generator=g) * torch.exp2(torch.randint(-12, 12, shape, generator=g).float() * (torch.rand(shape, generator=g) < 0.1))
+    x = x.to(dtype)
+    blocks, scales = T.mxfp4_quantize(x.cuda())
+    want_b, want_s = quantize_ref(x)
+    assert blocks.shape == (*shape[:-1], shape[-1] // 32, 16) and scales.shape == blocks.shape[:-1]
+    assert torch.equal(scales.cpu(), want_s) and torch.equal(blocks.cpu(), want_b)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantize_edges(dtype):
+    """Ties, saturation, zeros of both signs, subnormals, the type's largest, and blocks with NaN or infinity beside fine ones."""
+    info = torch.finfo(dtype)
+    x = torch.zeros(14, 32, dtype=torch.float64)
+    x[0] = torch.arange(32) / 4                                    # scale 2^0: every midpoint of the codes
+    x[1] = -torch.arange(32) / 4
+    x[2, 3] = 7.9                                                  # beyond 6: saturates
+    x[3] = -0.0
+    x[4, 5] = info.tiny
+    x[5] = info.smallest_normal * torch.arange(32) / 32            # subnormals (and the smallest normal's neighbours)
+    x[6, 0] = info.max
+    x[7, 31] = -info.max
+    x[8, 2] = math.nan
+    x[9, 2] = math.inf
+    x[10, 2] = -math.inf
+    x[11] = info.smallest_normal * torch.arange(32)
+    x[12, ::2] = 1.0
+    x[13] = torch.linspace(-1, 1, 32, dtype=torch.float64)
+    x = x.to(dtype)
+    blocks, scales = T.mxfp4_quantize(x.cuda())
+    want_b, want_s = quantize_ref(x)
+    assert torch.equal(scales.cpu(), want_s)
+    assert torch.equal(blocks.cpu(), want_b)
+    assert scales[8:11].eq(255).all() and blocks[8:11].eq(0).all()
+
+
+@gpu
+def test_quantize_strides():
+    x = torch.randn(9, 400, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    for view in (x[:, 8:360], x[:, 1:33], x[::2, :64], x.t()[:, :1].expand(400, 32), x[:0, :32], x[:, :0]):
+        blocks, scales = T.mxfp4_quantize(view)
+        want_b, want_s = quantize_ref(view.cpu().contiguous()) if view.numel() else (blocks.cpu(), scales.cpu())
+        assert torch.equal(blocks.cpu(), want_b) and torch.equal(scales.cpu(), want_s)
+    odd = torch.empty(33 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(33, 64).copy_(x.flatten()[: 33 * 64].view(33, 64))   # 2 bytes off
+    assert torch.equal(T.mxfp4_quantize(odd)[0].cpu(), quantize_ref(odd.cpu())[0])
+
+
+@gpu
+def test_quantized_values_come_back():
+    """What is in MXFP4 already stays as it is."""
+    g = torch.Generator().manual_seed(8)
+    blocks, scales = random_mx(g, 40, 320, lo=100, hi=140)
+    blocks[..., 0] = 7                                             # (a 6 in every block: its scale is the largest that holds it)
+    x = values(blocks, scales).float().cuda()
+    again, s = T.mxfp4_quantize(x)
+    assert torch.equal(s.cpu(), scales) and torch.equal(values(again.cpu(), s.cpu()).float(), x.cpu())
+
+
+# ---- the product ------------------------------------------------------------------------------------------------------------
+def linear_case(rows, n, k, acts, seed=0, bias=True):
+    g = torch.Generator().manual_seed(seed + rows * 7 + n * 3 + k)
+    w, ws = random_mx(g, n, k)
+    b = torch.randn(n, generator=g).bfloat16() if bias else None
+    if acts == "bf16":
+        x, xs = torch.randn(rows, k, generator=g).bfloat16(), None
+        xv = x.double()
+    else:
+        x, xs = random_mx(g, rows, k, lo=123, hi=128)
+        xv = values(x, xs)
+    wv = values(w, ws)
+    want, mag = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    if bias:
+        want, mag = want + b.double(), mag + b.double().abs()
+    return x, xs, w, ws, b, want, mag
+
+
+LINEAR = [(1, 2880, 4096), (1, 16, 32), (2, 1, 64), (3, 15, 96), (5, 17, 160), (16, 33, 224), (17, 127, 288), (31, 64, 2880), (33, 130, 512),
+          (65, 257, 608), (100, 100, 1024), (129, 320, 736), (200, 29, 2048), (257, 511, 352), (300, 640, 2880), (515, 1100, 160)]
+
+
+@gpu
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("rows,n,k", LINEAR)
+def test_linear(rows, n, k, acts):
+    x, xs, w, ws, b, want, mag = linear_case(rows, n, k, acts)
+    dx, dxs, dw, dws, db = cuda(x, xs, w, ws, b)
+    check_product(T.mxfp4_linear(dx, dw, dws, db, x_scales=dxs), want, mag, k)
+
+
+@gpu
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_linear_without_bias_and_odd_shapes(rows, acts):
+    x, xs, w, ws, b, want, mag = linear_case(rows, 48, 320, acts, bias=False)
+    dx, dxs, dw, dws = cuda(x, xs, w, ws)
+    got = T.mxfp4_linear(dx, dw, dws, x_scales=dxs)
+    check_product(got, want, mag, 320)
+    lead = (2, rows // 2) if rows % 2 == 0 else (1, 1, rows)
+    more = T.mxfp4_linear(dx.reshape(*lead, *dx.shape[1:]), dw, dws, x_scales=None if xs is None else dxs.reshape(*lead, -1))
+    assert torch.equal(more.reshape(rows, -1), got)
+    assert T.mxfp4_linear(dx[:0], dw, dws, x_scales=None if xs is None else dxs[:0]).shape == (0, 48)
+    if acts == "bf16":
+        wide = torch.randn(rows, 400).bfloat16().cuda()
+        for at in (8, 3):                                          # aligned rows of a wider matrix, and rows that have to be copied
+            wide[:, at: at + 320] = dx
+            assert torch.equal(T.mxfp4_linear(wide[:, at: at + 320], dw, dws), got)
+
+
+@gpu
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_linear_special_values(rows, acts):
+    """NaN blocks of the weight spoil their output alone, NaN and infinite activations their row; the smallest and largest scales count."""
+    x, xs, w, ws, b, _, _ = linear_case(rows, 70, 224, acts)
+    ws[3, 2] = 255
+    ws[69, 6] = 255
+    ws[5], ws[6] = 0, 1
+    ws[7] = 230
+    if acts == "bf16":
+        x[0, 100] = math.nan
+        if rows > 20:
+            x[17, 223] = math.inf
+            w[:, 6, 15] |= 0x10                                    # (no weight there is 0)
+        xv = x.double()
+    else:
+        xs[0, 3] = 255
+        if rows > 20:
+            xs[17] = 0
+        xv = values(x, xs)
+    wv = values(w, ws)
+    want = torch.stack([(xv * wv[i]).sum(1) for i in range(70)], 1) + b.double()
+    mag = (xv.abs()[:, None] * wv.abs()).sum(2).nan_to_num(0, 0, 0) + b.double().abs()
+    dx, dxs, dw, dws, db = cuda(x, xs, w, ws, b)
+    got = T.mxfp4_linear(dx, dw, dws, db, x_scales=dxs)
+    check_product(got, want, mag, 224)
+
+
+@gpu
+def test_quantize_then_linear_is_the_product_of_the_values():
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(77, 2880, generator=g).bfloat16()
+    w, ws = random_mx(g, 96, 2880)
+    xq, xs = T.mxfp4_quantize(x.cuda())
+    xv, wv = values(xq.cpu(), xs.cpu()), values(w, ws)
+    check_product(T.mxfp4_linear(xq, w.cuda(), ws.cuda(), x_scales=xs), xv @ wv.t(), xv.abs() @ wv.abs().t(), 2880)
+
+
+# ---- routing ----------------------------------------------------------------------------------------------------------------
+def route_ref(logits, top, score="softmax", bias=None, groups=1, kept=1, renorm=True, scale=1.0):
+    """In float64 and in plain loops over the choices; also how near the nearest choice that could go either way was."""
+    z = logits.double().clone()
+    z[z.isnan()] = -math.inf
+    tokens, n = z.shape
+    if score == "softmax":
+        m = z.amax(1, keepdim=True)
+        s = torch.where(z == -math.inf, 0.0, torch.where(z == m, 1.0, torch.exp(z - m.clamp(min=-1e300, max=1e300))))
+        s = s / s.sum(1, keepdim=True).clamp(min=1e-300)
+    else:
+        s = 1 / (1 + torch.exp(-z))
+    c = z.clone() if bias is None else s + bias.double()
+    c[c.isnan()] = -math.inf
+    near = torch.full((tokens,), math.inf, dtype=torch.float64)
+    if groups > 1:
+        by = (s if bias is None else c).view(tokens, groups, -1)
+        v = by.sort(2, descending=True).values[..., :2].sum(2)
+        o = torch.sort(v, dim=1, descending=True, stable=True)
+        if kept < groups:
+            near = torch.minimum(near, o.values[:, kept - 1] - o.values[:, kept])
+        keep = torch.zeros(tokens, groups, dtype=torch.bool).scatter_(1, o.indices[:, :kept], True)
+        out = ~keep.repeat_interleave(n // groups, 1)
+    else:
+        out = torch.zeros(tokens, n, dtype=torch.bool)
+    order = torch.empty(tokens, n, dtype=torch.long)
+    for t in range(tokens):
+        order[t] = torch.tensor(sorted(range(n), key=lambda e: (bool(out[t, e]), -c[t, e].item(), e)))
+    best = order[:, : min(top + 1, n)]
+    if bias is not None and best.shape[1] > 1:
+        gaps = -(c.gather(1, best).diff(dim=1))
+        same = (z.gather(1, best).diff(dim=1) == 0) & (bias.double()[best].diff(dim=1) == 0)    # equal in any precision
+        near = torch.minimum(near, torch.where(same | out.gather(1, best[:, 1:]), math.inf, gaps).amin(1))
+    best = best[:, :top]
+    w = s.gather(1, best)
+    if renorm:
+        w = w / w.sum(1, keepdim=True).clamp(min=1e-300)
+    return best, w * scale, near
+
+
+def check_plan(r, tokens, experts, top):
+    flat = r.experts.reshape(-1).cpu().long()
+    assert r.experts.dtype == r.order.dtype == r.offsets.dtype == torch.int32 and r.weights.dtype == torch.float32
+    assert torch.equal(r.order.cpu().long(), torch.sort(flat, stable=True).indices)
+    want = torch.zeros(experts + 1, dtype=torch.long)
+    want[1:] = torch.bincount(flat, minlength=experts).cumsum(0)
+    assert torch.equal(r.offsets.cpu().long(), want)
+
+
+def check_route(logits, top, near_at_least=1e-5, **how):
+    named = dict(score=how.get("score", "softmax"), bias=how.get("bias"), groups=how.get("groups", 1), kept=how.get("kept", 1),
+                 renorm=how.get("renorm", True), scale=how.get("scale", 1.0))
+    best, w, near = route_ref(logits, top, **named)
+    r = T.moe_route(logits.cuda(), top, score=named["score"], bias=None if named["bias"] is None else named["bias"].cuda(), n_groups=named["groups"],
+                    topk_groups=named["kept"], renormalize=named["renorm"], scale=named["scale"])
+    sure = near > near_at_least                                    # the others hang on fp32's last places
+    assert sure.double().mean() > 0.9
+    assert torch.equal(r.experts.cpu().long()[sure], best[sure])
+    torch.testing.assert_close(r.weights.cpu().double()[sure], w[sure], rtol=2e-6, atol=1e-7 * abs(named["scale"]))
+    check_plan(r, logits.shape[0], logits.shape[1], top)
+    return r
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,experts,top", [(1, 1, 1), (1, 32, 4), (8, 32, 4), (7, 5, 5), (63, 64, 8), (64, 65, 3), (65, 33, 2), (200, 128, 4), (300, 257, 8),
+                                                (129, 512, 32), (1000, 32, 4), (4097, 17, 2)])
+def test_route(tokens, experts, top, dtype):
+    g = torch.Generator().manual_seed(tokens + experts)
+    logits = (1.5 * torch.randn(tokens, experts, generator=g)).to(dtype)
+    check_route(logits, top)
+    check_route(logits, top, score="sigmoid", renorm=False, scale=2.5)
+
+
+@gpu
+@pytest.mark.parametrize("tokens,experts,top,groups,kept", [(1, 16, 2, 4, 2), (33, 256, 8, 8, 4), (70, 48, 6, 3, 2), (150, 512, 8, 64, 8), (90, 160, 6, 8, 3), (66, 8, 1, 8, 1),
+                                                            (500, 64, 8, 2, 1)])
+def test_route_groups(tokens, experts, top, groups, kept):
+    g = torch.Generator().manual_seed(tokens * experts)
+    logits = (1.5 * torch.randn(tokens, experts, generator=g)).bfloat16()
+    bias = 0.1 * torch.randn(experts, generator=g)
+    check_route(logits, top, score="sigmoid", bias=bias, groups=groups, kept=kept, scale=1.5)
+    check_route(logits, top, score="sigmoid", groups=groups, kept=kept)
+    check_route(logits, top, score="softmax", groups=groups, kept=kept, near_at_least=1e-7)
+    check_route(logits, top, score="softmax", bias=bias)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [5, 100])
+def test_route_ties_and_masks(tokens):
+    """Equal logits go to the lowest index; -inf, NaN and rows of nothing else; the lowest finite value is no mask."""
+    g = torch.Generator().manual_seed(tokens)
+    logits = torch.randint(-2, 3, (tokens, 40), generator=g).float()
+    check_route(logits, 6)
+    check_route(logits, 6, score="sigmoid")
+    logits[0] = 1.0
+    logits[1, 3:] = -math.inf                                      # three are left for six places
+    logits[2, ::2] = math.nan
+    logits[3] = -math.inf
+    logits[4] = torch.finfo(torch.float32).min
+    for score in ("softmax", "sigmoid"):
+        r = check_route(logits, 6, score=score)
+        assert r.experts[0].tolist() == list(range(6)) == r.experts[3].tolist()
+        assert r.weights[3].eq(0).all() and r.weights[1, 3:].eq(0).all() and r.weights.isfinite().all()
+    lowest = T.moe_route(logits.cuda(), 6).weights[4]
+    assert (lowest == lowest[0]).all() and lowest[0] > 0.1
+    inf = logits.clone()
+    inf[0, 7] = math.inf
+    r = T.moe_route(inf.cuda(), 2)
+    assert r.experts[0].tolist() == [7, 0] and r.weights[0].tolist() == [1.0, 0.0]
+
+
+@gpu
+def test_route_shapes():
+    r = T.moe_route(torch.empty(0, 32, device="cuda"), 4)
+    assert r.experts.shape == r.weights.shape == (0, 4) and r.order.shape == (0,) and r.offsets.tolist() == [0] * 33
+    x = torch.randn(6, 50, generator=torch.Generator().manual_seed(1))
+    want = T.moe_route(x[:, :32].contiguous().cuda(), 4)
+    for view in (x.cuda()[:, :32], x.cuda().t().contiguous().t()[:, :32], x[:, :32].reshape(2, 3, 32).cuda()):
+        for a, b in zip(T.moe_route(view, 4), want):
+            assert torch.equal(a, b)
+
+
+# ---- the experts ------------------------------------------------------------------------------------------------------------
+def plan_of(chosen, experts):
+    flat = chosen.reshape(-1).long()
+    offsets = torch.zeros(experts + 1, dtype=torch.int32)
+    offsets[1:] = torch.bincount(flat, minlength=experts).cumsum(0).int()
+    return torch.sort(flat, stable=True).indices.int(), offsets
+
+
+def experts_case(tokens, experts, top, hidden, inner, seed=0, spread=1.0):
+    """Routing (uneven with a small spread: some experts get nothing, few most) and both weights."""
+    g = torch.Generator().manual_seed(seed + tokens * 31 + experts)
+    favour = torch.randn(experts, generator=g) * 2 / spread
+    chosen = (torch.randn(tokens, experts, generator=g) + favour).topk(top, 1).indices.int()
+    weights = torch.softmax(torch.randn(tokens, top, generator=g), 1)
+    order, offsets = plan_of(chosen, experts)
+    return g, T.MoeRouting(chosen, weights, order, offsets), random_mx(g, experts, 2 * inner, hidden), random_mx(g, experts, hidden, inner)
+
+
+def by_expert(x, routing, w, ws, bias):
+    """rows in the plan's order -> (sums, magnitudes), float64"""
+    y = torch.empty(len(routing.order), w.shape[1], dtype=torch.float64)
+    m = torch.empty_like(y)
+    for e in range(w.shape[0]):
+        lo, hi = routing.offsets[e], routing.offsets[e + 1]
+        wv = values(w[e], ws[e])
+        y[lo:hi], m[lo:hi] = x[lo:hi] @ wv.t(), x[lo:hi].abs() @ wv.abs().t()
+        if bias is not None:
+            y[lo:hi] += bias[e].double()
+            m[lo:hi] += bias[e].double().abs()
+    return y, m
+
+
+EXPERTS = [(1, 4, 1, 32, 32), (1, 32, 4, 2880, 96), (2, 8, 2, 64, 160), (7, 8, 8, 96, 64), (8, 32, 4, 224, 352), (33, 17, 3, 160, 32), (40, 4, 2, 480, 96),
+           (64, 8, 4, 128, 288), (150, 3, 2, 352, 64), (300, 8, 3, 288, 160), (700, 2, 1, 64, 128), (257, 64, 4, 96, 96), (1000, 5, 4, 32, 32)]
+
+
+@gpu
+@pytest.mark.parametrize("limit,bias", [(7.0, True), (None, False)])
+@pytest.mark.parametrize("tokens,experts,top,hidden,inner", EXPERTS)
+def test_mlp1(tokens, experts, top, hidden, inner, limit, bias):
+    g, routing, (w, ws), _ = experts_case(tokens, experts, top, hidden, inner)
+    x = torch.randn(tokens, hidden, generator=g).bfloat16()
+    b = torch.randn(experts, 2 * inner, generator=g).bfloat16() if bias else None
+    y, m = by_expert(x.double()[(routing.order // top).long()], routing, w, ws, b)
+    off = hidden * 2.0**-23 * m
+    lim = math.inf if limit is None else limit
+    gate, lin = y[:, 0::2].clamp(max=lim), y[:, 1::2].clamp(-lim, lim)
+    want = gate * torch.sigmoid(ALPHA * gate) * (lin + 1)
+    # of g sigmoid(a g): the slope is at most 1.1; fp32's exp, division and products add a few of its places
+    room = 2.0**-8 * want.abs() + 1.1 * (lin + 1).abs() * off[:, 0::2] + gate.abs() * off[:, 1::2] + 1e-5 * want.abs() + 1e-30
+    got = T.moe_mlp1(x.cuda(), T.MoeRouting(*cuda(*routing)), *cuda(w, ws, b), alpha=ALPHA, limit=limit)
+    assert got.shape == want.shape and got.dtype == torch.bfloat16
+    d = (got.double().cpu() - want).abs()
+    assert (d <= room).all(), f"{(d > room).sum()} of {d.numel()} off, the worst {(d / room).max()} of the room"
+
+
+@gpu
+@pytest.mark.parametrize("residual,bias", [(True, True), (False, False)])
+@pytest.mark.parametrize("tokens,experts,top,hidden,inner", EXPERTS)
+def test_mlp2(tokens, experts, top, hidden, inner, residual, bias):
+    g, routing, _, (w, ws) = experts_case(tokens, experts, top, hidden, inner)
+    h = torch.randn(tokens * top, inner, generator=g).bfloat16()
+    b = torch.randn(experts, hidden, generator=g).bfloat16() if bias else None
+    res = torch.randn(tokens, hidden, generator=g).bfloat16() if residual else None
+    y, m = by_expert(h.double(), routing, w, ws, b)
+    wt = routing.weights.double().reshape(-1)[routing.order.long()][:, None]
+    token = (routing.order // top).long()
+    want = torch.zeros(tokens, hidden, dtype=torch.float64).index_add_(0, token, y * wt)
+    mag = torch.zeros_like(want).index_add_(0, token, m * wt)
+    if residual:
+        want, mag = want + res.double(), mag + res.double().abs()
+    dr = T.MoeRouting(*cuda(*routing))
+    dh, dw, dws, db, dres = cuda(h, w, ws, b, res)
+    got = T.moe_mlp2(dh, dr, dw, dws, db, residual=dres)
+    check_product(got, want, mag, inner + top)
+    assert torch.equal(T.moe_mlp2(dh, dr, dw, dws, db, residual=dres), got)      # the same order of sums every time
+    if residual:
+        assert T.moe_mlp2(dh, dr, dw, dws, db, residual=dres, out=dres) is dres and torch.equal(dres, got)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_experts_rows_from_strides_and_one_expert_for_all(tokens):
+    g, _, (w, ws), (w2, ws2) = experts_case(tokens, 6, 2, 96, 64)
+    chosen = torch.tensor([[5, 2]]).expand(tokens, 2).int().contiguous()
+    routing = T.MoeRouting(*cuda(chosen, torch.full((tokens, 2), 0.5), *plan_of(chosen, 6)))
+    wide = torch.randn(tokens, 200, generator=g).bfloat16().cuda()
+    dense = T.moe_mlp1(wide[:, 8:104].contiguous(), routing, w.cuda(), ws.cuda())
+    assert torch.equal(T.moe_mlp1(wide[:, 8:104], routing, w.cuda(), ws.cuda()), dense)
+    wide[:, 101:197] = wide[:, 8:104].clone()
+    assert torch.equal(T.moe_mlp1(wide[:, 101:197], routing, w.cuda(), ws.cuda()), dense)
+    y, m = by_expert(dense.double().cpu(), T.MoeRouting(*[t.cpu() for t in routing]), w2, ws2, None)
+    want = 0.5 * (y[:tokens] + y[tokens:])
+    check_product(T.moe_mlp2(dense, routing, w2.cuda(), ws2.cuda()), want, 0.5 * (m[:tokens] + m[tokens:]), 66)
+
+
+@gpu
+def test_experts_nothing_to_do():
+    g, routing, (w, ws), (w2, ws2) = experts_case(1, 4, 2, 64, 32)
+    empty = T.moe_route(torch.empty(0, 4, device="cuda"), 2)
+    h = T.moe_mlp1(torch.empty(0, 64, dtype=torch.bfloat16, device="cuda"), empty, w.cuda(), ws.cuda())
+    assert h.shape == (0, 32) and T.moe_mlp2(h, empty, w2.cuda(), ws2.cuda()).shape == (0, 64)
+
+
+@gpu
+def test_experts_nan_stays_with_its_token():
+    tokens = 50
+    g, routing, (w, ws), (w2, ws2) = experts_case(tokens, 6, 2, 96, 64)
+    x = torch.randn(tokens, 96, generator=g).bfloat16()
+    x[7, 5] = math.nan
+    dr = T.MoeRouting(*cuda(*routing))
+    h = T.moe_mlp1(x.cuda(), dr, w.cuda(), ws.cuda())
+    bad = (routing.order // 2 == 7)
+    assert h[bad.cuda()].isnan().all() and not h[~bad.cuda()].isnan().any()
+    y = T.moe_mlp2(h, dr, w2.cuda(), ws2.cuda())
+    assert y[7].isnan().all() and y.isnan().any(1).sum() == 1
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------------
+def _err():
+    return _lib.lib().tllm_last_error().decode()
+
+
+def test_entry_points_refuse_what_they_cannot_do():
+    lib, p, odd = _lib.lib(), C.c_void_p(4096), C.c_void_p(4104)
+    q = lib.tllm_mxfp4_quantize
+    assert q(None, 0, 0, None, None, 0, 64, None) == 0 and q(None, 0, 0, None, None, 3, 0, None) == 0
+    assert q(p, 0, 64, p, p, -1, 64, None) == -1 and q(p, 3, 64, p, p, 1, 64, None) == -1 and "type" in _err()
+    assert q(p, 0, 40, p, p, 2, 40, None) == -2 and q(None, 0, 64, p, p, 2, 64, None) == -1
+    assert q(p, 0, 32, p, p, 2, 64, None) == -1 and q(odd, 0, 64, p, p, 2, 64, None) == -3 and q(p, 0, 66, p, p, 2, 64, None) == -3
+    lin = lib.tllm_mxfp4_linear_bf16
+    assert lin(None, None, 0, None, None, None, None, 0, 0, 64, 64, None) == 0
+    assert lin(p, None, 64, p, p, None, p, 16, -1, 64, 16, None) == -1
+    assert lin(p, None, 48, p, p, None, p, 16, 2, 48, 16, None) == -2 and "32" in _err()
+    assert lin(p, None, 64, p, p, None, p, 16, 2, 64, 0, None) == -2
+    assert lin(p, None, 32, p, p, None, p, 16, 2, 64, 16, None) == -1 and lin(p, None, 64, p, p, None, p, 8, 2, 64, 16, None) == -1
+    assert lin(odd, None, 64, p, p, None, p, 16, 2, 64, 16, None) == -3 and lin(p, None, 64, odd, p, None, p, 16, 2, 64, 16, None) == -3
+    assert lin(p, None, 68, p, p, None, p, 16, 2, 64, 16, None) == -3
+    assert lin(p, None, 64, None, p, None, p, 16, 2, 64, 16, None) == -1 and lin(p, None, 64, p, p, None, None, 16, 2, 64, 16, None) == -1
+    assert lin(p, None, 4096, p, p, None, p, 16, 1 << 20, 4096, 16, None) == -2 and "4 GiB" in _err()
+    r = lib.tllm_moe_route
+
+    def route(logits=p, stride=32, groups=1, kept=1, tokens=8, experts=32, top=4, work=None, nbytes=0, offsets=p):
+        return r(logits, 0, stride, None, 0, groups, kept, 1, 1.0, p, p, p, offsets, work, nbytes, tokens, experts, top, None)
+
+    assert route(tokens=-1) == -1 and route(experts=0) == -2 and route(experts=513, stride=513) == -2 and route(top=0) == -2 and route(top=33) == -2
+    assert route(groups=5) == -2 and route(groups=4, kept=5) == -2 and route(groups=4, kept=0) == -2 and route(groups=16, kept=1) == -2
+    assert route(stride=31) == -1 and route(logits=None) == -1 and route(offsets=None) == -1 and route(tokens=1 << 30) == -2
+    need = lib.tllm_moe_route_workspace_bytes(1000, 32)
+    assert need > 0 and lib.tllm_moe_route_workspace_bytes(8, 32) == 0
+    assert route(tokens=1000) == -1 and route(tokens=1000, work=p, nbytes=need - 1) == -1 and "workspace" in _err()
+
+    def mlp1(x=p, stride=64, order=p, w=p, h=p, h_stride=32, tokens=8, experts=4, top=2, hidden=64, inner=32, limit=7.0):
+        return lib.tllm_moe_mlp1_bf16(x, stride, order, p, w, p, None, h, h_stride, tokens, experts, top, hidden, inner, 1.702, limit, 1, None)
+
+    assert mlp1(tokens=0) == 0 and mlp1(tokens=-1) == -1 and mlp1(top=0) == -2 and mlp1(top=5) == -2 and mlp1(hidden=40, stride=40) == -2
+    assert mlp1(x=None) == -1 and mlp1(order=None) == -1 and mlp1(w=odd) == -3 and mlp1(x=odd) == -3 and mlp1(h=None) == -1 and mlp1(h_stride=31) == -1
+    assert mlp1(stride=32) == -1 and mlp1(limit=-1.0) == -1 and mlp1(tokens=1 << 30) == -2 and mlp1(inner=0) == -2
+
+    def mlp2(h=p, weights=p, out=p, out_stride=64, work=p, nbytes=8 * 2 * 64 * 4, tokens=8, experts=4, top=2, inner=32, hidden=64, res=None, res_stride=64):
+        return lib.tllm_moe_mlp2_bf16(h, inner, p, p, weights, p, p, None, res, res_stride, out, out_stride, work, nbytes, tokens, experts, top, inner, hidden, None)
+
+    assert lib.tllm_moe_mlp2_workspace_bytes(8, 2, 64) <= 8 * 2 * 64 * 4
+    assert mlp2(tokens=0) == 0 and mlp2(tokens=-1) == -1 and mlp2(h=None) == -1 and mlp2(weights=None) == -1 and mlp2(out=None) == -1
+    assert mlp2(out_stride=63) == -1 and mlp2(res=p, res_stride=63) == -1 and mlp2(inner=33) == -2
+    assert lib.tllm_moe_mlp2_workspace_bytes(300, 2, 64) > 16 and mlp2(tokens=300, nbytes=16) == -1 and "workspace" in _err()
+
+
+def test_ops_refuse_cpu_tensors():
+    x, u8 = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 16, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        T.mxfp4_quantize(x)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        T.mxfp4_linear(x, u8, u8[..., 0])
+    with pytest.raises(RuntimeError, match="GPU only"):
+        T.moe_route(x, 2)
+    routing = T.MoeRouting(torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, 1), torch.arange(2, dtype=torch.int32), torch.tensor([0, 2], dtype=torch.int32))
+    for op in (T.moe_mlp1, T.moe_mlp2):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            op(x, routing, u8[None], u8[None, ..., 0])
+
+
+@gpu
+def test_ops_refuse_wrong_types_and_shapes():
+    c = dict(device="cuda")
+    x, w, ws = torch.zeros(2, 64, dtype=torch.bfloat16, **c), torch.zeros(6, 2, 16, dtype=torch.uint8, **c), torch.zeros(6, 2, dtype=torch.uint8, **c)
+    good = T.moe_route(torch.zeros(2, 3, **c), 1)
+    w3, ws3 = w.view(3, 2, 2, 16), ws.view(3, 2, 2)
+    bad = [lambda: T.mxfp4_quantize(x.double()), lambda: T.mxfp4_quantize(x[:, :40]), lambda: T.mxfp4_linear(x.float(), w, ws),
+           lambda: T.mxfp4_linear(x[:, :32], w, ws), lambda: T.mxfp4_linear(x, w, ws[:, :1]), lambda: T.mxfp4_linear(x, w[..., :8], ws),
+           lambda: T.mxfp4_linear(x, w.int(), ws), lambda: T.mxfp4_linear(x, w, ws, torch.zeros(5, dtype=torch.bfloat16, **c)),
+           lambda: T.mxfp4_linear(x, w, ws, torch.zeros(6, **c)), lambda: T.mxfp4_linear(w, w, ws, x_scales=ws[:, :1]),
+           lambda: T.mxfp4_linear(x, w, ws, x_scales=ws), lambda: T.moe_route(x.half(), 2), lambda: T.moe_route(x, 2, score="tanh"),
+           lambda: T.moe_route(x, 2, bias=torch.zeros(63, **c)), lambda: T.moe_route(x, 2, bias=torch.zeros(64, dtype=torch.bfloat16, **c)),
+           lambda: T.moe_mlp1(x[:1], good, w3, ws3), lambda: T.moe_mlp1(x[:, :32], good, w3, ws3), lambda: T.moe_mlp1(x, good, w3[:2], ws3[:2]),
+           lambda: T.moe_mlp1(x, good._replace(order=good.order.long()), w3, ws3), lambda: T.moe_mlp1(x, good, w3[:, :1], ws3[:, :1]),
+           lambda: T.moe_mlp2(x[:1], good, w3, ws3), lambda: T.moe_mlp2(x, good, w3, ws3, residual=x),
+           lambda: T.moe_mlp2(x, good, w3, ws3, out=torch.zeros(2, 3, dtype=torch.bfloat16, **c))]
+    for i, call in enumerate(bad):
+        with pytest.raises(AssertionError):
+            call()
+            print("call", i, "was let through")
+    with pytest.raises(RuntimeError, match="top"):
+        T.moe_route(x, 65)

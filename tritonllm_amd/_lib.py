@@ -79,6 +79,13 @@ SIGNATURES = {
                                            _f32, _i32, _vp, _i32, _vp]),
     "tllm_mxfp4_dequant_bf16": (_i32, [_vp, _vp, _vp, _i64, _vp]),
     "tllm_mxfp4_launch_threads": (_i64, [_i64]),
+    "tllm_mxfp4_quantize": (_i32, [_vp, _i32, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "tllm_mxfp4_linear_bf16": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "tllm_moe_route_workspace_bytes": (_i64, [_i64, _i32]),
+    "tllm_moe_route": (_i32, [_vp, _i32, _i64, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp]),
+    "tllm_moe_mlp1_bf16": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i64, _i64, _f32, _f32, _i32, _vp]),
+    "tllm_moe_mlp2_workspace_bytes": (_i64, [_i64, _i32, _i64]),
+    "tllm_moe_mlp2_bf16": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i64, _i64, _vp]),
     "tllm_qkv_rope_decode_w8_bf16": (_i32, [_vp, _vp, _i32, _f32, _vp, _vp] + _QKV_SIG[2:]),
 }
 

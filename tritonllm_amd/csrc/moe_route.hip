@@ -1,0 +1,347 @@
+// Routing to experts: every token's scores, its best experts and their weights, and the pairs in the order of their experts.
+//
+//   s = softmax(l) or 1 / (1 + exp(-l));   c = s + bias, or l itself without a bias (the order of the scores is that of the logits)
+//   groups: a group is worth the sum of its best two c (without a bias: of their s); the best of them stay, the others' c are out
+//   the `top` best c, descending, the lowest index where equal; weights = their s, over their sum if asked for, times `scale`
+//
+// A logit (or a bias) that is NaN counts as -infinity, and an expert of -infinity has the score 0; a row of nothing else gets the
+// first experts with weights of 0. All in fp32.
+//
+// A wavefront takes a token, its logits in registers, lane l those of experts l, l + 64, ...; a choice is two reductions over the
+// wavefront, of the values as sortable integers and of the indices that have the largest. The pairs are sorted by counting:
+// tokens are dealt in order to workgroups and their wavefronts, and a wavefront places its tokens one after the other -- a
+// token's experts are all different, so its lanes can place them at once. That makes the order stable and the same every time.
+#include "mx_common.h"
+
+namespace tllm {
+
+constexpr int ROUTE_E = 512, ROUTE_TOP = 32, ROUTE_GROUPS = 64;
+constexpr int ROUTE_WAVES = 16;           // wavefronts of a workgroup
+constexpr int ROUTE_RUNS = 256;           // most workgroups that count
+constexpr int ROUTE_ALONE = 64;           // tokens that one workgroup routes and sorts in one launch
+
+struct RouteArgs {
+  const void* logits;
+  int64_t row_stride;
+  const float* bias;
+  int* experts;
+  float* weights;
+  int* order;
+  int* offsets;
+  int* counts;                            // [runs][n_experts]
+  int64_t tokens;
+  int n_experts, top, groups, kept, renorm;
+  float scale;
+  int per_wave, runs;                     // tokens of a wavefront; workgroups
+};
+
+__device__ __forceinline__ unsigned wave_max_u32(unsigned v) {
+  auto dpp = [](unsigned x, auto ctrl) { return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+  v = max(v, dpp(v, std::integral_constant<int, 0xB1>{}));
+  v = max(v, dpp(v, std::integral_constant<int, 0x4E>{}));
+  v = max(v, dpp(v, std::integral_constant<int, 0x141>{}));
+  v = max(v, dpp(v, std::integral_constant<int, 0x140>{}));
+  const unsigned r0 = __builtin_amdgcn_readlane(v, 0), r1 = __builtin_amdgcn_readlane(v, 16), r2 = __builtin_amdgcn_readlane(v, 32), r3 = __builtin_amdgcn_readlane(v, 48);
+  return max(max(r0, r1), max(r2, r3));
+}
+
+// Lanes of one wavefront see each other's LDS writes in the order of the program; this keeps the compiler to it.
+__device__ __forceinline__ void lds_in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// fp32 as an unsigned integer of the same order; -0 is 0 and NaN -infinity. No float gives 0.
+__device__ __forceinline__ unsigned sortable(float v) {
+  v = v != v ? -__builtin_inff() : v + 0.0f;
+  const unsigned b = __builtin_bit_cast(unsigned, v);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// The largest key of the wavefront, the lowest index where several have it; `index` counts up with v in a lane.
+template <int V>
+__device__ __forceinline__ int take_best(unsigned (&key)[V], int lane) {
+  unsigned best = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) best = max(best, key[v]);
+  const unsigned top = wave_max_u32(best);
+  unsigned at = 0;                                          // complement of the lowest index
+#pragma unroll
+  for (int v = V - 1; v >= 0; --v)
+    if (key[v] == top) at = 0xffffu - (v * 64 + lane);
+  const int e = 0xffff - static_cast<int>(wave_max_u32(at));
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (v * 64 + lane == e) key[v] = 0;                     // taken
+  return e;
+}
+
+// One token: lane j < top has its j-th expert in `expert`, and writes that and the weight.
+template <int V, bool SIGMOID, class T>
+__device__ __forceinline__ int route_token(const RouteArgs& a, int64_t t, int lane, float* mine) {
+  const float ninf = -__builtin_inff();
+  const T* const row = static_cast<const T*>(a.logits) + t * a.row_stride;
+  float score[V];
+  unsigned key[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 64 + lane;
+    float l = e < a.n_experts ? static_cast<float>(row[e]) : ninf;
+    score[v] = l != l ? ninf : l;
+  }
+  float best = ninf, sum = 0.f;
+  if constexpr (!SIGMOID) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) best = fmaxf(best, score[v]);
+    best = wave_max(best);
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float l = score[v];
+    key[v] = v * 64 + lane < a.n_experts ? sortable(l) : 0;
+    if constexpr (SIGMOID) score[v] = 1.0f / (1.0f + expf(-l));
+    else score[v] = l == ninf ? 0.f : l == best ? 1.f : expf(l - best);     // (an infinite logit takes all)
+    sum += score[v];
+  }
+  if constexpr (!SIGMOID) {
+    sum = wave_sum(sum);
+#pragma unroll
+    for (int v = 0; v < V; ++v) score[v] = sum > 0.f ? score[v] / sum : 0.f;
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v * 64 + lane < a.n_experts) key[v] = sortable(score[v] + a.bias[v * 64 + lane]);
+  }
+  if (a.groups > 1) {
+    const int size = a.n_experts / a.groups;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = v * 64 + lane;
+      if (e < a.n_experts) mine[e] = a.bias ? score[v] + a.bias[e] : score[v];
+    }
+    lds_in_order();
+    unsigned gk[1] = {0};
+    if (lane < a.groups) {
+      float one = ninf, two = ninf;
+      for (int i = 0; i < size; ++i) {
+        float c = mine[lane * size + i];
+        c = c != c ? ninf : c;
+        two = c > one ? one : c > two ? c : two;
+        one = c > one ? c : one;
+      }
+      gk[0] = sortable(size > 1 ? one + two : one);
+    }
+    unsigned long long stay = 0;
+    for (int i = 0; i < a.kept; ++i) stay |= 1ull << take_best<1>(gk, lane);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (!(stay >> ((v * 64 + lane) / size & 63) & 1)) key[v] = 0;
+    lds_in_order();
+  }
+  int expert = 0;
+  float weight = 0.f, total = 0.f;
+  for (int j = 0; j < a.top; ++j) {
+    const int e = take_best<V>(key, lane);
+    float s = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v == e >> 6) s = score[v];
+    s = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), e & 63));
+    total += s;
+    if (lane == j) {
+      expert = e;
+      weight = s;
+    }
+  }
+  if (lane < a.top) {
+    if (a.renorm) weight = total > 0.f ? weight / total : 0.f;
+    a.experts[t * a.top + lane] = expert;
+    a.weights[t * a.top + lane] = weight * a.scale;
+  }
+  return expert;
+}
+
+// The tokens of workgroup b, wavefront w: per_wave of them from (b ROUTE_WAVES + w) per_wave on.
+template <int V, bool SIGMOID, class T, bool ALONE>
+__global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(RouteArgs a) {
+  __shared__ float choices[ROUTE_WAVES][V * 64];
+  __shared__ int count[ALONE ? ROUTE_WAVES : 1][V * 64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int i = threadIdx.x; i < static_cast<int>(sizeof(count) / 4); i += ROUTE_WAVES * 64) count[0][i] = 0;
+  __syncthreads();
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * ROUTE_WAVES + wave) * a.per_wave;
+  int chosen[ALONE ? ROUTE_ALONE / ROUTE_WAVES : 1];
+  if constexpr (ALONE) {
+#pragma unroll
+    for (int i = 0; i < ROUTE_ALONE / ROUTE_WAVES; ++i)
+      if (i < a.per_wave && t0 + i < a.tokens) {
+        chosen[i] = route_token<V, SIGMOID, T>(a, t0 + i, lane, choices[wave]);
+        if (lane < a.top) count[wave][chosen[i]] += 1;      // (a token's experts are different ones)
+        lds_in_order();
+      }
+  } else {
+    for (int i = 0; i < a.per_wave && t0 + i < a.tokens; ++i) {
+      const int e = route_token<V, SIGMOID, T>(a, t0 + i, lane, choices[wave]);
+      if (lane < a.top) atomicAdd(&count[0][e], 1);
+    }
+  }
+  __syncthreads();
+  if constexpr (!ALONE) {
+    for (int e = threadIdx.x; e < a.n_experts; e += ROUTE_WAVES * 64) a.counts[static_cast<int64_t>(blockIdx.x) * a.n_experts + e] = count[0][e];
+  } else {
+    // counts become first places: over the experts first, then over the wavefronts of one
+    if (wave == 0) {
+      int before = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int e = v * 64 + lane;
+        int n = 0;
+#pragma unroll
+        for (int w = 0; w < ROUTE_WAVES; ++w) n += count[w][e];
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const int u = __shfl_up(upto, d);
+          if (lane >= d) upto += u;
+        }
+        int at = before + upto - n;
+        if (e < a.n_experts) a.offsets[e] = at;
+#pragma unroll
+        for (int w = 0; w < ROUTE_WAVES; ++w) {
+          const int c = count[w][e];
+          count[w][e] = at;
+          at += c;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+      }
+      if (lane == 0) a.offsets[a.n_experts] = before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROUTE_ALONE / ROUTE_WAVES; ++i)
+      if (i < a.per_wave && t0 + i < a.tokens && lane < a.top) {
+        lds_in_order();
+        const int at = count[wave][chosen[i]];
+        count[wave][chosen[i]] = at + 1;
+        a.order[at] = static_cast<int>((t0 + i) * a.top + lane);
+      }
+  }
+}
+
+// Places the pairs of a run (the tokens of one workgroup of the kernel before): behind the experts before theirs, the runs
+// before this one, and the wavefronts before this one.
+__global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_place_kernel(RouteArgs a) {
+  __shared__ int first[ROUTE_E], here[ROUTE_E], count[ROUTE_WAVES][ROUTE_E];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int E = a.n_experts, run = blockIdx.x;
+  for (int i = tid; i < ROUTE_WAVES * ROUTE_E; i += ROUTE_WAVES * 64) count[0][i] = 0;
+  for (int e = tid; e < ROUTE_E; e += ROUTE_WAVES * 64) {
+    int all = 0, earlier = 0;
+    if (e < E)
+      for (int r = 0; r < a.runs; ++r) {
+        const int c = a.counts[static_cast<int64_t>(r) * E + e];
+        all += c;
+        earlier += r < run ? c : 0;
+      }
+    first[e] = all;
+    here[e] = earlier;
+  }
+  __syncthreads();
+  const int64_t t0 = (static_cast<int64_t>(run) * ROUTE_WAVES + wave) * a.per_wave;
+  for (int i = 0; i < a.per_wave && t0 + i < a.tokens; ++i) {
+    if (lane < a.top) count[wave][a.experts[(t0 + i) * a.top + lane]] += 1;
+    lds_in_order();
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int before = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+      const int e = e0 + lane;
+      const int n = e < ROUTE_E ? first[e] : 0;
+      int upto = n;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int u = __shfl_up(upto, d);
+        if (lane >= d) upto += u;
+      }
+      const int start = before + upto - n;
+      if (run == 0 && e < E) a.offsets[e] = start;
+      int at = start + here[e];
+      for (int w = 0; w < ROUTE_WAVES; ++w) {
+        const int c = count[w][e];
+        count[w][e] = at;
+        at += c;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (run == 0 && lane == 0) a.offsets[E] = before;
+  }
+  __syncthreads();
+  for (int i = 0; i < a.per_wave && t0 + i < a.tokens; ++i) {
+    lds_in_order();
+    if (lane < a.top) {
+      const int64_t p = (t0 + i) * a.top + lane;
+      int* const c = &count[wave][a.experts[p]];
+      const int at = *c;
+      *c = at + 1;
+      a.order[at] = static_cast<int>(p);
+    }
+  }
+}
+
+template <int V>
+static int launch_route(const RouteArgs& a, bool sigmoid, bool is_f32, bool alone, hipStream_t st) {
+  auto go = [&](auto* kernel) { hipLaunchKernelGGL(kernel, dim3(a.runs), dim3(ROUTE_WAVES * 64), 0, st, a); };
+  auto type = [&](auto sig, auto one) {
+    constexpr bool S = decltype(sig)::value, A = decltype(one)::value;
+    if (is_f32) go(moe_route_kernel<V, S, float, A>);
+    else go(moe_route_kernel<V, S, bf16, A>);
+  };
+  if (sigmoid) alone ? type(std::true_type{}, std::true_type{}) : type(std::true_type{}, std::false_type{});
+  else alone ? type(std::false_type{}, std::true_type{}) : type(std::false_type{}, std::false_type{});
+  return check_launch("moe_route");
+}
+
+static int route_runs(int64_t tokens, int* per_wave) {
+  const int64_t per = (tokens + ROUTE_RUNS * ROUTE_WAVES - 1) / (ROUTE_RUNS * ROUTE_WAVES);
+  *per_wave = static_cast<int>(tokens > ROUTE_ALONE ? per : tokens > 0 ? (tokens + ROUTE_WAVES - 1) / ROUTE_WAVES : 1);
+  return static_cast<int>((tokens + static_cast<int64_t>(*per_wave) * ROUTE_WAVES - 1) / (static_cast<int64_t>(*per_wave) * ROUTE_WAVES));
+}
+
+}  // namespace tllm
+
+using namespace tllm;
+
+extern "C" int64_t tllm_moe_route_workspace_bytes(int64_t tokens, int n_experts) {
+  if (tokens <= ROUTE_ALONE || n_experts < 1) return 0;
+  int per;
+  return static_cast<int64_t>(route_runs(tokens, &per)) * n_experts * 4;
+}
+
+extern "C" int tllm_moe_route(const void* logits, int logits_is_f32, int64_t logits_row_stride, const float* bias, int sigmoid, int n_groups, int topk_groups,
+                              int renormalize, float scale, int32_t* experts, float* weights, int32_t* order, int32_t* offsets, void* workspace,
+                              int64_t workspace_bytes, int64_t tokens, int n_experts, int top, void* stream) {
+  TLLM_REQUIRE(tokens >= 0, TLLM_E_ARG, "moe_route: tokens %lld", (long long)tokens);
+  TLLM_REQUIRE(n_experts >= 1 && n_experts <= ROUTE_E, TLLM_E_SHAPE, "moe_route: %d experts, 1 to %d are supported", n_experts, ROUTE_E);
+  TLLM_REQUIRE(n_groups >= 1 && n_groups <= ROUTE_GROUPS && n_experts % n_groups == 0, TLLM_E_SHAPE, "moe_route: %d experts in %d groups", n_experts, n_groups);
+  TLLM_REQUIRE(topk_groups >= 1 && topk_groups <= n_groups, TLLM_E_SHAPE, "moe_route: %d of %d groups", topk_groups, n_groups);
+  TLLM_REQUIRE(top >= 1 && top <= ROUTE_TOP && top <= n_experts / n_groups * topk_groups, TLLM_E_SHAPE,
+               "moe_route: top %d of %d experts (%d of %d groups); at most %d", top, n_experts, topk_groups, n_groups, ROUTE_TOP);
+  TLLM_REQUIRE(tokens * top < (1ll << 31), TLLM_E_SHAPE, "moe_route: %lld tokens x %d are too many", (long long)tokens, top);
+  TLLM_REQUIRE(offsets, TLLM_E_ARG, "moe_route: null pointer");
+  TLLM_REQUIRE(tokens == 0 || (logits && experts && weights && order), TLLM_E_ARG, "moe_route: null pointer");
+  TLLM_REQUIRE(logits_row_stride >= n_experts || tokens <= 1, TLLM_E_ARG, "moe_route: logits_row_stride %lld < %d experts", (long long)logits_row_stride, n_experts);
+  const int64_t need = tllm_moe_route_workspace_bytes(tokens, n_experts);
+  TLLM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), TLLM_E_ARG, "moe_route: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes,
+               (long long)need);
+  RouteArgs a{logits, logits_row_stride, bias, experts, weights, order, offsets, static_cast<int*>(workspace), tokens, n_experts, top, n_groups, topk_groups,
+              renormalize, scale, 0, 0};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool alone = tokens <= ROUTE_ALONE;
+  a.runs = route_runs(tokens, &a.per_wave);
+  if (tokens == 0) a.runs = 1;                             // (the offsets alone, all 0)
+  const bool s = sigmoid != 0, f = logits_is_f32 != 0;
+  const int rc = n_experts <= 64 ? launch_route<1>(a, s, f, alone, st) : n_experts <= 128 ? launch_route<2>(a, s, f, alone, st)
+               : n_experts <= 256 ? launch_route<4>(a, s, f, alone, st) : launch_route<8>(a, s, f, alone, st);
+  if (rc != TLLM_OK || alone) return rc;
+  hipLaunchKernelGGL(moe_place_kernel, dim3(a.runs), dim3(ROUTE_WAVES * 64), 0, st, a);
+  return check_launch("moe_route");
+}

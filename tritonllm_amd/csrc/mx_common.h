@@ -1,0 +1,124 @@
+// What the products with MXFP4 weights share: the operands, and which expert's rows a workgroup takes.
+//
+// An MXFP4 row of K values is K / 32 blocks of 16 bytes (32 e2m1 codes, the low nibble first) and as many e8m0 bytes, each the
+// block's power of two, biased by 127; 255 there makes the block NaN. That is how a checkpoint stores the experts
+// ([experts, N, K / 32, 16] and [experts, N, K / 32]) and how the kernels read it: nothing is laid out anew.
+#pragma once
+#include <utility>
+
+#include "common.h"
+
+namespace tllm {
+
+typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned u32x4;
+typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8;
+
+// y = x . W^T + b | SwiGLU of it, for rows by expert | a row per pair in fp32, for the weighted sum over a token's experts
+enum : int { kMxLinear = 0, kMxSwiglu = 1, kMxPairs = 2 };
+
+struct MxArgs {
+  const void* x;                    // rows of bf16, or of MXFP4 blocks
+  const unsigned char* x_scales;    // (MXFP4 rows alone)
+  int64_t x_pitch;                  // bytes from row to row
+  const unsigned char* w;           // blocks
+  const unsigned char* w_scales;
+  const bf16* bias;                 // [experts, N] or NULL
+  void* out;                        // bf16; fp32 for kMxPairs
+  int64_t out_stride;               // elements from row to row
+  const int* order;                 // pairs (token * top + choice) by expert, or NULL: one weight, rows as they are
+  const int* offsets;               // [experts + 1] places in `order`
+  int64_t rows;                     // rows, or pairs
+  int64_t tokens;
+  int experts, top;
+  int n, k;                         // weight rows (per expert) and values in each
+  float alpha, limit;               // SwiGLU; limit is infinity for none
+};
+
+// Items are runs of up to ROWS rows of one expert, in the order of the experts; a launch has as many as there can be
+// (mx_items), and the workgroups of those that are not there find no rows. All 64 lanes ask together: each loads one
+// expert's two offsets, a scan over the lanes counts the items before it, and a ballot finds the expert whose item this is.
+// Offsets are held to [0, rows], so that no content of theirs leads out of the tensors.
+struct MxItem {
+  int expert, first, rows;          // rows 0: none
+};
+static inline int64_t mx_items(int64_t rows, int experts, int per_item) {
+  return (rows < experts ? rows : experts) + rows / per_item;
+}
+__device__ __forceinline__ MxItem mx_find_item(const int* offsets, int experts, int rows, int per_item, int item) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int e0 = 0; e0 < experts; e0 += 64) {
+    const int e = e0 + lane;
+    int lo = offsets[e < experts ? e : experts], hi = offsets[e < experts ? e + 1 : experts];
+    lo = min(max(lo, 0), rows);
+    hi = min(max(hi, lo), rows);
+    const int mine = (hi - lo + per_item - 1) / per_item;
+    int upto = mine;                                       // items of the experts up to this lane's
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int v = __shfl_up(upto, d);
+      if (lane >= d) upto += v;
+    }
+    const unsigned long long has = __ballot(before + upto > item);
+    if (has) {
+      const int l = __builtin_ctzll(has);
+      const int at = item - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
+      const int first = __builtin_amdgcn_readlane(lo, l) + at * per_item, end = __builtin_amdgcn_readlane(hi, l);
+      return {e0 + l, first, min(per_item, end - first)};
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {0, 0, 0};
+}
+
+// A token's row: the pair at place s of the order, held to the pairs there are.
+__device__ __forceinline__ unsigned mx_pair(const MxArgs& a, int s) {
+  const unsigned p = static_cast<unsigned>(a.order[s]), last = static_cast<unsigned>(a.rows - 1);
+  return p < last ? p : last;
+}
+
+// Clamped SwiGLU of a gate and a linear value: g sigmoid(alpha g) (l + 1).
+__device__ __forceinline__ float mx_swiglu(float g, float l, float alpha, float limit) {
+  // (comparisons and not fminf: a NaN stays one)
+  g = g > limit ? limit : g;
+  l = l > limit ? limit : l < -limit ? -limit : l;
+  return g / (1.0f + __expf(-alpha * g)) * (l + 1.0f);
+}
+
+// A dword of eight codes times 2^(s - 127) as bf16, exactly (values of 2^128 and more, scale bytes 253 and 254, are infinite);
+// `scale` is the byte in an fp32's exponent, 0 there means 2^-127 and 255 NaN.
+__device__ __forceinline__ bf16x8 mx_bf16x8(unsigned codes, float scale) {
+  u32x4 o;
+  o[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
+  o[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
+  o[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
+  o[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
+  return __builtin_bit_cast(bf16x8, o);
+}
+
+// f(0), f(1), ... f(N - 1) with the numbers as types
+template <class F, int... I>
+__device__ __forceinline__ void mx_each(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void mx_each(F&& f) {
+  mx_each(f, std::make_integer_sequence<int, N>{});
+}
+
+// A buffer of `bytes` bytes from p on; loads behind its end give zeros and fetch nothing. MX_NONE is behind every end.
+constexpr unsigned MX_NONE = 0xfffffff0u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(bytes), 0x27000);
+}
+__device__ __forceinline__ u32x4 mx_load16(__amdgpu_buffer_rsrc_t b, unsigned at) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
+}
+__device__ __forceinline__ u32x4 mx_load16_once(__amdgpu_buffer_rsrc_t b, unsigned at) {   // (the nontemporal hint)
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 2));
+}
+__device__ __forceinline__ unsigned mx_load1(__amdgpu_buffer_rsrc_t b, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b8(b, at, 0, 0); }
+
+int mx_stream(const MxArgs& a, int mode, bool a4, hipStream_t st);
+
+}  // namespace tllm

@@ -72,9 +72,126 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const unsigned* __re
   }
 }
 
+// Quantisation to MXFP4 (the OCP microscaling format): the 32 values of a block share the power of two e = floor(log2 max|x|) - 2, at
+// least 2^-127, and become the nearest e2m1 value of x 2^-e, ties to the even code; beyond 6 is 6. A block that holds a NaN or an
+// infinity has the scale byte 255, which makes all of it NaN, and codes of 0.
+// The maximum is one of the values' bits: without the sign they order as integers, and the exponent field less 2 is the scale
+// byte. A lane takes eight values (16 or 32 bytes), four neighbouring lanes a block.
+template <class T>
+struct Eight;                        // eight values as loaded; the largest of their magnitudes as an fp32's bits; eight codes
+template <>
+struct Eight<bf16> {
+  u32x4 v;
+  __device__ void load(const void* p) { v = *static_cast<const u32x4*>(p); }
+  __device__ unsigned largest() const {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, max(v[i] << 16 & 0x7fff0000u, v[i] & 0x7fff0000u));
+    return m;
+  }
+  template <int I>
+  __device__ unsigned pair(unsigned old, float scale) const {
+    const unsigned two = v[I];       // (a scalar of its own: __builtin_bit_cast of a vector's element takes element 0 with this compiler)
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(bf16x2, two), scale, I);
+  }
+};
+template <>
+struct Eight<_Float16> {
+  typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2;
+  u32x4 v;
+  __device__ void load(const void* p) { v = *static_cast<const u32x4*>(p); }
+  __device__ unsigned largest() const {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, max(v[i] & 0x7fffu, v[i] >> 16 & 0x7fffu));
+    return __builtin_bit_cast(unsigned, static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(m))));
+  }
+  template <int I>
+  __device__ unsigned pair(unsigned old, float scale) const {
+    const unsigned two = v[I];
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(f16x2, two), scale, I);
+  }
+};
+template <>
+struct Eight<float> {
+  f32x4 v[2];
+  __device__ void load(const void* p) {
+    v[0] = static_cast<const f32x4*>(p)[0];
+    v[1] = static_cast<const f32x4*>(p)[1];
+  }
+  __device__ unsigned largest() const {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float one = v[i / 4][i % 4];
+      m = max(m, __builtin_bit_cast(unsigned, one) & 0x7fffffffu);
+    }
+    return m;
+  }
+  template <int I>
+  __device__ unsigned pair(unsigned old, float scale) const { return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, v[I / 2][I % 2 * 2], v[I / 2][I % 2 * 2 + 1], scale, I); }
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t row_stride, int per_row, unsigned* __restrict__ blocks,
+                                                             unsigned char* __restrict__ scales, int64_t n) {
+  const int64_t d = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;    // eight values each; n is a multiple of 4
+  if (d >= n) return;
+  const T* from = x + d * 8;
+  if (row_stride != 8ll * per_row) {
+    const int64_t row = d / per_row;
+    from = x + row * row_stride + (d - row * per_row) * 8;
+  }
+  Eight<T> e;
+  e.load(from);
+  unsigned m = e.largest();
+  m = max(m, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(m), 0xB1, 0xf, 0xf, true)));   // lane ^ 1
+  m = max(m, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(m), 0x4E, 0xf, 0xf, true)));   // lane ^ 2
+  const unsigned field = m >> 23, byte = field == 255 ? 255 : field > 2 ? field - 2 : 0;
+  const float scale = __builtin_bit_cast(float, byte << 23);                 // (a field of 0 is 2^-127 to the conversion)
+  unsigned codes = e.template pair<0>(0u, scale);
+  codes = e.template pair<1>(codes, scale);
+  codes = e.template pair<2>(codes, scale);
+  codes = e.template pair<3>(codes, scale);
+  blocks[d] = field == 255 ? 0 : codes;
+  if ((d & 3) == 0) scales[d >> 2] = static_cast<unsigned char>(byte);
+}
+
 }  // namespace tllm
 
 using namespace tllm;
+
+extern "C" int tllm_mxfp4_quantize(const void* x, int x_type, int64_t x_row_stride, void* blocks, void* scales, int64_t rows, int64_t cols, void* stream) {
+  TLLM_REQUIRE(rows >= 0 && cols >= 0, TLLM_E_ARG, "mxfp4_quantize: %lld x %lld values", (long long)rows, (long long)cols);
+  TLLM_REQUIRE(x_type == TLLM_BF16 || x_type == TLLM_F16 || x_type == TLLM_F32, TLLM_E_ARG, "mxfp4_quantize: type %d", x_type);
+  TLLM_REQUIRE(cols % 32 == 0 && cols < (1ll << 31), TLLM_E_SHAPE, "mxfp4_quantize: %lld values in a row, whole blocks of 32 are supported", (long long)cols);
+  if (rows == 0 || cols == 0) return TLLM_OK;
+  const int64_t size = x_type == TLLM_F32 ? 4 : 2;
+  TLLM_REQUIRE(x && blocks && scales, TLLM_E_ARG, "mxfp4_quantize: null pointer");
+  TLLM_REQUIRE(rows == 1 || x_row_stride >= cols, TLLM_E_ARG, "mxfp4_quantize: x_row_stride %lld < %lld", (long long)x_row_stride, (long long)cols);
+  TLLM_REQUIRE(aligned16(x) && aligned16(blocks) && (rows == 1 || x_row_stride * size % 16 == 0), TLLM_E_ALIGN, "mxfp4_quantize: rows of x and blocks must be 16-byte aligned");
+  TLLM_REQUIRE(rows < (1ll << 40) / cols, TLLM_E_SHAPE, "mxfp4_quantize: %lld x %lld values are too many", (long long)rows, (long long)cols);
+  if (rows == 1) x_row_stride = cols;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t rows_per_launch = (1ll << 31) / (cols / 8);      // (a launch holds fewer than 2^32 threads)
+  for (int64_t r = 0; r < rows; r += rows_per_launch) {
+    const int64_t m = (rows - r < rows_per_launch ? rows - r : rows_per_launch) * (cols / 8);
+    const dim3 grid((unsigned)((m + 255) / 256));
+    const char* const from = static_cast<const char*>(x) + r * x_row_stride * size;
+    unsigned* const to = static_cast<unsigned*>(blocks) + r * (cols / 8);
+    unsigned char* const sc = static_cast<unsigned char*>(scales) + r * (cols / 32);
+    const int per_row = static_cast<int>(cols / 8);
+    if (x_type == TLLM_BF16)
+      hipLaunchKernelGGL(mxfp4_quantize_kernel<bf16>, grid, dim3(256), 0, st, reinterpret_cast<const bf16*>(from), x_row_stride, per_row, to, sc, m);
+    else if (x_type == TLLM_F16)
+      hipLaunchKernelGGL(mxfp4_quantize_kernel<_Float16>, grid, dim3(256), 0, st, reinterpret_cast<const _Float16*>(from), x_row_stride, per_row, to, sc, m);
+    else
+      hipLaunchKernelGGL(mxfp4_quantize_kernel<float>, grid, dim3(256), 0, st, reinterpret_cast<const float*>(from), x_row_stride, per_row, to, sc, m);
+    const int rc = check_launch("mxfp4_quantize");
+    if (rc != TLLM_OK) return rc;
+  }
+  return TLLM_OK;
+}
 
 extern "C" int tllm_mxfp4_dequant_bf16(const void* blocks, const void* scales, void* out, int64_t n_blocks, void* stream) {
   TLLM_REQUIRE(n_blocks >= 0, TLLM_E_ARG, "mxfp4_dequant: n_blocks %lld", (long long)n_blocks);

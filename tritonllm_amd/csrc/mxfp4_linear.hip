@@ -1,0 +1,132 @@
+// Products with MXFP4 weights: the entry points, and the weighted sum over a token's experts.
+#include "mx_common.h"
+
+namespace tllm {
+
+// out[t, n] = residual[t, n] + sum_j weights[t, j] pairs[t top + j, n], in the order of j, in fp32, rounded once.
+__global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restrict__ pairs, const float* __restrict__ weights, const bf16* residual,
+                                                          int64_t res_stride, bf16* out, int64_t out_stride, int n, int top, int per_row) {
+  const int64_t t = blockIdx.x / per_row;
+  const int c = (blockIdx.x % per_row) * 256 + threadIdx.x;
+  if (c >= n) return;
+  float v = residual ? static_cast<float>(residual[t * res_stride + c]) : 0.f;
+  for (int j = 0; j < top; ++j) v = fmaf(weights[t * top + j], pairs[(t * top + j) * n + c], v);
+  out[t * out_stride + c] = static_cast<bf16>(v);
+}
+
+static int weight_ok(const char* what, const void* w, const void* ws, int64_t experts, int64_t k, int64_t n) {
+  TLLM_REQUIRE(n >= 1 && k >= 32 && k % 32 == 0, TLLM_E_SHAPE, "%s: a weight of %lld x %lld values; rows of whole blocks of 32 are supported", what, (long long)n, (long long)k);
+  TLLM_REQUIRE(k <= (1 << 24) && n <= (1 << 24), TLLM_E_SHAPE, "%s: a weight of %lld x %lld values is too large", what, (long long)n, (long long)k);
+  TLLM_REQUIRE(experts >= 1, TLLM_E_ARG, "%s: %lld experts", what, (long long)experts);
+  TLLM_REQUIRE(w && ws, TLLM_E_ARG, "%s: null pointer", what);
+  TLLM_REQUIRE(aligned16(w), TLLM_E_ALIGN, "%s: blocks must be 16-byte aligned", what);
+  return TLLM_OK;
+}
+
+// The last byte of x has a 32-bit offset.
+static int rows_ok(const char* what, const void* x, int64_t rows, int64_t pitch, int64_t row_bytes) {
+  TLLM_REQUIRE(x, TLLM_E_ARG, "%s: null pointer", what);
+  TLLM_REQUIRE(rows == 1 || pitch >= row_bytes, TLLM_E_ARG, "%s: rows of %lld bytes, %lld apart", what, (long long)row_bytes, (long long)pitch);
+  TLLM_REQUIRE(aligned16(x) && (rows == 1 || pitch % 16 == 0), TLLM_E_ALIGN, "%s: rows of x must be 16-byte aligned", what);
+  TLLM_REQUIRE((rows - 1) <= (int64_t)(MX_NONE - row_bytes) / (pitch > 0 ? pitch : 1), TLLM_E_SHAPE, "%s: x spans 4 GiB or more", what);
+  return TLLM_OK;
+}
+
+}  // namespace tllm
+
+using namespace tllm;
+
+#define TLLM_TRY(call)                 \
+  do {                                 \
+    const int rc_ = (call);            \
+    if (rc_ != TLLM_OK) return rc_;    \
+  } while (0)
+
+extern "C" int tllm_mxfp4_linear_bf16(const void* x, const void* x_scales, int64_t x_row_stride, const void* w_blocks, const void* w_scales, const void* bias,
+                                      void* out, int64_t out_row_stride, int64_t rows, int64_t in_dim, int64_t out_dim, void* stream) {
+  TLLM_REQUIRE(rows >= 0 && rows < (1ll << 31), TLLM_E_ARG, "mxfp4_linear: %lld rows", (long long)rows);
+  if (rows == 0) return TLLM_OK;
+  TLLM_TRY(weight_ok("mxfp4_linear", w_blocks, w_scales, 1, in_dim, out_dim));
+  const int64_t row_bytes = x_scales ? in_dim / 2 : in_dim * 2, pitch = x_scales ? row_bytes : x_row_stride * 2;
+  TLLM_TRY(rows_ok("mxfp4_linear", x, rows, pitch, row_bytes));
+  TLLM_REQUIRE(out, TLLM_E_ARG, "mxfp4_linear: null pointer");
+  TLLM_REQUIRE(rows == 1 || out_row_stride >= out_dim, TLLM_E_ARG, "mxfp4_linear: out_row_stride %lld < %lld", (long long)out_row_stride, (long long)out_dim);
+  MxArgs a{};
+  a.x = x;
+  a.x_scales = static_cast<const unsigned char*>(x_scales);
+  a.x_pitch = pitch;
+  a.w = static_cast<const unsigned char*>(w_blocks);
+  a.w_scales = static_cast<const unsigned char*>(w_scales);
+  a.bias = static_cast<const bf16*>(bias);
+  a.out = out;
+  a.out_stride = out_row_stride;
+  a.rows = a.tokens = rows;
+  a.experts = a.top = 1;
+  a.n = static_cast<int>(out_dim);
+  a.k = static_cast<int>(in_dim);
+  return mx_stream(a, kMxLinear, x_scales != nullptr, static_cast<hipStream_t>(stream));
+}
+
+static int experts_args(const char* what, MxArgs* a, const void* x, int64_t x_row_stride, int64_t x_rows, const int32_t* order, const int32_t* offsets,
+                        const void* w_blocks, const void* w_scales, const void* bias, int64_t tokens, int n_experts, int top, int64_t k, int64_t n) {
+  TLLM_REQUIRE(top >= 1 && n_experts >= top, TLLM_E_SHAPE, "%s: top %d of %d experts", what, top, n_experts);
+  TLLM_REQUIRE(tokens * top < (1ll << 31), TLLM_E_SHAPE, "%s: %lld tokens x %d are too many", what, (long long)tokens, top);
+  TLLM_TRY(weight_ok(what, w_blocks, w_scales, n_experts, k, n));
+  TLLM_TRY(rows_ok(what, x, x_rows, x_row_stride * 2, k * 2));
+  TLLM_REQUIRE(order && offsets, TLLM_E_ARG, "%s: null pointer", what);
+  a->x = x;
+  a->x_pitch = x_row_stride * 2;
+  a->w = static_cast<const unsigned char*>(w_blocks);
+  a->w_scales = static_cast<const unsigned char*>(w_scales);
+  a->bias = static_cast<const bf16*>(bias);
+  a->order = order;
+  a->offsets = offsets;
+  a->rows = tokens * top;
+  a->tokens = tokens;
+  a->experts = n_experts;
+  a->top = top;
+  a->n = static_cast<int>(n);
+  a->k = static_cast<int>(k);
+  return TLLM_OK;
+}
+
+extern "C" int tllm_moe_mlp1_bf16(const void* x, int64_t x_row_stride, const int32_t* order, const int32_t* offsets, const void* w_blocks, const void* w_scales,
+                                  const void* bias, void* h, int64_t h_row_stride, int64_t tokens, int n_experts, int top, int64_t hidden, int64_t inner,
+                                  float alpha, float limit, int has_limit, void* stream) {
+  TLLM_REQUIRE(tokens >= 0, TLLM_E_ARG, "moe_mlp1: tokens %lld", (long long)tokens);
+  if (tokens == 0) return TLLM_OK;
+  MxArgs a{};
+  TLLM_TRY(experts_args("moe_mlp1", &a, x, x_row_stride, tokens, order, offsets, w_blocks, w_scales, bias, tokens, n_experts, top, hidden, 2 * inner));
+  TLLM_REQUIRE(h && h_row_stride >= inner, TLLM_E_ARG, "moe_mlp1: null pointer, or h_row_stride %lld < %lld", (long long)h_row_stride, (long long)inner);
+  TLLM_REQUIRE(!has_limit || limit >= 0.f, TLLM_E_ARG, "moe_mlp1: limit %g", (double)limit);
+  a.out = h;
+  a.out_stride = h_row_stride;
+  a.alpha = alpha;
+  a.limit = has_limit ? limit : __builtin_inff();
+  return mx_stream(a, kMxSwiglu, false, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t tllm_moe_mlp2_workspace_bytes(int64_t tokens, int top, int64_t hidden) { return tokens > 0 && top > 0 && hidden > 0 ? tokens * top * hidden * 4 : 0; }
+
+extern "C" int tllm_moe_mlp2_bf16(const void* h, int64_t h_row_stride, const int32_t* order, const int32_t* offsets, const float* weights, const void* w_blocks,
+                                  const void* w_scales, const void* bias, const void* residual, int64_t res_row_stride, void* out, int64_t out_row_stride,
+                                  void* workspace, int64_t workspace_bytes, int64_t tokens, int n_experts, int top, int64_t inner, int64_t hidden, void* stream) {
+  TLLM_REQUIRE(tokens >= 0, TLLM_E_ARG, "moe_mlp2: tokens %lld", (long long)tokens);
+  if (tokens == 0) return TLLM_OK;
+  MxArgs a{};
+  TLLM_TRY(experts_args("moe_mlp2", &a, h, h_row_stride, tokens * top, order, offsets, w_blocks, w_scales, bias, tokens, n_experts, top, inner, hidden));
+  TLLM_REQUIRE(weights && out, TLLM_E_ARG, "moe_mlp2: null pointer");
+  TLLM_REQUIRE(tokens == 1 || (out_row_stride >= hidden && (!residual || res_row_stride >= hidden)), TLLM_E_ARG, "moe_mlp2: rows of %lld values, %lld (residual %lld) apart",
+               (long long)hidden, (long long)out_row_stride, (long long)res_row_stride);
+  const int64_t need = tllm_moe_mlp2_workspace_bytes(tokens, top, hidden), per_row = (hidden + 255) / 256;
+  TLLM_REQUIRE(tokens * per_row < (1ll << 24), TLLM_E_SHAPE, "moe_mlp2: %lld tokens of %lld values are too many", (long long)tokens, (long long)hidden);
+  TLLM_REQUIRE(workspace && workspace_bytes >= need && aligned16(workspace), TLLM_E_ARG, "moe_mlp2: a 16-byte aligned workspace of %lld bytes is needed, got %lld",
+               (long long)need, (long long)workspace_bytes);
+  a.out = workspace;
+  a.out_stride = hidden;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  TLLM_TRY(mx_stream(a, kMxPairs, false, st));
+  hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)(tokens * per_row)), dim3(256), 0, st, static_cast<const float*>(workspace), weights,
+                     static_cast<const bf16*>(residual), res_row_stride, static_cast<bf16*>(out), out_row_stride, (int)hidden, top, (int)per_row);
+  return check_launch("moe_mlp2");
+}

@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -814,3 +815,169 @@ def mxfp4_dequant(blocks: torch.Tensor, scales: torch.Tensor, out: torch.Tensor 
         _require(out.dtype == _BF16 and out.is_contiguous() and out.numel() == n_blocks * 32, "out must be contiguous bf16 of 32 values per block")
     check(lib().tllm_mxfp4_dequant_bf16(blocks.data_ptr(), scales.data_ptr(), out.data_ptr(), n_blocks, _stream()), "mxfp4_dequant")
     return out.view(shape) if out.shape != torch.Size(shape) else out
+
+
+_MX_TYPES = {_BF16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as a matrix whose rows are dense and begin at multiples of 16 bytes, a copy of it where they are not."""
+    t2 = t if t.ndim == 2 else t.reshape(-1, t.shape[-1])
+    size = t2.element_size()
+    if t2.shape[1] and (t2.stride(1) != 1 or t2.data_ptr() % 16 or (t2.shape[0] > 1 and (t2.stride(0) < t2.shape[1] or t2.stride(0) * size % 16))):
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2
+
+
+def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``x [..., K]`` (bf16, fp16 or fp32, K a multiple of 32) in MXFP4: ``(blocks [..., K / 32, 16], scales [..., K / 32])``, uint8, the
+    layout of a checkpoint's ``.blocks`` / ``.scales``.
+
+    The 32 values of a block share the power of two ``max(floor(log2 max|x|) - 2, -127)`` and go to the nearest e2m1 value,
+    ties to the even code, at most 6. A block that holds a NaN or an infinity gets the scale byte 255, which stands for NaN."""
+    _on_gpu(x)
+    _require(x.dtype in _MX_TYPES, "mxfp4_quantize: x must be bfloat16, float16 or float32")
+    _require(x.ndim >= 1 and x.shape[-1] % 32 == 0, "mxfp4_quantize: the last dimension must be whole blocks of 32 values")
+    shape = (*x.shape[:-1], x.shape[-1] // 32)
+    blocks = torch.empty((*shape, 16), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(shape, dtype=torch.uint8, device=x.device)
+    if x.numel():
+        x2 = _rows16(x)
+        check(lib().tllm_mxfp4_quantize(x2.data_ptr(), _MX_TYPES[x.dtype], x2.stride(0), blocks.data_ptr(), scales.data_ptr(), x2.shape[0], x2.shape[1],
+                                        _stream()), "mxfp4_quantize")
+    return blocks, scales
+
+
+def _mx_weight(blocks: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None, ndim: int):
+    _require(blocks.dtype == torch.uint8 and scales.dtype == torch.uint8, "MXFP4 blocks and scales are uint8")
+    _require(blocks.ndim == ndim + 1 and blocks.shape[-1] == 16, "an MXFP4 block is 16 bytes")
+    _require(blocks.shape[:-1] == scales.shape, f"{blocks.shape=} does not match {scales.shape=}")
+    _require(bias is None or (bias.dtype == _BF16 and bias.shape == scales.shape[:-1]), "the bias is bfloat16, one for each row of the weight")
+    return blocks.contiguous(), scales.contiguous(), bias if bias is None else bias.contiguous()
+
+
+def mxfp4_linear(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None,
+                 x_scales: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ W.T + bias`` with an MXFP4 weight ``W [N, K]`` (``blocks [N, K / 32, 16]``, ``scales [N, K / 32]``): ``[..., N]`` bf16.
+
+    ``x`` is ``[..., K]`` bf16 or, with ``x_scales [..., K / 32]``, MXFP4 blocks ``[..., K / 32, 16]`` as ``mxfp4_quantize`` makes
+    them. Products are exact, sums fp32, rounded once."""
+    _on_gpu(x, blocks, scales, bias, x_scales)
+    blocks, scales, bias = _mx_weight(blocks, scales, bias, 2)
+    n, g = scales.shape
+    if x_scales is not None:
+        _require(x.dtype == torch.uint8 and x_scales.dtype == torch.uint8 and x.shape == (*x_scales.shape, 16), "x: MXFP4 blocks of 16 bytes with a scale each")
+        _require(x_scales.ndim >= 1 and x_scales.shape[-1] == g, f"x has {x_scales.shape[-1]} blocks in a row, the weight {g}")
+        lead, x2, x_scales = x_scales.shape[:-1], x.contiguous(), x_scales.contiguous()
+        rows, stride = x_scales.numel() // g if g else 0, 0
+    else:
+        _require(x.dtype == _BF16 and x.ndim >= 1 and x.shape[-1] == 32 * g, f"x must be bfloat16 with {32 * g} values in a row")
+        lead, x2 = x.shape[:-1], _rows16(x)
+        rows, stride = x2.shape[0], x2.stride(0)
+    out = torch.empty((*lead, n), dtype=_BF16, device=x.device)
+    if out.numel():
+        check(lib().tllm_mxfp4_linear_bf16(x2.data_ptr(), x_scales.data_ptr() if x_scales is not None else None, stride, blocks.data_ptr(),
+                                           scales.data_ptr(), bias.data_ptr() if bias is not None else None, out.data_ptr(), n, rows, 32 * g, n,
+                                           _stream()), "mxfp4_linear")
+    return out
+
+
+class MoeRouting(NamedTuple):
+    """What ``moe_route`` answers: each token's experts, best first, and their weights; and the plan of the experts' products,
+    the pairs ``token * top + choice`` in the order of their experts and each expert's first place in that order."""
+
+    experts: torch.Tensor   # [tokens, top] int32
+    weights: torch.Tensor   # [tokens, top] float32
+    order: torch.Tensor     # [tokens * top] int32
+    offsets: torch.Tensor   # [experts + 1] int32
+
+
+def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: torch.Tensor | None = None, n_groups: int = 1,
+              topk_groups: int = 1, renormalize: bool = True, scale: float = 1.0) -> MoeRouting:
+    """Route tokens to experts by ``logits [..., experts]`` (bf16 or fp32).
+
+    The scores ``s`` are the logits' ``"softmax"`` or ``"sigmoid"``; the choice goes by ``s + bias`` (fp32 ``[experts]``, for balance) or,
+    without a bias, by the logits. With ``n_groups`` equal groups of experts, the ``topk_groups`` whose best two sum highest stay.
+    The ``top_k`` best are taken, the lowest index where equal, with the weights ``s`` there, divided by their sum under
+    ``renormalize``, times ``scale``. The defaults are gpt-oss's router (softmax over the chosen logits). A NaN counts as -inf; an
+    expert of -inf has a weight of 0."""
+    _on_gpu(logits, bias)
+    _require(logits.dtype in (_BF16, torch.float32) and logits.ndim >= 1, "moe_route: logits must be bfloat16 or float32")
+    _require(score in ("softmax", "sigmoid"), f"moe_route: score {score!r}")
+    experts = logits.shape[-1]
+    _require(bias is None or (bias.dtype == torch.float32 and bias.shape == (experts,)), "moe_route: the bias is float32, one for each expert")
+    x = logits if logits.ndim == 2 else logits.reshape(-1, experts)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < experts):
+        x = x.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    tokens, dev = x.shape[0], logits.device
+    chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
+    plan = torch.empty(tokens * top_k + experts + 1, dtype=torch.int32, device=dev)
+    order, offsets = plan[: tokens * top_k], plan[tokens * top_k:]
+    need = lib().tllm_moe_route_workspace_bytes(tokens, experts)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(lib().tllm_moe_route(x.data_ptr(), int(x.dtype == torch.float32), x.stride(0), bias.data_ptr() if bias is not None else None,
+                               int(score == "sigmoid"), n_groups, topk_groups, int(renormalize), float(scale), chosen.data_ptr(), weights.data_ptr(),
+                               order.data_ptr(), offsets.data_ptr(), work.data_ptr() if need else None, need, tokens, experts, top_k, _stream()),
+          "moe_route")
+    return MoeRouting(chosen, weights, order, offsets)
+
+
+def _routing_of(routing: MoeRouting, experts: int):
+    _, weights, order, offsets = routing
+    _require(weights.ndim == 2 and weights.dtype == torch.float32 and weights.is_contiguous(), "routing: weights are float32 [tokens, top]")
+    _require(order.dtype == torch.int32 and order.is_contiguous() and order.numel() == weights.numel(), "routing: order is int32, one for each pair")
+    _require(offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.shape == (experts + 1,), f"routing: offsets are int32 [{experts + 1}]")
+    return weights, order, offsets
+
+
+def moe_mlp1(x: torch.Tensor, routing: MoeRouting, blocks: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None, *,
+             alpha: float = 1.702, limit: float | None = 7.0) -> torch.Tensor:
+    """The experts' first product and its clamped SwiGLU (model.py:751-757, moe.py:25-33): ``x [..., hidden]`` bf16 and an MXFP4 weight
+    ``[experts, 2 * inner, hidden]`` (gate and linear rows in turn) give ``[tokens * top, inner]`` bf16, a row for each pair in the
+    order of ``routing.order``."""
+    _on_gpu(x, *routing, blocks, scales, bias)
+    blocks, scales, bias = _mx_weight(blocks, scales, bias, 3)
+    experts, n, g = scales.shape
+    _require(n % 2 == 0, "moe_mlp1: the weight has a gate and a linear row for each output")
+    _require(x.dtype == _BF16 and x.ndim >= 1 and x.shape[-1] == 32 * g, f"moe_mlp1: x must be bfloat16 with {32 * g} values in a row")
+    weights, order, offsets = _routing_of(routing, experts)
+    x2 = _rows16(x)
+    tokens, top = weights.shape
+    _require(x2.shape[0] == tokens, f"moe_mlp1: {x2.shape[0]} rows for {tokens} routed tokens")
+    h = torch.empty((tokens * top, n // 2), dtype=_BF16, device=x.device)
+    if h.numel():
+        check(lib().tllm_moe_mlp1_bf16(x2.data_ptr(), x2.stride(0), order.data_ptr(), offsets.data_ptr(), blocks.data_ptr(), scales.data_ptr(),
+                                       bias.data_ptr() if bias is not None else None, h.data_ptr(), n // 2, tokens, experts, top, 32 * g, n // 2,
+                                       float(alpha), float(limit) if limit is not None else 0.0, int(limit is not None), _stream()), "moe_mlp1")
+    return h
+
+
+def moe_mlp2(h: torch.Tensor, routing: MoeRouting, blocks: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None, *,
+             residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The experts' second product, weighted and summed over each token's experts, plus the residual (model.py:751-757):
+    ``h [tokens * top, inner]`` as ``moe_mlp1`` gives it and an MXFP4 weight ``[experts, hidden, inner]`` give ``[tokens, hidden]`` bf16
+    (in ``residual``'s shape if there is one). ``out`` may be ``residual``."""
+    _on_gpu(h, *routing, blocks, scales, bias, residual, out)
+    blocks, scales, bias = _mx_weight(blocks, scales, bias, 3)
+    experts, n, g = scales.shape
+    weights, order, offsets = _routing_of(routing, experts)
+    tokens, top = weights.shape
+    _require(h.dtype == _BF16 and h.shape == (tokens * top, 32 * g), f"moe_mlp2: h must be bfloat16 [{tokens * top}, {32 * g}]")
+    _require(residual is None or (residual.dtype == _BF16 and residual.numel() == tokens * n and residual.shape[-1] == n), f"moe_mlp2: the residual is bfloat16 [{tokens}, {n}]")
+    shape = tuple(residual.shape) if residual is not None else (tokens, n)
+    if out is None:
+        out = torch.empty(shape, dtype=_BF16, device=h.device)
+    _require(out.dtype == _BF16 and out.shape == shape and out.is_contiguous(), "moe_mlp2: out is contiguous bfloat16 in the residual's shape")
+    if residual is not None and not residual.is_contiguous():
+        residual = residual.contiguous()
+    h2 = _rows16(h)
+    if out.numel():
+        need = lib().tllm_moe_mlp2_workspace_bytes(tokens, top, n)
+        work = torch.empty(need, dtype=torch.uint8, device=h.device)
+        check(lib().tllm_moe_mlp2_bf16(h2.data_ptr(), h2.stride(0), order.data_ptr(), offsets.data_ptr(), weights.data_ptr(), blocks.data_ptr(),
+                                       scales.data_ptr(), bias.data_ptr() if bias is not None else None,
+                                       residual.data_ptr() if residual is not None else None, n, out.data_ptr(), n, work.data_ptr(), need, tokens,
+                                       experts, top, 32 * g, n, _stream()), "moe_mlp2")
+    return out
