@@ -71,6 +71,47 @@ __device__ __forceinline__ MxItem mx_find_item(const int* offsets, int experts, 
   return {0, 0, 0};
 }
 
+// The same for a grid in the order (expert, tile of weight rows, item): one of `tiles` x items, dealt so that the tiles of an XCD
+// (workgroups go to the eight of them in turn) are neighbours -- those of one run of weight rows, then the next run's.
+struct MxTile {
+  int expert, first, rows, tile_n;  // rows 0: none
+};
+__device__ __forceinline__ MxTile mx_find_tile(const int* offsets, int experts, int rows, int per_item, int tiles_n, int block) {
+  const int lane = threadIdx.x & 63;
+  auto counted = [&](int e, int* lo, int* hi) {
+    *lo = offsets[e < experts ? e : experts];
+    *hi = offsets[e < experts ? e + 1 : experts];
+    *lo = min(max(*lo, 0), rows);
+    *hi = min(max(*hi, *lo), rows);
+    return (*hi - *lo + per_item - 1) / per_item;
+  };
+  int lo, hi, total = 0;
+  for (int e0 = 0; e0 < experts; e0 += 64) total += counted(e0 + lane, &lo, &hi);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+  const int all = total * tiles_n, per = (all + 7) / 8, at = block >> 3, t = (block & 7) * per + at;
+  if (at >= per || t >= all) return {0, 0, 0, 0};
+  int before = 0;
+  for (int e0 = 0; e0 < experts; e0 += 64) {
+    const int mine = counted(e0 + lane, &lo, &hi);
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int v = __shfl_up(upto, d);
+      if (lane >= d) upto += v;
+    }
+    const unsigned long long has = __ballot((before + upto) * tiles_n > t);
+    if (has) {
+      const int l = __builtin_ctzll(has), items = __builtin_amdgcn_readlane(mine, l);
+      const int local = t - (before + __builtin_amdgcn_readlane(upto, l) - items) * tiles_n;
+      const int tile_n = local / items, first = __builtin_amdgcn_readlane(lo, l) + (local - tile_n * items) * per_item;
+      return {e0 + l, first, min(per_item, __builtin_amdgcn_readlane(hi, l) - first), tile_n};
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {0, 0, 0, 0};
+}
+
 // A token's row: the pair at place s of the order, held to the pairs there are.
 __device__ __forceinline__ unsigned mx_pair(const MxArgs& a, int s) {
   const unsigned p = static_cast<unsigned>(a.order[s]), last = static_cast<unsigned>(a.rows - 1);
@@ -117,8 +158,23 @@ __device__ __forceinline__ u32x4 mx_load16(__amdgpu_buffer_rsrc_t b, unsigned at
 __device__ __forceinline__ u32x4 mx_load16_once(__amdgpu_buffer_rsrc_t b, unsigned at) {   // (the nontemporal hint)
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 2));
 }
+// The same buffer as four words, for the load that goes straight to LDS: 16 bytes a lane, from `at` + `more` in the buffer to
+// `lds` + 16 x lane. The compiler does not know of it: its arrival is waited for by count.
+__device__ __forceinline__ u32x4 mx_buffer_words(const void* p, unsigned bytes) {
+  const uint64_t b = reinterpret_cast<uint64_t>(p);
+  u32x4 w;
+  w[0] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(b));
+  w[1] = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(b >> 32) & 0xffffu);
+  w[2] = __builtin_amdgcn_readfirstlane(bytes);
+  w[3] = 0x27000;
+  return w;
+}
+__device__ __forceinline__ void mx_load_lds(u32x4 buffer, unsigned at, unsigned more, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(at), "s"(buffer), "s"(more) : "memory", "m0");
+}
 __device__ __forceinline__ unsigned mx_load1(__amdgpu_buffer_rsrc_t b, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b8(b, at, 0, 0); }
 
 int mx_stream(const MxArgs& a, int mode, bool a4, hipStream_t st);
+int mx_tiles(const MxArgs& a, int mode, hipStream_t st);
 
 }  // namespace tllm

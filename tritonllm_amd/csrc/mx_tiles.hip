@@ -1,0 +1,203 @@
+// Products with an MXFP4 weight for many rows of bf16: tiles on the matrix cores.
+//
+//   D[r, n] = sum_k X[r, k] W[n, k]        X bf16, W MXFP4, a run of one expert's rows to a tile
+//
+// K goes in slices of 64: a slice of X is 128 bytes a row, of W 32 (two blocks). Both come into a ring of S slices in LDS as they are
+// (buffer loads straight to LDS); the codes become bf16 in registers, in front of v_mfma_f32_16x16x32_bf16, weight rows on M. In a
+// slice lane (m, g) of a fragment has the values k = 16 g .. 16 g + 15, half a block, eight for each of two MFMAs, of both operands.
+// The scale bytes of the tile's weight rows lie in LDS for the whole of K, a lane reads one for a fragment's slice.
+// A lane ends up with four neighbouring weight rows of one row of X and stores them from its registers.
+#include "mx_common.h"
+
+namespace tllm {
+
+template <int TB_, int RB_, int WM_, int WN_, int S_>
+struct MxTileShape {
+  static constexpr int TB = TB_, RB = RB_, WM = WM_, WN = WN_, S = S_, NW = WM * WN;
+  static constexpr int BM = 16 * TB * WM, BN = 16 * RB * WN;
+  static constexpr int XB = BM * 128, WB = BN * 32, STAGE = XB + WB;
+  static constexpr int XL = BM / 8 / NW, WL = BN / 32 / NW, LPW = XL + WL;        // loads of a wavefront per slice: 8 rows of X, 32 of W
+  static_assert(XL * 8 * NW == BM && WL * 32 * NW == BN && S >= 2, "whole loads");
+};
+
+template <class C, int MODE>
+__global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles_n) {
+  constexpr int TB = C::TB, RB = C::RB, S = C::S, BM = C::BM, BN = C::BN, XL = C::XL, WL = C::WL, LPW = C::LPW;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave % C::WN, wm = wave / C::WN, m16 = lane & 15, g = lane >> 4;
+  MxTile it;
+  if (a.order == nullptr) {
+    const int items = static_cast<int>((a.rows + BM - 1) / BM), all = items * tiles_n, per = (all + 7) / 8, at = blockIdx.x >> 3;
+    const int t = (blockIdx.x & 7) * per + at;
+    if (at >= per || t >= all) return;
+    const int64_t first = static_cast<int64_t>(t % items) * BM, left = a.rows - first;
+    it = {0, static_cast<int>(first), static_cast<int>(left < BM ? left : BM), t / items};
+  } else {
+    it = mx_find_tile(a.offsets, a.experts, static_cast<int>(a.rows), BM, tiles_n, blockIdx.x);
+  }
+  if (it.rows <= 0) return;
+  const int n0 = it.tile_n * BN, blocks = a.k / 32, slices = (blocks + 1) / 2;
+  const int nn = a.n - n0 < BN ? a.n - n0 : BN;
+  const int64_t wrow = static_cast<int64_t>(it.expert) * a.n + n0;
+  constexpr bool gather = MODE == kMxSwiglu;
+
+  // ---- loads
+  const unsigned char* const xb = static_cast<const unsigned char*>(a.x) + (gather ? 0 : it.first * a.x_pitch);
+  const unsigned x_span = static_cast<unsigned>(((gather ? a.tokens : it.rows) - 1) * a.x_pitch + a.k * 2);
+  const auto xr = mx_buffer_words(xb, x_span), wr = mx_buffer_words(a.w + wrow * blocks * 16, nn * blocks * 16);
+  unsigned xo[XL], wo[WL];
+#pragma unroll
+  for (int j = 0; j < XL; ++j) {
+    const int r = (wave * XL + j) * 8 + (lane >> 3), rr = r < it.rows ? r : 0;
+    const unsigned row = gather ? mx_pair(a, it.first + rr) / static_cast<unsigned>(a.top) : rr;
+    xo[j] = static_cast<unsigned>(row * a.x_pitch) + (((lane & 7) ^ (r >> 1 & 3)) << 4);
+  }
+#pragma unroll
+  for (int j = 0; j < WL; ++j) {
+    const int r = (wave * WL + j) * 32 + (lane >> 1);
+    wo[j] = (r < nn ? r : nn - 1) * (blocks * 16) + (lane & 1) * 16;
+  }
+  const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>(smem));
+  auto issue = [&](int slice, int place) {
+    const int s = slice < slices ? slice : slices - 1;     // (behind the last slice it again, so that the loads in flight can be counted)
+    const unsigned base = lds0 + place * C::STAGE;
+#pragma unroll
+    for (int j = 0; j < XL; ++j) mx_load_lds(xr, xo[j], s * 128, base + (wave * XL + j) * 1024);
+#pragma unroll
+    for (int j = 0; j < WL; ++j) mx_load_lds(wr, wo[j], s * 32, base + C::XB + (wave * WL + j) * 1024);
+  };
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue(s, s);
+
+  // ---- while they are on their way: scale bytes, four to a word, rows an odd number of words apart; the bias; the pairs' numbers
+  unsigned* const sc = reinterpret_cast<unsigned*>(smem + S * C::STAGE);
+  const int words = (blocks + 3) / 4, pitch = words | 1;
+  {
+    const unsigned char* const from = a.w_scales + wrow * blocks;
+    for (int i = tid; i < BN * words; i += C::NW * 64) {
+      const int r = i / words, w = i - r * words;
+      if (r >= nn) break;
+      unsigned v = 0;
+      if (blocks >= 4) {
+        const int at = min(4 * w, blocks - 4);
+        __builtin_memcpy(&v, from + static_cast<int64_t>(r) * blocks + at, 4);
+        v >>= 8 * (4 * w - at);
+      } else {
+        for (int b = 0; b < blocks; ++b) v |= static_cast<unsigned>(from[static_cast<int64_t>(r) * blocks + b]) << 8 * b;
+      }
+      sc[r * pitch + w] = v;
+    }
+  }
+  bf16 bias[RB][4];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = 16 * (RB * wn + rb) + 4 * g + i;
+      bias[rb][i] = a.bias ? a.bias[wrow + (n < nn ? n : nn - 1)] : static_cast<bf16>(0.f);
+    }
+  __syncthreads();
+
+  // ---- the walk over K
+  f32x4 acc[TB][RB];
+#pragma unroll
+  for (int t = 0; t < TB; ++t)
+#pragma unroll
+    for (int r = 0; r < RB; ++r) acc[t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const unsigned char* const scb = reinterpret_cast<const unsigned char*>(sc);
+  auto multiply = [&](int slice, int place, auto tail) {
+    const unsigned char* const st = smem + place * C::STAGE;
+    const bool none = decltype(tail)::value && g >= 2;     // the second block of the last slice is not there
+    typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
+    bf16x8 w[RB][2];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int row = 16 * (RB * wn + rb) + m16;
+      const u32x2 q = *reinterpret_cast<const u32x2*>(st + C::XB + row * 32 + g * 8);
+      unsigned lo = q[0], hi = q[1], e = scb[row * pitch * 4 + 2 * slice + (g >> 1)];
+      if (none) lo = hi = e = 0;
+      const float scale = __builtin_bit_cast(float, e << 23);
+      w[rb][0] = mx_bf16x8(lo, scale);
+      w[rb][1] = mx_bf16x8(hi, scale);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        const int row = 16 * (TB * wm + t) + m16;
+        u32x4 x = *reinterpret_cast<const u32x4*>(st + row * 128 + (((2 * g + i) ^ (m16 >> 1 & 3)) << 4));
+        if (none) x = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) acc[t][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[rb][i], __builtin_bit_cast(bf16x8, x), acc[t][rb], 0, 0, 0);
+      }
+  };
+  int place = 0;
+  const int whole = blocks / 2;
+  for (int s = 0; s < slices; ++s) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * LPW) : "memory");
+    issue(s + S - 1, place == 0 ? S - 1 : place - 1);
+    if (s < whole) multiply(s, place, std::false_type{});
+    else multiply(s, place, std::true_type{});
+    place = place + 1 == S ? 0 : place + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  // ---- lane (m16, g) holds weight rows 4 g .. + 3 of row m16 of X in each fragment pair
+#pragma unroll
+  for (int t = 0; t < TB; ++t) {
+    const int r = 16 * (TB * wm + t) + m16;
+    if (r >= it.rows) continue;
+    int64_t row = it.first + r;
+    if constexpr (MODE == kMxPairs) row = mx_pair(a, it.first + r);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int n = 16 * (RB * wn + rb) + 4 * g;
+      if (n >= nn) continue;
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = acc[t][rb][i] + static_cast<float>(bias[rb][i]);
+      const int64_t at = row * a.out_stride + n0 + n;
+      if constexpr (MODE == kMxSwiglu) {
+        bf16* const to = static_cast<bf16*>(a.out) + row * a.out_stride + (n0 + n) / 2;
+        const bf16 o0 = static_cast<bf16>(mx_swiglu(v[0], v[1], a.alpha, a.limit));
+        to[0] = o0;
+        if (n + 2 < nn) to[1] = static_cast<bf16>(mx_swiglu(v[2], v[3], a.alpha, a.limit));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < nn) {
+            if constexpr (MODE == kMxPairs) static_cast<float*>(a.out)[at + i] = v[i];
+            else static_cast<bf16*>(a.out)[at + i] = static_cast<bf16>(v[i]);
+          }
+      }
+    }
+  }
+}
+
+template <class C, int MODE>
+static int launch_tiles(const MxArgs& a, hipStream_t st) {
+  const int64_t tiles = (a.n + C::BN - 1) / C::BN;
+  const int64_t items = a.order ? mx_items(a.rows, a.experts, C::BM) : (a.rows + C::BM - 1) / C::BM;
+  const int blocks = a.k / 32, lds = C::S * C::STAGE + C::BN * (((blocks + 3) / 4) | 1) * 4;
+  TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
+  TLLM_REQUIRE(lds <= 160 * 1024, TLLM_E_SHAPE, "mxfp4 product: %d values in a row are too many for its tiles", a.k);
+  static std::atomic<uint64_t> done{0};
+  const void* const kernel = reinterpret_cast<const void*>(mx_tile_kernel<C, MODE>);
+  TLLM_REQUIRE(raise_lds_limit(kernel, 160 * 1024, done) == hipSuccess, TLLM_E_LAUNCH, "mxfp4 product: the LDS limit could not be raised");
+  hipLaunchKernelGGL((mx_tile_kernel<C, MODE>), dim3((unsigned)((tiles * items + 7) / 8 * 8)), dim3(C::NW * 64), lds, st, a, (int)tiles);
+  return check_launch("mxfp4 product");
+}
+
+#ifndef MX_SHAPE
+#define MX_SHAPE 4, 4, 1, 8, 3
+#endif
+typedef MxTileShape<MX_SHAPE> Big;
+
+int mx_tiles(const MxArgs& a, int mode, hipStream_t st) {
+  if (mode == kMxSwiglu) return launch_tiles<Big, kMxSwiglu>(a, st);
+  if (mode == kMxPairs) return launch_tiles<Big, kMxPairs>(a, st);
+  return launch_tiles<Big, kMxLinear>(a, st);
+}
+
+}  // namespace tllm

@@ -14,6 +14,11 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
   out[t * out_stride + c] = static_cast<bf16>(v);
 }
 
+static int product(const MxArgs& a, int mode, bool a4, hipStream_t st) {
+  if (!a4 && a.rows >= 24ll * a.experts && a.rows >= 512 && a.k <= 4096) return mx_tiles(a, mode, st);
+  return mx_stream(a, mode, a4, st);
+}
+
 static int weight_ok(const char* what, const void* w, const void* ws, int64_t experts, int64_t k, int64_t n) {
   TLLM_REQUIRE(n >= 1 && k >= 32 && k % 32 == 0, TLLM_E_SHAPE, "%s: a weight of %lld x %lld values; rows of whole blocks of 32 are supported", what, (long long)n, (long long)k);
   TLLM_REQUIRE(k <= (1 << 24) && n <= (1 << 24), TLLM_E_SHAPE, "%s: a weight of %lld x %lld values is too large", what, (long long)n, (long long)k);
@@ -64,7 +69,7 @@ extern "C" int tllm_mxfp4_linear_bf16(const void* x, const void* x_scales, int64
   a.experts = a.top = 1;
   a.n = static_cast<int>(out_dim);
   a.k = static_cast<int>(in_dim);
-  return mx_stream(a, kMxLinear, x_scales != nullptr, static_cast<hipStream_t>(stream));
+  return product(a, kMxLinear, x_scales != nullptr, static_cast<hipStream_t>(stream));
 }
 
 static int experts_args(const char* what, MxArgs* a, const void* x, int64_t x_row_stride, int64_t x_rows, const int32_t* order, const int32_t* offsets,
@@ -103,7 +108,7 @@ extern "C" int tllm_moe_mlp1_bf16(const void* x, int64_t x_row_stride, const int
   a.out_stride = h_row_stride;
   a.alpha = alpha;
   a.limit = has_limit ? limit : __builtin_inff();
-  return mx_stream(a, kMxSwiglu, false, static_cast<hipStream_t>(stream));
+  return product(a, kMxSwiglu, false, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t tllm_moe_mlp2_workspace_bytes(int64_t tokens, int top, int64_t hidden) { return tokens > 0 && top > 0 && hidden > 0 ? tokens * top * hidden * 4 : 0; }
@@ -125,7 +130,7 @@ extern "C" int tllm_moe_mlp2_bf16(const void* h, int64_t h_row_stride, const int
   a.out = workspace;
   a.out_stride = hidden;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  TLLM_TRY(mx_stream(a, kMxPairs, false, st));
+  TLLM_TRY(product(a, kMxPairs, false, st));
   hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)(tokens * per_row)), dim3(256), 0, st, static_cast<const float*>(workspace), weights,
                      static_cast<const bf16*>(residual), res_row_stride, static_cast<bf16*>(out), out_row_stride, (int)hidden, top, (int)per_row);
   return check_launch("moe_mlp2");
