@@ -68,35 +68,57 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
     for (int j = 0; j < WL; ++j) mx_load_lds(wr, wo[j], s * 32, base + C::XB + (wave * WL + j) * 1024);
   };
 #pragma unroll
-  for (int s = 0; s < S - 1; ++s) issue(s, s);
+  for (int s = 0; s < S; ++s) issue(s, s);
 
   // ---- while they are on their way: scale bytes, four to a word, rows an odd number of words apart; the bias; the pairs' numbers
   unsigned* const sc = reinterpret_cast<unsigned*>(smem + S * C::STAGE);
   const int words = (blocks + 3) / 4, pitch = words | 1;
   {
     const unsigned char* const from = a.w_scales + wrow * blocks;
-    for (int i = tid; i < BN * words; i += C::NW * 64) {
-      const int r = i / words, w = i - r * words;
-      if (r >= nn) break;
-      unsigned v = 0;
-      if (blocks >= 4) {
-        const int at = min(4 * w, blocks - 4);
-        __builtin_memcpy(&v, from + static_cast<int64_t>(r) * blocks + at, 4);
-        v >>= 8 * (4 * w - at);
-      } else {
-        for (int b = 0; b < blocks; ++b) v |= static_cast<unsigned>(from[static_cast<int64_t>(r) * blocks + b]) << 8 * b;
+    constexpr int THREADS = C::NW * 64, FLIGHT = 8;        // loads of a thread on their way together
+    const int step_r = THREADS / words, step_w = THREADS - step_r * words, last = blocks - 4;
+    int r = tid / words, w = tid - r * words;
+    while (r < nn) {
+      unsigned v[FLIGHT];
+      int at[FLIGHT];
+#pragma unroll
+      for (int j = 0; j < FLIGHT; ++j) {
+        at[j] = r < nn ? r * pitch + w : -1;
+        const int rr = r < nn ? r : nn - 1, off = 4 * w < last ? 4 * w : last;       // (a row's last word ends with the row)
+        if (blocks >= 4) {
+          __builtin_memcpy(&v[j], from + (rr * blocks + off), 4);
+          v[j] >>= 8 * (4 * w - off);
+        } else {
+          v[j] = 0;
+          for (int b = 0; b < blocks; ++b) v[j] |= static_cast<unsigned>(from[rr * blocks + b]) << 8 * b;
+        }
+        r += step_r;
+        w += step_w;
+        if (w >= words) {
+          w -= words;
+          ++r;
+        }
       }
-      sc[r * pitch + w] = v;
+#pragma unroll
+      for (int j = 0; j < FLIGHT; ++j)
+        if (at[j] >= 0) sc[at[j]] = v[j];
     }
   }
-  bf16 bias[RB][4];
+  // four neighbours of the bias, of a row of the result, at once: where their places are whole
+  const bool four = a.n % 4 == 0 && a.out_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(a.bias) % 8 == 0;
+  bf16x4 bias[RB];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
+  for (int rb = 0; rb < RB; ++rb) {
+    const int n = 16 * (RB * wn + rb) + 4 * g;
+    if (!a.bias) {
+      bias[rb] = bf16x4{};
+    } else if (four) {
+      bias[rb] = *reinterpret_cast<const bf16x4*>(a.bias + wrow + (n < nn ? n : 0));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = 16 * (RB * wn + rb) + 4 * g + i;
-      bias[rb][i] = a.bias ? a.bias[wrow + (n < nn ? n : nn - 1)] : static_cast<bf16>(0.f);
+      for (int i = 0; i < 4; ++i) bias[rb][i] = a.bias[wrow + (n + i < nn ? n + i : nn - 1)];
     }
+  }
   __syncthreads();
 
   // ---- the walk over K
@@ -106,40 +128,61 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
 #pragma unroll
     for (int r = 0; r < RB; ++r) acc[t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
   const unsigned char* const scb = reinterpret_cast<const unsigned char*>(sc);
-  auto multiply = [&](int slice, int place, auto tail) {
-    const unsigned char* const st = smem + place * C::STAGE;
-    const bool none = decltype(tail)::value && g >= 2;     // the second block of the last slice is not there
-    typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
-    bf16x8 w[RB][2];
+  typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
+  u32x2 q[RB];                                             // a slice's codes, and its scales as fp32
+  float qs[RB];
+  bf16x8 w[2][RB];
+  u32x4 x[2][TB];
+  const int xat = 16 * TB * wm + m16, wat = 16 * RB * wn + m16, flip = m16 >> 1 & 3;
+  auto read_w = [&](int slice, int place) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int row = 16 * (RB * wn + rb) + m16;
-      const u32x2 q = *reinterpret_cast<const u32x2*>(st + C::XB + row * 32 + g * 8);
-      unsigned lo = q[0], hi = q[1], e = scb[row * pitch * 4 + 2 * slice + (g >> 1)];
-      if (none) lo = hi = e = 0;
-      const float scale = __builtin_bit_cast(float, e << 23);
-      w[rb][0] = mx_bf16x8(lo, scale);
-      w[rb][1] = mx_bf16x8(hi, scale);
+      const int row = wat + 16 * rb;
+      q[rb] = *reinterpret_cast<const u32x2*>(smem + place * C::STAGE + C::XB + row * 32 + g * 8);
+      qs[rb] = __builtin_bit_cast(float, static_cast<unsigned>(scb[row * pitch * 4 + 2 * slice + (g >> 1)]) << 23);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        const int row = 16 * (TB * wm + t) + m16;
-        u32x4 x = *reinterpret_cast<const u32x4*>(st + row * 128 + (((2 * g + i) ^ (m16 >> 1 & 3)) << 4));
-        if (none) x = u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) acc[t][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[rb][i], __builtin_bit_cast(bf16x8, x), acc[t][rb], 0, 0, 0);
-      }
   };
+  auto read_x = [&](auto half, int place) {
+    constexpr int i = decltype(half)::value;
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+      x[i][t] = *reinterpret_cast<const u32x4*>(smem + place * C::STAGE + (xat + 16 * t) * 128 + (((2 * g + i) ^ flip) << 4));
+  };
+  // `none`: the second block of the last slice is not there
+  auto convert = [&](auto half, bool none) {
+    constexpr int i = decltype(half)::value;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) w[i][rb] = mx_bf16x8(none ? 0u : q[rb][i], none ? 1.0f : qs[rb]);
+    if (none)
+#pragma unroll
+      for (int t = 0; t < TB; ++t) x[i][t] = u32x4{0, 0, 0, 0};
+  };
+  auto multiply = [&](auto half) {
+    constexpr int i = decltype(half)::value;
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) acc[t][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i][rb], __builtin_bit_cast(bf16x8, x[i][t]), acc[t][rb], 0, 0, 0);
+  };
+  typedef std::integral_constant<int, 0> I0;
+  typedef std::integral_constant<int, 1> I1;
+  const bool odd = (blocks & 1) && g >= 2;
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * LPW) : "memory");
+  read_w(0, 0);
+  read_x(I0{}, 0);
   int place = 0;
-  const int whole = blocks / 2;
   for (int s = 0; s < slices; ++s) {
+    const bool none = odd && s + 1 == slices;
+    read_x(I1{}, place);
+    convert(I0{}, none);
+    multiply(I0{});
+    convert(I1{}, none);
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * LPW) : "memory");
-    issue(s + S - 1, place == 0 ? S - 1 : place - 1);
-    if (s < whole) multiply(s, place, std::false_type{});
-    else multiply(s, place, std::true_type{});
+    issue(s + S, place);
     place = place + 1 == S ? 0 : place + 1;
+    read_w(s + 1, place);                                  // (behind the last slice: the last one again, not used)
+    read_x(I0{}, place);
+    multiply(I1{});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
@@ -157,19 +200,34 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
       float v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = acc[t][rb][i] + static_cast<float>(bias[rb][i]);
-      const int64_t at = row * a.out_stride + n0 + n;
       if constexpr (MODE == kMxSwiglu) {
         bf16* const to = static_cast<bf16*>(a.out) + row * a.out_stride + (n0 + n) / 2;
-        const bf16 o0 = static_cast<bf16>(mx_swiglu(v[0], v[1], a.alpha, a.limit));
-        to[0] = o0;
-        if (n + 2 < nn) to[1] = static_cast<bf16>(mx_swiglu(v[2], v[3], a.alpha, a.limit));
-      } else {
+        const bf16x2 o = {static_cast<bf16>(mx_swiglu(v[0], v[1], a.alpha, a.limit)), static_cast<bf16>(mx_swiglu(v[2], v[3], a.alpha, a.limit))};
+        if (four) {
+          *reinterpret_cast<bf16x2*>(to) = o;
+        } else {
+          to[0] = o[0];
+          if (n + 2 < nn) to[1] = o[1];
+        }
+      } else if constexpr (MODE == kMxPairs) {
+        float* const to = static_cast<float*>(a.out) + row * a.out_stride + n0 + n;
+        if (four) {
+          *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < nn) {
-            if constexpr (MODE == kMxPairs) static_cast<float*>(a.out)[at + i] = v[i];
-            else static_cast<bf16*>(a.out)[at + i] = static_cast<bf16>(v[i]);
-          }
+          for (int i = 0; i < 4; ++i)
+            if (n + i < nn) to[i] = v[i];
+        }
+      } else {
+        bf16* const to = static_cast<bf16*>(a.out) + row * a.out_stride + n0 + n;
+        const bf16x4 o = {static_cast<bf16>(v[0]), static_cast<bf16>(v[1]), static_cast<bf16>(v[2]), static_cast<bf16>(v[3])};
+        if (four) {
+          *reinterpret_cast<bf16x4*>(to) = o;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + i < nn) to[i] = o[i];
+        }
       }
     }
   }
@@ -179,7 +237,7 @@ template <class C, int MODE>
 static int launch_tiles(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN;
   const int64_t items = a.order ? mx_items(a.rows, a.experts, C::BM) : (a.rows + C::BM - 1) / C::BM;
-  const int blocks = a.k / 32, lds = C::S * C::STAGE + C::BN * (((blocks + 3) / 4) | 1) * 4;
+  const int blocks = a.k / 32, lds = C::S * C::STAGE + C::BN * (((blocks + 3) / 4) | 1) * 4 + 16;
   TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
   TLLM_REQUIRE(lds <= 160 * 1024, TLLM_E_SHAPE, "mxfp4 product: %d values in a row are too many for its tiles", a.k);
   static std::atomic<uint64_t> done{0};
@@ -190,7 +248,7 @@ static int launch_tiles(const MxArgs& a, hipStream_t st) {
 }
 
 #ifndef MX_SHAPE
-#define MX_SHAPE 4, 4, 1, 8, 3
+#define MX_SHAPE 4, 2, 1, 8, 3
 #endif
 typedef MxTileShape<MX_SHAPE> Big;
 
