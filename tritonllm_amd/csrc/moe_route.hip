@@ -7,8 +7,8 @@
 // A logit (or a bias) that is NaN counts as -infinity, and an expert of -infinity has the score 0; a row of nothing else gets the
 // first experts with weights of 0. All in fp32.
 //
-// A wavefront takes a token, its logits in registers, lane l those of experts l, l + 64, ...; a choice is two reductions over the
-// wavefront, of the values as sortable integers and of the indices that have the largest. The pairs are sorted by counting:
+// A wavefront takes a token, its logits in registers, V neighbours to a lane; a choice is a maximum over the wavefront, of the
+// values as sortable integers, and the first lane that has it. The pairs are sorted by counting:
 // tokens are dealt in order to workgroups and their wavefronts, and a wavefront places its tokens one after the other -- a
 // token's experts are all different, so its lanes can place them at once. That makes the order stable and the same every time.
 #include "mx_common.h"
@@ -55,36 +55,43 @@ __device__ __forceinline__ unsigned sortable(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// The largest key of the wavefront, the lowest index where several have it; `index` counts up with v in a lane.
+// The largest key of the wavefront and its expert V lane + v, the lowest where several have it; it is taken out.
 template <int V>
 __device__ __forceinline__ int take_best(unsigned (&key)[V], int lane) {
-  unsigned best = 0;
+  unsigned best = key[0];
 #pragma unroll
-  for (int v = 0; v < V; ++v) best = max(best, key[v]);
+  for (int v = 1; v < V; ++v) best = max(best, key[v]);
   const unsigned top = wave_max_u32(best);
-  unsigned at = 0;                                          // complement of the lowest index
+  int at = V - 1;
 #pragma unroll
-  for (int v = V - 1; v >= 0; --v)
-    if (key[v] == top) at = 0xffffu - (v * 64 + lane);
-  const int e = 0xffff - static_cast<int>(wave_max_u32(at));
+  for (int v = V - 2; v >= 0; --v) at = key[v] == top ? v : at;
+  const int l = __builtin_ctzll(__ballot(best == top));
+  const int e = V * l + __builtin_amdgcn_readlane(at, l);
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (v * 64 + lane == e) key[v] = 0;                     // taken
+  for (int v = 0; v < V; ++v) key[v] = V * lane + v == e ? 0 : key[v];
   return e;
 }
 
-// One token: lane j < top has its j-th expert in `expert`, and writes that and the weight.
+// The best two of a pair of values and another's
+__device__ __forceinline__ void best_two(float& one, float& two, float a, float b) {
+  two = fmaxf(fminf(one, a), fmaxf(two, b));
+  one = fmaxf(one, a);
+}
+
+// One token: lane j < top has its j-th expert in the result, and writes that and the weight.
 template <int V, bool SIGMOID, class T>
-__device__ __forceinline__ int route_token(const RouteArgs& a, int64_t t, int lane, float* mine) {
+__device__ __forceinline__ int route_token(const RouteArgs& a, const float (&bias)[V], int64_t t, int lane, float* mine) {
   const float ninf = -__builtin_inff();
   const T* const row = static_cast<const T*>(a.logits) + t * a.row_stride;
   float score[V];
   unsigned key[V];
+  T l[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) l[v] = row[min(V * lane + v, a.n_experts - 1)];   // (no branch: the loads leave together)
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    float l = e < a.n_experts ? static_cast<float>(row[e]) : ninf;
-    score[v] = l != l ? ninf : l;
+    const float f = static_cast<float>(l[v]);
+    score[v] = V * lane + v >= a.n_experts || f != f ? ninf : f;
   }
   float best = ninf, sum = 0.f;
   if constexpr (!SIGMOID) {
@@ -95,7 +102,7 @@ __device__ __forceinline__ int route_token(const RouteArgs& a, int64_t t, int la
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const float l = score[v];
-    key[v] = v * 64 + lane < a.n_experts ? sortable(l) : 0;
+    key[v] = V * lane + v < a.n_experts ? sortable(l) : 0;
     if constexpr (SIGMOID) score[v] = 1.0f / (1.0f + expf(-l));
     else score[v] = l == ninf ? 0.f : l == best ? 1.f : expf(l - best);     // (an infinite logit takes all)
     sum += score[v];
@@ -108,48 +115,63 @@ __device__ __forceinline__ int route_token(const RouteArgs& a, int64_t t, int la
   if (a.bias) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (v * 64 + lane < a.n_experts) key[v] = sortable(score[v] + a.bias[v * 64 + lane]);
+      if (V * lane + v < a.n_experts) key[v] = sortable(score[v] + bias[v]);
   }
   if (a.groups > 1) {
-    const int size = a.n_experts / a.groups;
+    const int size = a.n_experts / a.groups, lanes = size / V;
+    float c[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int e = v * 64 + lane;
-      if (e < a.n_experts) mine[e] = a.bias ? score[v] + a.bias[e] : score[v];
+      c[v] = a.bias ? score[v] + bias[v] : score[v];
+      c[v] = c[v] != c[v] ? ninf : c[v];
     }
-    lds_in_order();
-    unsigned gk[1] = {0};
-    if (lane < a.groups) {
-      float one = ninf, two = ninf;
-      for (int i = 0; i < size; ++i) {
-        float c = mine[lane * size + i];
-        c = c != c ? ninf : c;
-        two = c > one ? one : c > two ? c : two;
-        one = c > one ? c : one;
-      }
-      gk[0] = sortable(size > 1 ? one + two : one);
-    }
-    unsigned long long stay = 0;
-    for (int i = 0; i < a.kept; ++i) stay |= 1ull << take_best<1>(gk, lane);
+    float value;                                            // of this lane's group, or of group `lane`
+    const bool spans = size == lanes * V && lanes > 0 && (lanes & (lanes - 1)) == 0;
+    if (spans) {                                            // a group is a power of two of whole lanes
+      float one = c[0], two = ninf;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (!(stay >> ((v * 64 + lane) / size & 63) & 1)) key[v] = 0;
-    lds_in_order();
+      for (int v = 1; v < V; ++v) best_two(one, two, c[v], ninf);
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2)
+        if (d < lanes) best_two(one, two, __shfl_xor(one, d), __shfl_xor(two, d));
+      value = size > 1 ? one + two : one;
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (V * lane + v < a.n_experts) mine[V * lane + v] = c[v];
+      lds_in_order();
+      float one = ninf, two = ninf;
+      if (lane < a.groups)
+        for (int i = 0; i < size; ++i) best_two(one, two, mine[lane * size + i], ninf);
+      value = size > 1 ? one + two : one;
+      lds_in_order();
+    }
+    // a group stays if fewer than `kept` are worth more, or as much with a lower number
+    const unsigned gk = sortable(value);
+    const int step = spans ? lanes : 1, group = lane / step;
+    int ahead = 0;
+    for (int j = 0; j < a.groups; ++j) {
+      const unsigned o = __builtin_amdgcn_readlane(gk, j * step);
+      ahead += o > gk || (o == gk && j < group);
+    }
+    const unsigned long long stay = __ballot(ahead < a.kept);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int of = spans ? lane : (V * lane + v) / size;  // the lane that knows of the group
+      if (of > 63 || !(stay >> (of & 63) & 1)) key[v] = 0;
+    }
   }
   int expert = 0;
   float weight = 0.f, total = 0.f;
   for (int j = 0; j < a.top; ++j) {
     const int e = take_best<V>(key, lane);
-    float s = 0.f;
+    float s = score[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v == e >> 6) s = score[v];
-    s = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), e & 63));
+    for (int v = 1; v < V; ++v) s = e % V == v ? score[v] : s;
+    s = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), e / V));
     total += s;
-    if (lane == j) {
-      expert = e;
-      weight = s;
-    }
+    expert = lane == j ? e : expert;
+    weight = lane == j ? s : weight;
   }
   if (lane < a.top) {
     if (a.renorm) weight = total > 0.f ? weight / total : 0.f;
@@ -159,27 +181,68 @@ __device__ __forceinline__ int route_token(const RouteArgs& a, int64_t t, int la
   return expert;
 }
 
+// Counts of a workgroup's wavefronts become their first places: each expert's `start` (the pairs before its own, of all experts
+// before and of the workgroups before), then the wavefronts one after the other.
+__device__ __forceinline__ void first_places(int* count, int pitch, const int* start, int n_experts) {
+  for (int e = threadIdx.x; e < n_experts; e += ROUTE_WAVES * 64) {
+    int at = start[e], c[ROUTE_WAVES];
+#pragma unroll
+    for (int w = 0; w < ROUTE_WAVES; ++w) c[w] = count[w * pitch + e];
+#pragma unroll
+    for (int w = 0; w < ROUTE_WAVES; ++w) {
+      count[w * pitch + e] = at;
+      at += c[w];
+    }
+  }
+}
+
+// One wavefront: all[e], pairs of expert e, becomes the pairs of the experts before it; so do the offsets, if they are to be written.
+__device__ __forceinline__ void scan_experts(int* all, int n_experts, int lane, int* offsets) {
+  int before = 0;
+  for (int e0 = 0; e0 < n_experts; e0 += 64) {
+    const int e = e0 + lane, n = e < n_experts ? all[e] : 0;
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int u = __shfl_up(upto, d);
+      if (lane >= d) upto += u;
+    }
+    const int start = before + upto - n;
+    if (e < n_experts) {
+      all[e] = start;
+      if (offsets) offsets[e] = start;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (offsets && lane == 0) offsets[n_experts] = before;
+}
+
 // The tokens of workgroup b, wavefront w: per_wave of them from (b ROUTE_WAVES + w) per_wave on.
 template <int V, bool SIGMOID, class T, bool ALONE>
 __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(RouteArgs a) {
   __shared__ float choices[ROUTE_WAVES][V * 64];
-  __shared__ int count[ALONE ? ROUTE_WAVES : 1][V * 64];
+  __shared__ int count[ALONE ? ROUTE_WAVES : 1][V * 64], start[ALONE ? V * 64 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int i = threadIdx.x; i < static_cast<int>(sizeof(count) / 4); i += ROUTE_WAVES * 64) count[0][i] = 0;
   __syncthreads();
   const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * ROUTE_WAVES + wave) * a.per_wave;
+  float bias[V] = {};
+  if (a.bias) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) bias[v] = a.bias[min(V * lane + v, a.n_experts - 1)];
+  }
   int chosen[ALONE ? ROUTE_ALONE / ROUTE_WAVES : 1];
   if constexpr (ALONE) {
 #pragma unroll
     for (int i = 0; i < ROUTE_ALONE / ROUTE_WAVES; ++i)
       if (i < a.per_wave && t0 + i < a.tokens) {
-        chosen[i] = route_token<V, SIGMOID, T>(a, t0 + i, lane, choices[wave]);
+        chosen[i] = route_token<V, SIGMOID, T>(a, bias, t0 + i, lane, choices[wave]);
         if (lane < a.top) count[wave][chosen[i]] += 1;      // (a token's experts are different ones)
         lds_in_order();
       }
   } else {
     for (int i = 0; i < a.per_wave && t0 + i < a.tokens; ++i) {
-      const int e = route_token<V, SIGMOID, T>(a, t0 + i, lane, choices[wave]);
+      const int e = route_token<V, SIGMOID, T>(a, bias, t0 + i, lane, choices[wave]);
       if (lane < a.top) atomicAdd(&count[0][e], 1);
     }
   }
@@ -187,33 +250,16 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(RouteArgs a
   if constexpr (!ALONE) {
     for (int e = threadIdx.x; e < a.n_experts; e += ROUTE_WAVES * 64) a.counts[static_cast<int64_t>(blockIdx.x) * a.n_experts + e] = count[0][e];
   } else {
-    // counts become first places: over the experts first, then over the wavefronts of one
-    if (wave == 0) {
-      int before = 0;
+    for (int e = threadIdx.x; e < a.n_experts; e += ROUTE_WAVES * 64) {
+      int n = 0;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int e = v * 64 + lane;
-        int n = 0;
-#pragma unroll
-        for (int w = 0; w < ROUTE_WAVES; ++w) n += count[w][e];
-        int upto = n;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const int u = __shfl_up(upto, d);
-          if (lane >= d) upto += u;
-        }
-        int at = before + upto - n;
-        if (e < a.n_experts) a.offsets[e] = at;
-#pragma unroll
-        for (int w = 0; w < ROUTE_WAVES; ++w) {
-          const int c = count[w][e];
-          count[w][e] = at;
-          at += c;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
-      }
-      if (lane == 0) a.offsets[a.n_experts] = before;
+      for (int w = 0; w < ROUTE_WAVES; ++w) n += count[w][e];
+      start[e] = n;
     }
+    __syncthreads();
+    if (wave == 0) scan_experts(start, a.n_experts, lane, a.offsets);
+    __syncthreads();
+    first_places(count[0], V * 64, start, a.n_experts);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < ROUTE_ALONE / ROUTE_WAVES; ++i)
@@ -229,51 +275,41 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(RouteArgs a
 // Places the pairs of a run (the tokens of one workgroup of the kernel before): behind the experts before theirs, the runs
 // before this one, and the wavefronts before this one.
 __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_place_kernel(RouteArgs a) {
-  __shared__ int first[ROUTE_E], here[ROUTE_E], count[ROUTE_WAVES][ROUTE_E];
+  __shared__ int all[ROUTE_E], earlier[ROUTE_E], count[ROUTE_WAVES][ROUTE_E];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int E = a.n_experts, run = blockIdx.x;
-  for (int i = tid; i < ROUTE_WAVES * ROUTE_E; i += ROUTE_WAVES * 64) count[0][i] = 0;
-  for (int e = tid; e < ROUTE_E; e += ROUTE_WAVES * 64) {
-    int all = 0, earlier = 0;
-    if (e < E)
-      for (int r = 0; r < a.runs; ++r) {
-        const int c = a.counts[static_cast<int64_t>(r) * E + e];
-        all += c;
-        earlier += r < run ? c : 0;
-      }
-    first[e] = all;
-    here[e] = earlier;
-  }
+  constexpr int THREADS = ROUTE_WAVES * 64;
+  for (int i = tid; i < ROUTE_WAVES * ROUTE_E; i += THREADS) count[0][i] = 0;
+  for (int e = tid; e < ROUTE_E; e += THREADS) all[e] = earlier[e] = 0;
   __syncthreads();
+  // the runs' counts, dealt to the threads by expert and by run, sixteen of a thread's on their way at a time
+  const int parts = THREADS / E, part = tid / E, mine = tid - part * E;
+  if (part < parts) {
+    int total = 0, before = 0;
+    for (int r0 = part; r0 < a.runs; r0 += 16 * parts) {
+      int c[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) c[j] = r0 + j * parts < a.runs ? a.counts[static_cast<int64_t>(r0 + j * parts) * E + mine] : 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        total += c[j];
+        before += r0 + j * parts < run ? c[j] : 0;
+      }
+    }
+    atomicAdd(&all[mine], total);
+    atomicAdd(&earlier[mine], before);
+  }
   const int64_t t0 = (static_cast<int64_t>(run) * ROUTE_WAVES + wave) * a.per_wave;
   for (int i = 0; i < a.per_wave && t0 + i < a.tokens; ++i) {
     if (lane < a.top) count[wave][a.experts[(t0 + i) * a.top + lane]] += 1;
     lds_in_order();
   }
   __syncthreads();
-  if (wave == 0) {
-    int before = 0;
-    for (int e0 = 0; e0 < E; e0 += 64) {
-      const int e = e0 + lane;
-      const int n = e < ROUTE_E ? first[e] : 0;
-      int upto = n;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int u = __shfl_up(upto, d);
-        if (lane >= d) upto += u;
-      }
-      const int start = before + upto - n;
-      if (run == 0 && e < E) a.offsets[e] = start;
-      int at = start + here[e];
-      for (int w = 0; w < ROUTE_WAVES; ++w) {
-        const int c = count[w][e];
-        count[w][e] = at;
-        at += c;
-      }
-      before += __builtin_amdgcn_readlane(upto, 63);
-    }
-    if (run == 0 && lane == 0) a.offsets[E] = before;
-  }
+  if (wave == 0) scan_experts(all, E, lane, run == 0 ? a.offsets : nullptr);
+  __syncthreads();
+  for (int e = tid; e < E; e += THREADS) all[e] += earlier[e];
+  __syncthreads();
+  first_places(count[0], ROUTE_E, all, E);
   __syncthreads();
   for (int i = 0; i < a.per_wave && t0 + i < a.tokens; ++i) {
     lds_in_order();
