@@ -174,7 +174,93 @@ __device__ __forceinline__ void mx_load_lds(u32x4 buffer, unsigned at, unsigned 
 }
 __device__ __forceinline__ unsigned mx_load1(__amdgpu_buffer_rsrc_t b, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b8(b, at, 0, 0); }
 
+// ---- what the tiles share
+// The scale bytes of a tile's rows in LDS, for the whole of K: four to a word, rows an odd number of words apart, so that sixteen
+// rows' words lie in different banks.
+static __host__ __device__ __forceinline__ int mx_scale_words(int blocks) { return ((blocks + 3) / 4) | 1; }
+template <int THREADS>
+__device__ __forceinline__ void mx_fetch_scales(unsigned* to, const unsigned char* from, int rows, int blocks, int tid) {
+  constexpr int FLIGHT = 8;                                // loads of a thread on their way together
+  const int words = (blocks + 3) / 4, pitch = words | 1, step_r = THREADS / words, step_w = THREADS - step_r * words, last = blocks - 4;
+  int r = tid / words, w = tid - r * words;
+  while (r < rows) {
+    unsigned v[FLIGHT];
+    int at[FLIGHT];
+#pragma unroll
+    for (int j = 0; j < FLIGHT; ++j) {
+      at[j] = r < rows ? r * pitch + w : -1;
+      const int rr = r < rows ? r : rows - 1, off = 4 * w < last ? 4 * w : last;     // (a row's last word ends with the row)
+      if (blocks >= 4) {
+        __builtin_memcpy(&v[j], from + (rr * blocks + off), 4);
+        v[j] >>= 8 * (4 * w - off);
+      } else {
+        v[j] = 0;
+        for (int b = 0; b < blocks; ++b) v[j] |= static_cast<unsigned>(from[rr * blocks + b]) << 8 * b;
+      }
+      r += step_r;
+      w += step_w;
+      if (w >= words) {
+        w -= words;
+        ++r;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < FLIGHT; ++j)
+      if (at[j] >= 0) to[at[j]] = v[j];
+  }
+}
+
+// Whether four neighbours of the bias and of a row of the result are whole accesses
+__device__ __forceinline__ bool mx_whole_fours(const MxArgs& a) {
+  return a.n % 4 == 0 && a.out_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(a.bias) % 8 == 0;
+}
+__device__ __forceinline__ bf16x4 mx_bias4(const MxArgs& a, bool four, int64_t wrow, int n, int nn) {
+  bf16x4 b = {};
+  if (a.bias == nullptr) return b;
+  if (four) return *reinterpret_cast<const bf16x4*>(a.bias + wrow + (n < nn ? n : 0));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = a.bias[wrow + (n + i < nn ? n + i : nn - 1)];
+  return b;
+}
+// Sums of weight rows n0 + n .. + 3 (nn of n0's tile are there) for a row of the result: bias, SwiGLU, one rounding
+template <int MODE>
+__device__ __forceinline__ void mx_store4(const MxArgs& a, bool four, int64_t row, int n0, int n, int nn, f32x4 sum, bf16x4 bias) {
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = sum[i] + static_cast<float>(bias[i]);
+  if constexpr (MODE == kMxSwiglu) {
+    bf16* const to = static_cast<bf16*>(a.out) + row * a.out_stride + (n0 + n) / 2;
+    const bf16x2 o = {static_cast<bf16>(mx_swiglu(v[0], v[1], a.alpha, a.limit)), static_cast<bf16>(mx_swiglu(v[2], v[3], a.alpha, a.limit))};
+    if (four) {
+      *reinterpret_cast<bf16x2*>(to) = o;
+    } else {
+      to[0] = o[0];
+      if (n + 2 < nn) to[1] = o[1];
+    }
+  } else if constexpr (MODE == kMxPairs) {
+    float* const to = static_cast<float*>(a.out) + row * a.out_stride + n0 + n;
+    if (four) {
+      *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < nn) to[i] = v[i];
+    }
+  } else {
+    bf16* const to = static_cast<bf16*>(a.out) + row * a.out_stride + n0 + n;
+    const bf16x4 o = {static_cast<bf16>(v[0]), static_cast<bf16>(v[1]), static_cast<bf16>(v[2]), static_cast<bf16>(v[3])};
+    if (four) {
+      *reinterpret_cast<bf16x4*>(to) = o;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < nn) to[i] = o[i];
+    }
+  }
+}
+
 int mx_stream(const MxArgs& a, int mode, bool a4, hipStream_t st);
+int mx_tiles4(const MxArgs& a, hipStream_t st);
 int mx_tiles(const MxArgs& a, int mode, hipStream_t st);
 
 }  // namespace tllm

@@ -70,55 +70,14 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
 #pragma unroll
   for (int s = 0; s < S; ++s) issue(s, s);
 
-  // ---- while they are on their way: scale bytes, four to a word, rows an odd number of words apart; the bias; the pairs' numbers
+  // ---- while they are on their way: scale bytes and bias
   unsigned* const sc = reinterpret_cast<unsigned*>(smem + S * C::STAGE);
-  const int words = (blocks + 3) / 4, pitch = words | 1;
-  {
-    const unsigned char* const from = a.w_scales + wrow * blocks;
-    constexpr int THREADS = C::NW * 64, FLIGHT = 8;        // loads of a thread on their way together
-    const int step_r = THREADS / words, step_w = THREADS - step_r * words, last = blocks - 4;
-    int r = tid / words, w = tid - r * words;
-    while (r < nn) {
-      unsigned v[FLIGHT];
-      int at[FLIGHT];
-#pragma unroll
-      for (int j = 0; j < FLIGHT; ++j) {
-        at[j] = r < nn ? r * pitch + w : -1;
-        const int rr = r < nn ? r : nn - 1, off = 4 * w < last ? 4 * w : last;       // (a row's last word ends with the row)
-        if (blocks >= 4) {
-          __builtin_memcpy(&v[j], from + (rr * blocks + off), 4);
-          v[j] >>= 8 * (4 * w - off);
-        } else {
-          v[j] = 0;
-          for (int b = 0; b < blocks; ++b) v[j] |= static_cast<unsigned>(from[rr * blocks + b]) << 8 * b;
-        }
-        r += step_r;
-        w += step_w;
-        if (w >= words) {
-          w -= words;
-          ++r;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < FLIGHT; ++j)
-        if (at[j] >= 0) sc[at[j]] = v[j];
-    }
-  }
-  // four neighbours of the bias, of a row of the result, at once: where their places are whole
-  const bool four = a.n % 4 == 0 && a.out_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(a.bias) % 8 == 0;
+  const int pitch = mx_scale_words(blocks);
+  mx_fetch_scales<C::NW * 64>(sc, a.w_scales + wrow * blocks, nn, blocks, tid);
+  const bool four = mx_whole_fours(a);
   bf16x4 bias[RB];
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int n = 16 * (RB * wn + rb) + 4 * g;
-    if (!a.bias) {
-      bias[rb] = bf16x4{};
-    } else if (four) {
-      bias[rb] = *reinterpret_cast<const bf16x4*>(a.bias + wrow + (n < nn ? n : 0));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bias[rb][i] = a.bias[wrow + (n + i < nn ? n + i : nn - 1)];
-    }
-  }
+  for (int rb = 0; rb < RB; ++rb) bias[rb] = mx_bias4(a, four, wrow, 16 * (RB * wn + rb) + 4 * g, nn);
   __syncthreads();
 
   // ---- the walk over K
@@ -197,38 +156,7 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
     for (int rb = 0; rb < RB; ++rb) {
       const int n = 16 * (RB * wn + rb) + 4 * g;
       if (n >= nn) continue;
-      float v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = acc[t][rb][i] + static_cast<float>(bias[rb][i]);
-      if constexpr (MODE == kMxSwiglu) {
-        bf16* const to = static_cast<bf16*>(a.out) + row * a.out_stride + (n0 + n) / 2;
-        const bf16x2 o = {static_cast<bf16>(mx_swiglu(v[0], v[1], a.alpha, a.limit)), static_cast<bf16>(mx_swiglu(v[2], v[3], a.alpha, a.limit))};
-        if (four) {
-          *reinterpret_cast<bf16x2*>(to) = o;
-        } else {
-          to[0] = o[0];
-          if (n + 2 < nn) to[1] = o[1];
-        }
-      } else if constexpr (MODE == kMxPairs) {
-        float* const to = static_cast<float*>(a.out) + row * a.out_stride + n0 + n;
-        if (four) {
-          *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + i < nn) to[i] = v[i];
-        }
-      } else {
-        bf16* const to = static_cast<bf16*>(a.out) + row * a.out_stride + n0 + n;
-        const bf16x4 o = {static_cast<bf16>(v[0]), static_cast<bf16>(v[1]), static_cast<bf16>(v[2]), static_cast<bf16>(v[3])};
-        if (four) {
-          *reinterpret_cast<bf16x4*>(to) = o;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + i < nn) to[i] = o[i];
-        }
-      }
+      mx_store4<MODE>(a, four, row, n0, n, nn, acc[t][rb], bias[rb]);
     }
   }
 }
@@ -237,7 +165,7 @@ template <class C, int MODE>
 static int launch_tiles(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN;
   const int64_t items = a.order ? mx_items(a.rows, a.experts, C::BM) : (a.rows + C::BM - 1) / C::BM;
-  const int blocks = a.k / 32, lds = C::S * C::STAGE + C::BN * (((blocks + 3) / 4) | 1) * 4 + 16;
+  const int blocks = a.k / 32, lds = C::S * C::STAGE + C::BN * mx_scale_words(blocks) * 4 + 16;
   TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
   TLLM_REQUIRE(lds <= 160 * 1024, TLLM_E_SHAPE, "mxfp4 product: %d values in a row are too many for its tiles", a.k);
   static std::atomic<uint64_t> done{0};

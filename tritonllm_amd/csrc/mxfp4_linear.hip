@@ -16,6 +16,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
 
 static int product(const MxArgs& a, int mode, bool a4, hipStream_t st) {
   if (!a4 && a.rows >= 24ll * a.experts && a.rows >= 512 && a.k <= 4096) return mx_tiles(a, mode, st);
+  if (a4 && a.rows >= 128 && a.k <= 4096) return mx_tiles4(a, st);
   return mx_stream(a, mode, a4, st);
 }
 
