@@ -3,10 +3,11 @@
 //
 //   D[r, n] = sum_k X[r, k] W[n, k]
 //
-// K goes in slices of 128, 64 bytes (four blocks) of a row: lane (m, g) of a fragment has block g of row m, one 16-byte read. Slices
-// of both operands come into a ring of S in LDS by buffer loads straight there, a row's four blocks in an order (block g at place g ^
-// (row / 4 % 2)) that keeps the sixteen lanes that a read serves together in different banks. Scale bytes of all rows lie in LDS
-// for the whole of K. A slice's fragments are read under the MFMAs of the one before.
+// K goes in slices of 256, eight blocks and a whole cache line of a row (with half lines a CU took in 30 GB/s). A slice is two
+// MFMAs deep: in the j-th lane (m, g) of a fragment has block 2 g + j of row m, one 16-byte read, and both blocks' scale bytes
+// side by side. Slices of both operands come into a ring of S in LDS by buffer loads straight there, block b of a row at place
+// b ^ (row / 2 % 8), which keeps the sixteen lanes that a read serves together (0 - 7 with 32 - 39, ...) in different banks. Scale
+// bytes of all rows lie in LDS for the whole of K. A half slice's fragments are read under the MFMAs of the one before.
 #include "mx_common.h"
 
 namespace tllm {
@@ -15,9 +16,9 @@ template <int TB_, int RB_, int WM_, int WN_, int S_>
 struct MxTile4 {
   static constexpr int TB = TB_, RB = RB_, WM = WM_, WN = WN_, S = S_, NW = WM * WN;
   static constexpr int BM = 16 * TB * WM, BN = 16 * RB * WN;
-  static constexpr int XB = BM * 64, STAGE = (BM + BN) * 64;
-  static constexpr int XL = BM / 16 / NW, WL = BN / 16 / NW, LPW = XL + WL;       // loads of a wavefront per slice: 16 rows each
-  static_assert(XL * 16 * NW == BM && WL * 16 * NW == BN && S >= 2, "whole loads");
+  static constexpr int XB = BM * 128, STAGE = (BM + BN) * 128;
+  static constexpr int XL = BM / 8 / NW, WL = BN / 8 / NW, LPW = XL + WL;         // loads of a wavefront per slice: 8 rows each
+  static_assert(XL * 8 * NW == BM && WL * 8 * NW == BN && S >= 2, "whole loads");
 };
 
 template <class C>
@@ -32,32 +33,38 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile4_kernel(MxArgs a, int tile
   const int n0 = t / items * BN;
   const int64_t r0 = static_cast<int64_t>(t % items) * BM, left = a.rows - r0;
   const int rows = static_cast<int>(left < BM ? left : BM), nn = a.n - n0 < BN ? a.n - n0 : BN;
-  const int blocks = a.k / 32, slices = (blocks + 3) / 4;
+  const int blocks = a.k / 32, slices = (blocks + 7) / 8;
 
   const u32x4 xr = mx_buffer_words(static_cast<const unsigned char*>(a.x) + r0 * blocks * 16, rows * blocks * 16);
   const u32x4 wr = mx_buffer_words(a.w + static_cast<int64_t>(n0) * blocks * 16, nn * blocks * 16);
   unsigned xo[XL], wo[WL];
-  const unsigned place_of = ((lane & 3) ^ (lane >> 4 & 1)) * 16;
+  // eight rows to a load, lane l at row l / 8 of them and at place l % 8, where the block (l % 8) ^ (row / 2 % 8) belongs
+  auto block_at = [&](int i) { return static_cast<unsigned>((lane & 7) ^ ((4 * i + (lane >> 4)) & 7)) * 16; };
 #pragma unroll
-  for (int j = 0; j < XL; ++j) xo[j] = min((wave * XL + j) * 16 + (lane >> 2), rows - 1) * (blocks * 16) + place_of;
+  for (int j = 0; j < XL; ++j) xo[j] = min((wave * XL + j) * 8 + (lane >> 3), rows - 1) * (blocks * 16) + block_at(wave * XL + j);
 #pragma unroll
-  for (int j = 0; j < WL; ++j) wo[j] = min((wave * WL + j) * 16 + (lane >> 2), nn - 1) * (blocks * 16) + place_of;
+  for (int j = 0; j < WL; ++j) wo[j] = min((wave * WL + j) * 8 + (lane >> 3), nn - 1) * (blocks * 16) + block_at(wave * WL + j);
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>(smem));
+  // Of the last slice blocks may not be there: their lanes ask behind the buffer's end and put zeros into LDS. Behind the last slice
+  // it comes again, so that the loads in flight can be counted.
   auto issue = [&](int slice, int place) {
-    const int s = slice < slices ? slice : slices - 1;     // (behind the last slice it again, so that the loads in flight can be counted)
+    const int s = slice < slices ? slice : slices - 1;
     const unsigned base = lds0 + place * C::STAGE;
 #pragma unroll
-    for (int j = 0; j < XL; ++j) mx_load_lds(xr, xo[j], s * 64, base + (wave * XL + j) * 1024);
+    for (int j = 0; j < XL; ++j)
+      mx_load_lds(xr, 8 * s + static_cast<int>(block_at(wave * XL + j) / 16) < blocks ? xo[j] : MX_NONE, s * 128, base + (wave * XL + j) * 1024);
 #pragma unroll
-    for (int j = 0; j < WL; ++j) mx_load_lds(wr, wo[j], s * 64, base + C::XB + (wave * WL + j) * 1024);
+    for (int j = 0; j < WL; ++j)
+      mx_load_lds(wr, 8 * s + static_cast<int>(block_at(wave * WL + j) / 16) < blocks ? wo[j] : MX_NONE, s * 128, base + C::XB + (wave * WL + j) * 1024);
   };
 #pragma unroll
   for (int s = 0; s < S; ++s) issue(s, s);
 
-  unsigned* const sc = reinterpret_cast<unsigned*>(smem + S * C::STAGE);
-  const int pitch = mx_scale_words(blocks);
-  mx_fetch_scales<C::NW * 64>(sc, a.x_scales + r0 * blocks, rows, blocks, tid);
-  mx_fetch_scales<C::NW * 64>(sc + BM * pitch, a.w_scales + static_cast<int64_t>(n0) * blocks, nn, blocks, tid);
+  unsigned char* const sc = smem + S * C::STAGE;
+  const int pitch = mx_scale_pitch(blocks), x_part = mx_scale_lds(BM, blocks);
+  const unsigned char *const x_scales = a.x_scales + r0 * blocks, *const w_scales = a.w_scales + static_cast<int64_t>(n0) * blocks;
+  mx_fetch_scales<C::NW * 64>(sc, x_scales, rows, blocks, tid);
+  mx_fetch_scales<C::NW * 64>(sc + x_part, w_scales, nn, blocks, tid);
   const bool four = mx_whole_fours(a);
   bf16x4 bias[RB];
 #pragma unroll
@@ -69,66 +76,65 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile4_kernel(MxArgs a, int tile
   for (int i = 0; i < TB; ++i)
 #pragma unroll
     for (int r = 0; r < RB; ++r) acc[i][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const unsigned char* const scb = reinterpret_cast<const unsigned char*>(sc);
   u32x4 x[2][TB], w[2][RB];
-  unsigned xs[2][TB], ws[2][RB];
-  const int xat = 16 * TB * wm + m16, wat = 16 * RB * wn + m16, at = (g ^ (m16 >> 2 & 1)) << 4;
-  auto read = [&](auto buf, int slice, int place) {
-    constexpr int b = decltype(buf)::value;
-    const unsigned char* const st = smem + place * C::STAGE;
+  unsigned xs[2][TB], ws[2][RB];                           // two scale bytes each, of this slice and the next
+  const int xat = 16 * TB * wm + m16, wat = 16 * RB * wn + m16, flip = m16 >> 1;
+  auto read = [&](auto half, int place) {
+    constexpr int j = decltype(half)::value;
+    const unsigned char* const st = smem + place * C::STAGE + (((2 * g + j) ^ flip) << 4);
 #pragma unroll
-    for (int i = 0; i < TB; ++i) {
-      x[b][i] = *reinterpret_cast<const u32x4*>(st + (xat + 16 * i) * 64 + at);
-      xs[b][i] = scb[(xat + 16 * i) * pitch * 4 + 4 * slice + g];
-    }
+    for (int i = 0; i < TB; ++i) x[j][i] = *reinterpret_cast<const u32x4*>(st + (xat + 16 * i) * 128);
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      w[b][i] = *reinterpret_cast<const u32x4*>(st + C::XB + (wat + 16 * i) * 64 + at);
-      ws[b][i] = scb[(BM + wat + 16 * i) * pitch * 4 + 4 * slice + g];
-    }
+    for (int i = 0; i < RB; ++i) w[j][i] = *reinterpret_cast<const u32x4*>(st + C::XB + (wat + 16 * i) * 128);
   };
-  auto multiply = [&](auto buf, int slice) {
+  const unsigned char *const my_xs = sc + mx_scale_shift(x_scales) + xat * pitch + 2 * g,
+                      *const my_ws = sc + x_part + mx_scale_shift(w_scales) + wat * pitch + 2 * g;
+  const int rest = blocks - 8 * (slices - 1) - 2 * g;      // of this lane's two blocks of the last slice: how many are there
+  const unsigned last_mask = rest >= 2 ? 0xffffu : rest == 1 ? 0xffu : 0u;
+  auto read_scales = [&](auto buf, int slice) {
     constexpr int b = decltype(buf)::value;
-    if (slice + 1 == slices && 4 * slice + g >= blocks) {  // blocks of the last slice that are not there
+    const unsigned mask = slice + 1 < slices ? 0xffffu : last_mask;      // (zeros times 2^-127, not times another row's scale)
+    auto two = [&](const unsigned char* p) { return (p[0] | static_cast<unsigned>(p[1]) << 8) & mask; };
 #pragma unroll
-      for (int i = 0; i < TB; ++i) {
-        x[b][i] = u32x4{0, 0, 0, 0};
-        xs[b][i] = 127;
-      }
+    for (int i = 0; i < TB; ++i) xs[b][i] = two(my_xs + 16 * i * pitch + 8 * slice);
 #pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        w[b][i] = u32x4{0, 0, 0, 0};
-        ws[b][i] = 127;
-      }
-    }
+    for (int i = 0; i < RB; ++i) ws[b][i] = two(my_ws + 16 * i * pitch + 8 * slice);
+  };
+  auto multiply = [&](auto half, auto buf) {
+    constexpr int j = decltype(half)::value, b = decltype(buf)::value;
 #pragma unroll
     for (int i = 0; i < TB; ++i)
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
         i32x8 wv = {}, xv = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          wv[j] = w[b][r][j];
-          xv[j] = x[b][i][j];
+        for (int e = 0; e < 4; ++e) {
+          wv[e] = w[j][r][e];
+          xv[e] = x[j][i][e];
         }
-        acc[i][r] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i][r], 4, 4, 0, ws[b][r], 0, xs[b][i]);
+        acc[i][r] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i][r], 4, 4, j, ws[b][r], j, xs[b][i]);
       }
   };
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * LPW) : "memory");
-  read(I0{}, 0, 0);
+  read(I0{}, 0);
+  read_scales(I0{}, 0);
   int place = 0;
   auto step = [&](auto buf, auto other, int s) {
+    read(I1{}, place);
+    multiply(I0{}, buf);
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * LPW) : "memory");
     issue(s + S, place);
     place = place + 1 == S ? 0 : place + 1;
-    read(other, s + 1, place);                             // (behind the last slice: the last one again, not used)
-    multiply(buf, s);
+    read(I0{}, place);                                     // (behind the last slice: the last one again, not used)
+    read_scales(other, s + 1);
+    multiply(I1{}, buf);
   };
   for (int s = 0; s < slices; s += 2) {
     step(I0{}, I1{}, s);
-    if (s + 1 < slices) step(I1{}, I0{}, s + 1);
+    if (s + 1 == slices) break;
+    step(I1{}, I0{}, s + 1);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
@@ -147,7 +153,7 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile4_kernel(MxArgs a, int tile
 template <class C>
 static int launch_tiles4(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN, items = (a.rows + C::BM - 1) / C::BM;
-  const int lds = C::S * C::STAGE + (C::BM + C::BN) * mx_scale_words(a.k / 32) * 4 + 16;
+  const int lds = C::S * C::STAGE + mx_scale_lds(C::BM, a.k / 32) + mx_scale_lds(C::BN, a.k / 32);
   TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
   TLLM_REQUIRE(lds <= 160 * 1024, TLLM_E_SHAPE, "mxfp4 product: %d values in a row are too many for its tiles", a.k);
   static std::atomic<uint64_t> done{0};
@@ -158,7 +164,7 @@ static int launch_tiles4(const MxArgs& a, hipStream_t st) {
 }
 
 #ifndef MX_SHAPE4
-#define MX_SHAPE4 4, 4, 2, 4, 4
+#define MX_SHAPE4 4, 4, 2, 4, 2
 #endif
 
 int mx_tiles4(const MxArgs& a, hipStream_t st) { return launch_tiles4<MxTile4<MX_SHAPE4>>(a, st); }

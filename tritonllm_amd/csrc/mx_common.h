@@ -175,38 +175,27 @@ __device__ __forceinline__ void mx_load_lds(u32x4 buffer, unsigned at, unsigned 
 __device__ __forceinline__ unsigned mx_load1(__amdgpu_buffer_rsrc_t b, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b8(b, at, 0, 0); }
 
 // ---- what the tiles share
-// The scale bytes of a tile's rows in LDS, for the whole of K: four to a word, rows an odd number of words apart, so that sixteen
-// rows' words lie in different banks.
-static __host__ __device__ __forceinline__ int mx_scale_words(int blocks) { return ((blocks + 3) / 4) | 1; }
+// The scale bytes of a tile's rows in LDS, for the whole of K: as they lie in memory, one row behind the other, from the sixteen bytes
+// on in which they begin; rows of whole sixteens have sixteen more between them, or sixteen rows' bytes would lie in few banks.
+// Byte b of row r is at mx_scale_shift + r mx_scale_pitch + b.
+static __host__ __device__ __forceinline__ int mx_scale_pitch(int blocks) { return blocks % 16 ? blocks : blocks + 16; }
+static __host__ __device__ __forceinline__ int mx_scale_lds(int rows, int blocks) { return (rows * mx_scale_pitch(blocks) + 47) / 16 * 16; }
+__device__ __forceinline__ int mx_scale_shift(const unsigned char* from) { return static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15); }
 template <int THREADS>
-__device__ __forceinline__ void mx_fetch_scales(unsigned* to, const unsigned char* from, int rows, int blocks, int tid) {
-  constexpr int FLIGHT = 8;                                // loads of a thread on their way together
-  const int words = (blocks + 3) / 4, pitch = words | 1, step_r = THREADS / words, step_w = THREADS - step_r * words, last = blocks - 4;
-  int r = tid / words, w = tid - r * words;
-  while (r < rows) {
-    unsigned v[FLIGHT];
-    int at[FLIGHT];
+__device__ __forceinline__ void mx_fetch_scales(unsigned char* to, const unsigned char* from, int rows, int blocks, int tid) {
+  constexpr int FLIGHT = 4;                                // loads of a thread on their way together
+  const int shift = mx_scale_shift(from), bytes = shift + rows * blocks, units = (bytes + 15) / 16;
+  // (to whole words: a word that the end cuts would come as zeros; its other bytes share the last one's sixteen)
+  const __amdgpu_buffer_rsrc_t buf = mx_buffer(from - shift, (bytes + 3) & ~3);
+  for (int i0 = tid; i0 < units; i0 += FLIGHT * THREADS) {
+    u32x4 v[FLIGHT];
+#pragma unroll
+    for (int j = 0; j < FLIGHT; ++j) v[j] = mx_load16(buf, i0 + j * THREADS < units ? 16 * (i0 + j * THREADS) : MX_NONE);
 #pragma unroll
     for (int j = 0; j < FLIGHT; ++j) {
-      at[j] = r < rows ? r * pitch + w : -1;
-      const int rr = r < rows ? r : rows - 1, off = 4 * w < last ? 4 * w : last;     // (a row's last word ends with the row)
-      if (blocks >= 4) {
-        __builtin_memcpy(&v[j], from + (rr * blocks + off), 4);
-        v[j] >>= 8 * (4 * w - off);
-      } else {
-        v[j] = 0;
-        for (int b = 0; b < blocks; ++b) v[j] |= static_cast<unsigned>(from[rr * blocks + b]) << 8 * b;
-      }
-      r += step_r;
-      w += step_w;
-      if (w >= words) {
-        w -= words;
-        ++r;
-      }
+      const int i = i0 + j * THREADS;
+      if (i < units) *reinterpret_cast<u32x4*>(to + 16 * (blocks % 16 ? i : i + i / (blocks / 16))) = v[j];
     }
-#pragma unroll
-    for (int j = 0; j < FLIGHT; ++j)
-      if (at[j] >= 0) to[at[j]] = v[j];
   }
 }
 

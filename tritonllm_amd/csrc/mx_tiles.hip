@@ -59,21 +59,27 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
     wo[j] = (r < nn ? r : nn - 1) * (blocks * 16) + (lane & 1) * 16;
   }
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>(smem));
+  // The last slice's second block may not be there: its lanes ask behind the buffer's end and put zeros into LDS. Behind the last
+  // slice it comes again, so that the loads in flight can be counted.
+  const bool x_second = ((lane & 7) ^ (lane >> 4 & 3)) >= 4;
   auto issue = [&](int slice, int place) {
-    const int s = slice < slices ? slice : slices - 1;     // (behind the last slice it again, so that the loads in flight can be counted)
+    const int s = slice < slices ? slice : slices - 1;
     const unsigned base = lds0 + place * C::STAGE;
+    const bool cut = (blocks & 1) && s + 1 == slices;
 #pragma unroll
-    for (int j = 0; j < XL; ++j) mx_load_lds(xr, xo[j], s * 128, base + (wave * XL + j) * 1024);
+    for (int j = 0; j < XL; ++j)
+      mx_load_lds(xr, cut && x_second ? MX_NONE : xo[j], s * 128, base + (wave * XL + j) * 1024);
 #pragma unroll
-    for (int j = 0; j < WL; ++j) mx_load_lds(wr, wo[j], s * 32, base + C::XB + (wave * WL + j) * 1024);
+    for (int j = 0; j < WL; ++j) mx_load_lds(wr, cut && (lane & 1) ? MX_NONE : wo[j], s * 32, base + C::XB + (wave * WL + j) * 1024);
   };
 #pragma unroll
   for (int s = 0; s < S; ++s) issue(s, s);
 
   // ---- while they are on their way: scale bytes and bias
-  unsigned* const sc = reinterpret_cast<unsigned*>(smem + S * C::STAGE);
-  const int pitch = mx_scale_words(blocks);
-  mx_fetch_scales<C::NW * 64>(sc, a.w_scales + wrow * blocks, nn, blocks, tid);
+  unsigned char* const sc = smem + S * C::STAGE;
+  const unsigned char* const scales = a.w_scales + wrow * blocks;
+  const int pitch = mx_scale_pitch(blocks);
+  mx_fetch_scales<C::NW * 64>(sc, scales, nn, blocks, tid);
   const bool four = mx_whole_fours(a);
   bf16x4 bias[RB];
 #pragma unroll
@@ -86,19 +92,21 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
   for (int t = 0; t < TB; ++t)
 #pragma unroll
     for (int r = 0; r < RB; ++r) acc[t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const unsigned char* const scb = reinterpret_cast<const unsigned char*>(sc);
   typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
   u32x2 q[RB];                                             // a slice's codes, and its scales as fp32
   float qs[RB];
   bf16x8 w[2][RB];
   u32x4 x[2][TB];
   const int xat = 16 * TB * wm + m16, wat = 16 * RB * wn + m16, flip = m16 >> 1 & 3;
+  const unsigned char* const my_scales = sc + mx_scale_shift(scales) + wat * pitch + (g >> 1);
+  const bool absent = (blocks & 1) && g >= 2;              // the last slice's second block is not there: zeros times 2^-127
   auto read_w = [&](int slice, int place) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int row = wat + 16 * rb;
-      q[rb] = *reinterpret_cast<const u32x2*>(smem + place * C::STAGE + C::XB + row * 32 + g * 8);
-      qs[rb] = __builtin_bit_cast(float, static_cast<unsigned>(scb[row * pitch * 4 + 2 * slice + (g >> 1)]) << 23);
+      q[rb] = *reinterpret_cast<const u32x2*>(smem + place * C::STAGE + C::XB + (wat + 16 * rb) * 32 + g * 8);
+      unsigned e = my_scales[16 * rb * pitch + 2 * slice];
+      if (absent && slice + 1 >= slices) e = 0;
+      qs[rb] = __builtin_bit_cast(float, e << 23);
     }
   };
   auto read_x = [&](auto half, int place) {
@@ -107,14 +115,10 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
     for (int t = 0; t < TB; ++t)
       x[i][t] = *reinterpret_cast<const u32x4*>(smem + place * C::STAGE + (xat + 16 * t) * 128 + (((2 * g + i) ^ flip) << 4));
   };
-  // `none`: the second block of the last slice is not there
-  auto convert = [&](auto half, bool none) {
+  auto convert = [&](auto half) {
     constexpr int i = decltype(half)::value;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) w[i][rb] = mx_bf16x8(none ? 0u : q[rb][i], none ? 1.0f : qs[rb]);
-    if (none)
-#pragma unroll
-      for (int t = 0; t < TB; ++t) x[i][t] = u32x4{0, 0, 0, 0};
+    for (int rb = 0; rb < RB; ++rb) w[i][rb] = mx_bf16x8(q[rb][i], qs[rb]);
   };
   auto multiply = [&](auto half) {
     constexpr int i = decltype(half)::value;
@@ -125,17 +129,15 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
   };
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
-  const bool odd = (blocks & 1) && g >= 2;
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * LPW) : "memory");
   read_w(0, 0);
   read_x(I0{}, 0);
   int place = 0;
   for (int s = 0; s < slices; ++s) {
-    const bool none = odd && s + 1 == slices;
     read_x(I1{}, place);
-    convert(I0{}, none);
+    convert(I0{});
     multiply(I0{});
-    convert(I1{}, none);
+    convert(I1{});
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * LPW) : "memory");
     issue(s + S, place);
     place = place + 1 == S ? 0 : place + 1;
@@ -165,7 +167,7 @@ template <class C, int MODE>
 static int launch_tiles(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN;
   const int64_t items = a.order ? mx_items(a.rows, a.experts, C::BM) : (a.rows + C::BM - 1) / C::BM;
-  const int blocks = a.k / 32, lds = C::S * C::STAGE + C::BN * mx_scale_words(blocks) * 4 + 16;
+  const int blocks = a.k / 32, lds = C::S * C::STAGE + mx_scale_lds(C::BN, blocks);
   TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
   TLLM_REQUIRE(lds <= 160 * 1024, TLLM_E_SHAPE, "mxfp4 product: %d values in a row are too many for its tiles", a.k);
   static std::atomic<uint64_t> done{0};

@@ -25,7 +25,7 @@ static int weight_ok(const char* what, const void* w, const void* ws, int64_t ex
   TLLM_REQUIRE(k <= (1 << 24) && n <= (1 << 24), TLLM_E_SHAPE, "%s: a weight of %lld x %lld values is too large", what, (long long)n, (long long)k);
   TLLM_REQUIRE(experts >= 1, TLLM_E_ARG, "%s: %lld experts", what, (long long)experts);
   TLLM_REQUIRE(w && ws, TLLM_E_ARG, "%s: null pointer", what);
-  TLLM_REQUIRE(aligned16(w), TLLM_E_ALIGN, "%s: blocks must be 16-byte aligned", what);
+  TLLM_REQUIRE(aligned16(w) && aligned16(ws), TLLM_E_ALIGN, "%s: blocks and scales must be 16-byte aligned", what);
   return TLLM_OK;
 }
 
@@ -56,6 +56,7 @@ extern "C" int tllm_mxfp4_linear_bf16(const void* x, const void* x_scales, int64
   const int64_t row_bytes = x_scales ? in_dim / 2 : in_dim * 2, pitch = x_scales ? row_bytes : x_row_stride * 2;
   TLLM_TRY(rows_ok("mxfp4_linear", x, rows, pitch, row_bytes));
   TLLM_REQUIRE(out, TLLM_E_ARG, "mxfp4_linear: null pointer");
+  TLLM_REQUIRE(aligned16(x_scales), TLLM_E_ALIGN, "mxfp4_linear: x_scales must be 16-byte aligned");
   TLLM_REQUIRE(rows == 1 || out_row_stride >= out_dim, TLLM_E_ARG, "mxfp4_linear: out_row_stride %lld < %lld", (long long)out_row_stride, (long long)out_dim);
   MxArgs a{};
   a.x = x;

@@ -848,12 +848,18 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return blocks, scales
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Dense from a multiple of 16 bytes on, a copy where it is not."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _mx_weight(blocks: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None, ndim: int):
     _require(blocks.dtype == torch.uint8 and scales.dtype == torch.uint8, "MXFP4 blocks and scales are uint8")
     _require(blocks.ndim == ndim + 1 and blocks.shape[-1] == 16, "an MXFP4 block is 16 bytes")
     _require(blocks.shape[:-1] == scales.shape, f"{blocks.shape=} does not match {scales.shape=}")
     _require(bias is None or (bias.dtype == _BF16 and bias.shape == scales.shape[:-1]), "the bias is bfloat16, one for each row of the weight")
-    return blocks.contiguous(), scales.contiguous(), bias if bias is None else bias.contiguous()
+    return _aligned(blocks), _aligned(scales), bias if bias is None else bias.contiguous()
 
 
 def mxfp4_linear(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None,
@@ -868,7 +874,7 @@ def mxfp4_linear(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bi
     if x_scales is not None:
         _require(x.dtype == torch.uint8 and x_scales.dtype == torch.uint8 and x.shape == (*x_scales.shape, 16), "x: MXFP4 blocks of 16 bytes with a scale each")
         _require(x_scales.ndim >= 1 and x_scales.shape[-1] == g, f"x has {x_scales.shape[-1]} blocks in a row, the weight {g}")
-        lead, x2, x_scales = x_scales.shape[:-1], x.contiguous(), x_scales.contiguous()
+        lead, x2, x_scales = x_scales.shape[:-1], _aligned(x), _aligned(x_scales)
         rows, stride = x_scales.numel() // g if g else 0, 0
     else:
         _require(x.dtype == _BF16 and x.ndim >= 1 and x.shape[-1] == 32 * g, f"x must be bfloat16 with {32 * g} values in a row")
