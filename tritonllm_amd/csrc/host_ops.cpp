@@ -618,6 +618,203 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return wrap(o);
 }
 
+// ---- MXFP4 and the experts ----------------------------------------------------------------------------------------------------
+inline bool u8(const Tensor& t) { return t.scalar_type() == at::kByte; }
+inline bool al16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+// blocks [..., G, 16] and scales [..., G], dense and aligned; `dim` dimensions of the scales (0: any)
+bool mx_ok(PyObject* b, PyObject* s, int64_t dim) {
+  if (!gpu_tensor(b) || !gpu_tensor(s)) return false;
+  const Tensor &blocks = tensor(b), &scales = tensor(s);
+  if (!u8(blocks) || !u8(scales) || scales.dim() < 1 || (dim && scales.dim() != dim) || blocks.dim() != scales.dim() + 1 || blocks.size(-1) != 16) return false;
+  if (blocks.sizes().slice(0, scales.dim()) != scales.sizes() || !blocks.is_contiguous() || !scales.is_contiguous()) return false;
+  return scales.numel() > 0 && al16(blocks) && al16(scales);
+}
+bool mx_bias_ok(PyObject* o, at::IntArrayRef shape) {
+  if (is_none(o)) return true;
+  if (!gpu_tensor(o)) return false;
+  const Tensor& t = tensor(o);
+  return bf16(t) && t.sizes() == shape && t.is_contiguous();
+}
+// bf16 rows of k values that the kernels read as they are: dense, or a matrix with rows apart
+bool mx_rows(PyObject* o, int64_t k, int64_t* rows, int64_t* stride) {
+  if (!gpu_tensor(o)) return false;
+  const Tensor& x = tensor(o);
+  if (!bf16(x) || x.dim() < 1 || x.size(-1) != k || x.numel() == 0 || !al16(x)) return false;
+  *rows = x.numel() / k;
+  *stride = k;
+  if (x.is_contiguous()) return true;
+  *stride = x.dim() == 2 ? x.stride(0) : 0;
+  return x.dim() == 2 && x.stride(1) == 1 && *stride >= k && *stride % 8 == 0;
+}
+
+// mxfp4_quantize(x)
+PyObject* mxfp4_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1 || !gpu_tensor(a[0])) return none();
+  const Tensor& x = tensor(a[0]);
+  const auto t = x.scalar_type();
+  const int type = t == at::kBFloat16 ? TLLM_BF16 : t == at::kHalf ? TLLM_F16 : t == at::kFloat ? TLLM_F32 : -1;
+  if (type < 0 || x.dim() < 1 || x.size(-1) % 32 || x.numel() == 0 || !x.is_contiguous() || !al16(x)) return none();
+  const int64_t k = x.size(-1);
+  at::DimVector shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = k / 32;
+  const Tensor scales = empty(shape, x.options().dtype(at::kByte));
+  shape.push_back(16);
+  const Tensor blocks = empty(shape, x.options().dtype(at::kByte));
+  const bool done = launch("mxfp4_quantize", [&] {
+    return tllm_mxfp4_quantize(x.const_data_ptr(), type, k, mut(blocks), mut(scales), x.numel() / k, k, stream());
+  });
+  if (!done) return none();
+  PyObject *b = wrap(blocks), *s = wrap(scales);
+  PyObject* r = PyTuple_Pack(2, b, s);
+  Py_XDECREF(b);
+  Py_XDECREF(s);
+  return r;
+}
+
+// mxfp4_dequant(blocks, scales)
+PyObject* mxfp4_dequant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 2 || !mx_ok(a[0], a[1], 0)) return none();
+  const Tensor& scales = tensor(a[1]);
+  at::DimVector shape(scales.sizes().begin(), scales.sizes().end());
+  shape.back() *= 32;
+  const Tensor out = empty(shape, scales.options().dtype(at::kBFloat16));
+  const bool done = launch("mxfp4_dequant", [&] {
+    return tllm_mxfp4_dequant_bf16(tensor(a[0]).const_data_ptr(), scales.const_data_ptr(), mut(out), scales.numel(), stream());
+  });
+  if (!done) return none();
+  return wrap(out);
+}
+
+// mxfp4_linear(x, blocks, scales, bias, x_scales)
+PyObject* mxfp4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5 || !mx_ok(a[1], a[2], 2)) return none();
+  const Tensor &w = tensor(a[1]), &ws = tensor(a[2]);
+  const int64_t out_dim = ws.size(0), k = 32 * ws.size(1);
+  if (!mx_bias_ok(a[3], {out_dim})) return none();
+  int64_t rows, stride = 0;
+  at::DimVector shape;
+  if (is_none(a[4])) {
+    if (!mx_rows(a[0], k, &rows, &stride)) return none();
+    shape.assign(tensor(a[0]).sizes().begin(), tensor(a[0]).sizes().end());
+  } else {
+    if (!mx_ok(a[0], a[4], 0) || tensor(a[4]).size(-1) != ws.size(1)) return none();
+    rows = tensor(a[4]).numel() / ws.size(1);
+    shape.assign(tensor(a[4]).sizes().begin(), tensor(a[4]).sizes().end());
+  }
+  shape.back() = out_dim;
+  const Tensor out = empty(shape, ws.options().dtype(at::kBFloat16));
+  const bool done = launch("mxfp4_linear", [&] {
+    return tllm_mxfp4_linear_bf16(ptr(a[0]), ptr(a[4]), stride, w.const_data_ptr(), ws.const_data_ptr(), ptr(a[3]), mut(out), out_dim, rows, k, out_dim, stream());
+  });
+  if (!done) return none();
+  return wrap(out);
+}
+
+// moe_route(logits, top_k, sigmoid, bias, n_groups, topk_groups, renormalize, scale)
+PyObject* moe_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t top, groups, kept;
+  double scale;
+  if (n != 8 || !gpu_tensor(a[0]) || !to_i64(a[1], &top) || !PyBool_Check(a[2]) || !to_i64(a[4], &groups) || !to_i64(a[5], &kept) || !PyBool_Check(a[6]) ||
+      !to_f64(a[7], &scale))
+    return none();
+  const Tensor& x = tensor(a[0]);
+  const bool f32 = x.scalar_type() == at::kFloat;
+  if ((!f32 && !bf16(x)) || x.dim() != 2 || !x.is_contiguous() || x.numel() == 0 || top < 1 || top > 1024 || groups < 1 || groups > INT32_MAX || kept > INT32_MAX) return none();
+  const int64_t tokens = x.size(0), experts = x.size(1);
+  if (experts > INT32_MAX) return none();
+  if (!is_none(a[3])) {
+    if (!gpu_tensor(a[3])) return none();
+    const Tensor& b = tensor(a[3]);
+    if (b.scalar_type() != at::kFloat || b.dim() != 1 || b.size(0) != experts || !b.is_contiguous()) return none();
+  }
+  const auto ints = x.options().dtype(at::kInt);
+  const Tensor chosen = empty({tokens, top}, ints), weights = empty({tokens, top}, x.options().dtype(at::kFloat));
+  const Tensor order = empty({tokens * top}, ints), offsets = empty({experts + 1}, ints);
+  const int64_t need = tllm_moe_route_workspace_bytes(tokens, static_cast<int>(experts));
+  Tensor work;
+  if (need) work = empty({need}, x.options().dtype(at::kByte));
+  const bool done = launch("moe_route", [&] {
+    return tllm_moe_route(x.const_data_ptr(), f32, experts, static_cast<const float*>(ptr(a[3])), a[2] == Py_True, static_cast<int>(groups), static_cast<int>(kept),
+                          a[6] == Py_True, static_cast<float>(scale), static_cast<int32_t*>(mut(chosen)), static_cast<float*>(mut(weights)),
+                          static_cast<int32_t*>(mut(order)), static_cast<int32_t*>(mut(offsets)), need ? mut(work) : nullptr, need, tokens,
+                          static_cast<int>(experts), static_cast<int>(top), stream());
+  });
+  if (!done) return none();
+  PyObject* t[4] = {wrap(chosen), wrap(weights), wrap(order), wrap(offsets)};
+  PyObject* r = PyTuple_Pack(4, t[0], t[1], t[2], t[3]);
+  for (PyObject* o : t) Py_XDECREF(o);
+  return r;
+}
+
+// a routing's weights [tokens, top], order and offsets
+bool routing_ok(PyObject* const* a, int64_t experts) {
+  for (int i = 0; i < 3; ++i)
+    if (!gpu_tensor(a[i]) || !tensor(a[i]).is_contiguous()) return false;
+  const Tensor &w = tensor(a[0]), &order = tensor(a[1]), &offsets = tensor(a[2]);
+  return w.scalar_type() == at::kFloat && w.dim() == 2 && w.numel() > 0 && order.scalar_type() == at::kInt && order.numel() == w.numel() &&
+         offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.size(0) == experts + 1;
+}
+
+// moe_mlp1(x, weights, order, offsets, blocks, scales, bias, alpha, limit)
+PyObject* moe_mlp1(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  double alpha, limit = 0.0;
+  if (n != 9 || !mx_ok(a[4], a[5], 3) || !to_f64(a[7], &alpha) || !(is_none(a[8]) || to_f64(a[8], &limit))) return none();
+  const Tensor& ws = tensor(a[5]);
+  const int64_t experts = ws.size(0), rows2 = ws.size(1), k = 32 * ws.size(2), tokens = routing_ok(a + 1, experts) ? tensor(a[1]).size(0) : 0;
+  int64_t rows, stride;
+  if (tokens == 0 || rows2 % 2 || experts > INT32_MAX || !mx_bias_ok(a[6], {experts, rows2}) || !mx_rows(a[0], k, &rows, &stride) || rows != tokens) return none();
+  const int64_t top = tensor(a[1]).size(1), inner = rows2 / 2;
+  const Tensor h = empty({tokens * top, inner}, tensor(a[0]).options());
+  const bool done = launch("moe_mlp1", [&] {
+    return tllm_moe_mlp1_bf16(ptr(a[0]), stride, static_cast<const int32_t*>(ptr(a[2])), static_cast<const int32_t*>(ptr(a[3])), ptr(a[4]), ptr(a[5]), ptr(a[6]),
+                              mut(h), inner, tokens, static_cast<int>(experts), static_cast<int>(top), k, inner, static_cast<float>(alpha),
+                              static_cast<float>(limit), !is_none(a[8]), stream());
+  });
+  if (!done) return none();
+  return wrap(h);
+}
+
+// moe_mlp2(h, weights, order, offsets, blocks, scales, bias, residual, out)
+PyObject* moe_mlp2(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 9 || !mx_ok(a[4], a[5], 3)) return none();
+  const Tensor& ws = tensor(a[5]);
+  const int64_t experts = ws.size(0), hidden = ws.size(1), k = 32 * ws.size(2), tokens = routing_ok(a + 1, experts) ? tensor(a[1]).size(0) : 0;
+  int64_t rows, stride;
+  if (tokens == 0 || experts > INT32_MAX || !mx_bias_ok(a[6], {experts, hidden}) || !mx_rows(a[0], k, &rows, &stride)) return none();
+  const int64_t top = tensor(a[1]).size(1);
+  const Tensor& h = tensor(a[0]);
+  if (h.dim() != 2 || rows != tokens * top) return none();
+  at::DimVector shape{tokens, hidden};
+  if (!is_none(a[7])) {
+    if (!gpu_tensor(a[7])) return none();
+    const Tensor& r = tensor(a[7]);
+    if (!bf16(r) || !r.is_contiguous() || r.dim() < 1 || r.numel() != tokens * hidden || r.size(-1) != hidden) return none();
+    shape.assign(r.sizes().begin(), r.sizes().end());
+  }
+  Tensor out;
+  if (is_none(a[8])) {
+    out = empty(shape, h.options());
+  } else {
+    if (!gpu_tensor(a[8])) return none();
+    out = tensor(a[8]);
+    if (!bf16(out) || out.sizes() != at::IntArrayRef(shape) || !out.is_contiguous()) return none();
+  }
+  const int64_t need = tllm_moe_mlp2_workspace_bytes(tokens, top, hidden);
+  Tensor work;
+  if (need) work = empty({need}, h.options().dtype(at::kByte));
+  const bool done = launch("moe_mlp2", [&] {
+    return tllm_moe_mlp2_bf16(h.const_data_ptr(), stride, static_cast<const int32_t*>(ptr(a[2])), static_cast<const int32_t*>(ptr(a[3])),
+                              static_cast<const float*>(ptr(a[1])), ptr(a[4]), ptr(a[5]), ptr(a[6]), ptr(a[7]), hidden, mut(out), hidden,
+                              need ? mut(work) : nullptr, need, tokens, static_cast<int>(experts), static_cast<int>(top), k, hidden, stream());
+  });
+  if (!done) return none();
+  if (!is_none(a[8])) {
+    Py_INCREF(a[8]);
+    return a[8];
+  }
+  return wrap(out);
+}
+
 // Whatever ATen throws (out of memory, ...) reaches Python as the RuntimeError it would be there.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -639,6 +836,7 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     TLLM_OP(rmsnorm), TLLM_OP(embedding), TLLM_OP(embedding_rmsnorm), TLLM_OP(swiglu), TLLM_OP(qkv_rope), TLLM_OP(qkv_rope_cache), TLLM_OP(linear),
     TLLM_OP(out_residual), TLLM_OP(unembedding), TLLM_OP(attention_decode), TLLM_OP(attention),
+    TLLM_OP(mxfp4_quantize), TLLM_OP(mxfp4_dequant), TLLM_OP(mxfp4_linear), TLLM_OP(moe_route), TLLM_OP(moe_mlp1), TLLM_OP(moe_mlp2),
     {"pool_get", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<pool_buffer>)), METH_FASTCALL, nullptr},
     {"pool_clear", py_pool_clear, METH_NOARGS, nullptr},
     {"pool_stats", py_pool_stats, METH_NOARGS, nullptr},

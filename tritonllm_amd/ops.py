@@ -800,6 +800,9 @@ def mxfp4_dequant(blocks: torch.Tensor, scales: torch.Tensor, out: torch.Tensor 
     ``[..., G]`` holds the shared power-of-two exponent, biased by 127. Returns ``[..., G * 32]`` bf16; ``out``, if
     given, must be a contiguous bf16 tensor of that many elements (it is filled in place, so a caller can expand
     straight into a slice of a preallocated parameter)."""
+    done = host().mxfp4_dequant(blocks, scales) if out is None else None
+    if done is not None:
+        return done
     _on_gpu(blocks, scales, out)
     _require(blocks.dtype == torch.uint8 and scales.dtype == torch.uint8, "MXFP4 blocks and scales are uint8")
     _require(blocks.shape[:-1] == scales.shape, f"{blocks.shape=} does not match {scales.shape=}")
@@ -835,6 +838,9 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
     The 32 values of a block share the power of two ``max(floor(log2 max|x|) - 2, -127)`` and go to the nearest e2m1 value,
     ties to the even code, at most 6. A block that holds a NaN or an infinity gets the scale byte 255, which stands for NaN."""
+    done = host().mxfp4_quantize(x)
+    if done is not None:
+        return done
     _on_gpu(x)
     _require(x.dtype in _MX_TYPES, "mxfp4_quantize: x must be bfloat16, float16 or float32")
     _require(x.ndim >= 1 and x.shape[-1] % 32 == 0, "mxfp4_quantize: the last dimension must be whole blocks of 32 values")
@@ -868,6 +874,9 @@ def mxfp4_linear(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bi
 
     ``x`` is ``[..., K]`` bf16 or, with ``x_scales [..., K / 32]``, MXFP4 blocks ``[..., K / 32, 16]`` as ``mxfp4_quantize`` makes
     them. Products are exact, sums fp32, rounded once."""
+    done = host().mxfp4_linear(x, blocks, scales, bias, x_scales)
+    if done is not None:
+        return done
     _on_gpu(x, blocks, scales, bias, x_scales)
     blocks, scales, bias = _mx_weight(blocks, scales, bias, 2)
     n, g = scales.shape
@@ -907,6 +916,10 @@ def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias:
     The ``top_k`` best are taken, the lowest index where equal, with the weights ``s`` there, divided by their sum under
     ``renormalize``, times ``scale``. The defaults are gpt-oss's router (softmax over the chosen logits). A NaN counts as -inf; an
     expert of -inf has a weight of 0."""
+    if score == "softmax" or score == "sigmoid":
+        done = host().moe_route(logits, top_k, score == "sigmoid", bias, n_groups, topk_groups, renormalize, scale)
+        if done is not None:
+            return MoeRouting(*done)
     _on_gpu(logits, bias)
     _require(logits.dtype in (_BF16, torch.float32) and logits.ndim >= 1, "moe_route: logits must be bfloat16 or float32")
     _require(score in ("softmax", "sigmoid"), f"moe_route: score {score!r}")
@@ -943,6 +956,9 @@ def moe_mlp1(x: torch.Tensor, routing: MoeRouting, blocks: torch.Tensor, scales:
     """The experts' first product and its clamped SwiGLU (model.py:751-757, moe.py:25-33): ``x [..., hidden]`` bf16 and an MXFP4 weight
     ``[experts, 2 * inner, hidden]`` (gate and linear rows in turn) give ``[tokens * top, inner]`` bf16, a row for each pair in the
     order of ``routing.order``."""
+    done = host().moe_mlp1(x, routing[1], routing[2], routing[3], blocks, scales, bias, alpha, limit)
+    if done is not None:
+        return done
     _on_gpu(x, *routing, blocks, scales, bias)
     blocks, scales, bias = _mx_weight(blocks, scales, bias, 3)
     experts, n, g = scales.shape
@@ -965,6 +981,9 @@ def moe_mlp2(h: torch.Tensor, routing: MoeRouting, blocks: torch.Tensor, scales:
     """The experts' second product, weighted and summed over each token's experts, plus the residual (model.py:751-757):
     ``h [tokens * top, inner]`` as ``moe_mlp1`` gives it and an MXFP4 weight ``[experts, hidden, inner]`` give ``[tokens, hidden]`` bf16
     (in ``residual``'s shape if there is one). ``out`` may be ``residual``."""
+    done = host().moe_mlp2(h, routing[1], routing[2], routing[3], blocks, scales, bias, residual, out)
+    if done is not None:
+        return done
     _on_gpu(h, *routing, blocks, scales, bias, residual, out)
     blocks, scales, bias = _mx_weight(blocks, scales, bias, 3)
     experts, n, g = scales.shape
