@@ -52,12 +52,19 @@ __device__ __forceinline__ MxItem mx_find_item(const int* offsets, int experts, 
     int lo = offsets[e < experts ? e : experts], hi = offsets[e < experts ? e + 1 : experts];
     lo = min(max(lo, 0), rows);
     hi = min(max(hi, lo), rows);
-    const int mine = (hi - lo + per_item - 1) / per_item;
-    int upto = mine;                                       // items of the experts up to this lane's
+    const int n = hi - lo;
+    int mine, upto;                                        // items of this lane's expert, and of all up to it
+    if (__ballot(n > per_item) == 0) {                     // at most one each: a count of bits
+      const unsigned long long some = __ballot(n > 0);
+      mine = n > 0;
+      upto = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(some >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(some), mine));
+    } else {
+      upto = mine = (n + per_item - 1) / per_item;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int v = __shfl_up(upto, d);
-      if (lane >= d) upto += v;
+      for (int d = 1; d < 64; d *= 2) {
+        const int v = __shfl_up(upto, d);
+        if (lane >= d) upto += v;
+      }
     }
     const unsigned long long has = __ballot(before + upto > item);
     if (has) {
@@ -155,9 +162,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void* p, unsig
 __device__ __forceinline__ u32x4 mx_load16(__amdgpu_buffer_rsrc_t b, unsigned at) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
 }
-__device__ __forceinline__ u32x4 mx_load16_once(__amdgpu_buffer_rsrc_t b, unsigned at) {   // (the nontemporal hint)
-  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 2));
-}
 // The same buffer as four words, for the load that goes straight to LDS: 16 bytes a lane, from `at` + `more` in the buffer to
 // `lds` + 16 x lane. The compiler does not know of it: its arrival is waited for by count.
 __device__ __forceinline__ u32x4 mx_buffer_words(const void* p, unsigned bytes) {
@@ -181,22 +185,43 @@ __device__ __forceinline__ unsigned mx_load1(__amdgpu_buffer_rsrc_t b, unsigned 
 static __host__ __device__ __forceinline__ int mx_scale_pitch(int blocks) { return blocks % 16 ? blocks : blocks + 16; }
 static __host__ __device__ __forceinline__ int mx_scale_lds(int rows, int blocks) { return (rows * mx_scale_pitch(blocks) + 47) / 16 * 16; }
 __device__ __forceinline__ int mx_scale_shift(const unsigned char* from) { return static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15); }
-template <int THREADS>
-__device__ __forceinline__ void mx_fetch_scales(unsigned char* to, const unsigned char* from, int rows, int blocks, int tid) {
-  constexpr int FLIGHT = 4;                                // loads of a thread on their way together
-  const int shift = mx_scale_shift(from), bytes = shift + rows * blocks, units = (bytes + 15) / 16;
-  // (to whole words: a word that the end cuts would come as zeros; its other bytes share the last one's sixteen)
-  const __amdgpu_buffer_rsrc_t buf = mx_buffer(from - shift, (bytes + 3) & ~3);
-  for (int i0 = tid; i0 < units; i0 += FLIGHT * THREADS) {
-    u32x4 v[FLIGHT];
-#pragma unroll
-    for (int j = 0; j < FLIGHT; ++j) v[j] = mx_load16(buf, i0 + j * THREADS < units ? 16 * (i0 + j * THREADS) : MX_NONE);
+// The fetch in two halves, loads and writes, FLIGHT loads of a thread on their way together; what is left, if anything, is `first`
+// units of sixteen bytes in.
+template <int THREADS, int FLIGHT>
+struct MxScaleFetch {
+  u32x4 v[FLIGHT];
+  __amdgpu_buffer_rsrc_t buf;
+  int units, blocks, tid;
+  __device__ __forceinline__ MxScaleFetch(const unsigned char* from, int rows, int blocks_, int tid_) : blocks(blocks_), tid(tid_) {
+    const int shift = mx_scale_shift(from), bytes = shift + rows * blocks;
+    units = (bytes + 15) / 16;
+    // (to whole words: a word that the end cuts would come as zeros; its other bytes share the last one's sixteen)
+    buf = mx_buffer(from - shift, (bytes + 3) & ~3);
+  }
+  __device__ __forceinline__ void load(int first) {
 #pragma unroll
     for (int j = 0; j < FLIGHT; ++j) {
-      const int i = i0 + j * THREADS;
+      const int i = first + tid + j * THREADS;
+      v[j] = mx_load16(buf, i < units ? 16 * i : MX_NONE);
+    }
+  }
+  __device__ __forceinline__ void write(unsigned char* to, int first) {
+#pragma unroll
+    for (int j = 0; j < FLIGHT; ++j) {
+      const int i = first + tid + j * THREADS;
       if (i < units) *reinterpret_cast<u32x4*>(to + 16 * (blocks % 16 ? i : i + i / (blocks / 16))) = v[j];
     }
   }
+  __device__ __forceinline__ void rest(unsigned char* to, int first) {
+    for (; first < units; first += THREADS * FLIGHT) {
+      load(first);
+      write(to, first);
+    }
+  }
+};
+template <int THREADS>
+__device__ __forceinline__ void mx_fetch_scales(unsigned char* to, const unsigned char* from, int rows, int blocks, int tid) {
+  MxScaleFetch<THREADS, 4>(from, rows, blocks, tid).rest(to, 0);
 }
 
 // Whether four neighbours of the bias and of a row of the result are whole accesses
