@@ -151,22 +151,56 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile4_kernel(MxArgs a, int tile
 }
 
 template <class C>
+static int64_t tile4_lds(int k) { return static_cast<int64_t>(C::S) * C::STAGE + mx_scale_lds(C::BM, k / 32) + mx_scale_lds(C::BN, k / 32); }
+
+template <class C>
 static int launch_tiles4(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN, items = (a.rows + C::BM - 1) / C::BM;
-  const int lds = C::S * C::STAGE + mx_scale_lds(C::BM, a.k / 32) + mx_scale_lds(C::BN, a.k / 32);
   TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
-  TLLM_REQUIRE(lds <= 160 * 1024, TLLM_E_SHAPE, "mxfp4 product: %d values in a row are too many for its tiles", a.k);
   static std::atomic<uint64_t> done{0};
   TLLM_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(mx_tile4_kernel<C>), 160 * 1024, done) == hipSuccess, TLLM_E_LAUNCH,
                "mxfp4 product: the LDS limit could not be raised");
-  hipLaunchKernelGGL(mx_tile4_kernel<C>, dim3((unsigned)((tiles * items + 7) / 8 * 8)), dim3(C::NW * 64), lds, st, a, (int)tiles);
+  hipLaunchKernelGGL(mx_tile4_kernel<C>, dim3((unsigned)((tiles * items + 7) / 8 * 8)), dim3(C::NW * 64), tile4_lds<C>(a.k), st, a, (int)tiles);
   return check_launch("mxfp4 product");
 }
 
-#ifndef MX_SHAPE4
-#define MX_SHAPE4 4, 4, 2, 4, 2
-#endif
+// The tiles, and what a launch of them takes: `fixed` us and, for each slice of K, `one` with up to one tile to a CU, `more` for each
+// of a CU's tiles beyond. Measured with 2880 and 4096 values a row (us; 128 x 256, 128 x 320, 128 x 128, 64 x 128, 64 x 64):
+//   2048 rows of [5120, 2880] 43.3 29.9 45.8 42.4 49.2     2048 of [4096, 2880] 25.1 28.4 31.9 33.0 40.9     1000 of [2880, 4096] 24.8 82.3 18.8 20.0 21.0
+//   512 of [4096, 2880] 21.3 25.9 16.0 13.7 12.8     300 of [5120, 2880] 21.6 25.6 15.6 13.1 11.9     64 of [5120, 2880] 18.5 21.5 13.1 11.1 8.7
+template <int TB, int RB, int WM, int WN, int S>
+static void weigh(const MxArgs& a, float fixed, float one, float more, int number, float* best, int* which) {
+  typedef MxTile4<TB, RB, WM, WN, S> C;
+  if (tile4_lds<C>(a.k) > 160 * 1024) return;
+  const int64_t tiles = (a.n + C::BN - 1) / C::BN * ((a.rows + C::BM - 1) / C::BM), each = (tiles + 255) / 256;
+  const float t = fixed + (a.k + 255) / 256 * (each == 1 ? one : more * each);
+  if (*which == 0 || t < *best) {
+    *best = t;
+    *which = number;
+  }
+}
+static int tile4_of(const MxArgs& a) {
+  float best = 0.f;
+  int which = 0;
+  weigh<4, 4, 2, 4, 2>(a, 9.4f, 1.36f, 1.36f, 1, &best, &which);
+  weigh<4, 5, 2, 4, 2>(a, 9.6f, 1.70f, 1.70f, 2, &best, &which);
+  weigh<4, 2, 2, 4, 2>(a, 7.5f, 0.71f, 1.02f, 3, &best, &which);
+  weigh<2, 2, 2, 4, 2>(a, 6.0f, 0.64f, 0.56f, 4, &best, &which);
+  weigh<2, 2, 2, 2, 3>(a, 5.0f, 0.37f, 0.35f, 5, &best, &which);
+  return which;
+}
 
-int mx_tiles4(const MxArgs& a, hipStream_t st) { return launch_tiles4<MxTile4<MX_SHAPE4>>(a, st); }
+// Up to 80 rows the weight stream is ahead: 64 rows of [5120, 2880] 7.9 us and 8.6 in tiles, 128 11.4 and 8.9.
+bool mx_tiles4_take(const MxArgs& a) { return a.rows > 80 && tile4_of(a) != 0; }
+
+int mx_tiles4(const MxArgs& a, hipStream_t st) {
+  switch (tile4_of(a)) {
+    case 1: return launch_tiles4<MxTile4<4, 4, 2, 4, 2>>(a, st);
+    case 2: return launch_tiles4<MxTile4<4, 5, 2, 4, 2>>(a, st);
+    case 3: return launch_tiles4<MxTile4<4, 2, 2, 4, 2>>(a, st);
+    case 4: return launch_tiles4<MxTile4<2, 2, 2, 4, 2>>(a, st);
+    default: return launch_tiles4<MxTile4<2, 2, 2, 2, 3>>(a, st);
+  }
+}
 
 }  // namespace tllm

@@ -275,6 +275,8 @@ __device__ __forceinline__ void mx_store4(const MxArgs& a, bool four, int64_t ro
 
 int mx_stream(const MxArgs& a, int mode, bool a4, hipStream_t st);
 int mx_tiles4(const MxArgs& a, hipStream_t st);
+bool mx_tiles_take(const MxArgs& a);
+bool mx_tiles4_take(const MxArgs& a);
 int mx_tiles(const MxArgs& a, int mode, hipStream_t st);
 
 }  // namespace tllm

@@ -249,14 +249,25 @@ static int launch(const MxArgs& a, hipStream_t st) {
   return check_launch("mxfp4 product");
 }
 
-#ifndef MX_S
-#define MX_S 2
-#define MX_R 4, 4, 3, 2
-#endif
+// The workgroup. Wide ones (64 weight rows) read the activations less often and pay where items are full: 128 tokens of 32 experts
+// mlp1 114 us with 32 rows, 107 with 64 (33 tokens 63.4 and 67.1), 65 rows of [5120, 2880] 14.8 and 12.3. Narrow ones, with their K
+// share in one piece, where the launch would have less than one for each CU otherwise: one row of [2880, 4096] 6.9 us with 32 weight
+// rows, 4.7 with 16; 64 rows of [1024, 1024] 5.8 with 64, 4.4 with 32. More steps on their way per wavefront cost wavefronts on the CU and more than
+// they bring: 33 tokens 63.8 us with 2 steps, 70 with 3, 85 with 6.
+template <int MODE>
+static int launch_bf16(const MxArgs& a, hipStream_t st) {
+  const int64_t items = a.order ? (a.rows < a.experts ? a.rows : a.experts) + a.rows / 32 : (a.rows + 15) / 16;
+  const bool full = a.rows > 12ll * a.experts;
+  if (full && (a.n + 63) / 64 * items >= 256) return launch<4, false, MODE, 4, 2, 2, 1>(a, st);
+  if ((a.n + 31) / 32 * items > 128) return launch<2, false, MODE, 4, 2, 2, 2>(a, st);
+  return launch<1, false, MODE, 8, 3, 3, 2>(a, st);
+}
+
 int mx_stream(const MxArgs& a, int mode, bool a4, hipStream_t st) {
-  if (mode == kMxSwiglu) return launch<MX_S, false, kMxSwiglu, MX_R>(a, st);
-  if (mode == kMxPairs) return launch<MX_S, false, kMxPairs, MX_R>(a, st);
-  return a4 ? launch<2, true, kMxLinear, 4, 4, 1, 1>(a, st) : launch<MX_S, false, kMxLinear, MX_R>(a, st);
+  if (mode == kMxSwiglu) return launch_bf16<kMxSwiglu>(a, st);
+  if (mode == kMxPairs) return launch_bf16<kMxPairs>(a, st);
+  if (!a4) return launch_bf16<kMxLinear>(a, st);
+  return (a.n + 31) / 32 * ((a.rows + 15) / 16) > 128 ? launch<2, true, kMxLinear, 4, 4, 1, 1>(a, st) : launch<1, true, kMxLinear, 8, 3, 1, 1>(a, st);
 }
 
 }  // namespace tllm

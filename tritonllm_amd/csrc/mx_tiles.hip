@@ -163,13 +163,15 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
   }
 }
 
+template <class C>
+static int64_t tile_lds(int k) { return static_cast<int64_t>(C::S) * C::STAGE + mx_scale_lds(C::BN, k / 32); }
+
 template <class C, int MODE>
 static int launch_tiles(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN;
   const int64_t items = a.order ? mx_items(a.rows, a.experts, C::BM) : (a.rows + C::BM - 1) / C::BM;
-  const int blocks = a.k / 32, lds = C::S * C::STAGE + mx_scale_lds(C::BN, blocks);
+  const int64_t lds = tile_lds<C>(a.k);
   TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
-  TLLM_REQUIRE(lds <= 160 * 1024, TLLM_E_SHAPE, "mxfp4 product: %d values in a row are too many for its tiles", a.k);
   static std::atomic<uint64_t> done{0};
   const void* const kernel = reinterpret_cast<const void*>(mx_tile_kernel<C, MODE>);
   TLLM_REQUIRE(raise_lds_limit(kernel, 160 * 1024, done) == hipSuccess, TLLM_E_LAUNCH, "mxfp4 product: the LDS limit could not be raised");
@@ -180,12 +182,26 @@ static int launch_tiles(const MxArgs& a, hipStream_t st) {
 #ifndef MX_SHAPE
 #define MX_SHAPE 4, 2, 1, 8, 3
 #endif
-typedef MxTileShape<MX_SHAPE> Big;
+typedef MxTileShape<MX_SHAPE> Large;              // 64 x 256, two workgroups to a CU
+typedef MxTileShape<2, 2, 1, 4, 3> Small;         // 32 x 128
+
+// Small tiles where large ones would leave CUs without any: 300 rows of [5120, 2880] 30.2 us in large, 22.9 in small ones.
+template <int MODE>
+static int tiles_of(const MxArgs& a, hipStream_t st) {
+  const int64_t large = (a.n + Large::BN - 1) / Large::BN * ((a.rows + Large::BM - 1) / Large::BM + (a.order ? a.experts / 2 : 0));
+  return large < 256 || tile_lds<Large>(a.k) > 160 * 1024 ? launch_tiles<Small, MODE>(a, st) : launch_tiles<Large, MODE>(a, st);
+}
+
+// Whether a product of these sizes is the tiles'. Below, the weight stream is ahead: 130 rows of [5120, 2880] 17.1 us, 18.7 in tiles
+// (300 29.8 and 22.9); experts of 32 and of 16 rows each on average mlp1 122 in tiles and 107 as a stream, 111.
+bool mx_tiles_take(const MxArgs& a) {
+  return a.rows > (a.order ? 24ll : 200ll) * a.experts && tile_lds<Small>(a.k) <= 160 * 1024;
+}
 
 int mx_tiles(const MxArgs& a, int mode, hipStream_t st) {
-  if (mode == kMxSwiglu) return launch_tiles<Big, kMxSwiglu>(a, st);
-  if (mode == kMxPairs) return launch_tiles<Big, kMxPairs>(a, st);
-  return launch_tiles<Big, kMxLinear>(a, st);
+  if (mode == kMxSwiglu) return tiles_of<kMxSwiglu>(a, st);
+  if (mode == kMxPairs) return tiles_of<kMxPairs>(a, st);
+  return tiles_of<kMxLinear>(a, st);
 }
 
 }  // namespace tllm

@@ -3,21 +3,47 @@
 
 namespace tllm {
 
-// out[t, n] = residual[t, n] + sum_j weights[t, j] pairs[t top + j, n], in the order of j, in fp32, rounded once.
+// out[t, n] = residual[t, n] + sum_j weights[t, j] pairs[t top + j, n], in the order of j, in fp32, rounded once. A thread takes V
+// neighbours of a token, four where rows are whole fours; up to four experts' loads leave together. 2000 tokens of 2880 and four
+// experts, 115 MB: 35 us an element at a time.
+template <int V>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restrict__ pairs, const float* __restrict__ weights, const bf16* residual,
                                                           int64_t res_stride, bf16* out, int64_t out_stride, int n, int top, int per_row) {
+  typedef __attribute__((__vector_size__(V * sizeof(float)))) float fv;
+  typedef __attribute__((__vector_size__(V * sizeof(bf16)))) bf16 bv;
   const int64_t t = blockIdx.x / per_row;
-  const int c = (blockIdx.x % per_row) * 256 + threadIdx.x;
+  const int c = ((blockIdx.x % per_row) * 256 + threadIdx.x) * V;
   if (c >= n) return;
-  float v = residual ? static_cast<float>(residual[t * res_stride + c]) : 0.f;
-  for (int j = 0; j < top; ++j) v = fmaf(weights[t * top + j], pairs[(t * top + j) * n + c], v);
-  out[t * out_stride + c] = static_cast<bf16>(v);
+  float v[V] = {};
+  if (residual) {
+    const bv r = *reinterpret_cast<const bv*>(residual + t * res_stride + c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = static_cast<float>(r[i]);
+  }
+  for (int j0 = 0; j0 < top; j0 += 4) {
+    fv p[4];
+    float w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = t * top + (j0 + j < top ? j0 + j : top - 1);
+      p[j] = *reinterpret_cast<const fv*>(pairs + at * n + c);
+      w[j] = weights[at];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j0 + j < top)
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = fmaf(w[j], p[j][i], v[i]);
+  }
+  bv o;
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = static_cast<bf16>(v[i]);
+  *reinterpret_cast<bv*>(out + t * out_stride + c) = o;
 }
 
 static int product(const MxArgs& a, int mode, bool a4, hipStream_t st) {
-  if (!a4 && a.rows >= 24ll * a.experts && a.rows >= 512 && a.k <= 4096) return mx_tiles(a, mode, st);
-  if (a4 && a.rows >= 128 && a.k <= 4096) return mx_tiles4(a, st);
-  return mx_stream(a, mode, a4, st);
+  if (a4) return mx_tiles4_take(a) ? mx_tiles4(a, st) : mx_stream(a, mode, true, st);
+  return mx_tiles_take(a) ? mx_tiles(a, mode, st) : mx_stream(a, mode, false, st);
 }
 
 static int weight_ok(const char* what, const void* w, const void* ws, int64_t experts, int64_t k, int64_t n) {
@@ -133,7 +159,12 @@ extern "C" int tllm_moe_mlp2_bf16(const void* h, int64_t h_row_stride, const int
   a.out_stride = hidden;
   hipStream_t st = static_cast<hipStream_t>(stream);
   TLLM_TRY(product(a, kMxPairs, false, st));
-  hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)(tokens * per_row)), dim3(256), 0, st, static_cast<const float*>(workspace), weights,
-                     static_cast<const bf16*>(residual), res_row_stride, static_cast<bf16*>(out), out_row_stride, (int)hidden, top, (int)per_row);
+  auto combine = [&](auto* kernel, int64_t per_row) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tokens * per_row)), dim3(256), 0, st, static_cast<const float*>(workspace), weights,
+                       static_cast<const bf16*>(residual), res_row_stride, static_cast<bf16*>(out), out_row_stride, (int)hidden, top, (int)per_row);
+  };
+  auto fours = [](const void* p, int64_t stride) { return reinterpret_cast<uintptr_t>(p) % 8 == 0 && stride % 4 == 0; };
+  if (hidden % 4 == 0 && fours(out, out_row_stride) && (!residual || fours(residual, res_row_stride))) combine(moe_combine_kernel<4>, (hidden + 1023) / 1024);
+  else combine(moe_combine_kernel<1>, per_row);
   return check_launch("moe_mlp2");
 }
