@@ -4,10 +4,10 @@
 //   D[r, n] = sum_k X[r, k] W[n, k]
 //
 // K goes in slices of 256, eight blocks and a whole cache line of a row (with half lines a CU took in 30 GB/s). A slice is two
-// MFMAs deep: in the j-th lane (m, g) of a fragment has block 2 g + j of row m, one 16-byte read, and both blocks' scale bytes
-// side by side. Slices of both operands come into a ring of S in LDS by buffer loads straight there, block b of a row at place
-// b ^ (row / 2 % 8), which keeps the sixteen lanes that a read serves together (0 - 7 with 32 - 39, ...) in different banks. Scale
-// bytes of all rows lie in LDS for the whole of K. A half slice's fragments are read under the MFMAs of the one before.
+// MFMAs deep: in the j-th lane (m, g) of a fragment has block 2 u + j of row m, u = mx_quarter(g), one 16-byte read, and both
+// blocks' scale bytes side by side. Slices of both operands come into a ring of S in LDS by buffer loads straight there, block b of a
+// row at place b ^ (row / 2 % 8). Scale bytes of all rows lie in LDS for the whole of K. A half slice's fragments are read under
+// the MFMAs of the one before.
 #include "mx_common.h"
 
 namespace tllm {
@@ -78,18 +78,18 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile4_kernel(MxArgs a, int tile
     for (int r = 0; r < RB; ++r) acc[i][r] = f32x4{0.f, 0.f, 0.f, 0.f};
   u32x4 x[2][TB], w[2][RB];
   unsigned xs[2][TB], ws[2][RB];                           // two scale bytes each, of this slice and the next
-  const int xat = 16 * TB * wm + m16, wat = 16 * RB * wn + m16, flip = m16 >> 1;
+  const int xat = 16 * TB * wm + m16, wat = 16 * RB * wn + m16, flip = m16 >> 1, u = mx_quarter(g);
   auto read = [&](auto half, int place) {
     constexpr int j = decltype(half)::value;
-    const unsigned char* const st = smem + place * C::STAGE + (((2 * g + j) ^ flip) << 4);
+    const unsigned char* const st = smem + place * C::STAGE + (((2 * u + j) ^ flip) << 4);
 #pragma unroll
     for (int i = 0; i < TB; ++i) x[j][i] = *reinterpret_cast<const u32x4*>(st + (xat + 16 * i) * 128);
 #pragma unroll
     for (int i = 0; i < RB; ++i) w[j][i] = *reinterpret_cast<const u32x4*>(st + C::XB + (wat + 16 * i) * 128);
   };
-  const unsigned char *const my_xs = sc + mx_scale_shift(x_scales) + xat * pitch + 2 * g,
-                      *const my_ws = sc + x_part + mx_scale_shift(w_scales) + wat * pitch + 2 * g;
-  const int rest = blocks - 8 * (slices - 1) - 2 * g;      // of this lane's two blocks of the last slice: how many are there
+  const unsigned char *const my_xs = sc + mx_scale_shift(x_scales) + xat * pitch + 2 * u,
+                      *const my_ws = sc + x_part + mx_scale_shift(w_scales) + wat * pitch + 2 * u;
+  const int rest = blocks - 8 * (slices - 1) - 2 * u;      // of this lane's two blocks of the last slice: how many are there
   const unsigned last_mask = rest >= 2 ? 0xffffu : rest == 1 ? 0xffu : 0u;
   auto read_scales = [&](auto buf, int slice) {
     constexpr int b = decltype(buf)::value;

@@ -179,6 +179,11 @@ __device__ __forceinline__ void mx_load_lds(u32x4 buffer, unsigned at, unsigned 
 __device__ __forceinline__ unsigned mx_load1(__amdgpu_buffer_rsrc_t b, unsigned at) { return __builtin_amdgcn_raw_buffer_load_b8(b, at, 0, 0); }
 
 // ---- what the tiles share
+// Which quarter of a slice's K the lanes of group g = lane / 16 have, in both operands. A 16-byte LDS read is served in four parts, of
+// lanes 0 - 3, 12 - 15, 20 - 27; 4 - 11, 16 - 19, 28 - 31; and the same of the upper half (measured). With 128-byte rows whose sixteens
+// are XORed with row / 2 % 8 the sixteen lanes of a part are in different banks if the quarters of groups 0 and 1, and of 2
+// and 3, are each other's complements.
+__device__ __forceinline__ int mx_quarter(int g) { return 0x2130 >> 4 * g & 3; }
 // The scale bytes of a tile's rows in LDS, for the whole of K: as they lie in memory, one row behind the other, from the sixteen bytes
 // on in which they begin; rows of whole sixteens have sixteen more between them, or sixteen rows' bytes would lie in few banks.
 // Byte b of row r is at mx_scale_shift + r mx_scale_pitch + b.

@@ -4,7 +4,8 @@
 //
 // K goes in slices of 64: a slice of X is 128 bytes a row, of W 32 (two blocks). Both come into a ring of S slices in LDS as they are
 // (buffer loads straight to LDS); the codes become bf16 in registers, in front of v_mfma_f32_16x16x32_bf16, weight rows on M. In a
-// slice lane (m, g) of a fragment has the values k = 16 g .. 16 g + 15, half a block, eight for each of two MFMAs, of both operands.
+// slice lane (m, g) of a fragment has the values k = 16 u .. 16 u + 15, u = mx_quarter(g), half a block, eight for each of two MFMAs,
+// of both operands.
 // The scale bytes of the tile's weight rows lie in LDS for the whole of K, a lane reads one for a fragment's slice.
 // A lane ends up with four neighbouring weight rows of one row of X and stores them from its registers.
 #include "mx_common.h"
@@ -51,26 +52,25 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
   for (int j = 0; j < XL; ++j) {
     const int r = (wave * XL + j) * 8 + (lane >> 3), rr = r < it.rows ? r : 0;
     const unsigned row = gather ? mx_pair(a, it.first + rr) / static_cast<unsigned>(a.top) : rr;
-    xo[j] = static_cast<unsigned>(row * a.x_pitch) + (((lane & 7) ^ (r >> 1 & 3)) << 4);
+    xo[j] = static_cast<unsigned>(row * a.x_pitch) + (((lane & 7) ^ (r >> 1 & 7)) << 4);
   }
 #pragma unroll
   for (int j = 0; j < WL; ++j) {
     const int r = (wave * WL + j) * 32 + (lane >> 1);
-    wo[j] = (r < nn ? r : nn - 1) * (blocks * 16) + (lane & 1) * 16;
+    wo[j] = (r < nn ? r : nn - 1) * (blocks * 16) + ((lane ^ lane >> 4) & 1) * 16;
   }
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>(smem));
   // The last slice's second block may not be there: its lanes ask behind the buffer's end and put zeros into LDS. Behind the last
   // slice it comes again, so that the loads in flight can be counted.
-  const bool x_second = ((lane & 7) ^ (lane >> 4 & 3)) >= 4;
   auto issue = [&](int slice, int place) {
     const int s = slice < slices ? slice : slices - 1;
     const unsigned base = lds0 + place * C::STAGE;
     const bool cut = (blocks & 1) && s + 1 == slices;
 #pragma unroll
     for (int j = 0; j < XL; ++j)
-      mx_load_lds(xr, cut && x_second ? MX_NONE : xo[j], s * 128, base + (wave * XL + j) * 1024);
+      mx_load_lds(xr, cut && (((lane & 7) ^ (4 * (wave * XL + j) + (lane >> 4))) & 4) ? MX_NONE : xo[j], s * 128, base + (wave * XL + j) * 1024);
 #pragma unroll
-    for (int j = 0; j < WL; ++j) mx_load_lds(wr, cut && (lane & 1) ? MX_NONE : wo[j], s * 32, base + C::XB + (wave * WL + j) * 1024);
+    for (int j = 0; j < WL; ++j) mx_load_lds(wr, cut && ((lane ^ lane >> 4) & 1) ? MX_NONE : wo[j], s * 32, base + C::XB + (wave * WL + j) * 1024);
   };
 #pragma unroll
   for (int s = 0; s < S; ++s) issue(s, s);
@@ -97,13 +97,13 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
   float qs[RB];
   bf16x8 w[2][RB];
   u32x4 x[2][TB];
-  const int xat = 16 * TB * wm + m16, wat = 16 * RB * wn + m16, flip = m16 >> 1 & 3;
-  const unsigned char* const my_scales = sc + mx_scale_shift(scales) + wat * pitch + (g >> 1);
-  const bool absent = (blocks & 1) && g >= 2;              // the last slice's second block is not there: zeros times 2^-127
+  const int xat = 16 * TB * wm + m16, wat = 16 * RB * wn + m16, flip = m16 >> 1, u = mx_quarter(g);
+  const unsigned char* const my_scales = sc + mx_scale_shift(scales) + wat * pitch + (u >> 1);
+  const bool absent = (blocks & 1) && u >= 2;              // the last slice's second block is not there: zeros times 2^-127
   auto read_w = [&](int slice, int place) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      q[rb] = *reinterpret_cast<const u32x2*>(smem + place * C::STAGE + C::XB + (wat + 16 * rb) * 32 + g * 8);
+      q[rb] = *reinterpret_cast<const u32x2*>(smem + place * C::STAGE + C::XB + (wat + 16 * rb) * 32 + (u ^ (m16 >> 2 & 2)) * 8);
       unsigned e = my_scales[16 * rb * pitch + 2 * slice];
       if (absent && slice + 1 >= slices) e = 0;
       qs[rb] = __builtin_bit_cast(float, e << 23);
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
     constexpr int i = decltype(half)::value;
 #pragma unroll
     for (int t = 0; t < TB; ++t)
-      x[i][t] = *reinterpret_cast<const u32x4*>(smem + place * C::STAGE + (xat + 16 * t) * 128 + (((2 * g + i) ^ flip) << 4));
+      x[i][t] = *reinterpret_cast<const u32x4*>(smem + place * C::STAGE + (xat + 16 * t) * 128 + (((2 * u + i) ^ flip) << 4));
   };
   auto convert = [&](auto half) {
     constexpr int i = decltype(half)::value;
