@@ -170,26 +170,28 @@ template <class C, int MODE>
 static int launch_tiles(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN;
   const int64_t items = a.order ? mx_items(a.rows, a.experts, C::BM) : (a.rows + C::BM - 1) / C::BM;
-  const int64_t lds = tile_lds<C>(a.k);
   TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
   static std::atomic<uint64_t> done{0};
   const void* const kernel = reinterpret_cast<const void*>(mx_tile_kernel<C, MODE>);
   TLLM_REQUIRE(raise_lds_limit(kernel, 160 * 1024, done) == hipSuccess, TLLM_E_LAUNCH, "mxfp4 product: the LDS limit could not be raised");
-  hipLaunchKernelGGL((mx_tile_kernel<C, MODE>), dim3((unsigned)((tiles * items + 7) / 8 * 8)), dim3(C::NW * 64), lds, st, a, (int)tiles);
+  hipLaunchKernelGGL((mx_tile_kernel<C, MODE>), dim3((unsigned)((tiles * items + 7) / 8 * 8)), dim3(C::NW * 64), tile_lds<C>(a.k), st, a, (int)tiles);
   return check_launch("mxfp4 product");
 }
 
-#ifndef MX_SHAPE
-#define MX_SHAPE 4, 2, 1, 8, 3
-#endif
-typedef MxTileShape<MX_SHAPE> Large;              // 64 x 256, two workgroups to a CU
+typedef MxTileShape<4, 4, 2, 2, 2> Tall;          // 128 x 128, four wavefronts of 64 x 64, three workgroups to a CU
+typedef MxTileShape<4, 2, 1, 8, 3> Wide;          // 64 x 256, eight of 64 x 32, two to a CU
 typedef MxTileShape<2, 2, 1, 4, 3> Small;         // 32 x 128
 
-// Small tiles where large ones would leave CUs without any: 300 rows of [5120, 2880] 30.2 us in large, 22.9 in small ones.
+// Tall tiles where an expert's rows fill them: 2048 tokens of 32 experts, 256 rows each, mlp1 315 us (wide ones 349), 512 tokens 168 (149);
+// 2048 rows of [5120, 2880] 62.7 (73.0). Small ones where the others would leave CUs without any: 300 rows of [5120, 2880] 30.2 in
+// wide, 22.9 in small ones.
 template <int MODE>
 static int tiles_of(const MxArgs& a, hipStream_t st) {
-  const int64_t large = (a.n + Large::BN - 1) / Large::BN * ((a.rows + Large::BM - 1) / Large::BM + (a.order ? a.experts / 2 : 0));
-  return large < 256 || tile_lds<Large>(a.k) > 160 * 1024 ? launch_tiles<Small, MODE>(a, st) : launch_tiles<Large, MODE>(a, st);
+  auto count = [&](int64_t bm, int64_t bn) { return (a.n + bn - 1) / bn * ((a.rows + bm - 1) / bm + (a.order ? a.experts / 2 : 0)); };
+  auto fits = [&](int64_t lds) { return lds <= 160 * 1024; };
+  if (a.rows > 128ll * a.experts && count(128, 128) >= 256 && fits(tile_lds<Tall>(a.k))) return launch_tiles<Tall, MODE>(a, st);
+  if (count(64, 256) >= 256 && fits(tile_lds<Wide>(a.k))) return launch_tiles<Wide, MODE>(a, st);
+  return launch_tiles<Small, MODE>(a, st);
 }
 
 // Whether a product of these sizes is the tiles'. Below, the weight stream is ahead: 130 rows of [5120, 2880] 17.1 us, 18.7 in tiles
