@@ -140,7 +140,8 @@ def linear_case(rows, n, k, acts, seed=0, bias=True):
     return x, xs, w, ws, b, want, mag
 
 
-LINEAR = [(1, 2880, 4096), (1, 16, 32), (2, 1, 64), (3, 15, 96), (5, 17, 160), (16, 33, 224), (17, 127, 288), (31, 64, 2880), (33, 130, 512),
+# (the last: long rows, and sizes that fill whole tiles of each shape)
+LINEAR = [(3, 40, 20480), (17, 70, 40960), (300, 33, 40960), (300, 64, 8192), (2100, 2000, 96), (1, 2880, 4096), (1, 16, 32), (2, 1, 64), (3, 15, 96), (5, 17, 160), (16, 33, 224), (17, 127, 288), (31, 64, 2880), (33, 130, 512),
           (65, 257, 608), (100, 100, 1024), (129, 320, 736), (200, 29, 2048), (257, 511, 352), (300, 640, 2880), (515, 1100, 160)]
 
 
@@ -199,6 +200,35 @@ def test_linear_special_values(rows, acts):
     dx, dxs, dw, dws, db = cuda(x, xs, w, ws, b)
     got = T.mxfp4_linear(dx, dw, dws, db, x_scales=dxs)
     check_product(got, want, mag, 224)
+
+
+@gpu
+@pytest.mark.parametrize("rows,n,k", [(2048, 4096, 1024), (2048, 5120, 1024), (1000, 2880, 2048), (700, 2880, 5120), (2048, 5120, 2880), (129, 200, 2880)])
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+def test_linear_of_prompts(rows, n, k, acts):
+    """The larger tiles; the reference is a float64 product on the GPU."""
+    g = torch.Generator().manual_seed(rows + n + k)
+    (w, ws), b = random_mx(g, n, k), torch.randn(n, generator=g).bfloat16()
+    x, xs = (torch.randn(rows, k, generator=g).bfloat16(), None) if acts == "bf16" else random_mx(g, rows, k, lo=123, hi=128)
+    xv, wv = (x.double() if xs is None else values(x, xs)).cuda(), values(w, ws).cuda()
+    want, mag = (xv @ wv.t()).cpu() + b.double(), (xv.abs() @ wv.abs().t()).cpu() + b.double().abs()
+    dx, dxs, dw, dws, db = cuda(x, xs, w, ws, b)
+    check_product(T.mxfp4_linear(dx, dw, dws, db, x_scales=dxs), want, mag, k)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [5, 300])
+def test_linear_of_unaligned_views(rows):
+    """Weights, scales and activations that begin anywhere are copied, or read as they are where that is possible."""
+    x, _, w, ws, b, want, mag = linear_case(rows, 61, 288, "bf16")
+    dx, dw, dws, db = cuda(x, w, ws, b)
+    big_w, big_s = torch.zeros(70, 9, 16, dtype=torch.uint8, device="cuda"), torch.zeros(70, 9, dtype=torch.uint8, device="cuda")
+    for at in (1, 5):
+        big_w[at: at + 61], big_s[at: at + 61] = dw, dws
+        check_product(T.mxfp4_linear(dx, big_w[at: at + 61], big_s[at: at + 61], db), want, mag, 288)
+    wide = torch.zeros(61, 12, 16, dtype=torch.uint8, device="cuda")
+    wide[:, 2:11] = dw
+    check_product(T.mxfp4_linear(dx.t().contiguous().t(), wide[:, 2:11], dws, db), want, mag, 288)
 
 
 @gpu
@@ -367,7 +397,7 @@ def by_expert(x, routing, w, ws, bias):
 
 
 EXPERTS = [(1, 4, 1, 32, 32), (1, 32, 4, 2880, 96), (2, 8, 2, 64, 160), (7, 8, 8, 96, 64), (8, 32, 4, 224, 352), (33, 17, 3, 160, 32), (40, 4, 2, 480, 96),
-           (64, 8, 4, 128, 288), (150, 3, 2, 352, 64), (300, 8, 3, 288, 160), (700, 2, 1, 64, 128), (257, 64, 4, 96, 96), (1000, 5, 4, 32, 32)]
+           (3000, 2, 2, 96, 352), (3000, 2, 2, 704, 64), (1000, 32, 4, 64, 544), (1000, 32, 4, 1088, 64), (64, 8, 4, 128, 288), (150, 3, 2, 352, 64), (300, 8, 3, 288, 160), (700, 2, 1, 64, 128), (257, 64, 4, 96, 96), (1000, 5, 4, 32, 32)]
 
 
 @gpu
@@ -450,6 +480,116 @@ def test_experts_nan_stays_with_its_token():
     assert h[bad.cuda()].isnan().all() and not h[~bad.cuda()].isnan().any()
     y = T.moe_mlp2(h, dr, w2.cuda(), ws2.cuda())
     assert y[7].isnan().all() and y.isnan().any(1).sum() == 1
+
+
+# ---- together ---------------------------------------------------------------------------------------------------------------
+def mlp_block(hidden=192, inner=160, experts=16, top=4, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    m = T.MLPBlock(hidden, inner, experts, top, device="cuda")
+    r = lambda *shape: (torch.randn(*shape, generator=g) / math.sqrt(shape[-1])).bfloat16()
+    with torch.no_grad():
+        m.norm.scale.copy_(1 + 0.1 * torch.randn(hidden, generator=g))
+        m.gate.weight.copy_(3 * r(experts, hidden))
+        m.gate.bias.copy_(r(experts))
+        m.mlp1_bias.copy_(0.1 * torch.randn(experts, 2 * inner, generator=g))
+        m.mlp2_bias.copy_(0.1 * torch.randn(experts, hidden, generator=g))
+    return m.quantize_experts(r(experts, 2 * inner, hidden).cuda(), r(experts, hidden, inner).cuda())
+
+
+def block_ref(m, x):
+    """The block in float64, rounded to bf16 where one kernel hands over to the next; the routing is by its own logits."""
+    bf = lambda v: v.bfloat16().double()
+    t = x.double()
+    t = bf(t * torch.rsqrt(t.square().mean(-1, keepdim=True) + m.norm.eps) * m.norm.scale.detach().cpu().double())
+    logits = bf(t @ m.gate.weight.detach().cpu().double().t() + m.gate.bias.detach().cpu().double())
+    v, e = torch.sort(logits, dim=1, descending=True, stable=True)
+    top = m.experts_per_token
+    sure = v[:, top - 1] - v[:, top] > 0.05                        # (a place of bf16 in a logit cannot change these tokens' experts)
+    w = torch.softmax(v[:, :top], 1)
+    w1, w2 = values(m.mlp1_blocks.cpu(), m.mlp1_scales.cpu()), values(m.mlp2_blocks.cpu(), m.mlp2_scales.cpu())
+    out = x.double().clone()
+    for i in range(len(x)):
+        for j in range(top):
+            k = e[i, j]
+            y = w1[k] @ t[i] + m.mlp1_bias[k].detach().cpu().double()
+            gate, lin = y[0::2].clamp(max=LIMIT), y[1::2].clamp(-LIMIT, LIMIT)
+            h = bf(gate * torch.sigmoid(ALPHA * gate) * (lin + 1))
+            out[i] += w[i, j] * (w2[k] @ h + m.mlp2_bias[k].detach().cpu().double())
+    return out, sure
+
+
+@gpu
+@pytest.mark.parametrize("tokens,experts", [(1, 16), (7, 16), (70, 32), (300, 16), (9, 10)])
+def test_mlp_block(tokens, experts):
+    m = mlp_block(experts=experts)
+    x = torch.randn(tokens, 192, generator=torch.Generator().manual_seed(tokens)).bfloat16()
+    want, sure = block_ref(m, x)
+    assert sure.double().mean() > 0.7 or tokens == 1
+    got = m(x.cuda())
+    # a place of bf16 in t, the logits and h each, and in the result: the kernels' tolerance here is twice the reference model's rounding
+    torch.testing.assert_close(got.double().cpu()[sure], want[sure], rtol=2e-2, atol=2e-2)
+    assert torch.equal(m(x.cuda().view(1, tokens, 192)).view(tokens, 192), got)
+
+
+@gpu
+def test_mlp_block_in_a_graph():
+    """Nothing of a call lives on the host: a captured block replays with other tokens, also other experts, and between eager work."""
+    m = mlp_block()
+    for tokens in (3, 100):
+        x = torch.randn(tokens, 192, device="cuda").bfloat16()
+        m(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m(x)
+        for seed in range(4):
+            x.copy_(torch.randn(tokens, 192, generator=torch.Generator().manual_seed(seed)))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, m(x))
+
+
+@gpu
+def test_ops_on_two_streams():
+    """Outputs and workspaces belong to a call: the same calls on two streams at once give what they give alone."""
+    m = mlp_block()
+    xs = [torch.randn(200, 192, generator=torch.Generator().manual_seed(i)).bfloat16().cuda() for i in range(2)]
+    want = [m(x) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in xs], [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                t = T.router_logits(xs[i], m.gate.weight.detach(), m.gate.bias.detach())          # (the norm's buffer is borrowed: one stream's at a time)
+                r = T.moe_route(t, 4)
+                h = T.moe_mlp1(xs[i], r, m.mlp1_blocks, m.mlp1_scales, m.mlp1_bias.detach())
+                got[i].append(T.moe_mlp2(h, r, m.mlp2_blocks, m.mlp2_scales, m.mlp2_bias.detach(), residual=xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        r = T.moe_route(T.router_logits(xs[i], m.gate.weight.detach(), m.gate.bias.detach()), 4)
+        h = T.moe_mlp1(xs[i], r, m.mlp1_blocks, m.mlp1_scales, m.mlp1_bias.detach())
+        alone = T.moe_mlp2(h, r, m.mlp2_blocks, m.mlp2_scales, m.mlp2_bias.detach(), residual=xs[i])
+        assert all(torch.equal(g, alone) for g in got[i]) and want[i].shape == alone.shape
+
+
+@gpu
+def test_mlp_block_from_a_checkpoint(tmp_path):
+    from safetensors.torch import save_file
+
+    m = mlp_block(seed=3)
+    n = "block.1.mlp."
+    save_file({n + "norm.scale": m.norm.scale.detach().cpu().clone(), n + "gate.weight": m.gate.weight.detach().cpu().clone(),
+               n + "gate.bias": m.gate.bias.detach().cpu().clone(), n + "mlp1_bias": m.mlp1_bias.detach().cpu().clone(),
+               n + "mlp2_bias": m.mlp2_bias.detach().cpu().clone(), n + "mlp1_weight.blocks": m.mlp1_blocks.cpu(), n + "mlp1_weight.scales": m.mlp1_scales.cpu(),
+               n + "mlp2_weight.blocks": m.mlp2_blocks.cpu(), n + "mlp2_weight.scales": m.mlp2_scales.cpu()}, str(tmp_path / "a.safetensors"))
+    ck = T.Checkpoint(str(tmp_path), torch.device("cuda"))
+    with pytest.raises(AssertionError, match="not stored in MXFP4"):
+        ck.get_mxfp4(n + "mlp1_bias")
+    loaded = T.MLPBlock(192, 160, 16, 4, device="cuda").load(ck, 1)
+    x = torch.randn(11, 192, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    assert torch.equal(loaded(x), m(x))
+    expanded = ck.get(n + "mlp1_weight")                           # the same weights, expanded: what the products multiply with
+    assert torch.equal(expanded.double().cpu(), values(m.mlp1_blocks.cpu(), m.mlp1_scales.cpu()))
 
 
 # ---- refusals ---------------------------------------------------------------------------------------------------------------

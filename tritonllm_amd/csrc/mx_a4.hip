@@ -156,7 +156,7 @@ static int64_t tile4_lds(int k) { return static_cast<int64_t>(C::S) * C::STAGE +
 template <class C>
 static int launch_tiles4(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN, items = (a.rows + C::BM - 1) / C::BM;
-  TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
+  TLLM_REQUIRE(tiles * items < (1ll << 32) / (C::NW * 64) - 8, TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
   static std::atomic<uint64_t> done{0};
   TLLM_REQUIRE(raise_lds_limit(reinterpret_cast<const void*>(mx_tile4_kernel<C>), 160 * 1024, done) == hipSuccess, TLLM_E_LAUNCH,
                "mxfp4 product: the LDS limit could not be raised");

@@ -244,8 +244,14 @@ template <int NT, bool A4, int MODE, int NW, int U4, int U8, int U16>
 static int launch(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + 16 * NT - 1) / (16 * NT);
   const int64_t items = a.order ? mx_items(a.rows, a.experts, 16) : (a.rows + 15) / 16;
-  TLLM_REQUIRE(tiles * items < (1ll << 31), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
-  hipLaunchKernelGGL((mx_stream_kernel<NT, A4, MODE, NW, U4, U8, U16>), dim3((unsigned)(tiles * items)), dim3(NW * 64), mx_scale_lds(16 * NT, a.k / 32), st, a, (int)tiles);
+  TLLM_REQUIRE(tiles * items < (1ll << 32) / (NW * 64), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
+  const int lds = mx_scale_lds(16 * NT, a.k / 32);
+  if (lds > 40 * 1024) {                                   // (long rows; with the sums more than a kernel has without asking)
+    static std::atomic<uint64_t> done{0};
+    const void* const kernel = reinterpret_cast<const void*>(mx_stream_kernel<NT, A4, MODE, NW, U4, U8, U16>);
+    TLLM_REQUIRE(raise_lds_limit(kernel, 140 * 1024, done) == hipSuccess, TLLM_E_LAUNCH, "mxfp4 product: the LDS limit could not be raised");
+  }
+  hipLaunchKernelGGL((mx_stream_kernel<NT, A4, MODE, NW, U4, U8, U16>), dim3((unsigned)(tiles * items)), dim3(NW * 64), lds, st, a, (int)tiles);
   return check_launch("mxfp4 product");
 }
 
@@ -258,8 +264,8 @@ template <int MODE>
 static int launch_bf16(const MxArgs& a, hipStream_t st) {
   const int64_t items = a.order ? (a.rows < a.experts ? a.rows : a.experts) + a.rows / 32 : (a.rows + 15) / 16;
   const bool full = a.rows > 12ll * a.experts;
-  if (full && (a.n + 63) / 64 * items >= 256) return launch<4, false, MODE, 4, 2, 2, 1>(a, st);
-  if ((a.n + 31) / 32 * items > 128) return launch<2, false, MODE, 4, 2, 2, 2>(a, st);
+  if (full && (a.n + 63) / 64 * items >= 256 && a.k <= 16384) return launch<4, false, MODE, 4, 2, 2, 1>(a, st);
+  if ((a.n + 31) / 32 * items > 128 && a.k <= 32768) return launch<2, false, MODE, 4, 2, 2, 2>(a, st);
   return launch<1, false, MODE, 8, 3, 3, 2>(a, st);
 }
 
@@ -267,7 +273,7 @@ int mx_stream(const MxArgs& a, int mode, bool a4, hipStream_t st) {
   if (mode == kMxSwiglu) return launch_bf16<kMxSwiglu>(a, st);
   if (mode == kMxPairs) return launch_bf16<kMxPairs>(a, st);
   if (!a4) return launch_bf16<kMxLinear>(a, st);
-  return (a.n + 31) / 32 * ((a.rows + 15) / 16) > 128 ? launch<2, true, kMxLinear, 4, 4, 1, 1>(a, st) : launch<1, true, kMxLinear, 8, 3, 1, 1>(a, st);
+  return (a.n + 31) / 32 * ((a.rows + 15) / 16) > 128 && a.k <= 32768 ? launch<2, true, kMxLinear, 4, 4, 1, 1>(a, st) : launch<1, true, kMxLinear, 8, 3, 1, 1>(a, st);
 }
 
 }  // namespace tllm

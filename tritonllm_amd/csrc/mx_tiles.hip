@@ -170,7 +170,7 @@ template <class C, int MODE>
 static int launch_tiles(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + C::BN - 1) / C::BN;
   const int64_t items = a.order ? mx_items(a.rows, a.experts, C::BM) : (a.rows + C::BM - 1) / C::BM;
-  TLLM_REQUIRE(tiles * items < (1ll << 30), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
+  TLLM_REQUIRE(tiles * items < (1ll << 32) / (C::NW * 64) - 8, TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
   static std::atomic<uint64_t> done{0};
   const void* const kernel = reinterpret_cast<const void*>(mx_tile_kernel<C, MODE>);
   TLLM_REQUIRE(raise_lds_limit(kernel, 160 * 1024, done) == hipSuccess, TLLM_E_LAUNCH, "mxfp4 product: the LDS limit could not be raised");

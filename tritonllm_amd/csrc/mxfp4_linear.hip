@@ -48,7 +48,8 @@ static int product(const MxArgs& a, int mode, bool a4, hipStream_t st) {
 
 static int weight_ok(const char* what, const void* w, const void* ws, int64_t experts, int64_t k, int64_t n) {
   TLLM_REQUIRE(n >= 1 && k >= 32 && k % 32 == 0, TLLM_E_SHAPE, "%s: a weight of %lld x %lld values; rows of whole blocks of 32 are supported", what, (long long)n, (long long)k);
-  TLLM_REQUIRE(k <= (1 << 24) && n <= (1 << 24), TLLM_E_SHAPE, "%s: a weight of %lld x %lld values is too large", what, (long long)n, (long long)k);
+  // (a workgroup keeps the scale bytes of at least sixteen weight rows in LDS)
+  TLLM_REQUIRE(k <= (1 << 18) && n <= (1 << 24), TLLM_E_SHAPE, "%s: a weight of %lld x %lld values is too large", what, (long long)n, (long long)k);
   TLLM_REQUIRE(experts >= 1, TLLM_E_ARG, "%s: %lld experts", what, (long long)experts);
   TLLM_REQUIRE(w && ws, TLLM_E_ARG, "%s: null pointer", what);
   TLLM_REQUIRE(aligned16(w) && aligned16(ws), TLLM_E_ALIGN, "%s: blocks and scales must be 16-byte aligned", what);

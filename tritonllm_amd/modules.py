@@ -1,6 +1,6 @@
 """Leaf modules with the constructor and forward signatures of the reference's
 ``gpt_oss/triton/model.py``: ``RMSNorm`` (:55-68), ``QKV`` (:119-167), ``OUT`` (:170-216), ``UnEmbedding`` (:70-117),
-``RotaryEmbedding`` (:218-337) and the token ``Embedding`` (``torch.nn.Embedding``
+``RotaryEmbedding`` (:218-337), ``MLPBlock`` (:751-757) and the token ``Embedding`` (``torch.nn.Embedding``
 at :906-908). A model file written against the reference can import these instead.
 
 Unlike the reference modules there is no torch fallback branch: inputs must be bf16
@@ -213,3 +213,57 @@ class Embedding(torch.nn.Module):
         if self._oob is not None and int(self._oob.item()) != 0:
             self._oob.zero_()
             raise IndexError("index out of range in Embedding")
+
+
+class MLPBlock(torch.nn.Module):
+    """The expert half of a block (model.py:751-757): norm, gate, routing, the experts' two products and the residual, with the
+    experts' weights in MXFP4 as a checkpoint holds them (a quarter of their bf16 size, and what bounds a decode step).
+
+    ``mlp1_blocks [experts, 2 * intermediate, hidden / 32, 16]`` with gate and linear rows in turn and ``mlp2_blocks [experts, hidden,
+    intermediate / 32, 16]`` are uint8 buffers with their ``_scales``; ``gate`` and both biases are bf16 parameters. Without a checkpoint,
+    ``quantize_experts`` makes them from bf16 weights."""
+
+    def __init__(self, hidden_size: int, intermediate_size: int, num_experts: int, experts_per_token: int, swiglu_limit: float = 7.0,
+                 eps: float = 1e-05, device: torch.device | None = None):
+        super().__init__()
+        _require(hidden_size % 32 == 0 and intermediate_size % 32 == 0, "MXFP4 rows are whole blocks of 32 values")
+        self.experts_per_token, self.swiglu_limit = experts_per_token, swiglu_limit
+        self.norm = RMSNorm(hidden_size, eps, device=device)
+        self.gate = torch.nn.Linear(hidden_size, num_experts, device=device, dtype=torch.bfloat16)
+        u8 = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=device)
+        self.register_buffer("mlp1_blocks", u8(num_experts, 2 * intermediate_size, hidden_size // 32, 16))
+        self.register_buffer("mlp1_scales", u8(num_experts, 2 * intermediate_size, hidden_size // 32))
+        self.register_buffer("mlp2_blocks", u8(num_experts, hidden_size, intermediate_size // 32, 16))
+        self.register_buffer("mlp2_scales", u8(num_experts, hidden_size, intermediate_size // 32))
+        self.mlp1_bias = torch.nn.Parameter(torch.zeros((num_experts, 2 * intermediate_size), device=device, dtype=torch.bfloat16))
+        self.mlp2_bias = torch.nn.Parameter(torch.zeros((num_experts, hidden_size), device=device, dtype=torch.bfloat16))
+
+    @torch.no_grad()
+    def load(self, checkpoint, block: int) -> "MLPBlock":
+        """Fill the module from block ``block`` of a ``weights.Checkpoint``; the experts' weights stay in MXFP4."""
+        name = f"block.{block}.mlp."
+        for to, key in ((self.norm.scale, "norm.scale"), (self.gate.weight, "gate.weight"), (self.gate.bias, "gate.bias"),
+                        (self.mlp1_bias, "mlp1_bias"), (self.mlp2_bias, "mlp2_bias")):
+            to.copy_(checkpoint.get(name + key))
+        for mlp in ("mlp1", "mlp2"):
+            blocks, scales = checkpoint.get_mxfp4(f"{name}{mlp}_weight")
+            getattr(self, mlp + "_blocks").copy_(blocks)
+            getattr(self, mlp + "_scales").copy_(scales)
+        return self
+
+    @torch.no_grad()
+    def quantize_experts(self, mlp1_weight: torch.Tensor, mlp2_weight: torch.Tensor) -> "MLPBlock":
+        """Take the experts' weights ``[experts, 2 * intermediate, hidden]`` and ``[experts, hidden, intermediate]`` in MXFP4."""
+        for mlp, weight in (("mlp1", mlp1_weight), ("mlp2", mlp2_weight)):
+            blocks, scales = ops.mxfp4_quantize(weight)
+            getattr(self, mlp + "_blocks").copy_(blocks)
+            getattr(self, mlp + "_scales").copy_(scales)
+        return self
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """``x [..., hidden]`` bf16 -> ``x + the experts' answer`` of the same shape."""
+        t = self.norm(x).view(-1, x.shape[-1])
+        routing = ops.moe_route(ops.router_logits(t, self.gate.weight, self.gate.bias), self.experts_per_token)
+        h = ops.moe_mlp1(t, routing, self.mlp1_blocks, self.mlp1_scales, self.mlp1_bias, limit=self.swiglu_limit)
+        return ops.moe_mlp2(h, routing, self.mlp2_blocks, self.mlp2_scales, self.mlp2_bias, residual=x)

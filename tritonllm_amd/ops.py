@@ -897,6 +897,26 @@ def mxfp4_linear(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bi
     return out
 
 
+def router_logits(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
+    """The router's gate, ``F.linear(x, weight, bias)`` of ``x [tokens, hidden]`` with ``weight [experts, hidden]`` (model.py:751-757): few
+    outputs, as heads of sixteen through the general decode projection or, beyond its rows, a GEMM tile."""
+    _on_gpu(x, weight, bias)
+    experts, hidden = weight.shape
+    _require(x.ndim == 2 and x.shape[1] == hidden and x.dtype == _BF16 and weight.dtype == _BF16, "router_logits: bfloat16 [tokens, hidden] and [experts, hidden]")
+    if experts % 16 or hidden % 64:
+        return linear_qkv_forward(x, weight, bias)
+    x, weight, bias = _prep_linear(x, weight, bias)
+    out = torch.empty((x.shape[0], experts), dtype=_BF16, device=x.device)
+    if x.shape[0] == 0:
+        return out
+    if x.shape[0] <= DECODE_MAX_ROWS:
+        _launch_qkv("decode", x, weight, bias, out, None, None, experts, 0, 0, 0, experts // 16, 0, 16, None)
+    else:
+        check(lib().tllm_linear_bf16(x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None, out.data_ptr(), experts, x.shape[0],
+                                     hidden, experts, _stream()), "router_logits")
+    return out
+
+
 class MoeRouting(NamedTuple):
     """What ``moe_route`` answers: each token's experts, best first, and their weights; and the plan of the experts' products,
     the pairs ``token * top + choice`` in the order of their experts and each expert's first place in that order."""

@@ -57,6 +57,15 @@ class Checkpoint:
             return out
         return t
 
+    def get_mxfp4(self, name: str) -> tuple[torch.Tensor, torch.Tensor]:
+        """The ``(blocks, scales)`` of an MXFP4 parameter as they are stored, on the checkpoint's device: what the products with
+        MXFP4 weights take (``ops.moe_mlp1``, ``ops.moe_mlp2``)."""
+        names = _param_names(name)
+        _require(isinstance(names, tuple), f"{name} is not stored in MXFP4")
+        blocks, scales = map(self._get_tensor, names)
+        _require(blocks.shape[:-1] == scales.shape, f"{blocks.shape=} does not match {scales.shape=}")
+        return blocks, scales
+
     def _get_tensor(self, name: str) -> torch.Tensor:
         _require(name in self.tensor_name_to_file, f"Tensor {name} not found in checkpoint.")
         with safe_open(self.tensor_name_to_file[name], framework="pt", device=self.device_str) as f:
