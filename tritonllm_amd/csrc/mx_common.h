@@ -119,6 +119,10 @@ __device__ __forceinline__ MxTile mx_find_tile(const int* offsets, int experts, 
   return {0, 0, 0, 0};
 }
 
+// Read through the scalar cache, at places that all lanes share.
+typedef const __attribute__((address_space(4))) int* ScalarInts;
+__device__ __forceinline__ ScalarInts mx_scalar(const int* p) { return (ScalarInts)(uintptr_t)p; }
+
 // A token's row: the pair at place s of the order, held to the pairs there are.
 __device__ __forceinline__ unsigned mx_pair(const MxArgs& a, int s) {
   const unsigned p = static_cast<unsigned>(a.order[s]), last = static_cast<unsigned>(a.rows - 1);

@@ -2,100 +2,114 @@
 //
 //   D[n, r] = sum_k W[n, k] X[r, k]        W MXFP4 [N, K], X bf16 or MXFP4
 //
-// What bounds it is the weight's arrival, N K 17 / 32 bytes of every expert that has rows, and with one token the chain of latencies
-// before and after. A workgroup of NW wavefronts owns 16 NT weight rows and up to 16 activation rows; the wavefronts deal the
-// K steps of 128 between them, U neighbouring ones each (sums meet in LDS, added in a fixed order), and ask for all U at once: with K
-// up to 128 NW U everything is on its way together, behind two reads (the plan's offsets, and the rows' numbers where rows are
-// gathered). The loads are buffer loads: what lies behind the tensors' end, rows that are not there and steps behind the last one read
-// as zeros without a fetch and without a branch.
+// What bounds it is the weight's arrival, N K 17 / 32 bytes of every expert that has rows (8 tokens of 32 experts, 186 MB: mlp1 35.7 us,
+// 5.2 TB/s; a plain read reaches 6.1), and with one token the chain of latencies around it (10.4 us for 35 MB). A workgroup of NW
+// wavefronts owns 16 NT weight rows and up to 16 activation rows; the wavefronts deal the K steps of 128 between them (sums meet in
+// LDS, added in a fixed order). Weights and activations go straight to LDS, U steps of a wavefront at a time in a ring that is its
+// alone, so that nothing but the wavefront's own count of arrivals is waited for. That path is what the addresses ask for: a
+// 16-byte load takes one turn of the address unit for four neighbouring lanes with 64 neighbouring bytes and one for each lane
+// otherwise, and a matrix operand has its rows in neighbouring lanes (loaded to registers that way the address units were busy
+// 73 % of the time: 33 tokens 63.8 us, 59.5 now).
 //
-// In a step lane l has block l / 16 of weight row l % 16: one 16-byte load is a whole MXFP4 block. For bf16 activations the four lanes of a
-// row exchange their words (two swaps of half and quarter wavefronts each), after which word i of all of them is of block i:
-// the i-th of the step's four v_mfma_f32_16x16x32_bf16 then takes k = 32 i + 8 (l / 16) .. + 7, and a load of activations 64
-// neighbouring bytes of a row (without the exchange its sixteens were 64 bytes apart, and every line was asked for four times: 33 tokens
-// 78 us). The codes become bf16 on the way, exactly, once per step for all rows; the scale bytes lie in LDS, fetched sixteen at a
-// time (byte by byte 10 % of the time). With MXFP4 activations the step is one v_mfma_scale_f32_16x16x128_f8f6f4, which takes
-// both blocks and scales as they are. The weight's loads carry no nontemporal hint: a step takes half a line, and with the hint
-// the other half's request fetched the line again (one token 14.4 us with, 10.1 without).
+// In a step lane (m, g) of a fragment has block mx_quarter(g) of weight row m, and the four v_mfma_f32_16x16x32_bf16 take 8 of its 32
+// values each, from both operands. The codes become bf16 on the way, exactly, once per step for all rows; a lane reads its block's scale
+// byte from LDS, where the tile's lie as in memory. With MXFP4 activations, in registers, the step is one
+// v_mfma_scale_f32_16x16x128_f8f6f4, which takes both blocks and scales as they are. All loads are buffer loads: what lies behind the
+// tensors' end, rows that are not there and blocks behind the last one come as zeros without a fetch. None carries the nontemporal
+// hint: a step takes half a line, and with the hint the other half's request fetched the line again (one token 14.4 us with, 10.1
+// without).
 #include "mx_common.h"
 
 namespace tllm {
 
-// b of the lower half (of the first and third quarter) of the wavefront for a of the upper half (of the second and fourth)
-__device__ __forceinline__ void lanes_swap32(unsigned& a, unsigned& b) {
-  const unsigned long long u = __builtin_bit_cast(unsigned long long, __builtin_amdgcn_permlane32_swap(a, b, false, false));
-  a = static_cast<unsigned>(u);
-  b = static_cast<unsigned>(u >> 32);
-}
-__device__ __forceinline__ void lanes_swap16(unsigned& a, unsigned& b) {
-  const unsigned long long u = __builtin_bit_cast(unsigned long long, __builtin_amdgcn_permlane16_swap(a, b, false, false));
-  a = static_cast<unsigned>(u);
-  b = static_cast<unsigned>(u >> 32);
-}
-
-// What a walk over K reads: the weight rows' buffer, the activation rows' buffer and each lane's row in it, and both scales.
+// A wavefront's walk over its steps: wave, wave + NW, ... of K, through a ring of its own in LDS.
 struct MxWalk {
-  __amdgpu_buffer_rsrc_t w, x, x_scales;
-  const unsigned char* scale_bytes;                        // LDS: this lane's weight row's
-  unsigned row_at, row_scales_at;                          // of this lane's activation row; MX_NONE: there is none
-  int blocks, pitch;                                       // blocks of a row; scale bytes from row to row
+  u32x4 w, x;                                              // buffers
+  __amdgpu_buffer_rsrc_t x_scales;                         // (MXFP4 rows alone)
+  const unsigned char* scales;                             // LDS: scale bytes of this lane's weight row
+  unsigned char* ring;                                     // LDS: this wavefront's
+  int blocks, nn, wave, lane;
 };
 
-// Up to RP bf16 rows, 4, 8 or 16. The columns of a product are sixteen: with up to 8 rows a load of activations takes two of the
-// step's four pieces of K for all of them, with up to 4 all four (lane (m, g): row m % RP, piece p + m / RP), and the products with
-// piece p's weights then are good in the columns of that piece and nonsense in the others, so each piece has its own sums, of which
-// only those columns are kept. `ready` is called when the first loads are on their way.
-template <int NT, int RP, int NW, int U, class F>
-__device__ __forceinline__ void mx_walk(const MxWalk& m, int wave, int lane, float* sums, int sums_pitch, F&& ready) {
-  constexpr int C = 16 / RP, X = 4 / C;                    // pieces that share a load; loads of a step
-  const int m16 = lane & 15, g = lane >> 4, steps = (m.blocks + 3) / 4, mine = m16 / RP;
-  u32x4 wq[U][NT], xq[U][X];
+template <int N, int LOADS>
+__device__ __forceinline__ void wait_steps_left(int left) {  // at most `left` (<= N) steps of LOADS loads still on their way
+  if constexpr (N == 0) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  } else {
+    if (left >= N) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N * LOADS) : "memory");
+    else wait_steps_left<N - 1, LOADS>(left);
+  }
+}
+
+// Up to RP bf16 rows, 4, 8 or 16. In a step a row is 256 bytes, four loads of four rows; weights 64 bytes, a load of sixteen rows.
+// The columns of a product are sixteen: with up to 8 rows they hold two of the step's four pieces of K for all rows (column c: row c %
+// RP, piece c / RP), with up to 4 all four. The products with a piece's weights are then good in that piece's columns and nonsense in
+// the others, so each piece has its own sums, of which only those columns are kept: fewer reads for the same products.
+// In LDS a row's sixteens are XORed so that the lanes that a read serves together (mx_quarter) are in different banks.
+// `row_at(r)`: where row r begins in x. `ready`: called when the first loads are on their way.
+template <int NT, int RP, int NW, int U, class Row, class F>
+__device__ __forceinline__ void mx_walk(const MxWalk& m, float* sums, int sums_pitch, Row&& row_at, F&& ready) {
+  constexpr int C = 16 / RP, X = 4 / C, XI = RP / 4, LOADS = NT + XI, SLOT = LOADS * 1024;
+  const int lane = m.lane, m16 = lane & 15, g = lane >> 4, u = mx_quarter(g), steps = (m.blocks + 3) / 4, mine = m16 / RP, r = m16 % RP;
+  const int n = (steps - m.wave + NW - 1) / NW;            // steps of this wavefront; may be none
+  auto fold = [](int row) { return 4 * (row & 3) + (row >> 2) * C; };
+  unsigned wo[NT], xo[XI];
+  int xb[XI];                                              // which block of the step this lane loads of x
+  const int wrow = lane >> 2, wb = (lane & 3) ^ (wrow >> 3);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) wo[t] = static_cast<unsigned>(min(16 * t + wrow, m.nn - 1) * m.blocks + wb) * 16;
+#pragma unroll
+  for (int j = 0; j < XI; ++j) {
+    const int row = 4 * j + (lane >> 4), c = (lane & 15) ^ fold(row);
+    xo[j] = row_at(row);
+    xb[j] = c >> 2;
+    if (xo[j] != MX_NONE) xo[j] += 16 * c;
+  }
+  const unsigned ring = static_cast<unsigned>(reinterpret_cast<uintptr_t>(m.ring));
+  auto issue = [&](int j, int slot) {
+    const int b = 4 * (m.wave + NW * j);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) mx_load_lds(m.w, b + wb < m.blocks ? wo[t] : MX_NONE, b * 16, ring + slot * SLOT + t * 1024);
+#pragma unroll
+    for (int i = 0; i < XI; ++i) mx_load_lds(m.x, b + xb[i] < m.blocks ? xo[i] : MX_NONE, b * 64, ring + slot * SLOT + (NT + i) * 1024);
+  };
   f32x4 acc[NT][C];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int base = 0; base < steps; base += NW * U) {
-    const int step0 = base + wave * U;
+  const int first = n < U ? n : U;
+#pragma unroll 1
+  for (int j = 0; j < first; ++j) issue(j, j);
+  ready(first * LOADS);
+  int slot = 0;
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    const int left = n - 1 - j;
+    wait_steps_left<U - 1, LOADS>(left < U - 1 ? left : U - 1);
+    const unsigned char* const at = m.ring + slot * SLOT;
+    const int b = 4 * (m.wave + NW * j) + u;
+    u32x4 wq[NT], xq[X];
+    unsigned e[NT];
 #pragma unroll
-    for (int s = 0; s < U; ++s) {
-      const int b = 4 * (step0 + s) + g;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) wq[s][t] = mx_load16(m.w, b < m.blocks ? ((16 * t + m16) * m.blocks + b) * 16 : MX_NONE);
+    for (int t = 0; t < NT; ++t) {
+      wq[t] = *reinterpret_cast<const u32x4*>(at + t * 1024 + m16 * 64 + ((u ^ (m16 >> 3)) << 4));
+      e[t] = b < m.blocks ? m.scales[16 * t * m.blocks + b] : 0u;         // (of blocks that are not there: 0, not another row's)
     }
 #pragma unroll
-    for (int s = 0; s < U; ++s)
+    for (int i = 0; i < X; ++i) xq[i] = *reinterpret_cast<const u32x4*>(at + NT * 1024 + r * 256 + (((4 * u + C * i + mine) ^ fold(r)) << 4));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // read, before the slot is filled again
+    if (j + U < n) issue(j + U, slot);
+    slot = slot + 1 == U ? 0 : slot + 1;
 #pragma unroll
-      for (int j = 0; j < X; ++j) {
-        const int b = 4 * (step0 + s) + C * j + mine;
-        xq[s][j] = mx_load16(m.x, b < m.blocks && m.row_at != MX_NONE ? m.row_at + 64 * b + 16 * g : MX_NONE);
-      }
-    if (base == 0) ready();
+    for (int t = 0; t < NT; ++t) {
+      const float scale = __builtin_bit_cast(float, e[t] << 23);
 #pragma unroll
-    for (int s = 0; s < U; ++s) {
-      const int b = 4 * (step0 + s);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        unsigned four = 0;                                  // (of blocks that are not there: 0, not another row's)
-        if (b < m.blocks) {
-          __builtin_memcpy(&four, m.scale_bytes + 16 * t * m.pitch + b, 4);
-          if (b + 4 > m.blocks) four &= (1u << 8 * (m.blocks - b)) - 1;
-        }
-        unsigned w0 = wq[s][t][0], w1 = wq[s][t][1], w2 = wq[s][t][2], w3 = wq[s][t][3];
-        lanes_swap32(w0, w2);
-        lanes_swap32(w1, w3);
-        lanes_swap16(w0, w1);
-        lanes_swap16(w2, w3);
-        const unsigned words[4] = {w0, w1, w2, w3};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned e = i == 0 ? four << 23 : four >> (8 * i) << 23;
-          const bf16x8 wv = mx_bf16x8(words[i], __builtin_bit_cast(float, e & 0x7f800000u));
-          acc[t][i % C] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8, xq[s][i / C]), acc[t][i % C], 0, 0, 0);
-        }
-      }
+      for (int i = 0; i < 4; ++i)
+        acc[t][i % C] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_bf16x8(wq[t][i], scale), __builtin_bit_cast(bf16x8, xq[i / C]), acc[t][i % C], 0, 0, 0);
     }
   }
+  __syncthreads();                                         // (the sums lie over the rings)
   // lane (m16, g) holds weight rows 4 g .. + 3 of its column
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -108,33 +122,34 @@ __device__ __forceinline__ void mx_walk(const MxWalk& m, int wave, int lane, flo
   }
 }
 
-// The same for up to 16 rows of MXFP4.
+// The same for up to 16 rows of MXFP4, which come to registers.
 template <int NT, int NW, int U, class F>
-__device__ __forceinline__ void mx_walk4(const MxWalk& m, int wave, int lane, float* sums, int sums_pitch, F&& ready) {
-  const int m16 = lane & 15, g = lane >> 4, steps = (m.blocks + 3) / 4;
+__device__ __forceinline__ void mx_walk4(const MxWalk& m, __amdgpu_buffer_rsrc_t w, __amdgpu_buffer_rsrc_t x, unsigned row_at, unsigned row_scales_at, float* sums,
+                                         int sums_pitch, F&& ready) {
+  const int m16 = m.lane & 15, g = m.lane >> 4, steps = (m.blocks + 3) / 4;
   u32x4 wq[U][NT], xq[U];
   unsigned xs[U];
   f32x4 acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int base = 0; base < steps; base += NW * U) {
-    const int step0 = base + wave * U;
+    const int step0 = base + m.wave * U;
 #pragma unroll
     for (int s = 0; s < U; ++s) {
       const int b = 4 * (step0 + s) + g;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) wq[s][t] = mx_load16(m.w, b < m.blocks ? ((16 * t + m16) * m.blocks + b) * 16 : MX_NONE);
-      const bool ok = b < m.blocks && m.row_at != MX_NONE;
-      xq[s] = mx_load16(m.x, ok ? m.row_at + 16 * b : MX_NONE);
-      xs[s] = mx_load1(m.x_scales, ok ? m.row_scales_at + b : MX_NONE);
+      for (int t = 0; t < NT; ++t) wq[s][t] = mx_load16(w, b < m.blocks ? ((16 * t + m16) * m.blocks + b) * 16 : MX_NONE);
+      const bool ok = b < m.blocks && row_at != MX_NONE;
+      xq[s] = mx_load16(x, ok ? row_at + 16 * b : MX_NONE);
+      xs[s] = mx_load1(m.x_scales, ok ? row_scales_at + b : MX_NONE);
     }
-    if (base == 0) ready();
+    if (base == 0) ready(0);
 #pragma unroll
     for (int s = 0; s < U; ++s) {
       const int b = 4 * (step0 + s) + g;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const unsigned scale = b < m.blocks ? m.scale_bytes[16 * t * m.pitch + b] : 0u;
+        const unsigned scale = b < m.blocks ? m.scales[16 * t * m.blocks + b] : 0u;
         i32x8 wv = {}, xv = {};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -145,17 +160,34 @@ __device__ __forceinline__ void mx_walk4(const MxWalk& m, int wave, int lane, fl
       }
     }
   }
+  __syncthreads();
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[m16 * sums_pitch + 16 * t + 4 * g + i] = acc[t][i];
 }
 
+// Scale bytes in LDS as they lie in memory, from the sixteen on in which the first row begins.
+static __host__ __device__ __forceinline__ int stream_scale_lds(int rows, int blocks) { return (rows * blocks + 15 + 1023) / 1024 * 1024; }
+
+// LDS of a wavefront's ring: KB a step is NT + RP / 4
+template <int NT, bool A4, int U4, int U8, int U16>
+constexpr int stream_ring() {
+  int most = (NT + 1) * U4;
+  if ((NT + 2) * U8 > most) most = (NT + 2) * U8;
+  if ((NT + 4) * U16 > most) most = (NT + 4) * U16;
+  return A4 ? 0 : most * 1024;
+}
+template <int NT, bool A4, int NW, int U4, int U8, int U16>
+static __host__ __device__ __forceinline__ int stream_lds(int blocks) {
+  constexpr int sums = NW * 16 * (16 * NT + 1) * 4, rings = NW * stream_ring<NT, A4, U4, U8, U16>();
+  return (sums > rings ? sums : rings) + stream_scale_lds(16 * NT, blocks);
+}
+
 template <int NT, bool A4, int MODE, int NW, int U4, int U8, int U16>
 __global__ __launch_bounds__(NW * 64) void mx_stream_kernel(MxArgs a, int tiles_n) {
-  constexpr int BN = 16 * NT, BR = 16, THREADS = NW * 64, PITCH = BN + 1;
-  __shared__ float sums[NW][BR][PITCH];
-  extern __shared__ __align__(16) unsigned char scale_bytes[];
+  constexpr int BN = 16 * NT, BR = 16, THREADS = NW * 64, PITCH = BN + 1, RING = stream_ring<NT, A4, U4, U8, U16>();
+  extern __shared__ __align__(1024) unsigned char smem[];  // rings, later sums [NW][BR][PITCH]; scale bytes
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m16 = lane & 15;
   const int item = blockIdx.x / tiles_n, n0 = (blockIdx.x - item * tiles_n) * BN;
@@ -172,16 +204,68 @@ __global__ __launch_bounds__(NW * 64) void mx_stream_kernel(MxArgs a, int tiles_
   const int blocks = a.k / 32;
   const int nn = a.n - n0 < BN ? a.n - n0 : BN;             // weight rows of this tile
   const int64_t wrow = static_cast<int64_t>(it.expert) * a.n + n0;
-  MxScaleFetch<THREADS, 1> fetch(a.w_scales + wrow * blocks, nn, blocks, tid);
-  fetch.load(0);
+  const unsigned char* const scales_from = a.w_scales + wrow * blocks;
+  const int shift = mx_scale_shift(scales_from);
+  unsigned char* const scale_bytes = smem + stream_lds<NT, A4, NW, U4, U8, U16>(blocks) - stream_scale_lds(BN, blocks);
 
-  // the rows' numbers, if they are gathered or scattered, and this thread's bias go out ahead of the weight
+  // The pairs of the item's rows, if the rows are gathered: through the scalar cache, since vector loads would come back behind
+  // the weights that are asked for on this CU already.
   constexpr bool gather = MODE == kMxSwiglu;
-  const int r16 = m16 & (columns - 1);
-  const bool there = r16 < it.rows;
-  unsigned row = r16;
-  if (gather) row = a.tokens > 1 ? mx_pair(a, it.first + (there ? r16 : 0)) / static_cast<unsigned>(a.top) : 0;
-  constexpr int OUTS = BR * BN / (MODE == kMxSwiglu ? 2 : 1), PER = (OUTS + THREADS - 1) / THREADS;   // results of a thread
+  const ScalarInts order = mx_scalar(a.order) + it.first;
+  const unsigned last_pair = static_cast<unsigned>(a.rows - 1);
+  auto row_of = [&](int r) {                                // row r of the item in x; r differs from lane to lane
+    if (!gather) return static_cast<unsigned>(r);
+    unsigned pair = 0;
+    for (int j = 0; j < it.rows; ++j) {
+      const unsigned p = min(static_cast<unsigned>(order[j]), last_pair);
+      pair = r == j ? p : pair;
+    }
+    return pair / static_cast<unsigned>(a.top);
+  };
+  const int row_bytes = A4 ? blocks * 16 : a.k * 2;
+  const unsigned char* const xb = static_cast<const unsigned char*>(a.x) + (gather ? 0 : it.first * a.x_pitch);
+  const unsigned x_span = static_cast<unsigned>(((gather ? a.tokens : it.rows) - 1) * a.x_pitch + row_bytes);
+  MxWalk m;
+  m.w = mx_buffer_words(a.w + wrow * blocks * 16, nn * blocks * 16);
+  m.x = mx_buffer_words(xb, x_span);
+  m.scales = scale_bytes + shift + m16 * blocks;
+  m.ring = smem + wave * RING;
+  m.blocks = blocks;
+  m.nn = nn;
+  m.wave = wave;
+  m.lane = lane;
+  float* const sums = reinterpret_cast<float*>(smem);
+  float* const mine = sums + wave * BR * PITCH;
+
+  // the scale bytes, 1 KB a load, dealt to the wavefronts (to whole words: a word that the end cuts would come as zeros)
+  {
+    const int bytes = (shift + nn * blocks + 3) & ~3;
+    const u32x4 from = mx_buffer_words(scales_from - shift, bytes);
+    const unsigned to = static_cast<unsigned>(reinterpret_cast<uintptr_t>(scale_bytes));
+    for (int i = wave * 1024; i < bytes; i += NW * 1024) mx_load_lds(from, 16 * lane, i, to + i);
+  }
+  auto ready = [&](int loads) {                             // behind the scales' loads, `loads` others
+    if (loads >= 12) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    else if (loads >= 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  if constexpr (A4) {
+    const auto w = mx_buffer(a.w + wrow * blocks * 16, nn * blocks * 16), x = mx_buffer(xb, x_span);
+    m.x_scales = mx_buffer(a.x_scales + static_cast<int64_t>(it.first) * blocks, it.rows * blocks);
+    mx_walk4<NT, NW, U4>(m, w, x, m16 < it.rows ? static_cast<unsigned>(m16 * a.x_pitch) : MX_NONE, m16 * blocks, mine, PITCH, ready);
+  } else {
+    auto row_at = [&](int r) {
+      const unsigned row = row_of(r);
+      return r < it.rows ? static_cast<unsigned>(row * a.x_pitch) : MX_NONE;
+    };
+    if (columns == 4) mx_walk<NT, 4, NW, U4>(m, mine, PITCH, row_at, ready);
+    else if (columns == 8) mx_walk<NT, 8, NW, U8>(m, mine, PITCH, row_at, ready);
+    else mx_walk<NT, 16, NW, U16>(m, mine, PITCH, row_at, ready);
+  }
+
+  // this thread's results: where they go, and their bias
+  constexpr int OUTS = BR * BN / (MODE == kMxSwiglu ? 2 : 1), PER = (OUTS + THREADS - 1) / THREADS;
   unsigned pair[PER] = {};
   float bias[PER][2] = {};
 #pragma unroll
@@ -193,36 +277,12 @@ __global__ __launch_bounds__(NW * 64) void mx_stream_kernel(MxArgs a, int tiles_
       if (MODE == kMxSwiglu) bias[p][1] = static_cast<float>(a.bias[wrow + min(n + 1, nn - 1)]);
     }
   }
-
-  // the rows' bytes: of a token anywhere in x, or counted from the item's first row
-  MxWalk m;
-  const int row_bytes = A4 ? blocks * 16 : a.k * 2;
-  const unsigned char* const xb = static_cast<const unsigned char*>(a.x) + (gather ? 0 : it.first * a.x_pitch);
-  m.w = mx_buffer(a.w + wrow * blocks * 16, nn * blocks * 16);
-  m.x = mx_buffer(xb, static_cast<unsigned>(((gather ? a.tokens : it.rows) - 1) * a.x_pitch + row_bytes));
-  m.x_scales = A4 ? mx_buffer(a.x_scales + static_cast<int64_t>(it.first) * blocks, it.rows * blocks) : m.x;
-  m.blocks = blocks;
-  m.pitch = mx_scale_pitch(blocks);
-  m.scale_bytes = scale_bytes + mx_scale_shift(a.w_scales + wrow * blocks) + m16 * m.pitch;
-  m.row_at = there ? static_cast<unsigned>(row * a.x_pitch) : MX_NONE;
-  m.row_scales_at = row * blocks;
-  auto ready = [&] {
-    fetch.write(scale_bytes, 0);
-    fetch.rest(scale_bytes, THREADS);
-    __syncthreads();
-  };
-  float* const mine = sums[wave][0];
-  if constexpr (A4) mx_walk4<NT, NW, U4>(m, wave, lane, mine, PITCH, ready);
-  else if (columns == 4) mx_walk<NT, 4, NW, U4>(m, wave, lane, mine, PITCH, ready);
-  else if (columns == 8) mx_walk<NT, 8, NW, U8>(m, wave, lane, mine, PITCH, ready);
-  else mx_walk<NT, 16, NW, U16>(m, wave, lane, mine, PITCH, ready);
   __syncthreads();
-
   auto total = [&](int r, int n) {
     float v = 0.f;
     for (int c = r; c < 16; c += columns)
 #pragma unroll
-      for (int w = 0; w < NW; ++w) v += sums[w][c][n];
+      for (int w = 0; w < NW; ++w) v += sums[(w * BR + c) * PITCH + n];
     return v;
   };
 #pragma unroll
@@ -245,28 +305,27 @@ static int launch(const MxArgs& a, hipStream_t st) {
   const int64_t tiles = (a.n + 16 * NT - 1) / (16 * NT);
   const int64_t items = a.order ? mx_items(a.rows, a.experts, 16) : (a.rows + 15) / 16;
   TLLM_REQUIRE(tiles * items < (1ll << 32) / (NW * 64), TLLM_E_SHAPE, "mxfp4 product: %lld rows of %d outputs are too many", (long long)a.rows, a.n);
-  const int lds = mx_scale_lds(16 * NT, a.k / 32);
-  if (lds > 40 * 1024) {                                   // (long rows; with the sums more than a kernel has without asking)
-    static std::atomic<uint64_t> done{0};
-    const void* const kernel = reinterpret_cast<const void*>(mx_stream_kernel<NT, A4, MODE, NW, U4, U8, U16>);
-    TLLM_REQUIRE(raise_lds_limit(kernel, 140 * 1024, done) == hipSuccess, TLLM_E_LAUNCH, "mxfp4 product: the LDS limit could not be raised");
-  }
+  const int lds = stream_lds<NT, A4, NW, U4, U8, U16>(a.k / 32);
+  static std::atomic<uint64_t> done{0};
+  const void* const kernel = reinterpret_cast<const void*>(mx_stream_kernel<NT, A4, MODE, NW, U4, U8, U16>);
+  TLLM_REQUIRE(raise_lds_limit(kernel, 160 * 1024, done) == hipSuccess, TLLM_E_LAUNCH, "mxfp4 product: the LDS limit could not be raised");
+  TLLM_REQUIRE(lds <= 160 * 1024, TLLM_E_SHAPE, "mxfp4 product: %d values in a row are too many", a.k);
   hipLaunchKernelGGL((mx_stream_kernel<NT, A4, MODE, NW, U4, U8, U16>), dim3((unsigned)(tiles * items)), dim3(NW * 64), lds, st, a, (int)tiles);
   return check_launch("mxfp4 product");
 }
 
 // The workgroup. Wide ones (64 weight rows) read the activations less often and pay where items are full: 128 tokens of 32 experts
-// mlp1 114 us with 32 rows, 107 with 64 (33 tokens 63.4 and 67.1), 65 rows of [5120, 2880] 14.8 and 12.3. Narrow ones, with their K
-// share in one piece, where the launch would have less than one for each CU otherwise: one row of [2880, 4096] 6.9 us with 32 weight
-// rows, 4.7 with 16; 64 rows of [1024, 1024] 5.8 with 64, 4.4 with 32. More steps on their way per wavefront cost wavefronts on the CU and more than
-// they bring: 33 tokens 63.8 us with 2 steps, 70 with 3, 85 with 6.
+// mlp1 107 us with 32 rows, 96 with 64 (33 tokens 59.5 and 63), 65 rows of [5120, 2880] 11.7 and 9.0. Narrow ones, with their K
+// share in one piece, where the launch would have less than one for every other CU otherwise: one row of [2880, 4096] 6.9 us with 32
+// weight rows, 4.7 with 16; 64 rows of [1024, 1024] 5.8 with 64, 4.4 with 32. Few steps in the rings: workgroups on the CU bring
+// more than a longer ring does (33 tokens 59.5 us with rings of 6 KB, 59.8 with 9, 64 with 12, 78 with 18).
 template <int MODE>
 static int launch_bf16(const MxArgs& a, hipStream_t st) {
   const int64_t items = a.order ? (a.rows < a.experts ? a.rows : a.experts) + a.rows / 32 : (a.rows + 15) / 16;
   const bool full = a.rows > 12ll * a.experts;
-  if (full && (a.n + 63) / 64 * items >= 256 && a.k <= 16384) return launch<4, false, MODE, 4, 2, 2, 1>(a, st);
-  if ((a.n + 31) / 32 * items > 128 && a.k <= 32768) return launch<2, false, MODE, 4, 2, 2, 2>(a, st);
-  return launch<1, false, MODE, 8, 3, 3, 2>(a, st);
+  if (full && (a.n + 63) / 64 * items >= 256 && a.k <= 16384) return launch<4, false, MODE, 4, 1, 1, 1>(a, st);
+  if ((a.n + 31) / 32 * items > 128 && a.k <= 32768) return launch<2, false, MODE, 4, 2, 1, 1>(a, st);
+  return launch<1, false, MODE, 8, 3, 2, 1>(a, st);
 }
 
 int mx_stream(const MxArgs& a, int mode, bool a4, hipStream_t st) {
