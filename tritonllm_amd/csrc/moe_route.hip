@@ -11,6 +11,8 @@
 // values as sortable integers, and the first lane that has it. The pairs are sorted by counting:
 // tokens are dealt in order to workgroups and their wavefronts, and a wavefront places its tokens one after the other -- a
 // token's experts are all different, so its lanes can place them at once. That makes the order stable and the same every time.
+// What bounds it are latencies: 8 tokens of 32 experts 3.2 us in one launch; 8191 of 256, 4.2 MB of logits, 14.6 + 9.2 us in two
+// (branches around single loads, one wait each, had made the first 19.5; counts summed one load at a time the second 60).
 #include "mx_common.h"
 
 namespace tllm {
@@ -196,18 +198,24 @@ __device__ __forceinline__ void first_places(int* count, int pitch, const int* s
   }
 }
 
+// Sum over the lanes up to this one: inside the rows of sixteen, then the first row's last to the second and the third's to the
+// fourth, then the second's to the upper half.
+__device__ __forceinline__ int wave_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 // One wavefront: all[e], pairs of expert e, becomes the pairs of the experts before it; so do the offsets, if they are to be written.
 __device__ __forceinline__ void scan_experts(int* all, int n_experts, int lane, int* offsets) {
   int before = 0;
   for (int e0 = 0; e0 < n_experts; e0 += 64) {
     const int e = e0 + lane, n = e < n_experts ? all[e] : 0;
-    int upto = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int u = __shfl_up(upto, d);
-      if (lane >= d) upto += u;
-    }
-    const int start = before + upto - n;
+    const int upto = wave_upto(n), start = before + upto - n;
     if (e < n_experts) {
       all[e] = start;
       if (offsets) offsets[e] = start;
@@ -215,6 +223,170 @@ __device__ __forceinline__ void scan_experts(int* all, int n_experts, int lane, 
     before += __builtin_amdgcn_readlane(upto, 63);
   }
   if (offsets && lane == 0) offsets[n_experts] = before;
+}
+
+// Many tokens: four to a wavefront, a token's experts in the sixteen lanes of a DPP row, V neighbours to a lane. All of a choice is
+// then vector work of four tokens at once -- a maximum inside the row, the first lane that has it, its first value. A wavefront takes
+// longer over its tokens that way, but there is a quarter as much to issue: of 256 experts in groups, the best 8, both launches,
+// 32768 tokens 61.5 us with a token to a wavefront, 51.0 so, 8191 24.4 and 23.3, 2048 15.2 and 18.5. Groups have to be whole
+// lanes, a power of two of them, and `top` at most sixteen, one to a lane. The tokens of workgroup b are those of the kernel below, so
+// that the pairs are placed by the same counts.
+constexpr int FOURS_WAVES = 8, FOURS_FROM = 6000;
+__device__ __forceinline__ unsigned row_max_u32(unsigned v) {
+  auto dpp = [](unsigned x, auto ctrl) { return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+  v = max(v, dpp(v, std::integral_constant<int, 0xB1>{}));
+  v = max(v, dpp(v, std::integral_constant<int, 0x4E>{}));
+  v = max(v, dpp(v, std::integral_constant<int, 0x141>{}));
+  return max(v, dpp(v, std::integral_constant<int, 0x140>{}));
+}
+template <class Op>
+__device__ __forceinline__ float row_all(float v, Op op) {
+  auto dpp = [](float x, auto ctrl) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+  v = op(v, dpp(v, std::integral_constant<int, 0xB1>{}));
+  v = op(v, dpp(v, std::integral_constant<int, 0x4E>{}));
+  v = op(v, dpp(v, std::integral_constant<int, 0x141>{}));
+  return op(v, dpp(v, std::integral_constant<int, 0x140>{}));
+}
+template <int V, bool SIGMOID, class T>
+__global__ __launch_bounds__(FOURS_WAVES * 64) void moe_route_fours_kernel(RouteArgs a) {
+  __shared__ int count[16 * V];
+  const float ninf = -__builtin_inff();
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, base = lane & 48;
+  for (int i = tid; i < 16 * V; i += FOURS_WAVES * 64) count[i] = 0;
+  float bias[V] = {};
+  if (a.bias) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) bias[v] = a.bias[min(V * l16 + v, a.n_experts - 1)];
+  }
+  __syncthreads();
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * ROUTE_WAVES * a.per_wave;
+  const int per_run = ROUTE_WAVES * a.per_wave;
+  // rows of whole sixteens come in as such
+  const bool whole = a.n_experts == 16 * V && V * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.row_stride * sizeof(T) % 16 == 0;
+  for (int i0 = 4 * wave; i0 < per_run && first + i0 < a.tokens; i0 += 4 * FOURS_WAVES) {
+    const int64_t mine = first + i0 + (lane >> 4);
+    const bool there = mine < a.tokens;
+    const int64_t t = there ? mine : a.tokens - 1;
+    const T* const row = static_cast<const T*>(a.logits) + t * a.row_stride;
+    T l[V];
+    if (whole) {
+      typedef __attribute__((__vector_size__(16))) T T16;
+      constexpr int N = 16 / sizeof(T);
+#pragma unroll
+      for (int v = 0; v + N <= V; v += N) {
+        const T16 x = *reinterpret_cast<const T16*>(row + V * l16 + v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) l[v + i] = x[i];
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) l[v] = row[min(V * l16 + v, a.n_experts - 1)];
+    }
+    float s[V];                                             // logits, then scores
+    float best = ninf, sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float f = static_cast<float>(l[v]);
+      s[v] = V * l16 + v >= a.n_experts || f != f ? ninf : f;
+      best = fmaxf(best, s[v]);
+    }
+    unsigned key[V];
+    if constexpr (!SIGMOID) best = row_all(best, [](float x, float y) { return fmaxf(x, y); });
+    // the scores of all are needed for softmax's sum, a bias or groups; otherwise the chosen ones' alone, below
+    auto score_of = [&](float x) {
+      if constexpr (SIGMOID) return 1.0f / (1.0f + expf(-x));
+      else return x == ninf ? 0.f : x == best ? 1.f : expf(x - best);       // (an infinite logit takes all)
+    };
+    const bool all = !SIGMOID || a.bias || a.groups > 1;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      key[v] = V * l16 + v < a.n_experts ? sortable(s[v]) : 0;
+      if (all) {
+        s[v] = score_of(s[v]);
+        sum += s[v];
+      }
+    }
+    if constexpr (!SIGMOID) {
+      sum = row_all(sum, [](float x, float y) { return x + y; });
+      if (a.bias || a.groups > 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) s[v] = sum > 0.f ? s[v] / sum : 0.f;
+      }
+    }
+    if (a.bias) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        s[v] += bias[v];
+        key[v] = V * l16 + v < a.n_experts ? sortable(s[v]) : 0;
+      }
+    }
+    if (a.groups > 1) {
+      const int lanes = a.n_experts / a.groups / V;
+      float one = ninf, two = ninf;
+#pragma unroll
+      for (int v = 0; v < V; ++v) best_two(one, two, s[v] != s[v] ? ninf : s[v], ninf);
+#pragma unroll
+      for (int d = 1; d < 16; d *= 2)
+        if (d < lanes) best_two(one, two, __shfl_xor(one, d), __shfl_xor(two, d));
+      const unsigned gk = sortable(V * lanes > 1 ? one + two : one);
+      const int group = l16 / lanes;
+      int ahead = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const unsigned o = __shfl(gk, base + ((j * lanes) & 15));
+        ahead += j < a.groups && (o > gk || (o == gk && j < group));
+      }
+      if (ahead >= a.kept) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = 0;
+      }
+    }
+    int expert = 0;
+    T chosen = static_cast<T>(0.f);
+    for (int j = 0; j < a.top; ++j) {
+      unsigned half[V];                                     // (a tree: the steps of a chain would wait for one another)
+#pragma unroll
+      for (int v = 0; v < V; ++v) half[v] = key[v];
+#pragma unroll
+      for (int d = V / 2; d >= 1; d /= 2)
+#pragma unroll
+        for (int v = 0; v < d; ++v) half[v] = max(half[v], half[v + d]);
+      const unsigned own = half[0], top = row_max_u32(own);
+      const unsigned has = static_cast<unsigned>(__ballot(own == top) >> base) & 0xffffu;
+      const int who = __builtin_ctz(has);
+      unsigned hits[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) hits[v] = key[v] == top ? 1u << v : 0u;
+#pragma unroll
+      for (int d = V / 2; d >= 1; d /= 2)
+#pragma unroll
+        for (int v = 0; v < d; ++v) hits[v] |= hits[v + d];
+      const int at = __builtin_ctz(hits[0] | 0x80000000u);
+      const int gone = l16 == who ? at : -1;
+#pragma unroll
+      for (int v = 0; v < V; ++v) key[v] = v == gone ? 0 : key[v];
+      const int e = V * who + __shfl(at, base + who);
+      if (l16 == j) {
+        expert = e;
+        chosen = row[e];
+      }
+    }
+    float weight = 0.f;
+    if (l16 < a.top) {
+      const float f = static_cast<float>(chosen);
+      weight = score_of(f != f ? ninf : f);
+      if (!SIGMOID) weight = sum > 0.f ? weight / sum : 0.f;
+    }
+    const float total = row_all(weight, [](float x, float y) { return x + y; });
+    if (a.renorm) weight = total > 0.f ? weight / total : 0.f;
+    if (there && l16 < a.top) {
+      a.experts[t * a.top + l16] = expert;
+      a.weights[t * a.top + l16] = weight * a.scale;
+      atomicAdd(&count[expert], 1);
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e < a.n_experts; e += FOURS_WAVES * 64) a.counts[static_cast<int64_t>(blockIdx.x) * a.n_experts + e] = count[e];
 }
 
 // The tokens of workgroup b, wavefront w: per_wave of them from (b ROUTE_WAVES + w) per_wave on.
@@ -282,16 +454,26 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_place_kernel(RouteArgs a
   for (int i = tid; i < ROUTE_WAVES * ROUTE_E; i += THREADS) count[0][i] = 0;
   for (int e = tid; e < ROUTE_E; e += THREADS) all[e] = earlier[e] = 0;
   __syncthreads();
-  // the runs' counts, dealt to the threads by expert and by run, sixteen of a thread's on their way at a time
+  // this wavefront's first tokens' experts, read once where there are few
+  constexpr int HELD = 4;
+  const int64_t t0 = (static_cast<int64_t>(run) * ROUTE_WAVES + wave) * a.per_wave;
+  int held[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    const int64_t t = t0 + i < a.tokens ? t0 + i : a.tokens - 1;
+    held[i] = a.experts[t * a.top + (lane < a.top ? lane : 0)];
+  }
+  auto expert_of = [&](int i) { return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : i == 3 ? held[3] : a.experts[(t0 + i) * a.top + lane]; };
+  // the runs' counts, dealt to the threads by expert and by run, thirty-two of a thread's on their way at a time
   const int parts = THREADS / E, part = tid / E, mine = tid - part * E;
   if (part < parts) {
     int total = 0, before = 0;
-    for (int r0 = part; r0 < a.runs; r0 += 16 * parts) {
-      int c[16];
+    for (int r0 = part; r0 < a.runs; r0 += 32 * parts) {
+      int c[32];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) c[j] = r0 + j * parts < a.runs ? a.counts[static_cast<int64_t>(r0 + j * parts) * E + mine] : 0;
+      for (int j = 0; j < 32; ++j) c[j] = r0 + j * parts < a.runs ? a.counts[static_cast<int64_t>(r0 + j * parts) * E + mine] : 0;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < 32; ++j) {
         total += c[j];
         before += r0 + j * parts < run ? c[j] : 0;
       }
@@ -299,9 +481,8 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_place_kernel(RouteArgs a
     atomicAdd(&all[mine], total);
     atomicAdd(&earlier[mine], before);
   }
-  const int64_t t0 = (static_cast<int64_t>(run) * ROUTE_WAVES + wave) * a.per_wave;
   for (int i = 0; i < a.per_wave && t0 + i < a.tokens; ++i) {
-    if (lane < a.top) count[wave][a.experts[(t0 + i) * a.top + lane]] += 1;
+    if (lane < a.top) count[wave][expert_of(i)] += 1;
     lds_in_order();
   }
   __syncthreads();
@@ -315,12 +496,27 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_place_kernel(RouteArgs a
     lds_in_order();
     if (lane < a.top) {
       const int64_t p = (t0 + i) * a.top + lane;
-      int* const c = &count[wave][a.experts[p]];
+      int* const c = &count[wave][expert_of(i)];
       const int at = *c;
       *c = at + 1;
       a.order[at] = static_cast<int>(p);
     }
   }
+}
+
+// Whether the choice can be made in a row of sixteen lanes with V experts each
+static bool in_fours(const RouteArgs& a, int V) {
+  if (a.top > 16) return false;
+  if (a.groups == 1) return true;
+  const int size = a.n_experts / a.groups, lanes = size / V;
+  return size % V == 0 && lanes > 0 && (lanes & (lanes - 1)) == 0;
+}
+template <int V>
+static int launch_fours(const RouteArgs& a, bool sigmoid, bool is_f32, hipStream_t st) {
+  auto go = [&](auto* kernel) { hipLaunchKernelGGL(kernel, dim3(a.runs), dim3(FOURS_WAVES * 64), 0, st, a); };
+  if (sigmoid) is_f32 ? go(moe_route_fours_kernel<V, true, float>) : go(moe_route_fours_kernel<V, true, bf16>);
+  else is_f32 ? go(moe_route_fours_kernel<V, false, float>) : go(moe_route_fours_kernel<V, false, bf16>);
+  return check_launch("moe_route");
 }
 
 template <int V>
@@ -375,7 +571,14 @@ extern "C" int tllm_moe_route(const void* logits, int logits_is_f32, int64_t log
   a.runs = route_runs(tokens, &a.per_wave);
   if (tokens == 0) a.runs = 1;                             // (the offsets alone, all 0)
   const bool s = sigmoid != 0, f = logits_is_f32 != 0;
-  const int rc = n_experts <= 64 ? launch_route<1>(a, s, f, alone, st) : n_experts <= 128 ? launch_route<2>(a, s, f, alone, st)
+  const int per_lane = n_experts <= 32 ? 2 : n_experts <= 64 ? 4 : n_experts <= 128 ? 8 : n_experts <= 256 ? 16 : 32;
+  const bool fours = tokens >= FOURS_FROM && in_fours(a, per_lane);
+  const int rc = fours ? (per_lane == 2   ? launch_fours<2>(a, s, f, st)
+                          : per_lane == 4  ? launch_fours<4>(a, s, f, st)
+                          : per_lane == 8  ? launch_fours<8>(a, s, f, st)
+                          : per_lane == 16 ? launch_fours<16>(a, s, f, st)
+                                           : launch_fours<32>(a, s, f, st))
+               : n_experts <= 64 ? launch_route<1>(a, s, f, alone, st) : n_experts <= 128 ? launch_route<2>(a, s, f, alone, st)
                : n_experts <= 256 ? launch_route<4>(a, s, f, alone, st) : launch_route<8>(a, s, f, alone, st);
   if (rc != TLLM_OK || alone) return rc;
   hipLaunchKernelGGL(moe_place_kernel, dim3(a.runs), dim3(ROUTE_WAVES * 64), 0, st, a);
