@@ -8,6 +8,9 @@
 // blocks' scale bytes side by side. Slices of both operands come into a ring of S in LDS by buffer loads straight there, block b of a
 // row at place b ^ (row / 2 % 8). Scale bytes of all rows lie in LDS for the whole of K. A half slice's fragments are read under
 // the MFMAs of the one before.
+//
+// What bounds it: 2048 rows of [5120, 2880] take 30 us, one 128 x 320 tile to a CU, 2.0 PFLOP/s: 9 us of beginning and end, then 1.7 us a
+// slice, of which the MFMAs are 0.7 and the LDS reads as much; 4096 x 4096 x 4096 54 us, 2.5 PFLOP/s.
 #include "mx_common.h"
 
 namespace tllm {

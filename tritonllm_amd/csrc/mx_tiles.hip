@@ -3,11 +3,18 @@
 //   D[r, n] = sum_k X[r, k] W[n, k]        X bf16, W MXFP4, a run of one expert's rows to a tile
 //
 // K goes in slices of 64: a slice of X is 128 bytes a row, of W 32 (two blocks). Both come into a ring of S slices in LDS as they are
-// (buffer loads straight to LDS); the codes become bf16 in registers, in front of v_mfma_f32_16x16x32_bf16, weight rows on M. In a
-// slice lane (m, g) of a fragment has the values k = 16 u .. 16 u + 15, u = mx_quarter(g), half a block, eight for each of two MFMAs,
-// of both operands.
-// The scale bytes of the tile's weight rows lie in LDS for the whole of K, a lane reads one for a fragment's slice.
-// A lane ends up with four neighbouring weight rows of one row of X and stores them from its registers.
+// (buffer loads straight to LDS); the codes become bf16 in registers, in front of v_mfma_f32_16x16x32_bf16, weight rows on M: a
+// wavefront converts each of its weight fragments once per slice, five issue cycles a pair of values next to the sixteen of an MFMA,
+// and they run side by side. In a slice lane (m, g) of a fragment has the values k = 16 u .. 16 u + 15, u = mx_quarter(g), half a block,
+// eight for each of two MFMAs, of both operands. The next half slice's fragments are read under the MFMAs of this one. The
+// scale bytes of the tile's weight rows lie in LDS for the whole of K, a lane reads one for a fragment's slice. A lane ends up with four
+// neighbouring weight rows of one row of X and stores them from its registers.
+//
+// What bounds it: the matrix cores at the clock that they leave (one 128 x 256 tile to a CU, [4096] outputs of 2048 rows, goes
+// through K at 1.18 PFLOP/s, where a large library product reaches 1.24), behind 11 us of a launch's beginning and end per round
+// of tiles, which workgroups that share a CU cover for one another, and the rows that an expert's last tile lacks. 2048 tokens of
+// 32 experts, four each, hidden and inner 2880: mlp1 312 us (870 TFLOP/s), mlp2's product 166 and its weighted sum 17. Built and
+// slower: three slices in the ring of the 128 x 128 tile (two workgroups to a CU instead of three; 340 us), 64 x 512 (472), 128 x 256 (367).
 #include "mx_common.h"
 
 namespace tllm {
@@ -130,20 +137,28 @@ __global__ __launch_bounds__(C::NW * 64) void mx_tile_kernel(MxArgs a, int tiles
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * LPW) : "memory");
-  read_w(0, 0);
-  read_x(I0{}, 0);
+  // a wavefront whose rows, or weight rows, are not there keeps step and leaves the matrix cores to others
+  const bool live = 16 * TB * wm < it.rows && 16 * RB * wn < nn;
+  if (live) {
+    read_w(0, 0);
+    read_x(I0{}, 0);
+  }
   int place = 0;
   for (int s = 0; s < slices; ++s) {
-    read_x(I1{}, place);
-    convert(I0{});
-    multiply(I0{});
-    convert(I1{});
+    if (live) {
+      read_x(I1{}, place);
+      convert(I0{});
+      multiply(I0{});
+      convert(I1{});
+    }
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * LPW) : "memory");
     issue(s + S, place);
     place = place + 1 == S ? 0 : place + 1;
-    read_w(s + 1, place);                                  // (behind the last slice: the last one again, not used)
-    read_x(I0{}, place);
-    multiply(I1{});
+    if (live) {
+      read_w(s + 1, place);                                // (behind the last slice: the last one again, not used)
+      read_x(I0{}, place);
+      multiply(I1{});
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 

@@ -76,7 +76,8 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const unsigned* __re
 // least 2^-127, and become the nearest e2m1 value of x 2^-e, ties to the even code; beyond 6 is 6. A block that holds a NaN or an
 // infinity has the scale byte 255, which makes all of it NaN, and codes of 0.
 // The maximum is one of the values' bits: without the sign they order as integers, and the exponent field less 2 is the scale
-// byte. A lane takes eight values (16 or 32 bytes), four neighbouring lanes a block.
+// byte. A lane takes eight values (16 or 32 bytes), four neighbouring lanes a block. The bytes bound it: 40960 x 2880 fp32 values, 472 MB
+// read and 63 MB written, 87 us, 6.1 TB/s (a plain read's rate); one row of 2880 1.6 us.
 template <class T>
 struct Eight;                        // eight values as loaded; the largest of their magnitudes as an fp32's bits; eight codes
 template <>

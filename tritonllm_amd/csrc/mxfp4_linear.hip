@@ -5,7 +5,8 @@ namespace tllm {
 
 // out[t, n] = residual[t, n] + sum_j weights[t, j] pairs[t top + j, n], in the order of j, in fp32, rounded once. A thread takes V
 // neighbours of a token, four where rows are whole fours; up to four experts' loads leave together. 2000 tokens of 2880 and four
-// experts, 115 MB: 35 us an element at a time.
+// experts, 115 MB: 17.5 us, 6.6 TB/s (the pairs are in the Infinity Cache still; an element at a time 35). The pairs stay in fp32: as bf16
+// they would be half the bytes, 8 us, and a second rounding in every result.
 template <int V>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restrict__ pairs, const float* __restrict__ weights, const bf16* residual,
                                                           int64_t res_stride, bf16* out, int64_t out_stride, int n, int top, int per_row) {
