@@ -7,9 +7,9 @@
 // wavefronts owns 16 NT weight rows and up to 16 activation rows; the wavefronts deal the K steps of 128 between them (sums meet in
 // LDS, added in a fixed order). Weights and activations go straight to LDS, U steps of a wavefront at a time in a ring that is its
 // alone, so that nothing but the wavefront's own count of arrivals is waited for. That path is what the addresses ask for: a
-// 16-byte load takes one turn of the address unit for four neighbouring lanes with 64 neighbouring bytes and one for each lane
-// otherwise, and a matrix operand has its rows in neighbouring lanes (loaded to registers that way the address units were busy
-// 73 % of the time: 33 tokens 63.8 us, 59.5 now).
+// 16-byte load is one access of the cache for four neighbouring lanes with 64 neighbouring bytes and one for each lane otherwise, and a
+// matrix operand has its rows in neighbouring lanes (33 tokens, loaded to registers that way: 24.2 million accesses, 63.8 us; 7.8
+// million and 59.5 now).
 //
 // In a step lane (m, g) of a fragment has block mx_quarter(g) of weight row m, and the four v_mfma_f32_16x16x32_bf16 take 8 of its 32
 // values each, from both operands. The codes become bf16 on the way, exactly, once per step for all rows; a lane reads its block's scale
