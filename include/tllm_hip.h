@@ -357,7 +357,7 @@ int tllm_mxfp4_quantize(const void* x, int x_type, int64_t x_row_stride, void* b
 
 /* out[r, n] = sum_k x[r, k] W[n, k] + bias[n] with W MXFP4 [out_dim, in_dim] (fp32 accumulate, one RNE to bf16). x is bf16
  * with x_row_stride values from row to row, or, with x_scales not NULL, dense MXFP4 blocks. bias bf16 [out_dim] or NULL. in_dim a
- * multiple of 32; rows of x, W's blocks and all scales 16-byte aligned, x within 4 GiB. Any number of rows. */
+ * multiple of 32; rows of x, W's blocks and all scales 16-byte aligned, 128 rows of x within 4 GiB. Any number of rows. */
 int tllm_mxfp4_linear_bf16(const void* x, const void* x_scales, int64_t x_row_stride, const void* w_blocks, const void* w_scales,
                            const void* bias, void* out, int64_t out_row_stride, int64_t rows, int64_t in_dim, int64_t out_dim,
                            void* stream);
@@ -380,7 +380,7 @@ int tllm_moe_route(const void* logits, int logits_is_f32, int64_t logits_row_str
 /* The experts' first product with its SwiGLU, a row per pair in the order of tllm_moe_route's plan:
  *   h[s, :] = swiglu(x[order[s] / top, :] . W[e]^T + bias[e])     e: the expert whose offsets hold s
  * x [tokens, hidden] bf16, W MXFP4 [n_experts, 2 * inner, hidden] with gate and linear rows in turn, bias bf16 [n_experts,
- * 2 * inner] or NULL, h [tokens * top, inner] bf16; SwiGLU as tllm_swiglu_bf16, on the fp32 sums. Replaces the gathered
+ * 2 * inner] or NULL, h [tokens * top, inner] bf16, x within 4 GiB; SwiGLU as tllm_swiglu_bf16, on the fp32 sums. Replaces the gathered
  * mlp1 matmul and swiglu of MLPBlock (model.py:751-757, moe.py:25-33). */
 int tllm_moe_mlp1_bf16(const void* x, int64_t x_row_stride, const int32_t* order, const int32_t* offsets, const void* w_blocks,
                        const void* w_scales, const void* bias, void* h, int64_t h_row_stride, int64_t tokens, int n_experts, int top,

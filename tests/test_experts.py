@@ -232,6 +232,27 @@ def test_linear_of_unaligned_views(rows):
 
 
 @gpu
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+def test_linear_of_rows_beyond_32_bits(acts):
+    """Activations of more than 4 GiB: the first rows, ones from the middle and the last."""
+    rows, k, n = ((1 << 22) + 133, 512, 16) if acts == "bf16" else ((1 << 23) + 133, 1024, 16)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w, ws = random_mx(torch.Generator().manual_seed(2), n, k)
+    if acts == "bf16":
+        x, xs = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda").normal_(generator=g), None
+    else:
+        x = torch.randint(0, 256, (rows, k // 32, 16), generator=g, dtype=torch.uint8, device="cuda")
+        xs = torch.randint(120, 130, (rows, k // 32), generator=g, dtype=torch.uint8, device="cuda")
+    assert x.numel() * x.element_size() > 1 << 32
+    got = T.mxfp4_linear(x, *cuda(w, ws), x_scales=xs)
+    wv = values(w, ws)
+    for first in (0, rows // 2, rows - 300):
+        part = slice(first, first + 300)
+        xv = x[part].cpu().double() if xs is None else values(x[part].cpu(), xs[part].cpu())
+        check_product(got[part], xv @ wv.t(), xv.abs() @ wv.abs().t(), k, f"rows from {first} on")
+
+
+@gpu
 def test_quantize_then_linear_is_the_product_of_the_values():
     g = torch.Generator().manual_seed(3)
     x = torch.randn(77, 2880, generator=g).bfloat16()
@@ -616,7 +637,7 @@ def test_entry_points_refuse_what_they_cannot_do():
     assert lin(odd, None, 64, p, p, None, p, 16, 2, 64, 16, None) == -3 and lin(p, None, 64, odd, p, None, p, 16, 2, 64, 16, None) == -3
     assert lin(p, None, 68, p, p, None, p, 16, 2, 64, 16, None) == -3
     assert lin(p, None, 64, None, p, None, p, 16, 2, 64, 16, None) == -1 and lin(p, None, 64, p, p, None, None, 16, 2, 64, 16, None) == -1
-    assert lin(p, None, 4096, p, p, None, p, 16, 1 << 20, 4096, 16, None) == -2 and "4 GiB" in _err()
+    assert lin(p, None, 1 << 25, p, p, None, p, 16, 300, 4096, 16, None) == -2 and "4 GiB" in _err()
     r = lib.tllm_moe_route
 
     def route(logits=p, stride=32, groups=1, kept=1, tokens=8, experts=32, top=4, work=None, nbytes=0, offsets=p):
@@ -634,6 +655,7 @@ def test_entry_points_refuse_what_they_cannot_do():
 
     assert mlp1(tokens=0) == 0 and mlp1(tokens=-1) == -1 and mlp1(top=0) == -2 and mlp1(top=5) == -2 and mlp1(hidden=40, stride=40) == -2
     assert mlp1(x=None) == -1 and mlp1(order=None) == -1 and mlp1(w=odd) == -3 and mlp1(x=odd) == -3 and mlp1(h=None) == -1 and mlp1(h_stride=31) == -1
+    assert mlp1(tokens=1 << 20, stride=4096) == -2 and "4 GiB" in _err()
     assert mlp1(stride=32) == -1 and mlp1(limit=-1.0) == -1 and mlp1(tokens=1 << 30) == -2 and mlp1(inner=0) == -2
 
     def mlp2(h=p, weights=p, out=p, out_stride=64, work=p, nbytes=8 * 2 * 64 * 4, tokens=8, experts=4, top=2, inner=32, hidden=64, res=None, res_stride=64):

@@ -57,12 +57,14 @@ static int weight_ok(const char* what, const void* w, const void* ws, int64_t ex
   return TLLM_OK;
 }
 
-// The last byte of x has a 32-bit offset.
-static int rows_ok(const char* what, const void* x, int64_t rows, int64_t pitch, int64_t row_bytes) {
+// Bytes of x have 32-bit offsets: from its beginning where rows are gathered, from a tile's first row (of 128 at most) otherwise.
+static int rows_ok(const char* what, const void* x, int64_t rows, int64_t pitch, int64_t row_bytes, bool gathered) {
   TLLM_REQUIRE(x, TLLM_E_ARG, "%s: null pointer", what);
   TLLM_REQUIRE(rows == 1 || pitch >= row_bytes, TLLM_E_ARG, "%s: rows of %lld bytes, %lld apart", what, (long long)row_bytes, (long long)pitch);
   TLLM_REQUIRE(aligned16(x) && (rows == 1 || pitch % 16 == 0), TLLM_E_ALIGN, "%s: rows of x must be 16-byte aligned", what);
-  TLLM_REQUIRE((rows - 1) <= (int64_t)(MX_NONE - row_bytes) / (pitch > 0 ? pitch : 1), TLLM_E_SHAPE, "%s: x spans 4 GiB or more", what);
+  const int64_t together = gathered || rows < 128 ? rows : 128;
+  TLLM_REQUIRE(together - 1 <= (int64_t)(MX_NONE - row_bytes) / (pitch > 0 ? pitch : 1), TLLM_E_SHAPE, "%s: %lld rows of x span 4 GiB or more", what,
+               (long long)together);
   return TLLM_OK;
 }
 
@@ -82,7 +84,7 @@ extern "C" int tllm_mxfp4_linear_bf16(const void* x, const void* x_scales, int64
   if (rows == 0) return TLLM_OK;
   TLLM_TRY(weight_ok("mxfp4_linear", w_blocks, w_scales, 1, in_dim, out_dim));
   const int64_t row_bytes = x_scales ? in_dim / 2 : in_dim * 2, pitch = x_scales ? row_bytes : x_row_stride * 2;
-  TLLM_TRY(rows_ok("mxfp4_linear", x, rows, pitch, row_bytes));
+  TLLM_TRY(rows_ok("mxfp4_linear", x, rows, pitch, row_bytes, false));
   TLLM_REQUIRE(out, TLLM_E_ARG, "mxfp4_linear: null pointer");
   TLLM_REQUIRE(aligned16(x_scales), TLLM_E_ALIGN, "mxfp4_linear: x_scales must be 16-byte aligned");
   TLLM_REQUIRE(rows == 1 || out_row_stride >= out_dim, TLLM_E_ARG, "mxfp4_linear: out_row_stride %lld < %lld", (long long)out_row_stride, (long long)out_dim);
@@ -102,12 +104,12 @@ extern "C" int tllm_mxfp4_linear_bf16(const void* x, const void* x_scales, int64
   return product(a, kMxLinear, x_scales != nullptr, static_cast<hipStream_t>(stream));
 }
 
-static int experts_args(const char* what, MxArgs* a, const void* x, int64_t x_row_stride, int64_t x_rows, const int32_t* order, const int32_t* offsets,
+static int experts_args(const char* what, MxArgs* a, bool gathered, const void* x, int64_t x_row_stride, int64_t x_rows, const int32_t* order, const int32_t* offsets,
                         const void* w_blocks, const void* w_scales, const void* bias, int64_t tokens, int n_experts, int top, int64_t k, int64_t n) {
   TLLM_REQUIRE(top >= 1 && n_experts >= top, TLLM_E_SHAPE, "%s: top %d of %d experts", what, top, n_experts);
   TLLM_REQUIRE(tokens * top < (1ll << 31), TLLM_E_SHAPE, "%s: %lld tokens x %d are too many", what, (long long)tokens, top);
   TLLM_TRY(weight_ok(what, w_blocks, w_scales, n_experts, k, n));
-  TLLM_TRY(rows_ok(what, x, x_rows, x_row_stride * 2, k * 2));
+  TLLM_TRY(rows_ok(what, x, x_rows, x_row_stride * 2, k * 2, gathered));
   TLLM_REQUIRE(order && offsets, TLLM_E_ARG, "%s: null pointer", what);
   a->x = x;
   a->x_pitch = x_row_stride * 2;
@@ -131,7 +133,7 @@ extern "C" int tllm_moe_mlp1_bf16(const void* x, int64_t x_row_stride, const int
   TLLM_REQUIRE(tokens >= 0, TLLM_E_ARG, "moe_mlp1: tokens %lld", (long long)tokens);
   if (tokens == 0) return TLLM_OK;
   MxArgs a{};
-  TLLM_TRY(experts_args("moe_mlp1", &a, x, x_row_stride, tokens, order, offsets, w_blocks, w_scales, bias, tokens, n_experts, top, hidden, 2 * inner));
+  TLLM_TRY(experts_args("moe_mlp1", &a, true, x, x_row_stride, tokens, order, offsets, w_blocks, w_scales, bias, tokens, n_experts, top, hidden, 2 * inner));
   TLLM_REQUIRE(h && h_row_stride >= inner, TLLM_E_ARG, "moe_mlp1: null pointer, or h_row_stride %lld < %lld", (long long)h_row_stride, (long long)inner);
   TLLM_REQUIRE(!has_limit || limit >= 0.f, TLLM_E_ARG, "moe_mlp1: limit %g", (double)limit);
   a.out = h;
@@ -149,7 +151,7 @@ extern "C" int tllm_moe_mlp2_bf16(const void* h, int64_t h_row_stride, const int
   TLLM_REQUIRE(tokens >= 0, TLLM_E_ARG, "moe_mlp2: tokens %lld", (long long)tokens);
   if (tokens == 0) return TLLM_OK;
   MxArgs a{};
-  TLLM_TRY(experts_args("moe_mlp2", &a, h, h_row_stride, tokens * top, order, offsets, w_blocks, w_scales, bias, tokens, n_experts, top, inner, hidden));
+  TLLM_TRY(experts_args("moe_mlp2", &a, false, h, h_row_stride, tokens * top, order, offsets, w_blocks, w_scales, bias, tokens, n_experts, top, inner, hidden));
   TLLM_REQUIRE(weights && out, TLLM_E_ARG, "moe_mlp2: null pointer");
   TLLM_REQUIRE(tokens == 1 || (out_row_stride >= hidden && (!residual || res_row_stride >= hidden)), TLLM_E_ARG, "moe_mlp2: rows of %lld values, %lld (residual %lld) apart",
                (long long)hidden, (long long)out_row_stride, (long long)res_row_stride);
