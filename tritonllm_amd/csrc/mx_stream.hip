@@ -8,8 +8,8 @@
 // LDS, added in a fixed order). Weights and activations go straight to LDS, U steps of a wavefront at a time in a ring that is its
 // alone, so that nothing but the wavefront's own count of arrivals is waited for. That path is what the addresses ask for: a
 // 16-byte load is one access of the cache for four neighbouring lanes with 64 neighbouring bytes and one for each lane otherwise, and a
-// matrix operand has its rows in neighbouring lanes (33 tokens, loaded to registers that way: 24.2 million accesses, 63.8 us; 7.8
-// million and 59.5 now).
+// matrix operand has its rows in neighbouring lanes (33 tokens, loaded to registers that way: 24.2 million accesses, 63.8 us; this
+// way, with 32 weight rows as there, 7.8 million and 59.5).
 //
 // In a step lane (m, g) of a fragment has block mx_quarter(g) of weight row m, and the four v_mfma_f32_16x16x32_bf16 take 8 of its 32
 // values each, from both operands. The codes become bf16 on the way, exactly, once per step for all rows; a lane reads its block's scale
@@ -46,7 +46,7 @@ __device__ __forceinline__ void wait_steps_left(int left) {  // at most `left` (
 // RP, piece c / RP), with up to 4 all four. The products with a piece's weights are then good in that piece's columns and nonsense in
 // the others, so each piece has its own sums, of which only those columns are kept: fewer reads for the same products.
 // In LDS a row's sixteens are XORed so that the lanes that a read serves together (mx_quarter) are in different banks.
-// `row_at(r)`: where row r begins in x. `ready`: called when the first loads are on their way.
+// `row_at(RP, r)`: where row r, of up to RP, begins in x. `ready`: called when the first loads are on their way.
 template <int NT, int RP, int NW, int U, class Row, class F>
 __device__ __forceinline__ void mx_walk(const MxWalk& m, float* sums, int sums_pitch, Row&& row_at, F&& ready) {
   constexpr int C = 16 / RP, X = 4 / C, XI = RP / 4, LOADS = NT + XI, SLOT = LOADS * 1024;
@@ -61,7 +61,7 @@ __device__ __forceinline__ void mx_walk(const MxWalk& m, float* sums, int sums_p
 #pragma unroll
   for (int j = 0; j < XI; ++j) {
     const int row = 4 * j + (lane >> 4), c = (lane & 15) ^ fold(row);
-    xo[j] = row_at(row);
+    xo[j] = row_at(std::integral_constant<int, RP>{}, row);
     xb[j] = c >> 2;
     if (xo[j] != MX_NONE) xo[j] += 16 * c;
   }
@@ -213,14 +213,15 @@ __global__ __launch_bounds__(NW * 64) void mx_stream_kernel(MxArgs a, int tiles_
   constexpr bool gather = MODE == kMxSwiglu;
   const ScalarInts order = mx_scalar(a.order) + it.first;
   const unsigned last_pair = static_cast<unsigned>(a.rows - 1);
-  auto row_of = [&](int r) {                                // row r of the item in x; r differs from lane to lane
+  auto row_of = [&](auto most, int r) {                     // row r of the item in x; r differs from lane to lane
+    constexpr int RP = decltype(most)::value;
     if (!gather) return static_cast<unsigned>(r);
-    unsigned pair = 0;
-    for (int j = 0; j < it.rows; ++j) {
-      const unsigned p = min(static_cast<unsigned>(order[j]), last_pair);
-      pair = r == j ? p : pair;
-    }
-    return pair / static_cast<unsigned>(a.top);
+    unsigned pair[RP], mine = 0;                            // (all asked for together)
+#pragma unroll
+    for (int j = 0; j < RP; ++j) pair[j] = static_cast<unsigned>(order[min(j, it.rows - 1)]);
+#pragma unroll
+    for (int j = 0; j < RP; ++j) mine = r == j ? pair[j] : mine;
+    return min(mine, last_pair) / static_cast<unsigned>(a.top);
   };
   const int row_bytes = A4 ? blocks * 16 : a.k * 2;
   const unsigned char* const xb = static_cast<const unsigned char*>(a.x) + (gather ? 0 : it.first * a.x_pitch);
@@ -255,8 +256,8 @@ __global__ __launch_bounds__(NW * 64) void mx_stream_kernel(MxArgs a, int tiles_
     m.x_scales = mx_buffer(a.x_scales + static_cast<int64_t>(it.first) * blocks, it.rows * blocks);
     mx_walk4<NT, NW, U4>(m, w, x, m16 < it.rows ? static_cast<unsigned>(m16 * a.x_pitch) : MX_NONE, m16 * blocks, mine, PITCH, ready);
   } else {
-    auto row_at = [&](int r) {
-      const unsigned row = row_of(r);
+    auto row_at = [&](auto most, int r) {
+      const unsigned row = row_of(most, r);
       return r < it.rows ? static_cast<unsigned>(row * a.x_pitch) : MX_NONE;
     };
     if (columns == 4) mx_walk<NT, 4, NW, U4>(m, mine, PITCH, row_at, ready);
@@ -315,15 +316,18 @@ static int launch(const MxArgs& a, hipStream_t st) {
 }
 
 // The workgroup. Wide ones (64 weight rows) read the activations less often and pay where items are full: 128 tokens of 32 experts
-// mlp1 107 us with 32 rows, 96 with 64 (33 tokens 59.5 and 63), 65 rows of [5120, 2880] 11.7 and 9.0. Narrow ones, with their K
-// share in one piece, where the launch would have less than one for every other CU otherwise: one row of [2880, 4096] 6.9 us with 32
-// weight rows, 4.7 with 16; 64 rows of [1024, 1024] 5.8 with 64, 4.4 with 32. Few steps in the rings: workgroups on the CU bring
-// more than a longer ring does (33 tokens 59.5 us with rings of 6 KB, 59.8 with 9, 64 with 12, 78 with 18).
+// mlp1 97.7 us with 32 rows, 89.5 with 64; 33 tokens, four pairs an expert, 58.4 and 57.6, 24 tokens 53.0 and 54.0; mlp2, half as many
+// weight rows, 64 tokens 43.7 and 43.6, 33 34.9 and 36.2; 16 rows of [32768, 2880] 13.2 and 12.1, 8 rows 11.6 and 11.7. And where
+// there are enough of them: 33 rows of [8192, 2880], 384 workgroups, 8.0 and 9.3; 65 rows of [5120, 2880], 400, 9.2 and 8.8. Narrow
+// ones, with their K share in one piece, where the launch would have less than one for every other CU otherwise: one row of
+// [2880, 4096] 6.9 us with 32 weight rows, 4.7 with 16; 64 rows of [1024, 1024] 5.8 with 64, 4.4 with 32. Few steps in the rings:
+// workgroups on the CU bring more than a longer ring does (33 tokens 59.5 us with rings of 6 KB, 59.8 with 9, 64 with 12, 78 with 18,
+// before a row's pairs were asked for together).
 template <int MODE>
 static int launch_bf16(const MxArgs& a, hipStream_t st) {
   const int64_t items = a.order ? (a.rows < a.experts ? a.rows : a.experts) + a.rows / 32 : (a.rows + 15) / 16;
-  const bool full = a.rows > 12ll * a.experts;
-  if (full && (a.n + 63) / 64 * items >= 256 && a.k <= 16384) return launch<4, false, MODE, 4, 1, 1, 1>(a, st);
+  const bool full = a.rows > (MODE == kMxSwiglu ? 4ll : MODE == kMxPairs ? 8ll : 12ll) * a.experts;
+  if (full && (a.n + 63) / 64 * items > 384 && a.k <= 16384) return launch<4, false, MODE, 4, 1, 1, 1>(a, st);
   if ((a.n + 31) / 32 * items > 128 && a.k <= 32768) return launch<2, false, MODE, 4, 2, 1, 1>(a, st);
   return launch<1, false, MODE, 8, 3, 2, 1>(a, st);
 }

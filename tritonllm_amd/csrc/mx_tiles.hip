@@ -210,7 +210,7 @@ static int tiles_of(const MxArgs& a, hipStream_t st) {
 }
 
 // Whether a product of these sizes is the tiles'. Below, the weight stream is ahead: 130 rows of [5120, 2880] 17.1 us, 18.7 in tiles
-// (300 29.8 and 22.9); experts of 32 and of 16 rows each on average mlp1 122 in tiles and 107 as a stream, 111.
+// (300 29.8 and 22.9); 32 experts of 24 rows each on average mlp1 115.7 in tiles and 108.0 as a stream, of 32 rows 122.0 and 128.3.
 bool mx_tiles_take(const MxArgs& a) {
   return a.rows > (a.order ? 24ll : 200ll) * a.experts && tile_lds<Small>(a.k) <= 160 * 1024;
 }
