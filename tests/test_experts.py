@@ -203,7 +203,8 @@ def test_linear_special_values(rows, acts):
 
 
 @gpu
-@pytest.mark.parametrize("rows,n,k", [(2048, 4096, 1024), (2048, 5120, 1024), (1000, 2880, 2048), (700, 2880, 5120), (2048, 5120, 2880), (129, 200, 2880)])
+@pytest.mark.parametrize("rows,n,k", [(2048, 4096, 1024), (2048, 5120, 1024), (1000, 2880, 2048), (700, 2880, 5120), (2048, 5120, 2880), (129, 200, 2880),
+                                      (520, 5001, 2880), (330, 8000, 96), (3000, 1100, 160)])
 @pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
 def test_linear_of_prompts(rows, n, k, acts):
     """The larger tiles; the reference is a float64 product on the GPU."""

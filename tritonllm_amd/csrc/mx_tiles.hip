@@ -195,22 +195,31 @@ static int launch_tiles(const MxArgs& a, hipStream_t st) {
 
 typedef MxTileShape<4, 4, 2, 2, 2> Tall;          // 128 x 128, four wavefronts of 64 x 64, three workgroups to a CU
 typedef MxTileShape<4, 2, 1, 8, 3> Wide;          // 64 x 256, eight of 64 x 32, two to a CU
+typedef MxTileShape<4, 2, 1, 4, 2> Middle;        // 64 x 128, four of 64 x 32, four to a CU
 typedef MxTileShape<2, 2, 1, 4, 3> Small;         // 32 x 128
 
 // Tall tiles where an expert's rows fill them: 2048 tokens of 32 experts, 256 rows each, mlp1 315 us (wide ones 349), 512 tokens 168 (149);
 // 2048 rows of [5120, 2880] 62.7 (73.0). Small ones where the others would leave CUs without any: 300 rows of [5120, 2880] 30.2 in
-// wide, 22.9 in small ones.
+// wide, 20.6 in small ones. Between tall and small, for one weight, middle ones where a CU gets one and a quarter to three (rows of [5120, 2880]
+// in middle tiles and in what is chosen otherwise: 400, 280 tiles, 25.3 and 24.6; 512, 320, 26.1 and 29.9; 700 26.8 and 39.1; 1000
+// 35.0 and 42.0; 1300, 840, 49.4 and 43.7; 700 of [8192, 2880], 704, 38.2 and 42.4; 2000 of [2880, 4096], 736, 52.5 and 57.2).
+// Experts' rows have no use for them (512 tokens of 32 mlp1 166, wide ones 147; mlp2 110 and 100).
 template <int MODE>
 static int tiles_of(const MxArgs& a, hipStream_t st) {
   auto count = [&](int64_t bm, int64_t bn) { return (a.n + bn - 1) / bn * ((a.rows + bm - 1) / bm + (a.order ? a.experts / 2 : 0)); };
   auto fits = [&](int64_t lds) { return lds <= 160 * 1024; };
+  if constexpr (MODE == kMxLinear) {
+    const int64_t middle = count(64, 128);
+    if (middle >= 320 && middle <= 768 && fits(tile_lds<Middle>(a.k))) return launch_tiles<Middle, MODE>(a, st);
+  }
   if (a.rows > 128ll * a.experts && count(128, 128) >= 256 && fits(tile_lds<Tall>(a.k))) return launch_tiles<Tall, MODE>(a, st);
-  if (count(64, 256) >= 256 && fits(tile_lds<Wide>(a.k))) return launch_tiles<Wide, MODE>(a, st);
+  if constexpr (MODE != kMxLinear)
+    if (count(64, 256) >= 256 && fits(tile_lds<Wide>(a.k))) return launch_tiles<Wide, MODE>(a, st);
   return launch_tiles<Small, MODE>(a, st);
 }
 
 // Whether a product of these sizes is the tiles'. Below, the weight stream is ahead: 130 rows of [5120, 2880] 17.1 us, 18.7 in tiles
-// (300 29.8 and 22.9); 32 experts of 24 rows each on average mlp1 115.7 in tiles and 108.0 as a stream, of 32 rows 122.0 and 128.3.
+// (300 29.8 and 20.6); 32 experts of 24 rows each on average mlp1 115.7 in tiles and 108.0 as a stream, of 32 rows 122.0 and 128.3.
 bool mx_tiles_take(const MxArgs& a) {
   return a.rows > (a.order ? 24ll : 200ll) * a.experts && tile_lds<Small>(a.k) <= 160 * 1024;
 }
