@@ -682,6 +682,27 @@ def test_ops_refuse_cpu_tensors():
             op(x, routing, u8[None], u8[None, ..., 0])
 
 
+def test_linear_operands_with_a_bias_of_another_length_are_refused():
+    """The kernels read a bias value for each row of the weight: one that is shorter would be read beyond its end."""
+    x, w = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(32, 64, dtype=torch.bfloat16)
+    for n in (0, 1, 31, 33):
+        with pytest.raises(AssertionError, match=f"{n} values for 32"):
+            T.ops._prep_linear(x, w, torch.zeros(n, dtype=torch.bfloat16))
+    T.ops._prep_linear(x, w, torch.zeros(32, dtype=torch.bfloat16))
+    T.ops._prep_linear(x, w, None)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [1, 65])
+@pytest.mark.parametrize("experts", [32, 10])
+def test_router_logits_refuses_a_bias_of_another_length(tokens, experts):
+    x, w = torch.zeros(tokens, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(experts, 64, dtype=torch.bfloat16, device="cuda")
+    for n in (1, experts - 1, experts + 1):
+        for op in (T.router_logits, T.linear_qkv_forward):
+            with pytest.raises(AssertionError, match="bias"):
+                op(x, w, torch.zeros(n, dtype=torch.bfloat16, device="cuda"))
+
+
 @gpu
 def test_ops_refuse_wrong_types_and_shapes():
     c = dict(device="cuda")

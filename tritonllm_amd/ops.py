@@ -341,6 +341,8 @@ def _prep_weight_scale(weight, weight_scale):
 
 def _prep_linear(hidden2, weight, bias):
     _require(hidden2.dtype == _BF16 and weight.dtype in (_BF16, _FP8) and (bias is None or bias.dtype == _BF16))
+    # (the kernels read one for each row of the weight; they do not broadcast)
+    _require(bias is None or bias.numel() == weight.shape[0], f"the bias holds {0 if bias is None else bias.numel()} values for {weight.shape[0]} outputs")
     if not hidden2.is_contiguous():
         hidden2 = hidden2.contiguous()
     if not weight.is_contiguous():
