@@ -598,6 +598,38 @@ def test_ops_on_two_streams():
 
 
 @gpu
+@pytest.mark.parametrize("tokens", [2, 70])
+def test_mlp_block_of_a_borrowed_buffer(tokens):
+    """The rows that a norm has lent out are rows as others: the block's own norm leaves them alone, and the residual is theirs."""
+    m, before = mlp_block(), T.RMSNorm(192, device="cuda")
+    rows = torch.randn(tokens, 192, generator=torch.Generator().manual_seed(tokens)).bfloat16().cuda()
+    for shape in ((tokens, 192), (1, tokens, 192)):
+        x = before(rows.view(shape))                               # (the pool's buffer of this shape)
+        kept = x.clone()
+        want = m(kept)
+        assert torch.equal(m(x), want) and torch.equal(x, kept)
+    wide = torch.cat([rows, rows], 1)[:, 3:195]                    # rows that lie apart
+    assert torch.equal(m(wide), m(wide.contiguous()))
+
+
+@gpu
+def test_mlp_blocks_on_two_streams():
+    """Two blocks of one shape, each on its stream at the same time, give what they give alone."""
+    ms = [mlp_block(seed=i) for i in range(2)]
+    xs = [torch.randn(200, 192, generator=torch.Generator().manual_seed(i)).bfloat16().cuda() for i in range(2)]
+    want = [m(x) for m, x in zip(ms, xs)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in ms], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ms[i](xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@gpu
 def test_mlp_block_from_a_checkpoint(tmp_path):
     from safetensors.torch import save_file
 

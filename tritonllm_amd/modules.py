@@ -263,7 +263,8 @@ class MLPBlock(torch.nn.Module):
     @torch.no_grad()
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """``x [..., hidden]`` bf16 -> ``x + the experts' answer`` of the same shape."""
-        t = self.norm(x).view(-1, x.shape[-1])
+        # (a buffer of the call's own: it lives across three launches, and the pool's may be x itself or another stream's)
+        t = self.norm(x, out=torch.empty_like(x, memory_format=torch.contiguous_format)).view(-1, x.shape[-1])
         routing = ops.moe_route(ops.router_logits(t, self.gate.weight, self.gate.bias), self.experts_per_token)
         h = ops.moe_mlp1(t, routing, self.mlp1_blocks, self.mlp1_scales, self.mlp1_bias, limit=self.swiglu_limit)
         return ops.moe_mlp2(h, routing, self.mlp2_blocks, self.mlp2_scales, self.mlp2_bias, residual=x)
