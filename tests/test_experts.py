@@ -736,6 +736,25 @@ def test_router_logits_refuses_a_bias_of_another_length(tokens, experts):
 
 
 @gpu
+def test_products_over_rows_of_no_values_are_refused():
+    """K = 0, with both types of activations; without rows or without outputs there is nothing to compute."""
+    u8 = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device="cuda")
+    bf = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+    for lead in ((3,), (2, 5), ()):
+        for bias in (None, bf(6)):
+            with pytest.raises(RuntimeError, match="whole blocks"):
+                T.mxfp4_linear(u8(*lead, 0, 16), u8(6, 0, 16), u8(6, 0), bias, x_scales=u8(*lead, 0))
+    with pytest.raises(RuntimeError, match="whole blocks"):
+        T.mxfp4_linear(bf(3, 0), u8(6, 0, 16), u8(6, 0))
+    assert T.mxfp4_linear(u8(0, 2, 16), u8(6, 2, 16), u8(6, 2), x_scales=u8(0, 2)).shape == (0, 6)
+    assert T.mxfp4_linear(u8(4, 2, 16), u8(0, 2, 16), u8(0, 2), x_scales=u8(4, 2)).shape == (4, 0)
+    routing = T.moe_route(torch.zeros(2, 3, device="cuda"), 1)
+    for op in (T.moe_mlp1, T.moe_mlp2):
+        with pytest.raises(RuntimeError, match="whole blocks"):
+            op(bf(2, 0), routing, u8(3, 4, 0, 16), u8(3, 4, 0))
+
+
+@gpu
 def test_ops_refuse_wrong_types_and_shapes():
     c = dict(device="cuda")
     x, w, ws = torch.zeros(2, 64, dtype=torch.bfloat16, **c), torch.zeros(6, 2, 16, dtype=torch.uint8, **c), torch.zeros(6, 2, dtype=torch.uint8, **c)

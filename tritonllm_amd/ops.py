@@ -886,7 +886,7 @@ def mxfp4_linear(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bi
         _require(x.dtype == torch.uint8 and x_scales.dtype == torch.uint8 and x.shape == (*x_scales.shape, 16), "x: MXFP4 blocks of 16 bytes with a scale each")
         _require(x_scales.ndim >= 1 and x_scales.shape[-1] == g, f"x has {x_scales.shape[-1]} blocks in a row, the weight {g}")
         lead, x2, x_scales = x_scales.shape[:-1], _aligned(x), _aligned(x_scales)
-        rows, stride = x_scales.numel() // g if g else 0, 0
+        rows, stride = math.prod(lead), 0
     else:
         _require(x.dtype == _BF16 and x.ndim >= 1 and x.shape[-1] == 32 * g, f"x must be bfloat16 with {32 * g} values in a row")
         lead, x2 = x.shape[:-1], _rows16(x)
