@@ -507,6 +507,58 @@ def test_experts_nan_stays_with_its_token():
     assert y[7].isnan().all() and y.isnan().any(1).sum() == 1
 
 
+def whole_case(g, n, k, *lead):
+    """Weights of [..., n, k] that are multiples of a quarter, and rows' worth of them times -1, 0 and 1 exact in fp32 in any order
+    (below 12 * 2^18, a multiple of 2^-2)."""
+    return random_mx(g, *lead, n, k, lo=126, hi=129)
+
+
+LONG = [229344, 229376, 262144]                                    # (whole blocks, the last an odd number of steps' worth; the longest rows)
+
+
+@gpu
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("rows,n", [(1, 17), (5, 16), (17, 40), (220, 9)])
+@pytest.mark.parametrize("k", LONG)
+def test_linear_of_the_longest_rows(k, rows, n, acts):
+    """All sums are exact: the result is the exact one, rounded once."""
+    g = torch.Generator().manual_seed(k + rows)
+    w, ws = whole_case(g, n, k)
+    b = torch.randint(-9, 10, (n,), generator=g).bfloat16()
+    x = torch.randint(-1, 2, (rows, k), generator=g).bfloat16().cuda()
+    want = (x.double() @ values(w, ws).cuda().t() + b.cuda().double()).float().bfloat16()
+    if acts == "mxfp4":
+        x, xs = T.mxfp4_quantize(x)
+        assert torch.equal(T.mxfp4_linear(x, *cuda(w, ws, b), x_scales=xs), want)
+    else:
+        assert torch.equal(T.mxfp4_linear(x, *cuda(w, ws, b)), want)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [1, 21, 120])
+@pytest.mark.parametrize("k", LONG)
+def test_experts_of_the_longest_rows(k, tokens):
+    g = torch.Generator().manual_seed(k + tokens)
+    chosen = torch.randint(0, 3, (tokens, 1), generator=g).int()
+    chosen = torch.cat([chosen, (chosen + 1) % 3], 1)
+    routing = T.MoeRouting(chosen, torch.full((tokens, 2), 0.5), *plan_of(chosen, 3))
+    dr = T.MoeRouting(*cuda(*routing))
+    w, ws = whole_case(g, 10, k, 3)
+    b = torch.randint(-9, 10, (3, 10), generator=g).bfloat16()
+    wv = values(w, ws).cuda()
+    x = torch.randint(-1, 2, (tokens, k), generator=g).bfloat16().cuda()
+    y = torch.einsum("tk,enk->ten", x.double(), wv) + b.cuda().double()
+    pair = y.gather(1, chosen.cuda().long()[..., None].expand(-1, -1, 10))           # [tokens, 2, 10]
+    rows = pair.reshape(-1, 10)[routing.order.cuda().long()]
+    want = rows[:, 0::2] * torch.sigmoid(ALPHA * rows[:, 0::2]) * (rows[:, 1::2] + 1)
+    got = T.moe_mlp1(x, dr, *cuda(w, ws, b), alpha=ALPHA, limit=None).double()
+    assert ((got - want).abs() <= (2.0**-8 + 1e-5) * want.abs() + 1e-30).all()
+    h = x.repeat_interleave(2, 0)[routing.order.cuda().long()]
+    res = torch.randint(-9, 10, (tokens, 10), generator=g).bfloat16().cuda()
+    want = (0.5 * (pair[:, 0] + pair[:, 1]) + res.double()).float().bfloat16()
+    assert torch.equal(T.moe_mlp2(h, dr, *cuda(w, ws, b), residual=res), want)
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------------
 def mlp_block(hidden=192, inner=160, experts=16, top=4, seed=0):
     g = torch.Generator().manual_seed(seed)
@@ -698,6 +750,14 @@ def test_entry_points_refuse_what_they_cannot_do():
     assert mlp2(tokens=0) == 0 and mlp2(tokens=-1) == -1 and mlp2(h=None) == -1 and mlp2(weights=None) == -1 and mlp2(out=None) == -1
     assert mlp2(out_stride=63) == -1 and mlp2(res=p, res_stride=63) == -1 and mlp2(inner=33) == -2
     assert lib.tllm_moe_mlp2_workspace_bytes(300, 2, 64) > 16 and mlp2(tokens=300, nbytes=16) == -1 and "workspace" in _err()
+
+
+def test_rows_beyond_the_longest_are_refused():
+    lib, p = _lib.lib(), C.c_void_p(4096)
+    k = (1 << 18) + 32
+    assert lib.tllm_mxfp4_linear_bf16(p, None, k, p, p, None, p, 16, 2, k, 16, None) == -2 and "too large" in _err()
+    assert lib.tllm_mxfp4_linear_bf16(p, p, 0, p, p, None, p, 16, 2, k, 16, None) == -2 and "too large" in _err()
+    assert lib.tllm_moe_mlp1_bf16(p, k, p, p, p, p, None, p, 32, 8, 4, 2, k, 32, 1.702, 7.0, 1, None) == -2 and "too large" in _err()
 
 
 def test_ops_refuse_cpu_tensors():

@@ -322,13 +322,15 @@ static int launch(const MxArgs& a, hipStream_t st) {
 // ones, with their K share in one piece, where the launch would have less than one for every other CU otherwise: one row of
 // [2880, 4096] 6.9 us with 32 weight rows, 4.7 with 16; 64 rows of [1024, 1024] 5.8 with 64, 4.4 with 32. Few steps in the rings:
 // workgroups on the CU bring more than a longer ring does (33 tokens 59.5 us with rings of 6 KB, 59.8 with 9, 64 with 12, 78 with 18,
-// before a row's pairs were asked for together).
+// before a row's pairs were asked for together). Beyond 229344 values a row the scale bytes of sixteen weight rows, 112 KB and up to 129, leave
+// eight wavefronts' rings (48 KB) no room, four's do: one row of [4096, 229376] 136 us, of [4096, 229344] in eight 99.
 template <int MODE>
 static int launch_bf16(const MxArgs& a, hipStream_t st) {
   const int64_t items = a.order ? (a.rows < a.experts ? a.rows : a.experts) + a.rows / 32 : (a.rows + 15) / 16;
   const bool full = a.rows > (MODE == kMxSwiglu ? 4ll : MODE == kMxPairs ? 8ll : 12ll) * a.experts;
   if (full && (a.n + 63) / 64 * items > 384 && a.k <= 16384) return launch<4, false, MODE, 4, 1, 1, 1>(a, st);
   if ((a.n + 31) / 32 * items > 128 && a.k <= 32768) return launch<2, false, MODE, 4, 2, 1, 1>(a, st);
+  if (stream_lds<1, false, 8, 3, 2, 1>(a.k / 32) > 160 * 1024) return launch<1, false, MODE, 4, 3, 2, 1>(a, st);
   return launch<1, false, MODE, 8, 3, 2, 1>(a, st);
 }
 
