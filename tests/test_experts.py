@@ -559,6 +559,34 @@ def test_experts_of_the_longest_rows(k, tokens):
     assert torch.equal(T.moe_mlp2(h, dr, *cuda(w, ws, b), residual=res), want)
 
 
+@gpu
+@pytest.mark.parametrize("tokens", [1, 9, 64, 65, 449])
+@pytest.mark.parametrize("experts", [1, 5, 10, 16, 17, 32, 33, 48, 128])
+@pytest.mark.parametrize("hidden", [96, 192, 2880])
+def test_router_logits(tokens, experts, hidden):
+    """Any number of experts, of any tokens."""
+    g = torch.Generator().manual_seed(tokens + experts + hidden)
+    x, w, b = torch.randn(tokens, hidden, generator=g).bfloat16(), torch.randn(experts, hidden, generator=g).bfloat16(), torch.randn(experts, generator=g).bfloat16()
+    want, mag = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+    dx, dw, db = cuda(x, w, b)
+    check_product(T.router_logits(dx, dw, None), want, mag, hidden)
+    check_product(T.router_logits(dx, dw, db), want + b.double(), mag + b.double().abs(), hidden)
+    apart = torch.cat([x, x], 1)[:, hidden // 2 + 1: hidden // 2 + 1 + hidden]        # rows of a wider matrix, at any address
+    v = apart.double()
+    check_product(T.router_logits(torch.cat([dx, dx], 1)[:, hidden // 2 + 1: hidden // 2 + 1 + hidden], dw, db), v @ w.double().t() + b.double(),
+                  v.abs() @ w.double().abs().t() + b.double().abs(), hidden)
+
+
+@gpu
+@pytest.mark.parametrize("hidden", [32, 33])
+def test_router_logits_of_an_odd_number_for_many_tokens(hidden):
+    tokens = 65535 + 70
+    g = torch.Generator().manual_seed(hidden)
+    x, w, b = torch.randn(tokens, hidden, generator=g).bfloat16(), torch.randn(3, hidden, generator=g).bfloat16(), torch.randn(3, generator=g).bfloat16()
+    want, mag = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t() + b.double().abs()
+    check_product(T.router_logits(*cuda(x, w, b)), want, mag, hidden)
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------------
 def mlp_block(hidden=192, inner=160, experts=16, top=4, seed=0):
     g = torch.Generator().manual_seed(seed)
@@ -606,6 +634,17 @@ def test_mlp_block(tokens, experts):
     # a place of bf16 in t, the logits and h each, and in the result: the kernels' tolerance here is twice the reference model's rounding
     torch.testing.assert_close(got.double().cpu()[sure], want[sure], rtol=2e-2, atol=2e-2)
     assert torch.equal(m(x.cuda().view(1, tokens, 192)).view(tokens, 192), got)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [6, 130])
+@pytest.mark.parametrize("experts,top", [(17, 3), (5, 4)])
+def test_mlp_block_of_an_odd_number_of_experts(tokens, experts, top):
+    m = mlp_block(experts=experts, top=top)
+    x = torch.randn(tokens, 192, generator=torch.Generator().manual_seed(tokens)).bfloat16()
+    want, sure = block_ref(m, x)
+    assert sure.double().mean() > 0.5
+    torch.testing.assert_close(m(x.cuda()).double().cpu()[sure], want[sure], rtol=2e-2, atol=2e-2)
 
 
 @gpu

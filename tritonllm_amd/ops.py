@@ -901,21 +901,27 @@ def mxfp4_linear(x: torch.Tensor, blocks: torch.Tensor, scales: torch.Tensor, bi
 
 def router_logits(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
     """The router's gate, ``F.linear(x, weight, bias)`` of ``x [tokens, hidden]`` with ``weight [experts, hidden]`` (model.py:751-757): few
-    outputs, as heads of sixteen through the general decode projection or, beyond its rows, a GEMM tile."""
+    outputs, as heads of sixteen through the general decode projection or, beyond its rows, a GEMM tile. Pairs of outputs that are not
+    sixteens go through the QKV projection, odd numbers of them through the out-projection, whose outputs may be any number."""
     _on_gpu(x, weight, bias)
     experts, hidden = weight.shape
     _require(x.ndim == 2 and x.shape[1] == hidden and x.dtype == _BF16 and weight.dtype == _BF16, "router_logits: bfloat16 [tokens, hidden] and [experts, hidden]")
-    if experts % 16 or hidden % 64:
+    if experts % 2 == 0 and (experts % 16 or hidden % 64):
         return linear_qkv_forward(x, weight, bias)
     x, weight, bias = _prep_linear(x, weight, bias)
-    out = torch.empty((x.shape[0], experts), dtype=_BF16, device=x.device)
-    if x.shape[0] == 0:
+    rows = x.shape[0]
+    out = torch.empty((rows, experts), dtype=_BF16, device=x.device)
+    if rows == 0:
         return out
-    if x.shape[0] <= DECODE_MAX_ROWS:
+    b = bias.data_ptr() if bias is not None else None
+    if experts % 2:
+        for r in range(0, rows, 65535):                    # (what its kernel for any operands takes at once)
+            check(lib().tllm_out_residual_decode_bf16(x[r].data_ptr(), weight.data_ptr(), None, b, None, out[r].data_ptr(), experts, experts,
+                                                      min(rows - r, 65535), hidden, experts, _stream()), "router_logits")
+    elif rows <= DECODE_MAX_ROWS:
         _launch_qkv("decode", x, weight, bias, out, None, None, experts, 0, 0, 0, experts // 16, 0, 16, None)
     else:
-        check(lib().tllm_linear_bf16(x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None, out.data_ptr(), experts, x.shape[0],
-                                     hidden, experts, _stream()), "router_logits")
+        check(lib().tllm_linear_bf16(x.data_ptr(), weight.data_ptr(), b, out.data_ptr(), experts, rows, hidden, experts, _stream()), "router_logits")
     return out
 
 
