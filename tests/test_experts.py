@@ -578,6 +578,15 @@ def test_router_logits(tokens, experts, hidden):
 
 
 @gpu
+@pytest.mark.parametrize("experts", [10, 16, 17])
+def test_mlp_block_of_no_tokens(experts):
+    m = mlp_block(experts=experts)
+    x = torch.empty(0, 192, dtype=torch.bfloat16, device="cuda")
+    assert T.router_logits(x, m.gate.weight, m.gate.bias).shape == (0, experts)
+    assert m(x).shape == (0, 192) and m(x.view(2, 0, 192)).shape == (2, 0, 192)
+
+
+@gpu
 @pytest.mark.parametrize("hidden", [32, 33])
 def test_router_logits_of_an_odd_number_for_many_tokens(hidden):
     tokens = 65535 + 70

@@ -906,10 +906,10 @@ def router_logits(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     _on_gpu(x, weight, bias)
     experts, hidden = weight.shape
     _require(x.ndim == 2 and x.shape[1] == hidden and x.dtype == _BF16 and weight.dtype == _BF16, "router_logits: bfloat16 [tokens, hidden] and [experts, hidden]")
-    if experts % 2 == 0 and (experts % 16 or hidden % 64):
+    rows = x.shape[0]
+    if rows and experts % 2 == 0 and (experts % 16 or hidden % 64):
         return linear_qkv_forward(x, weight, bias)
     x, weight, bias = _prep_linear(x, weight, bias)
-    rows = x.shape[0]
     out = torch.empty((rows, experts), dtype=_BF16, device=x.device)
     if rows == 0:
         return out
