@@ -578,6 +578,23 @@ def test_router_logits(tokens, experts, hidden):
 
 
 @gpu
+@pytest.mark.parametrize("tokens", [3, 70])
+@pytest.mark.parametrize("experts,hidden", [(32, 192), (10, 192), (17, 192), (48, 96)])
+def test_router_logits_of_operands_anywhere(tokens, experts, hidden):
+    """Dense operands whose first value lies at any address."""
+    g = torch.Generator().manual_seed(tokens + experts)
+    ts = [torch.randn(shape, generator=g).bfloat16() for shape in ((tokens, hidden), (experts, hidden), (experts,))]
+    x, w, b = (t.double() for t in ts)
+    want, mag = x @ w.t() + b, x.abs() @ w.abs().t() + b.abs()
+    for off in (1, 4):
+        for which in range(3):
+            d = cuda(*ts)
+            d[which] = torch.zeros(d[which].numel() + off, dtype=torch.bfloat16, device="cuda")[off:].view(d[which].shape).copy_(d[which])
+            assert d[which].is_contiguous() and d[which].data_ptr() % 16
+            check_product(T.router_logits(*d), want, mag, hidden)
+
+
+@gpu
 @pytest.mark.parametrize("experts", [10, 16, 17])
 def test_mlp_block_of_no_tokens(experts):
     m = mlp_block(experts=experts)

@@ -921,6 +921,7 @@ def router_logits(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     elif rows <= DECODE_MAX_ROWS:
         _launch_qkv("decode", x, weight, bias, out, None, None, experts, 0, 0, 0, experts // 16, 0, 16, None)
     else:
+        x, weight = _aligned(x), _aligned(weight)
         check(lib().tllm_linear_bf16(x.data_ptr(), weight.data_ptr(), b, out.data_ptr(), experts, rows, hidden, experts, _stream()), "router_logits")
     return out
 
