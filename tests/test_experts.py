@@ -217,6 +217,75 @@ def test_linear_of_prompts(rows, n, k, acts):
     check_product(T.mxfp4_linear(dx, dw, dws, db, x_scales=dxs), want, mag, k)
 
 
+# Sizes by the kernels that take them, few rows: 16, 32 and 64 weight rows to a workgroup, with 1 - 4, 5 - 8 and up to 16 rows in the last
+# run of rows; and the tiles, with edges in both directions.
+STREAMS = [(16, 100, 352), (23, 90, 736), (40, 1500, 96), (3, 4200, 288), (7, 4130, 224), (12, 4160, 736), (64, 5120, 2880), (20, 9001, 1056), (33, 8200, 96),
+           (190, 2500, 160), (130, 3333, 416), (25, 32770, 64), (22, 16388, 224)]
+TILES = [(1900, 4801, 1312), (1025, 4800, 2880), (2600, 4321, 1120), (2333, 5100, 480)]
+
+
+def linear_on_gpu(x, xs, w, ws, b):
+    """float64 on the GPU: the product, the magnitudes"""
+    v = lambda t, s: values(t, s).cuda()
+    xv, wv = x.double().cuda() if xs is None else v(x, xs), v(w, ws)
+    add = torch.zeros((), dtype=torch.float64) if b is None else b.double()
+    return (xv @ wv.t()).cpu() + add, (xv.abs().nan_to_num(0, 0, 0) @ wv.abs().nan_to_num(0, 0, 0).t()).cpu() + add.abs()
+
+
+@gpu
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("rows,n,k", STREAMS + TILES)
+def test_linear_of_each_kernel(rows, n, k, acts):
+    """NaN blocks of the weight and NaN rows among the others, and rows of a wider matrix."""
+    g = torch.Generator().manual_seed(rows + n + k)
+    (w, ws), b = random_mx(g, n, k), torch.randn(n, generator=g).bfloat16()
+    x, xs = (torch.randn(rows, k, generator=g).bfloat16(), None) if acts == "bf16" else random_mx(g, rows, k, lo=123, hi=128)
+    for i in (0, n // 2, n - 1):
+        ws[i, (i * 5 + k // 32 - 1) % (k // 32)] = 255
+    bad = rows - 1 - rows // 3
+    if acts == "bf16":
+        x[bad, k - 1] = math.nan
+    else:
+        xs[bad, -1] = 255
+    want, mag = linear_on_gpu(x, xs, w, ws, b)
+    assert want[bad].isnan().all() and want.isnan().sum() == n + 3 * rows - 3
+    dx, dxs, dw, dws, db = cuda(x, xs, w, ws, b)
+    got = T.mxfp4_linear(dx, dw, dws, db, x_scales=dxs)
+    check_product(got, want, mag, k)
+    if acts == "bf16":
+        wide = torch.full((rows, k + 24), math.nan, dtype=torch.bfloat16, device="cuda")
+        wide[:, 8: 8 + k] = dx
+        assert torch.equal(T.mxfp4_linear(wide[:, 8: 8 + k], dw, dws, db).view(torch.int16), got.view(torch.int16))
+
+
+@gpu
+@pytest.mark.parametrize("acts", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("rows,n", [(1, 70), (40, 1500), (33, 8200), (16, 100), (300, 70), (700, 5000), (1900, 4800), (2333, 5100)])
+def test_linear_with_the_smallest_and_largest_scales(rows, n, acts):
+    """Weights down to 2^-128 (subnormal in bf16) and up to the last scale bytes, with activations that bring the sums back, and nothing
+    beside them. Values of 2^128 and more are infinite beside bf16 activations, and as they are beside MXFP4 ones."""
+    g = torch.Generator().manual_seed(rows + n)
+    k = 224
+    for at, lo, hi in ((100, 0, 4), (-110, 250, 253), (-110, 253, 255)):
+        w, ws = random_mx(g, n, k, lo=lo, hi=hi)
+        if acts == "bf16":
+            x, xs = (torch.randn(rows, k, generator=g).bfloat16().float() * 2.0**at).bfloat16(), None
+            xv = x.double()
+        else:
+            x, xs = random_mx(g, rows, k, lo=127 + at, hi=130 + at)
+            xv = values(x, xs)
+        wv = values(w, ws)
+        if acts == "bf16":
+            wv = torch.where(wv.abs() >= 2.0**128, torch.sign(wv) * math.inf, wv)
+        want = (xv.cuda() @ wv.cuda().t()).cpu()
+        mag = (xv.abs().cuda() @ wv.abs().nan_to_num(0, 0, 0).cuda().t()).cpu().nan_to_num(0, 0, 0)
+        assert (want[want.isfinite()].abs() < 2.0**60).all() and (hi < 255 or acts == "mxfp4") == bool(want.isfinite().all())
+        if hi < 255 or acts == "mxfp4":
+            assert want.abs().median() > 2.0**-60
+        dx, dxs, dw, dws = cuda(x, xs, w, ws)
+        check_product(T.mxfp4_linear(dx, dw, dws, x_scales=dxs), want, mag, k, f"scales from {lo}")
+
+
 @gpu
 @pytest.mark.parametrize("rows", [5, 300])
 def test_linear_of_unaligned_views(rows):
@@ -354,6 +423,21 @@ def test_route_groups(tokens, experts, top, groups, kept):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,experts,top", [(1, 512, 8), (64, 300, 32), (17, 512, 8), (33, 257, 5), (9, 200, 3)])
+def test_route_of_few_tokens_to_many_experts(tokens, experts, top, dtype):
+    g = torch.Generator().manual_seed(tokens + experts + 1)
+    logits = (1.5 * torch.randn(tokens, experts, generator=g)).to(dtype)
+    bias = 0.5 * torch.randn(experts, generator=g)
+    check_route(logits, top)
+    check_route(logits, top, score="sigmoid", renorm=False, scale=2.5)
+    for groups, kept in ((64, 9), (8, 4)):
+        if experts % groups == 0:
+            check_route(logits, top, score="sigmoid", bias=bias, groups=groups, kept=kept)
+            check_route(logits, top, groups=groups, kept=kept, near_at_least=1e-7)
+
+
+@gpu
 @pytest.mark.parametrize("tokens", [5, 100, 6500])
 def test_route_ties_and_masks(tokens):
     """Equal logits go to the lowest index; -inf, NaN and rows of nothing else; the lowest finite value is no mask."""
@@ -467,6 +551,53 @@ def test_mlp2(tokens, experts, top, hidden, inner, residual, bias):
     assert torch.equal(T.moe_mlp2(dh, dr, dw, dws, db, residual=dres), got)      # the same order of sums every time
     if residual:
         assert T.moe_mlp2(dh, dr, dw, dws, db, residual=dres, out=dres) is dres and torch.equal(dres, got)
+
+
+COUNTS = [1, 3, 4, 5, 8, 9, 16, 17, 40, 0, 33]                     # tokens of each expert: every number of rows that the weight streams past
+
+
+def by_expert_on_gpu(x, routing, w, ws, bias):
+    y, m = [], []
+    for e in range(w.shape[0]):
+        rows = x[routing.offsets[e]: routing.offsets[e + 1]].cuda()
+        wv, b = values(w[e], ws[e]).cuda(), bias[e].double().cuda()
+        y.append(rows @ wv.t() + b)
+        m.append(rows.abs() @ wv.abs().nan_to_num(0, 0, 0).t() + b.abs())
+    return torch.cat(y).cpu(), torch.cat(m).cpu()
+
+
+@gpu
+@pytest.mark.parametrize("n", [100, 500, 1730, 4160])
+@pytest.mark.parametrize("k", [160, 1056])
+@pytest.mark.parametrize("scale", [1, 3])
+def test_experts_of_each_number_of_rows(n, k, scale):
+    """Experts of none, one and up to forty tokens (or three times as many, in tiles) at each width of a workgroup; a NaN block in one expert's weight."""
+    counts = [c * scale for c in COUNTS]
+    tokens, experts = sum(counts), len(counts)
+    g = torch.Generator().manual_seed(n + k + scale)
+    chosen = torch.repeat_interleave(torch.arange(experts), torch.tensor(counts))[torch.randperm(tokens, generator=g)].int()[:, None]
+    routing = T.MoeRouting(chosen, torch.rand(tokens, 1, generator=g) + 0.1, *plan_of(chosen, experts))
+    w, ws = random_mx(g, experts, n, k)
+    ws[7, n - 1, k // 32 - 1] = 255
+    b = torch.randn(experts, n, generator=g).bfloat16()
+    x = torch.randn(tokens, k, generator=g).bfloat16()
+    dr = T.MoeRouting(*cuda(*routing))
+    dx, dw, dws, db = cuda(x, w, ws, b)
+    y, m = by_expert_on_gpu(x.double()[routing.order.long()], routing, w, ws, b)
+    gate, lin = y[:, 0::2].clamp(max=LIMIT), y[:, 1::2].clamp(-LIMIT, LIMIT)
+    want = gate * torch.sigmoid(ALPHA * gate) * (lin + 1)
+    off = k * 2.0**-23 * m
+    room = 2.0**-8 * want.abs() + 1.1 * (lin + 1).abs() * off[:, 0::2] + gate.abs() * off[:, 1::2] + 1e-5 * want.abs() + 1e-30
+    got = T.moe_mlp1(dx, dr, dw, dws, db, alpha=ALPHA, limit=LIMIT).double().cpu()
+    assert want.isnan().sum() == counts[7] and torch.equal(got.isnan(), want.isnan())
+    assert ((got - want).abs() <= room)[~want.isnan()].all()
+    y, m = by_expert_on_gpu(x.double(), routing, w, ws, b)
+    wt = routing.weights.double()[routing.order.long()]
+    at = routing.order.long()
+    want, mag = torch.empty_like(y), torch.empty_like(m)
+    want[at], mag[at] = y * wt, m * wt
+    res = torch.randn(tokens, n, generator=g).bfloat16()
+    check_product(T.moe_mlp2(dx, dr, dw, dws, db, residual=res.cuda()), want + res.double(), mag + res.double().abs(), k + 1)
 
 
 @gpu
@@ -660,6 +791,68 @@ def test_mlp_block(tokens, experts):
     # a place of bf16 in t, the logits and h each, and in the result: the kernels' tolerance here is twice the reference model's rounding
     torch.testing.assert_close(got.double().cpu()[sure], want[sure], rtol=2e-2, atol=2e-2)
     assert torch.equal(m(x.cuda().view(1, tokens, 192)).view(tokens, 192), got)
+
+
+def gpt_oss_block(seed):
+    """A block of gpt-oss's sizes: 32 experts, four to a token, 2880 wide."""
+    m = T.MLPBlock(2880, 2880, 32, 4, device="cuda")
+    g, d = torch.Generator().manual_seed(seed), torch.Generator(device="cuda").manual_seed(seed)
+    with torch.no_grad():
+        m.norm.scale.copy_(1 + 0.1 * torch.randn(2880, generator=g))
+        m.gate.weight.copy_(3 * torch.randn(32, 2880, generator=g) / math.sqrt(2880))
+        m.gate.bias.copy_(torch.randn(32, generator=g))
+        m.mlp1_bias.copy_(0.1 * torch.randn(32, 5760, generator=g))
+        m.mlp2_bias.copy_(0.1 * torch.randn(32, 2880, generator=g))
+        for blocks, scales in ((m.mlp1_blocks, m.mlp1_scales), (m.mlp2_blocks, m.mlp2_scales)):
+            blocks.copy_(torch.randint(0, 256, blocks.shape, generator=d, dtype=torch.uint8, device="cuda"))
+            scales.copy_(torch.randint(118, 122, scales.shape, generator=d, dtype=torch.uint8, device="cuda"))
+    return m
+
+
+def gpt_oss_routing(m, x):
+    """The norm's rows, the logits, and which tokens' experts a place of bf16 in a logit cannot change; float64 on the CPU."""
+    t = x.double()
+    t = (t * torch.rsqrt(t.square().mean(-1, keepdim=True) + m.norm.eps) * m.norm.scale.detach().cpu().double()).bfloat16().double()
+    logits = (t @ m.gate.weight.detach().cpu().double().t() + m.gate.bias.detach().cpu().double()).bfloat16().double()
+    v, e = torch.sort(logits, dim=1, descending=True, stable=True)
+    return t, e[:, :4], torch.softmax(v[:, :4], 1), v[:, 3] - v[:, 4] > 0.05
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [1, 8, 40, 300])
+def test_mlp_block_of_gpt_oss_sizes(tokens):
+    m = gpt_oss_block(1)
+    x = torch.randn(tokens, 2880, generator=torch.Generator().manual_seed(tokens)).bfloat16()
+    t, chosen, weights, sure = gpt_oss_routing(m, x)
+    assert sure.double().mean() > 0.7
+    want, t, on = x.double().cuda(), t.cuda(), lambda p: p.detach().double()
+    table = FP4.cuda()
+
+    def dense(blocks, scales):
+        v = torch.stack((table[(blocks & 15).int()], table[(blocks >> 4).int()]), -1).flatten(-2)
+        return (v * torch.exp2(scales.double() - 127)[..., None]).flatten(-2)
+
+    for e in range(32):
+        at, j = (chosen == e).cuda().nonzero(as_tuple=True)
+        if len(at):
+            y = t[at] @ dense(m.mlp1_blocks[e], m.mlp1_scales[e]).t() + on(m.mlp1_bias[e])
+            gate, lin = y[:, 0::2].clamp(max=LIMIT), y[:, 1::2].clamp(-LIMIT, LIMIT)
+            h = (gate * torch.sigmoid(ALPHA * gate) * (lin + 1)).bfloat16().double()
+            want.index_add_(0, at, weights.cuda()[at, j, None] * (h @ dense(m.mlp2_blocks[e], m.mlp2_scales[e]).t() + on(m.mlp2_bias[e])))
+    got = m(x.cuda())
+    # (as for the small blocks: a place of bf16 in t, the logits and h each, and in the result)
+    torch.testing.assert_close(got.double().cpu()[sure], want.cpu()[sure], rtol=2e-2, atol=2e-2)
+
+
+@gpu
+def test_mlp_block_of_one_token():
+    """One token whose experts are sure, for each of several."""
+    m = mlp_block()
+    x = torch.randn(24, 192, generator=torch.Generator().manual_seed(3)).bfloat16()
+    want, sure = block_ref(m, x)
+    assert sure.sum() > 12
+    for i in sure.nonzero()[:, 0].tolist():
+        torch.testing.assert_close(m(x[i: i + 1].cuda()).double().cpu(), want[i: i + 1], rtol=2e-2, atol=2e-2)
 
 
 @gpu
