@@ -194,43 +194,26 @@ __device__ __forceinline__ int mx_quarter(int g) { return 0x2130 >> 4 * g & 3; }
 static __host__ __device__ __forceinline__ int mx_scale_pitch(int blocks) { return blocks % 16 ? blocks : blocks + 16; }
 static __host__ __device__ __forceinline__ int mx_scale_lds(int rows, int blocks) { return (rows * mx_scale_pitch(blocks) + 47) / 16 * 16; }
 __device__ __forceinline__ int mx_scale_shift(const unsigned char* from) { return static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15); }
-// The fetch in two halves, loads and writes, FLIGHT loads of a thread on their way together; what is left, if anything, is `first`
-// units of sixteen bytes in.
-template <int THREADS, int FLIGHT>
-struct MxScaleFetch {
-  u32x4 v[FLIGHT];
-  __amdgpu_buffer_rsrc_t buf;
-  int units, blocks, tid;
-  __device__ __forceinline__ MxScaleFetch(const unsigned char* from, int rows, int blocks_, int tid_) : blocks(blocks_), tid(tid_) {
-    const int shift = mx_scale_shift(from), bytes = shift + rows * blocks;
-    units = (bytes + 15) / 16;
-    // (to whole words: a word that the end cuts would come as zeros; its other bytes share the last one's sixteen)
-    buf = mx_buffer(from - shift, (bytes + 3) & ~3);
-  }
-  __device__ __forceinline__ void load(int first) {
+// The fetch, four loads of a thread on their way together.
+template <int THREADS>
+__device__ __forceinline__ void mx_fetch_scales(unsigned char* to, const unsigned char* from, int rows, int blocks, int tid) {
+  constexpr int FLIGHT = 4;
+  const int shift = mx_scale_shift(from), bytes = shift + rows * blocks, units = (bytes + 15) / 16;
+  // (to whole words: a word that the end cuts would come as zeros; its other bytes share the last one's sixteen)
+  const auto buf = mx_buffer(from - shift, (bytes + 3) & ~3);
+  for (int first = 0; first < units; first += THREADS * FLIGHT) {
+    u32x4 v[FLIGHT];
 #pragma unroll
     for (int j = 0; j < FLIGHT; ++j) {
       const int i = first + tid + j * THREADS;
       v[j] = mx_load16(buf, i < units ? 16 * i : MX_NONE);
     }
-  }
-  __device__ __forceinline__ void write(unsigned char* to, int first) {
 #pragma unroll
     for (int j = 0; j < FLIGHT; ++j) {
       const int i = first + tid + j * THREADS;
       if (i < units) *reinterpret_cast<u32x4*>(to + 16 * (blocks % 16 ? i : i + i / (blocks / 16))) = v[j];
     }
   }
-  __device__ __forceinline__ void rest(unsigned char* to, int first) {
-    for (; first < units; first += THREADS * FLIGHT) {
-      load(first);
-      write(to, first);
-    }
-  }
-};
-template <int THREADS>
-__device__ __forceinline__ void mx_fetch_scales(unsigned char* to, const unsigned char* from, int rows, int blocks, int tid) {
-  MxScaleFetch<THREADS, 4>(from, rows, blocks, tid).rest(to, 0);
 }
 
 // Whether four neighbours of the bias and of a row of the result are whole accesses
