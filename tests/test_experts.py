@@ -744,6 +744,32 @@ def test_router_logits_of_an_odd_number_for_many_tokens(hidden):
     check_product(T.router_logits(*cuda(x, w, b)), want, mag, hidden)
 
 
+@gpu
+@pytest.mark.parametrize("tokens", [3, 31, 250])
+def test_rows_far_apart(tokens):
+    """Rows that span almost 4 GiB are read where they lie; x of moe_mlp1 that spans more is refused."""
+    g, routing, (w, ws), (w2, ws2) = experts_case(tokens, 4, 2, 288, 160)
+    dr = T.MoeRouting(*cuda(*routing))
+    dw, dws, dw2, dws2 = cuda(w, ws, w2, ws2)
+
+    def far(rows, k, pitch):
+        dense = torch.randn(rows, k, generator=g).bfloat16().cuda()
+        return dense, torch.empty((rows - 1) * pitch + k, dtype=torch.bfloat16, device="cuda").as_strided((rows, k), (pitch, 1)).copy_(dense)
+
+    most = ((1 << 31) - 2048) // (tokens - 1) // 8 * 8             # values between rows
+    dense, x = far(tokens, 288, most)
+    assert (tokens - 1) * most * 2 > 4000 << 20
+    assert torch.equal(T.moe_mlp1(x, dr, dw, dws), T.moe_mlp1(dense, dr, dw, dws))
+    assert torch.equal(T.mxfp4_linear(x, dw[0], dws[0]), T.mxfp4_linear(dense, dw[0], dws[0]))
+    del x
+    dense, x = far(tokens, 288, most + 2048)
+    with pytest.raises(RuntimeError, match="4 GiB"):
+        T.moe_mlp1(x, dr, dw, dws)
+    del x
+    dense, h = far(2 * tokens, 160, ((1 << 31) - 2048) // (2 * tokens - 1) // 8 * 8)
+    assert torch.equal(T.moe_mlp2(h, dr, dw2, dws2), T.moe_mlp2(dense, dr, dw2, dws2))
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------------
 def mlp_block(hidden=192, inner=160, experts=16, top=4, seed=0):
     g = torch.Generator().manual_seed(seed)
