@@ -12,7 +12,8 @@
 // tokens are dealt in order to workgroups and their wavefronts, and a wavefront places its tokens one after the other -- a
 // token's experts are all different, so its lanes can place them at once. That makes the order stable and the same every time.
 // What bounds it are latencies: 8 tokens of 32 experts 3.2 us in one launch; 8191 of 256, 4.2 MB of logits, 14.6 + 9.2 us in two
-// (branches around single loads, one wait each, had made the first 19.5; counts summed one load at a time the second 60).
+// (branches around single loads, one wait each, had made the first 19.5; counts summed one load at a time the second 60). In the second each
+// of 256 workgroups reads every workgroup's counts, 67 MB in all, and one wavefront of it scans them; of 32 experts, softmax, 4.4 + 6.6.
 #include "mx_common.h"
 
 namespace tllm {

@@ -193,7 +193,7 @@ static int tile4_of(const MxArgs& a) {
   return which;
 }
 
-// Up to 80 rows the weight stream is ahead: 64 rows of [5120, 2880] 7.9 us and 8.6 in tiles, 128 11.4 and 8.9.
+// The weight stream and the tiles meet between 64 and 80 rows: 64 rows of [5120, 2880] 8.2 us and 8.8 in tiles, 80 9.9 and 8.6, 128 11.8 and 9.1.
 bool mx_tiles4_take(const MxArgs& a) { return a.rows > 80 && tile4_of(a) != 0; }
 
 int mx_tiles4(const MxArgs& a, hipStream_t st) {

@@ -2,8 +2,9 @@
 //
 //   D[n, r] = sum_k W[n, k] X[r, k]        W MXFP4 [N, K], X bf16 or MXFP4
 //
-// What bounds it is the weight's arrival, N K 17 / 32 bytes of every expert that has rows (8 tokens of 32 experts, 186 MB: mlp1 35.7 us,
-// 5.2 TB/s; a plain read reaches 6.1), and with one token the chain of latencies around it (10.4 us for 35 MB). A workgroup of NW
+// What bounds it is the weight's arrival, N K 17 / 32 bytes of every expert that has rows (8 tokens of 32 experts, 186 MB: mlp1 34.0 us,
+// 5.5 TB/s; a plain read reaches 6.1), and with one token the chain of latencies around it (9.8 us for 35 MB: a workgroup's first weights
+// leave with its rows, whose addresses are the pairs'). A workgroup of NW
 // wavefronts owns 16 NT weight rows and up to 16 activation rows; the wavefronts deal the K steps of 128 between them (sums meet in
 // LDS, added in a fixed order). Weights and activations go straight to LDS, U steps of a wavefront at a time in a ring that is its
 // alone, so that nothing but the wavefront's own count of arrivals is waited for. That path is what the addresses ask for: a

@@ -13,7 +13,7 @@
 // What bounds it: the matrix cores at the clock that they leave (one 128 x 256 tile to a CU, [4096] outputs of 2048 rows, goes
 // through K at 1.18 PFLOP/s, where a large library product reaches 1.24), behind 11 us of a launch's beginning and end per round
 // of tiles, which workgroups that share a CU cover for one another, and the rows that an expert's last tile lacks. 2048 tokens of
-// 32 experts, four each, hidden and inner 2880: mlp1 312 us (870 TFLOP/s), mlp2's product 166 and its weighted sum 17. Built and
+// 32 experts, four each, hidden and inner 2880: mlp1 312 us (870 TFLOP/s), mlp2's product 173 and its weighted sum 17. Built and
 // slower: three slices in the ring of the 128 x 128 tile (two workgroups to a CU instead of three; 340 us), 64 x 512 (472), 128 x 256 (367).
 #include "mx_common.h"
 
@@ -218,8 +218,8 @@ static int tiles_of(const MxArgs& a, hipStream_t st) {
   return launch_tiles<Small, MODE>(a, st);
 }
 
-// Whether a product of these sizes is the tiles'. Below, the weight stream is ahead: 130 rows of [5120, 2880] 17.1 us, 18.7 in tiles
-// (300 29.8 and 20.6); 32 experts of 24 rows each on average mlp1 115.7 in tiles and 108.0 as a stream, of 32 rows 122.0 and 128.3.
+// Whether a product of these sizes is the tiles'. Below, the weight stream is ahead: 130 rows of [5120, 2880] 12.4 us, 16.4 in tiles,
+// 200 16.8 and 19.2, 300 21.5 and 21.2; 32 experts of 24 rows each on average mlp1 113.3 and 113.8 in tiles, of 32 rows 129.4 and 120.5.
 bool mx_tiles_take(const MxArgs& a) {
   return a.rows > (a.order ? 24ll : 200ll) * a.experts && tile_lds<Small>(a.k) <= 160 * 1024;
 }
