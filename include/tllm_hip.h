@@ -357,7 +357,8 @@ int tllm_mxfp4_quantize(const void* x, int x_type, int64_t x_row_stride, void* b
 
 /* out[r, n] = sum_k x[r, k] W[n, k] + bias[n] with W MXFP4 [out_dim, in_dim] (fp32 accumulate, one RNE to bf16). x is bf16
  * with x_row_stride values from row to row, or, with x_scales not NULL, dense MXFP4 blocks. bias bf16 [out_dim] or NULL. in_dim a
- * multiple of 32; rows of x, W's blocks and all scales 16-byte aligned, 128 rows of x within 4 GiB. Any number of rows. */
+ * multiple of 32, 32 to 2^18 (of the experts' products too); rows of x, W's blocks and all scales 16-byte aligned, 128 rows of x within
+ * 4 GiB. Any number of rows. */
 int tllm_mxfp4_linear_bf16(const void* x, const void* x_scales, int64_t x_row_stride, const void* w_blocks, const void* w_scales,
                            const void* bias, void* out, int64_t out_row_stride, int64_t rows, int64_t in_dim, int64_t out_dim,
                            void* stream);
