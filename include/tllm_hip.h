@@ -399,6 +399,47 @@ int tllm_moe_mlp2_bf16(const void* h, int64_t h_row_stride, const int32_t* order
                        void* out, int64_t out_row_stride, void* workspace, int64_t workspace_bytes, int64_t tokens, int n_experts,
                        int top, int64_t inner, int64_t hidden, void* stream);
 
+/* ---- A KV cache in MXFP4 ------------------------------------------------------------------------------------------------
+ * Codes [batch][n_slots][n_kv_heads][head_dim / 32][16] and scale bytes [batch][n_slots][n_kv_heads][head_dim / 32], for keys and for
+ * values; the last two dimensions of the codes and the last of the scales are dense, the others have strides in bytes, the same for keys
+ * and values: those of the codes multiples of 16, none negative, those between slots below 2^24. Device pointers, codes 16-byte aligned.
+ * Attention reads fastest where a head's slots are neighbours (slot_stride = head_dim / 2). batch and n_kv_heads up to 65535,
+ * n_slots below 2^30, head_dim a multiple of 32 up to 1024 (attention: 64). */
+typedef struct TllmMxCache {
+  void *k_blocks, *k_scales, *v_blocks, *v_scales;
+  int64_t batch_stride, slot_stride, head_stride;
+  int64_t scale_batch_stride, scale_slot_stride, scale_head_stride;
+  int64_t batch, n_slots;
+  int32_t n_kv_heads, head_dim;
+} TllmMxCache;
+
+/* k, v [batch, tokens, n_kv_heads, head_dim] of `type` -> the cache, quantised as tllm_mxfp4_quantize does it: token t of row b goes to slot
+ * offset[b] + t (offset[0] + t without offset_per_row). Slots outside the cache and, with lengths (NULL: none), tokens t >= lengths[b] are
+ * not written; everything else in the cache stays as it is. k_strides / v_strides: elements between rows, tokens and heads, 16-byte
+ * multiples. offset and lengths: device, int32 or int64. The cache's rows must not share memory. */
+int tllm_mxfp4_cache_write(const TllmMxCache* cache, const void* k, const void* v, int type, const int64_t* k_strides,
+                           const int64_t* v_strides, int64_t tokens, const void* offset, int offset_is_i64, int offset_per_row,
+                           const void* lengths, int lengths_is_i64, int lengths_per_row, void* stream);
+
+/* Slots first .. first + tokens - 1 as bf16: k_out, v_out [batch, tokens, n_kv_heads, head_dim] dense. A scale byte of 255 gives NaN;
+ * values beyond bf16's range (scale bytes 253 and 254, which the quantisation never writes) are infinite. */
+int tllm_mxfp4_cache_read_bf16(const TllmMxCache* cache, int64_t first, int64_t tokens, void* k_out, void* v_out, void* stream);
+
+/* Attention over the cache with learned sinks and an optional sliding window: query i of row b sits at position start_q[b] + i (start_q[0] + i
+ * without start_q_per_row) and sees the slots n <= position, n < n_slots and, when window > 0, n > position - window; otherwise
+ * as tllm_attention_prefill_bf16. q [batch, n_q, n_kv_heads * group, 64] bf16 with batch / token strides in elements, out
+ * [batch, n_q, n_kv_heads * group * 64] likewise; sinks bf16 [n_kv_heads * group] or NULL (logit 0). A row that sees nothing gives zeros.
+ * What a slot holds that a query does not see, NaN included, is nothing to it. start_q: device, int32 or int64. group up to 64,
+ * sm_scale positive. kv_len_hint (0: none) plans the launch for that many visible keys instead of n_slots; results do not depend on it.
+ * workspace: device memory of tllm_mxfp4_attention_workspace_bytes() for the same arguments, 4-byte aligned (may be 0 bytes). */
+int tllm_mxfp4_attention_splits(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint);
+int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window,
+                                             int64_t kv_len_hint);
+int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, int64_t q_token_stride, const TllmMxCache* cache, const void* sinks,
+                              void* out, int64_t out_batch_stride, int64_t out_token_stride, int64_t n_q, int group, float sm_scale,
+                              int window, const void* start_q, int start_q_is_i64, int start_q_per_row, int64_t kv_len_hint,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

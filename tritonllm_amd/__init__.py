@@ -5,6 +5,7 @@ from . import scratch_pool
 from .modules import OUT, QKV, Embedding, MLPBlock, RMSNorm, RotaryEmbedding, UnEmbedding
 from .ops import (
     MoeRouting,
+    Mxfp4Cache,
     attention,
     attention_decode,
     embed_qkv_rope_forward,
@@ -14,6 +15,11 @@ from .ops import (
     moe_mlp1,
     moe_mlp2,
     moe_route,
+    mxfp4_attention,
+    mxfp4_attention_decode,
+    mxfp4_cache,
+    mxfp4_cache_read,
+    mxfp4_cache_write,
     mxfp4_dequant,
     mxfp4_linear,
     mxfp4_quantize,
@@ -43,4 +49,5 @@ __all__ = [
     "qkv_rope_forward", "quantize_fp8_rows", "rmsnorm_forward", "rope_forward", "swiglu", "UnEmbedding", "unembedding_decode_forward", "unembedding_decode_argmax_forward", "unembedding_decode_argmax_noalloc", "unembedding_decode_argmax_noalloc_init",
     "unembedding_decode_fp8_forward", "unembedding_decode_fp8_argmax_forward", "unembedding_forward",
     "MLPBlock", "MoeRouting", "router_logits", "moe_mlp1", "moe_mlp2", "moe_route", "mxfp4_linear", "mxfp4_quantize",
+    "Mxfp4Cache", "mxfp4_cache", "mxfp4_cache_write", "mxfp4_cache_read", "mxfp4_attention", "mxfp4_attention_decode",
 ]

@@ -34,6 +34,13 @@ class TllmRope(C.Structure):
     ]
 
 
+class TllmMxCache(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("k_blocks", "k_scales", "v_blocks", "v_scales")] + [
+        (name, C.c_int64)
+        for name in ("batch_stride", "slot_stride", "head_stride", "scale_batch_stride", "scale_slot_stride", "scale_head_stride", "batch", "n_slots")
+    ] + [("n_kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
 _vp, _i64, _i32, _f32 = C.c_void_p, C.c_int64, C.c_int, C.c_float
 _QKV_SIG = [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, C.POINTER(TllmRope), _vp]
 
@@ -86,6 +93,12 @@ SIGNATURES = {
     "tllm_moe_mlp1_bf16": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i64, _i64, _f32, _f32, _i32, _vp]),
     "tllm_moe_mlp2_workspace_bytes": (_i64, [_i64, _i32, _i64]),
     "tllm_moe_mlp2_bf16": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i64, _i64, _vp]),
+    "tllm_mxfp4_cache_write": (_i32, [C.POINTER(TllmMxCache), _vp, _vp, _i32, C.POINTER(_i64), C.POINTER(_i64), _i64, _vp, _i32, _i32, _vp, _i32, _i32, _vp]),
+    "tllm_mxfp4_cache_read_bf16": (_i32, [C.POINTER(TllmMxCache), _i64, _i64, _vp, _vp, _vp]),
+    "tllm_mxfp4_attention_splits": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32, _i64]),
+    "tllm_mxfp4_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i64]),
+    "tllm_mxfp4_attention_bf16": (_i32, [_vp, _i64, _i64, C.POINTER(TllmMxCache), _vp, _vp, _i64, _i64, _i64, _i32, _f32, _i32, _vp, _i32, _i32, _i64, _vp,
+                                         _i64, _vp]),
     "tllm_qkv_rope_decode_w8_bf16": (_i32, [_vp, _vp, _i32, _f32, _vp, _vp] + _QKV_SIG[2:]),
 }
 

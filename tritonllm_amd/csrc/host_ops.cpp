@@ -815,6 +815,98 @@ PyObject* moe_mlp2(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return wrap(out);
 }
 
+// ---- a KV cache in MXFP4 ------------------------------------------------------------------------------------------------------
+// (k_blocks, k_scales, v_blocks, v_scales) on the current device, laid out as ops.py describes it
+bool mx_cache_of(PyObject* const* a, TllmMxCache* c) {
+  for (int i = 0; i < 4; ++i)
+    if (!gpu_tensor(a[i]) || !u8(tensor(a[i])) || tensor(a[i]).device().index() != c10::hip::current_device()) return false;
+  const Tensor &kb = tensor(a[0]), &ks = tensor(a[1]), &vb = tensor(a[2]), &vs = tensor(a[3]);
+  if (kb.dim() != 5 || ks.dim() != 4 || kb.size(4) != 16 || kb.size(3) < 1 || kb.sizes().slice(0, 4) != ks.sizes() || vb.sizes() != kb.sizes() || vs.sizes() != ks.sizes() ||
+      vb.strides() != kb.strides() || vs.strides() != ks.strides() || kb.stride(4) != 1 || kb.stride(3) != 16 || ks.stride(3) != 1 || kb.numel() == 0)
+    return false;
+  if (kb.size(2) > INT32_MAX || kb.size(3) > 1024) return false;
+  *c = TllmMxCache{mut(kb), mut(ks), mut(vb), mut(vs), kb.stride(0), kb.stride(1), kb.stride(2), ks.stride(0), ks.stride(1), ks.stride(2), kb.size(0), kb.size(1),
+                   static_cast<int32_t>(kb.size(2)), static_cast<int32_t>(32 * kb.size(3))};
+  return true;
+}
+bool row_ints_ok(PyObject* o, int64_t batch) {
+  if (!gpu_tensor(o) || tensor(o).device().index() != c10::hip::current_device()) return false;
+  const Tensor& t = tensor(o);
+  return (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.dim() == 1 && (t.size(0) == 1 || t.size(0) == batch) && t.is_contiguous();
+}
+
+// mxfp4_cache_write(k_blocks, k_scales, v_blocks, v_scales, k, v, offset, lengths): True behind a launch
+PyObject* mxfp4_cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  TllmMxCache c;
+  if (n != 8 || !mx_cache_of(a, &c) || !row_ints_ok(a[6], c.batch) || !(is_none(a[7]) || row_ints_ok(a[7], c.batch))) return none();
+  int64_t strides[2][3];
+  for (int i = 0; i < 2; ++i) {
+    if (!gpu_tensor(a[4 + i]) || tensor(a[4 + i]).device() != tensor(a[0]).device()) return none();
+    const Tensor& t = tensor(a[4 + i]);
+    if (t.dim() != 4 || t.size(0) != c.batch || t.size(2) != c.n_kv_heads || t.size(3) != c.head_dim || t.stride(3) != 1 || t.numel() == 0) return none();
+    for (int d = 0; d < 3; ++d) strides[i][d] = t.stride(d);
+  }
+  const Tensor &k = tensor(a[4]), &v = tensor(a[5]), &off = tensor(a[6]);
+  const auto t = k.scalar_type();
+  const int type = t == at::kBFloat16 ? TLLM_BF16 : t == at::kHalf ? TLLM_F16 : t == at::kFloat ? TLLM_F32 : -1;
+  if (type < 0 || v.scalar_type() != t || v.size(1) != k.size(1)) return none();
+  const bool done = launch("mxfp4_cache_write", [&] {
+    return tllm_mxfp4_cache_write(&c, k.const_data_ptr(), v.const_data_ptr(), type, strides[0], strides[1], k.size(1), off.const_data_ptr(),
+                                  off.scalar_type() == at::kLong, off.size(0) > 1, ptr(a[7]), !is_none(a[7]) && tensor(a[7]).scalar_type() == at::kLong,
+                                  !is_none(a[7]) && tensor(a[7]).size(0) > 1, stream());
+  });
+  if (!done) return none();
+  Py_RETURN_TRUE;
+}
+
+// mxfp4_cache_read(k_blocks, k_scales, v_blocks, v_scales, first, tokens)
+PyObject* mxfp4_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  TllmMxCache c;
+  int64_t first, tokens;
+  if (n != 6 || !mx_cache_of(a, &c) || !to_i64(a[4], &first) || !to_i64(a[5], &tokens) || first < 0 || tokens < 1 || first > c.n_slots || tokens > c.n_slots - first)
+    return none();
+  const auto options = tensor(a[0]).options().dtype(at::kBFloat16);
+  const Tensor k = empty({c.batch, tokens, c.n_kv_heads, c.head_dim}, options), v = empty({c.batch, tokens, c.n_kv_heads, c.head_dim}, options);
+  const bool done = launch("mxfp4_cache_read", [&] { return tllm_mxfp4_cache_read_bf16(&c, first, tokens, mut(k), mut(v), stream()); });
+  if (!done) return none();
+  PyObject *pk = wrap(k), *pv = wrap(v);
+  PyObject* r = PyTuple_Pack(2, pk, pv);
+  Py_XDECREF(pk);
+  Py_XDECREF(pv);
+  return r;
+}
+
+// mxfp4_attention(q, k_blocks, k_scales, v_blocks, v_scales, sinks, sm_scale, bandwidth, start_q, kv_len_hint)
+PyObject* mxfp4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  TllmMxCache c;
+  double scale;
+  int64_t window = 0, hint = 0;
+  if (n != 10 || !mx_cache_of(a + 1, &c) || !gpu_tensor(a[0]) || !to_f64(a[6], &scale) || !row_ints_ok(a[8], c.batch) || !(is_none(a[9]) || to_i64(a[9], &hint))) return none();
+  if (!is_none(a[7]) && (!to_i64(a[7], &window) || window < 0 || window > INT32_MAX)) return none();
+  const Tensor &q = tensor(a[0]), &start = tensor(a[8]);
+  if (q.device() != tensor(a[1]).device() || !bf16(q) || q.dim() != 5 || q.size(0) != c.batch || q.size(2) != c.n_kv_heads || q.size(4) != 64 || c.head_dim != 64 || q.numel() == 0)
+    return none();
+  const int64_t n_ctx = q.size(1), group = q.size(3), n_heads = c.n_kv_heads * group;
+  if (group > 64 || q.stride(4) != 1 || q.stride(3) != 64 || q.stride(2) != 64 * group || q.stride(1) % 8 || q.stride(0) % 8 || !al16(q)) return none();
+  if (!is_none(a[5])) {
+    if (!gpu_tensor(a[5]) || tensor(a[5]).device() != q.device()) return none();
+    const Tensor& z = tensor(a[5]);
+    if (!bf16(z) || z.dim() != 1 || z.size(0) != n_heads || !z.is_contiguous()) return none();
+  }
+  if (!is_none(a[9]) && hint < 1) hint = 1;
+  const Tensor o = empty({c.batch, n_ctx, n_heads * 64}, q.options());
+  const int64_t need = tllm_mxfp4_attention_workspace_bytes(c.batch, n_ctx, c.n_slots, c.n_kv_heads, static_cast<int>(group), static_cast<int>(window), hint);
+  Tensor work;
+  if (need) work = empty({need}, q.options().dtype(at::kByte));
+  const bool done = launch("mxfp4_attention", [&] {
+    return tllm_mxfp4_attention_bf16(q.const_data_ptr(), q.stride(0), q.stride(1), &c, ptr(a[5]), mut(o), o.stride(0), o.stride(1), n_ctx, static_cast<int>(group),
+                                     static_cast<float>(scale), static_cast<int>(window), start.const_data_ptr(), start.scalar_type() == at::kLong,
+                                     start.size(0) > 1, hint, need ? mut(work) : nullptr, need, stream());
+  });
+  if (!done) return none();
+  return wrap(o);
+}
+
 // Whatever ATen throws (out of memory, ...) reaches Python as the RuntimeError it would be there.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -837,6 +929,7 @@ PyMethodDef kMethods[] = {
     TLLM_OP(rmsnorm), TLLM_OP(embedding), TLLM_OP(embedding_rmsnorm), TLLM_OP(swiglu), TLLM_OP(qkv_rope), TLLM_OP(qkv_rope_cache), TLLM_OP(linear),
     TLLM_OP(out_residual), TLLM_OP(unembedding), TLLM_OP(attention_decode), TLLM_OP(attention),
     TLLM_OP(mxfp4_quantize), TLLM_OP(mxfp4_dequant), TLLM_OP(mxfp4_linear), TLLM_OP(moe_route), TLLM_OP(moe_mlp1), TLLM_OP(moe_mlp2),
+    TLLM_OP(mxfp4_cache_write), TLLM_OP(mxfp4_cache_read), TLLM_OP(mxfp4_attention),
     {"pool_get", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<pool_buffer>)), METH_FASTCALL, nullptr},
     {"pool_clear", py_pool_clear, METH_NOARGS, nullptr},
     {"pool_stats", py_pool_stats, METH_NOARGS, nullptr},

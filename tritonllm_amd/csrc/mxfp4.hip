@@ -3,7 +3,7 @@
 // The arithmetic follows the
 // reference's torch.ldexp on a bf16 tensor: the product is formed in fp32 and rounded once to bf16 (exact for every
 // scale a checkpoint holds; scale bytes >= 255 give inf / nan there and here).
-#include "common.h"
+#include "mx_quantize.h"
 
 namespace tllm {
 
@@ -13,8 +13,6 @@ __device__ __forceinline__ float fp4_value(unsigned nib) {
   const float m = mag < 2u ? 0.5f * static_cast<float>(mag) : static_cast<float>(2u + (mag & 1u)) * static_cast<float>(1u << ((mag >> 1) - 1u)) * 0.5f;
   return (nib & 8u) ? -m : m;
 }
-
-typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned u32x4;
 
 // A lane expands one dword (4 bytes -> 8 values -> one 16-byte store), so that a wave's store covers 1 KB of
 // consecutive output and its load 256 consecutive bytes; a work-group takes UNROLL * 256 dwords and each lane issues its
@@ -75,64 +73,8 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const unsigned* __re
 // Quantisation to MXFP4 (the OCP microscaling format): the 32 values of a block share the power of two e = floor(log2 max|x|) - 2, at
 // least 2^-127, and become the nearest e2m1 value of x 2^-e, ties to the even code; beyond 6 is 6. A block that holds a NaN or an
 // infinity has the scale byte 255, which makes all of it NaN, and codes of 0.
-// The maximum is one of the values' bits: without the sign they order as integers, and the exponent field less 2 is the scale
-// byte. A lane takes eight values (16 or 32 bytes), four neighbouring lanes a block. The bytes bound it: 40960 x 2880 fp32 values, 472 MB
+// A lane takes eight values (16 or 32 bytes), four neighbouring lanes a block. The bytes bound it: 40960 x 2880 fp32 values, 472 MB
 // read and 63 MB written, 87 us, 6.1 TB/s (a plain read's rate); one row of 2880 1.6 us.
-template <class T>
-struct Eight;                        // eight values as loaded; the largest of their magnitudes as an fp32's bits; eight codes
-template <>
-struct Eight<bf16> {
-  u32x4 v;
-  __device__ void load(const void* p) { v = *static_cast<const u32x4*>(p); }
-  __device__ unsigned largest() const {
-    unsigned m = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = max(m, max(v[i] << 16 & 0x7fff0000u, v[i] & 0x7fff0000u));
-    return m;
-  }
-  template <int I>
-  __device__ unsigned pair(unsigned old, float scale) const {
-    const unsigned two = v[I];       // (a scalar of its own: __builtin_bit_cast of a vector's element takes element 0 with this compiler)
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(bf16x2, two), scale, I);
-  }
-};
-template <>
-struct Eight<_Float16> {
-  typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2;
-  u32x4 v;
-  __device__ void load(const void* p) { v = *static_cast<const u32x4*>(p); }
-  __device__ unsigned largest() const {
-    unsigned m = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = max(m, max(v[i] & 0x7fffu, v[i] >> 16 & 0x7fffu));
-    return __builtin_bit_cast(unsigned, static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(m))));
-  }
-  template <int I>
-  __device__ unsigned pair(unsigned old, float scale) const {
-    const unsigned two = v[I];
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(f16x2, two), scale, I);
-  }
-};
-template <>
-struct Eight<float> {
-  f32x4 v[2];
-  __device__ void load(const void* p) {
-    v[0] = static_cast<const f32x4*>(p)[0];
-    v[1] = static_cast<const f32x4*>(p)[1];
-  }
-  __device__ unsigned largest() const {
-    unsigned m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float one = v[i / 4][i % 4];
-      m = max(m, __builtin_bit_cast(unsigned, one) & 0x7fffffffu);
-    }
-    return m;
-  }
-  template <int I>
-  __device__ unsigned pair(unsigned old, float scale) const { return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, v[I / 2][I % 2 * 2], v[I / 2][I % 2 * 2 + 1], scale, I); }
-};
-
 template <class T>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t row_stride, int per_row, unsigned* __restrict__ blocks,
                                                              unsigned char* __restrict__ scales, int64_t n) {
@@ -145,16 +87,8 @@ __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict
   }
   Eight<T> e;
   e.load(from);
-  unsigned m = e.largest();
-  m = max(m, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(m), 0xB1, 0xf, 0xf, true)));   // lane ^ 1
-  m = max(m, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(m), 0x4E, 0xf, 0xf, true)));   // lane ^ 2
-  const unsigned field = m >> 23, byte = field == 255 ? 255 : field > 2 ? field - 2 : 0;
-  const float scale = __builtin_bit_cast(float, byte << 23);                 // (a field of 0 is 2^-127 to the conversion)
-  unsigned codes = e.template pair<0>(0u, scale);
-  codes = e.template pair<1>(codes, scale);
-  codes = e.template pair<2>(codes, scale);
-  codes = e.template pair<3>(codes, scale);
-  blocks[d] = field == 255 ? 0 : codes;
+  unsigned byte;
+  blocks[d] = mx_quantize8(e, &byte);
   if ((d & 3) == 0) scales[d >> 2] = static_cast<unsigned char>(byte);
 }
 

@@ -33,7 +33,7 @@ from typing import NamedTuple
 import torch
 
 from . import scratch_pool
-from ._lib import TllmRope, check, host, lib
+from ._lib import TllmMxCache, TllmRope, check, host, lib
 from ._lib import require as _require
 from .yarn import YarnParams
 
@@ -1035,3 +1035,140 @@ def moe_mlp2(h: torch.Tensor, routing: MoeRouting, blocks: torch.Tensor, scales:
                                        residual.data_ptr() if residual is not None else None, n, out.data_ptr(), n, work.data_ptr(), need, tokens,
                                        experts, top, 32 * g, n, _stream()), "moe_mlp2")
     return out
+
+
+# --------------------------------------------------------------------------------------- a KV cache in MXFP4
+class Mxfp4Cache(NamedTuple):
+    """Keys and values in MXFP4, 17 bytes for 32 of them: ``blocks [batch, n_ctx, n_kv_heads, head_dim / 32, 16]`` and ``scales [batch, n_ctx,
+    n_kv_heads, head_dim / 32]``, uint8, of any strides outside a head (keys' and values' alike). ``mxfp4_cache`` makes one."""
+
+    k_blocks: torch.Tensor
+    k_scales: torch.Tensor
+    v_blocks: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def mxfp4_cache(batch: int, n_ctx: int, n_kv_heads: int, head_dim: int = 64, device: torch.device | None = None) -> Mxfp4Cache:
+    """An empty cache (zeros) whose heads' slots are neighbours in memory, which attention reads fastest."""
+    _require(head_dim % 32 == 0, "mxfp4_cache: a head is whole blocks of 32 values")
+    shape = (batch, n_kv_heads, n_ctx, head_dim // 32)
+    make = lambda *last: torch.zeros(*shape, *last, dtype=torch.uint8, device="cuda" if device is None else device).transpose(1, 2)
+    return Mxfp4Cache(make(16), make(), make(16), make())
+
+
+def _mx_cache_desc(cache, *others: torch.Tensor) -> TllmMxCache:
+    """The C descriptor of a cache, checked: every tensor on one GPU, blocks of 16 dense bytes, keys laid out as values are."""
+    kb, ks, vb, vs = cache
+    _on_gpu(kb, ks, vb, vs, *others)
+    _require(all(t is None or t.device == kb.device for t in (ks, vb, vs, *others)), "the cache and its operands must be on one device")
+    _require(all(t.dtype == torch.uint8 for t in (kb, ks, vb, vs)), "MXFP4 blocks and scales are uint8")
+    _require(kb.ndim == 5 and kb.shape[-1] == 16 and ks.shape == kb.shape[:-1], f"a cache holds blocks [batch, n_ctx, n_kv_heads, head_dim / 32, 16] and their scales, not {tuple(kb.shape)} and {tuple(ks.shape)}")
+    _require(vb.shape == kb.shape and vs.shape == ks.shape, "a cache holds as many keys as values")
+    groups = kb.shape[3]
+    _require(groups >= 1, "a cache's heads hold no values")
+    _require(kb.stride()[3:] == (16, 1) or (groups == 1 and kb.stride(4) == 1), "a cache's blocks must be dense inside a head")
+    _require(groups == 1 or ks.stride(3) == 1, "a cache's scales must be dense inside a head")
+    _require(vb.stride() == kb.stride() and vs.stride() == ks.stride(), "a cache's keys and values must have the same strides")
+    return TllmMxCache(kb.data_ptr(), ks.data_ptr(), vb.data_ptr(), vs.data_ptr(), kb.stride(0), kb.stride(1), kb.stride(2), ks.stride(0), ks.stride(1),
+                       ks.stride(2), kb.shape[0], kb.shape[1], kb.shape[2], 32 * groups)
+
+
+def _row_ints(t: torch.Tensor, batch: int, what: str) -> torch.Tensor:
+    """int32 or int64 numbers on the device, one for the whole batch or one for each row."""
+    _require(t.dtype in (torch.int32, torch.int64) and t.ndim == 1 and t.shape[0] in (1, batch), f"{what}: one int32 or int64 for the batch, or one for each of its {batch} rows")
+    return t.contiguous()
+
+
+def mxfp4_cache_write(cache: Mxfp4Cache, k: torch.Tensor, v: torch.Tensor, offset: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
+    """Quantise new keys and values, ``[batch, tokens, n_kv_heads, head_dim]`` (bf16, fp16 or fp32), into the cache, as ``mxfp4_quantize`` does
+    it: token ``t`` of row ``b`` goes to slot ``offset[b] + t``.
+
+    ``offset`` (int32 or int64 on the device, one element or one per row) is read by the kernel, so that a captured call follows a
+    growing context. Of a padded batch, ``lengths`` (likewise) says how many tokens of a row there are. What lies behind them, and slots
+    outside the cache, are left as they are."""
+    if host().mxfp4_cache_write(*cache, k, v, offset, lengths):
+        return
+    desc = _mx_cache_desc(cache, k, v, offset, lengths)
+    _require(k.dtype in _MX_TYPES and v.dtype == k.dtype, "mxfp4_cache_write: k and v must both be bfloat16, float16 or float32")
+    _require(k.ndim == 4 and v.shape == k.shape, f"mxfp4_cache_write: k {tuple(k.shape)} and v {tuple(v.shape)}")
+    batch, tokens, heads, dim = k.shape
+    _require((batch, heads, dim) == (desc.batch, desc.n_kv_heads, desc.head_dim), f"mxfp4_cache_write: k {tuple(k.shape)} for a cache of {desc.batch} rows of {desc.n_kv_heads} heads of {desc.head_dim}")
+    offset = _row_ints(offset, batch, "mxfp4_cache_write: offset")
+    lengths = lengths if lengths is None else _row_ints(lengths, batch, "mxfp4_cache_write: lengths")
+
+    def rows(t):
+        size = t.element_size()
+        ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(st * size % 16 == 0 for st in t.stride()[:3])
+        return t if ok else _aligned(t)
+
+    if k.numel() == 0:
+        return
+    k, v = rows(k), rows(v)
+    strides = [(C.c_int64 * 3)(*t.stride()[:3]) for t in (k, v)]
+    with torch.cuda.device(k.device):
+        check(lib().tllm_mxfp4_cache_write(C.byref(desc), k.data_ptr(), v.data_ptr(), _MX_TYPES[k.dtype], *strides, tokens, offset.data_ptr(),
+                                           int(offset.dtype == torch.int64), int(offset.shape[0] > 1), lengths.data_ptr() if lengths is not None else None,
+                                           int(lengths is not None and lengths.dtype == torch.int64), int(lengths is not None and lengths.shape[0] > 1),
+                                           _stream()), "mxfp4_cache_write")
+
+
+def mxfp4_cache_read(cache: Mxfp4Cache, first: int = 0, tokens: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Slots ``first`` to ``first + tokens`` (``None``: to the end) as ``(k, v)``, bf16 ``[batch, tokens, n_kv_heads, head_dim]``, exactly; a scale
+    byte of 255 gives NaN."""
+    n_ctx = cache[0].shape[1]
+    if tokens is None:
+        tokens = n_ctx - first
+    done = host().mxfp4_cache_read(*cache, first, tokens)
+    if done is not None:
+        return done
+    desc = _mx_cache_desc(cache)
+    _require(0 <= first <= n_ctx and 0 <= tokens <= n_ctx - first, f"mxfp4_cache_read: slots {first} to {first + tokens} of {n_ctx}")
+    k, v = (torch.empty((desc.batch, tokens, desc.n_kv_heads, desc.head_dim), dtype=_BF16, device=cache[0].device) for _ in range(2))
+    if k.numel():
+        with torch.cuda.device(k.device):
+            check(lib().tllm_mxfp4_cache_read_bf16(C.byref(desc), first, tokens, k.data_ptr(), v.data_ptr(), _stream()), "mxfp4_cache_read")
+    return k, v
+
+
+def mxfp4_attention(q: torch.Tensor, cache: Mxfp4Cache, sinks: torch.Tensor | None, sm_scale: float, bandwidth: int | None, start_q: torch.Tensor,
+                    kv_len_hint: int | None = None) -> torch.Tensor:
+    """``attention`` over a cache in MXFP4: ``q [bs, n_ctx, n_kv_heads, repeat_kv, 64]`` bf16 -> ``[bs, n_ctx, n_heads * 64]``.
+
+    ``start_q`` (int32 or int64, read on the device) has one element or one per row: query ``i`` of row ``b`` sits at position ``start_q[b] + i``
+    and sees the slots up to there (``bandwidth`` of them, if given). A query that sees none gives zeros; what it does not see, NaN
+    included, is nothing to it. Any number of queries: drafts to verify, a chat's next turn, a prompt. ``kv_len_hint`` (the most keys that
+    a query sees, as far as the host knows) plans the launch; the result never depends on it."""
+    done = host().mxfp4_attention(q, *cache, sinks, sm_scale, bandwidth, start_q, kv_len_hint)
+    if done is not None:
+        return done
+    desc = _mx_cache_desc(cache, q, sinks, start_q)
+    _require(q.ndim == 5 and q.dtype == _BF16, "mxfp4_attention: q must be bfloat16 [bs, n_ctx, n_kv_heads, repeat_kv, 64]")
+    bs, n_ctx, n_kv_heads, repeat_kv, head_dim = q.shape
+    _require((bs, n_kv_heads, head_dim) == (desc.batch, desc.n_kv_heads, desc.head_dim), f"mxfp4_attention: q {tuple(q.shape)} for a cache of {desc.batch} rows of {desc.n_kv_heads} heads of {desc.head_dim}")
+    if head_dim != 64:
+        raise NotImplementedError("mxfp4_attention: the HIP kernels are built for head_dim 64")
+    n_heads = n_kv_heads * repeat_kv
+    _require(sinks is None or (sinks.dtype == _BF16 and sinks.shape == (n_heads,)), f"mxfp4_attention: sinks are bfloat16 [{n_heads}]")
+    start_q = _row_ints(start_q, bs, "mxfp4_attention: start_q")
+    sinks = sinks if sinks is None else sinks.contiguous()
+    ok = q.stride(4) == 1 and q.stride(3) == 64 and q.stride(2) == 64 * repeat_kv and q.stride(1) % 8 == 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+    q = q if ok else _aligned(q)
+    window = min(int(bandwidth), 2**31 - 1) if bandwidth else 0
+    hint = 0 if kv_len_hint is None else max(int(kv_len_hint), 1)
+    o = torch.empty((bs, n_ctx, n_heads * 64), dtype=_BF16, device=q.device)
+    if o.numel():
+        need = lib().tllm_mxfp4_attention_workspace_bytes(bs, n_ctx, desc.n_slots, n_kv_heads, repeat_kv, window, hint)
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        with torch.cuda.device(q.device):
+            check(lib().tllm_mxfp4_attention_bf16(q.data_ptr(), q.stride(0), q.stride(1), C.byref(desc), sinks.data_ptr() if sinks is not None else None,
+                                                  o.data_ptr(), o.stride(0), o.stride(1), n_ctx, repeat_kv, float(sm_scale), window, start_q.data_ptr(),
+                                                  int(start_q.dtype == torch.int64), int(start_q.shape[0] > 1), hint, work.data_ptr(), need, _stream()),
+                  "mxfp4_attention")
+    return o
+
+
+def mxfp4_attention_decode(q: torch.Tensor, cache: Mxfp4Cache, sinks: torch.Tensor | None, sm_scale: float, bandwidth: int | None,
+                           start_q: torch.Tensor, kv_len_hint: int | None = None) -> torch.Tensor:
+    """``attention_decode`` over a cache in MXFP4: one new token per row, ``q [bs, 1, n_kv_heads, repeat_kv, 64]``; else as ``mxfp4_attention``."""
+    _require(q.ndim == 5 and q.shape[1] == 1, "mxfp4_attention_decode: one token per row")
+    return mxfp4_attention(q, cache, sinks, sm_scale, bandwidth, start_q, kv_len_hint)
