@@ -21,29 +21,25 @@ struct MxAttnArgs {
   MxCache c;
   int batch, n_q, n_kv_heads, group, window;
   int row_groups;         // runs of rows (queries x heads of a KV head) that a workgroup takes
-  int splits, fill, keys_shift;
+  int splits, fill, most_shift, least_shift;
   float scale_log2;       // sm_scale * log2 e
 };
 
 namespace {
-constexpr int kNW = 4;                // wavefronts of a workgroup
-constexpr int VROW = 128 + 32;        // V tile row in LDS, bytes: eight keys' 32-byte pieces in different banks
-constexpr int VTILE = 32 * VROW;
-constexpr int AROW = 64 + 1;          // accumulator row in LDS, floats
 constexpr int PART = 66;              // floats of a record in the workspace
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRaise = 8.f;         // log2 units by which a block must exceed the running maximum to move it
+constexpr float kNoRef = -3.0e38f;    // no key has been seen: the reference (finite, so that a masked logit's weight is exp2(-inf); the first key's is infinite and raises it)
+constexpr float kMost = 256.f;        // a block's weights may sum to so much before the reference is raised
 }  // namespace
 
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
 typedef __attribute__((__vector_size__(8 * sizeof(short)))) short i16x8;
-typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
 
-// Context splits for `fill` workgroups a stream over `ctx` visible keys: enough to fill the CUs, beyond that about 2^keys_shift keys each,
-// never less than 128, at most 64. The host plans the launch with it from the size of the cache (or the caller's hint), the kernels evaluate
-// it again with the length that they read.
-__host__ __device__ inline int mx_attn_splits(int fill, int ctx, int keys_shift) {
-  const int cap = ((ctx - 1) >> 7) + 1, by_work = ((ctx - 1) >> keys_shift) + 1;
+// Context splits for `fill` workgroups a stream over `ctx` visible keys: enough to fill the CUs, beyond that about 2^most_shift keys each,
+// never less than 2^least_shift, at most 64. The host plans the launch with it from the size of the cache (or the caller's hint), the
+// kernels evaluate it again with the length that they read.
+__host__ __device__ inline int mx_attn_splits(int fill, int ctx, int most_shift, int least_shift) {
+  const int cap = ((ctx - 1) >> least_shift) + 1, by_work = ((ctx - 1) >> most_shift) + 1;
   int s = fill > by_work ? fill : by_work;
   s = s < cap ? s : cap;
   s = s > 1 ? s : 1;
@@ -60,14 +56,14 @@ __device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int b, int first_
   s.start = mx_row_int(a.start_q, a.start_is_i64, static_cast<int64_t>(b) * a.start_stride);
   const int64_t far = 1ll << 40;                               // (beyond any slot; sums of it stay within 64 bits)
   s.start = s.start < -far ? -far : s.start > far ? far : s.start;
-  const int q0 = first_row / a.group, q1 = last_row / a.group;
+  const int q0 = a.n_q == 1 ? 0 : first_row / a.group, q1 = a.n_q == 1 ? 0 : last_row / a.group;
   int64_t hi = s.start + (q1 < a.n_q ? q1 : a.n_q - 1) + 1;
   hi = hi < 0 ? 0 : hi < a.c.n_slots ? hi : a.c.n_slots;
   int64_t lo = a.window > 0 ? s.start + q0 - a.window + 1 : 0;
   lo = lo < 0 ? 0 : lo < hi ? lo : hi;
   s.lo = static_cast<int>(lo);
   s.hi = static_cast<int>(hi);
-  const int live = mx_attn_splits(a.fill, hi > lo ? s.hi - s.lo : 1, a.keys_shift);
+  const int live = mx_attn_splits(a.fill, hi > lo ? s.hi - s.lo : 1, a.most_shift, a.least_shift);
   s.live = live < a.splits ? live : a.splits;
   return s;
 }
@@ -77,20 +73,31 @@ __device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int b, int first_
 __device__ __forceinline__ float mx_norm(const MxAttnArgs& a, int head, float m, float l) {
   const float sink = a.sinks ? static_cast<float>(a.sinks[head]) * kLog2e : 0.f;
   const float top = fmaxf(m, sink);
-  if (top == -INFINITY) return l == l ? 0.f : l;
   const float f = __builtin_amdgcn_exp2f(m - top);
-  return f / (l * f + __builtin_amdgcn_exp2f(sink - top));
+  const float z = l * f + __builtin_amdgcn_exp2f(sink - top);
+  return z == 0.f ? 0.f : f / z;
 }
 
-// Rows of a workgroup: RT tiles of 16 of the rows r = query * G + head of a KV head. ONE: a single query of up to eight heads, which are
-// held twice, once for each half of a block's keys.
-template <int RT, bool ONE>
-__global__ __launch_bounds__(kNW * 64) void mxfp4_attn_kernel(MxAttnArgs a) {
-  constexpr int RB = ONE ? 8 : 16 * RT;
-  __shared__ __align__(16) unsigned char vt[kNW * VTILE];
-  __shared__ float s_m[kNW][16], s_l[kNW][16];
+__device__ __forceinline__ float mx_power(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// Where 16 bytes (eight values) of a V tile's row are in LDS: rows of 128 bytes, their chunks XORed so that the transposing reads (eight
+// rows x two chunks at a time) and the writes (eight rows x one chunk of either half) have every bank once.
+__device__ __forceinline__ int mx_v_chunk(int key, int chunk) { return key * 128 + ((chunk ^ ((key >> 1 & 3) << 1) ^ (chunk >> 2)) << 4); }
+
+// One query of up to eight heads. A wavefront takes 64 keys at a time: keys 0 - 31 and 32 - 63 of a block are dealt to the two halves of the
+// matrix instruction's sixteen columns, so that eight heads fill it.
+//   S^T = K . Q^T, keys on M, in two tiles of 16 x 2 keys: the k slots of the lane groups g = 0, 1 are a key's two blocks of 32 values, those of
+//   g = 2, 3 the key 32 places on; the columns 0 - 7 have Q in the former and zeros in the latter, the columns 8 - 15 the reverse.
+//   A lane loads 16 bytes of codes and their scale byte straight into that layout. A lane's scores are then four of a tile, all of use.
+//   O = P . V, the weights' registers being the A operand for the block's keys 0 - 31 in the rows 0 - 7 and for 32 - 63 in the rows 8 - 15: two
+//   accumulators, each of which is looked at in one half of its rows. V passes LDS as bf16, for transposing reads.
+template <int NW>
+__global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a) {
+  constexpr int VTILE = 64 * 128;
+  constexpr int AROW = 64 + 1;                                 // accumulator row in LDS, floats
+  __shared__ __align__(16) unsigned char vt[NW * VTILE];
+  __shared__ float s_m[NW][16], s_l[NW][16];
   static_assert(16 * AROW * 4 <= VTILE, "an accumulator fits a tile");
-  static_assert(!ONE || RT == 1, "a single query is one tile");
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
@@ -99,278 +106,484 @@ __global__ __launch_bounds__(kNW * 64) void mxfp4_attn_kernel(MxAttnArgs a) {
   unsigned id = blockIdx.x;
   const int kvh = id % a.n_kv_heads;
   id /= a.n_kv_heads;
-  const int rg = id % a.row_groups;
-  id /= a.row_groups;
   const int b = id % a.batch, split = id / a.batch;
-  const int rows = a.n_q * a.group, row0 = rg * RB;
-  const MxSpan sp = mx_span(a, b, row0, row0 + RB - 1);
-  if (split >= sp.live) return;
-  int chunk = (sp.hi - sp.lo + sp.live - 1) / sp.live;
-  chunk = (chunk + 31) & ~31;
-  const int s_lo = sp.lo + split * chunk < sp.hi ? sp.lo + split * chunk : sp.hi;
-  const int s_hi = s_lo + chunk < sp.hi ? s_lo + chunk : sp.hi;
-  const int nblk = (s_hi - s_lo + 31) >> 5;
+  const int G = a.group;
 
-  // ---- Q as the B operand of S^T = K . Q^T: lane (row r16, k slots 8 g + j)
-  // ONE: the slots of g = 0, 1 are one key's two blocks of 32, those of g = 2, 3 the two of the key 16 places on. The columns 0 - 7 have
-  // Q in the former and zeros in the latter, the columns 8 - 15 the reverse, so that they are the same heads over other keys, no
-  // column is empty, and a lane's scores are four.
-  bf16x8 qf[RT][ONE ? 4 : 2];
-  int upper[RT], lower[RT];                                    // the keys that the lane's row sees
+  bf16x8 qf[4];
+  {
+    const int head = kvh * G + ((r16 & 7) < G ? r16 & 7 : G - 1);                  // (columns beyond the group repeat its last head; never stored)
+    const bf16* const qr = a.q + b * a.q_bs + head * 64 + 32 * (g & 1);
+    const bool mine = (g >> 1) == (r16 >> 3);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    int row = row0 + (ONE ? r16 & 7 : 16 * rt + r16);
-    row = row < rows ? row : rows - 1;                         // (rows that are not there repeat the last one; never stored)
-    const int i = row / a.group, head = kvh * a.group + row - i * a.group;
-    const bf16* const qr = a.q + b * a.q_bs + i * a.q_ts + head * 64;
-    const int64_t up = sp.start + i < a.c.n_slots - 1 ? sp.start + i : a.c.n_slots - 1, low = a.window > 0 ? sp.start + i - a.window + 1 : 0;
-    upper[rt] = static_cast<int>(up > -1 ? up : -1);
-    lower[rt] = static_cast<int>(low < 0 ? 0 : low < a.c.n_slots ? low : a.c.n_slots);
-    if constexpr (ONE) {
-      const bool mine = (g >> 1) == (r16 >> 3);
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(qr + 32 * (g & 1) + 8 * st);
-        qf[rt][st] = __builtin_bit_cast(bf16x8, mine ? w : u32x4{0u, 0u, 0u, 0u});
-      }
-    } else {
-#pragma unroll
-      for (int st = 0; st < 2; ++st) qf[rt][st] = *reinterpret_cast<const bf16x8*>(qr + 16 * g + 8 * st);
+    for (int t = 0; t < 4; ++t) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(qr + 8 * t);
+      qf[t] = __builtin_bit_cast(bf16x8, mine ? w : u32x4{0u, 0u, 0u, 0u});
     }
   }
+  const MxSpan sp = mx_span(a, b, 0, 0);
+  if (split >= sp.live) return;
+  const int len = sp.hi - sp.lo, nblk = (len + 63) >> 6;
+  const int first = split * NW + wave, step = sp.live * NW;     // the stream's wavefronts take its blocks in turn
 
-  const int64_t kv_off = b * a.c.bs + kvh * a.c.hs, sc_off = b * a.c.sbs + kvh * a.c.shs;
+  const int64_t kv_off = b * a.c.bs + kvh * a.c.hs + sp.lo * a.c.ts, sc_off = b * a.c.sbs + kvh * a.c.shs + sp.lo * a.c.sts;
   const unsigned char *const kp = a.c.blocks[0] + kv_off, *const vp = a.c.blocks[1] + kv_off;
   const unsigned char *const ksp = a.c.scales[0] + sc_off, *const vsp = a.c.scales[1] + sc_off;
-  const unsigned ts = static_cast<unsigned>(a.c.ts), sts = static_cast<unsigned>(a.c.sts);
   unsigned char* const vtile = vt + wave * VTILE;
 
-  float m_run[RT], l_run[RT];                                  // of row r16 (the sum: this lane's share of it)
-  f32x4 acc[RT][4];                                            // O: lane (d = 16 nb + r16, rows 4 g + i)
+  // A lane's places in a block: of the two tiles of K, of the two halves of V. In the last block rows past the end are held to the last key,
+  // a visible one, so that no byte that the query does not see gets near the matrix cores.
+  const int64_t blk_bytes = 64 * a.c.ts, blk_scales = 64 * a.c.sts;
+  unsigned off[2][8];                                          // [whole, last]: K, K + 16 rows, V, V + 32 rows; their scales
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m_run[rt] = -INFINITY;
-    l_run[rt] = 0.f;
+  for (int e = 0; e < 2; ++e) {
+    const unsigned last = e == 0 ? 63u : static_cast<unsigned>((len - 1) & 63);
+    const unsigned ts = static_cast<unsigned>(a.c.ts), sts = static_cast<unsigned>(a.c.sts);
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) acc[rt][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 2; ++t) {
+      const unsigned kr = min(16u * t + r16 + 32u * (g >> 1), last), vr = min(32u * t + (lane >> 1), last);
+      off[e][t] = kr * ts + 16 * (g & 1);
+      off[e][2 + t] = vr * ts + 16 * (lane & 1);
+      off[e][4 + t] = kr * sts + (g & 1);
+      off[e][6 + t] = vr * sts + (lane & 1);
+    }
   }
-
-  // A block's loads. Rows past the end are clamped to the last key, which is a visible one; their weights are zero.
-  struct Block {
-    u32x4 k, v;
-    unsigned ks[2], vs;
+  u32x4 kc[2], vc[2];
+  unsigned ks[2], vs[2];
+  auto load_block = [&](int blk) __attribute__((always_inline)) {
+    const unsigned char *const kb = kp + blk * blk_bytes, *const vb = vp + blk * blk_bytes, *const ksb = ksp + blk * blk_scales, *const vsb = vsp + blk * blk_scales;
+    const bool end = blk == nblk - 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      kc[t] = *reinterpret_cast<const u32x4*>(kb + (end ? off[1][t] : off[0][t]));
+      ks[t] = ksb[end ? off[1][4 + t] : off[0][4 + t]];
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      vc[t] = *reinterpret_cast<const u32x4*>(vb + (end ? off[1][2 + t] : off[0][2 + t]));
+      vs[t] = vsb[end ? off[1][6 + t] : off[0][6 + t]];
+    }
   };
-  auto load_block = [&](int blk, Block& w) __attribute__((always_inline)) {
-    const int k0 = s_lo + 32 * blk;
-    const unsigned last = s_hi - k0 - 1;
-    const unsigned char *const kb = kp + static_cast<int64_t>(k0) * a.c.ts, *const vb = vp + static_cast<int64_t>(k0) * a.c.ts;
-    const unsigned char *const ksb = ksp + static_cast<int64_t>(k0) * a.c.sts, *const vsb = vsp + static_cast<int64_t>(k0) * a.c.sts;
-    auto held = [&](unsigned r) { return r < last ? r : last; };
-    if constexpr (ONE) {
-      const unsigned r = held(r16 + 16 * (g >> 1));
-      w.k = *reinterpret_cast<const u32x4*>(kb + r * ts + 16 * (g & 1));
-      w.ks[0] = ksb[r * sts + (g & 1)];
-    } else {
+  // where the lane's 64 bytes of V go, and where the transposing reads want them from: within 16 lanes, lane 4 r + c has the address of four d
+  // (quad c of sixteen) of key r and gets one d (its own of the sixteen) of the four keys
+  unsigned char* const v_to = vtile + (lane >> 1) * 128;
+  int v_chunk[4], v_from[4];
 #pragma unroll
-      for (int kb2 = 0; kb2 < 2; ++kb2) {
-        const unsigned r = held(16 * kb2 + r16);
-        const u32x2 two = *reinterpret_cast<const u32x2*>(kb + r * ts + 8 * g);
-        w.k[2 * kb2] = two[0];
-        w.k[2 * kb2 + 1] = two[1];
-        w.ks[kb2] = ksb[r * sts + (g >> 1)];
-      }
-    }
-    const unsigned r = held(lane >> 1);
-    w.v = *reinterpret_cast<const u32x4*>(vb + r * ts + 16 * (lane & 1));
-    w.vs = vsb[r * sts + (lane & 1)];
-  };
-  // keys up to `seen_hi` and from `seen_lo` on are seen by every row
-  const int64_t first_at = sp.start + row0 / a.group, last_i = (row0 + RB - 1) / a.group;
-  const int64_t last_low = a.window > 0 ? sp.start + (last_i < a.n_q ? last_i : a.n_q - 1) - a.window + 1 : 0;
-  const int seen_hi = static_cast<int>(first_at < s_hi - 1 ? (first_at > -1 ? first_at : -1) : s_hi - 1);
-  const int seen_lo = static_cast<int>(last_low < 0 ? 0 : last_low < a.c.n_slots ? last_low : a.c.n_slots);
-  auto power = [](unsigned byte) { return __builtin_bit_cast(float, byte << 23); };
+  for (int t = 0; t < 4; ++t) v_chunk[t] = mx_v_chunk(lane >> 1, 4 * (lane & 1) + t) - (lane >> 1) * 128;
+#pragma unroll
+  for (int nb = 0; nb < 4; ++nb) v_from[nb] = mx_v_chunk(4 * g + (r16 >> 2), 2 * nb + (r16 >> 1 & 1)) + (r16 & 1) * 8;
 
-  Block cur;
-  if (wave < nblk) load_block(wave, cur);
-  for (int blk = wave; blk < nblk; blk += kNW) {
-    const int k0 = s_lo + 32 * blk;
-    // ---- S^T
-    f32x4 st[RT][ONE ? 1 : 2];
-    if constexpr (ONE) {
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  float ref = kNoRef, l_run = 0.f;                             // of column r16 (the sum: this lane's share of it)
+  f32x4 acc[2][4];                                             // [half of the keys]; lane (d = 16 nb + r16, rows 4 g + i)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_bf16x8(cur.k[t], power(cur.ks[0])), qf[0][t], s, 0, 0, 0);
-      st[0][0] = s;
-    } else {
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const bf16x8 k0f = mx_bf16x8(cur.k[2 * kb], power(cur.ks[kb])), k1f = mx_bf16x8(cur.k[2 * kb + 1], power(cur.ks[kb]));
+    for (int nb = 0; nb < 4; ++nb) acc[h][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (first < nblk) load_block(first);
+  for (int blk = first; blk < nblk; blk += step) {
+    f32x4 st[2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          f32x4 s = {0.f, 0.f, 0.f, 0.f};
-          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0f, qf[rt][0], s, 0, 0, 0);
-          st[rt][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1f, qf[rt][1], s, 0, 0, 0);
-        }
-      }
-    }
-    // ---- V into the wavefront's tile, as bf16
-    // A NaN that only some of the rows see may not reach the others as 0 x NaN: it is put aside as zeros and added behind (rare).
-    unsigned long long bad = 0;
-    unsigned vs = cur.vs;
-    u32x4 vc = cur.v;
-    if constexpr (!ONE) {
-      bad = __builtin_amdgcn_ballot_w64(vs == 255u);
-      if (bad != 0) {
-        vc = vs == 255u ? u32x4{0u, 0u, 0u, 0u} : vc;
-        vs = vs == 255u ? 0u : vs;
-      }
+    for (int t = 0; t < 2; ++t) {
+      st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_bf16x8(kc[t][w], mx_power(ks[t])), qf[w], st[t], 0, 0, 0);
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) *reinterpret_cast<bf16x8*>(vtile + (lane >> 1) * VROW + (lane & 1) * 64 + t * 16) = mx_bf16x8(vc[t], power(vs));
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) *reinterpret_cast<bf16x8*>(v_to + 4096 * t + v_chunk[w]) = mx_bf16x8(vc[t][w], mx_power(vs[t]));
     // The next block's loads go out before the rest of this one. Unconditional: the last round asks for its own block again.
-    load_block(blk + kNW < nblk ? blk + kNW : blk, cur);
+    load_block(blk + step < nblk ? blk + step : blk);
 
-    // ---- online softmax: this lane holds keys k0 + 4 g + i of row r16 (ONE: 16 on in the columns 8 - 15), and 16 on
-    bf16x8 pa[RT];                                             // A operand of P . V: k slot j <-> key 4 g + j (j < 4), 16 + 4 g + j - 4
-    const bool masked = ONE ? k0 + 31 >= s_hi : k0 + 31 > seen_hi || k0 < seen_lo;     // (a single query sees all of its span)
+    // ---- weights: this lane has keys 16 t + 4 g + i of its half of the block
+    float sc[8], p[8];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      constexpr int NK = ONE ? 4 : 8;
-      float sc[NK];
+    for (int j = 0; j < 8; ++j) sc[j] = st[j >> 2][j & 3];
+    if (blk == nblk - 1) {
 #pragma unroll
-      for (int j = 0; j < NK; ++j) sc[j] = st[rt][j >> 2][j & 3];
-      if (masked) {
+      for (int j = 0; j < 8; ++j) sc[j] = 64 * blk + 16 * (j >> 2) + 4 * g + (j & 3) + 32 * (r16 >> 3) < len ? sc[j] : -INFINITY;
+    }
+    auto weights = [&]() __attribute__((always_inline)) {
+      float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < NK; ++j) {
-          const int key = k0 + 4 * g + (j & 3) + 16 * (ONE ? r16 >> 3 : j >> 2);
-          sc[j] = key < s_hi && (ONE || (key <= upper[rt] && key >= lower[rt])) ? sc[j] : -INFINITY;
-        }
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(fmaf(sc[j], a.scale_log2, -ref));
+        sum += p[j];
       }
+      return sum;
+    };
+    float sum = weights();
+    // The reference -- the largest logit, when it was last raised -- is raised only where a lane's weights have outgrown it.
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMost) != 0, 0)) {
       float top = sc[0];
 #pragma unroll
-      for (int j = 1; j < NK; ++j) top = fmaxf(top, sc[j]);
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j]);
       top = max_over_lane_bits_16_32(top) * a.scale_log2;
-      const bool raise = top > m_run[rt] + kRaise;
-      if (__any(raise)) {
-        const float m_new = raise ? top : m_run[rt];
-        const float alpha = raise ? __builtin_amdgcn_exp2f(m_run[rt] - m_new) : 1.f;
-        m_run[rt] = m_new;
-        l_run[rt] *= alpha;
+      const float moved = top > ref ? top : ref;
+      const float alpha = __builtin_amdgcn_exp2f(ref - moved);
+      ref = moved;
+      l_run *= alpha;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float al = __shfl(alpha, 4 * g + i, 64);
+      for (int i = 0; i < 4; ++i) {
+        const float al = __shfl(alpha, 4 * g + i, 64);
 #pragma unroll
-          for (int nb = 0; nb < 4; ++nb) acc[rt][nb][i] *= al;
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int nb = 0; nb < 4; ++nb) acc[h][nb][i] *= al;
       }
-      const float ref = m_run[rt] == -INFINITY ? 0.f : m_run[rt];
-      bf16 p[NK];
+      // (pinned as whole registers: the copies that join the two paths stay in this one)
 #pragma unroll
-      for (int j = 0; j < NK; ++j) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(sc[j], a.scale_log2, -ref));
-        p[j] = static_cast<bf16>(e);                           // the weights in bf16, as the matrix cores take them; their fp32 values are summed
-        l_run[rt] += e;
-      }
-      if constexpr (ONE) {
-        const bf16 z = static_cast<bf16>(0.f);
-        const bool second = r16 >= 8;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          pa[rt][j] = second ? z : p[j];
-          pa[rt][4 + j] = second ? p[j] : z;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pa[rt][j] = p[j];
-      }
+        for (int nb = 0; nb < 4; ++nb) asm volatile("" : "+v"(acc[h][nb]));
+      sum = weights();
     }
-    // ---- O += P . V: the B operand (lane: d = 16 nb + r16, eight keys) out of transposing reads
+    l_run += sum;
+    bf16x8 pa;                                                 // A operand of P . V: k slot j <-> key 4 g + j (j < 4), 16 + 4 g + j - 4 of the half
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pa[j] = static_cast<bf16>(p[j]);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
-      i16x4 half[2];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) i16x4*)(vtile + (16 * u + 4 * g + (r16 >> 2)) * VROW + (16 * nb + 4 * (r16 & 3)) * 2));
-      const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      for (int nb = 0; nb < 4; ++nb) {
+        i16x4 part[2];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) acc[rt][nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[rt], vf, acc[rt][nb], 0, 0, 0);
-    }
+        for (int u = 0; u < 2; ++u)
+          part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(vtile + v_from[nb] + 4096 * h + 2048 * u));
+        acc[h][nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa, __builtin_bit_cast(bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7)),
+                                                             acc[h][nb], 0, 0, 0);
+      }
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if constexpr (!ONE) {
-      for (; bad != 0; bad &= bad - 1) {
-        const int at = __builtin_ctzll(bad), key = k0 + (at >> 1);
+  }
+
+  // ---- the wavefronts meet: sixteen columns of each, the heads over either half of the keys
+  const float l = sum_over_lane_bits_16_32(l_run);
+  if (g == 0) {
+    s_m[wave][r16] = ref;
+    s_l[wave][r16] = l;
+  }
+  float* const mine = reinterpret_cast<float*>(vtile);         // (this wavefront is past its last read of the tile)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+  for (int nb = 0; nb < 4; ++nb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t p = sp.start + (row0 + 16 * rt + 4 * g + i) / a.group;
-            if (key < s_hi && key <= p && (a.window == 0 || key > p - a.window)) {
+    for (int i = 0; i < 4; ++i) {
+      const float x = acc[0][nb][i], y = acc[1][nb][i];
+      mine[(4 * g + i) * AROW + 16 * nb + r16] = g < 2 ? x : y;
+    }
+  __syncthreads();
+  // thread -> (head, every TPR-th of its 64 values)
+  constexpr int TPR = NW * 64 / 8, DPT = 64 / TPR > 0 ? 64 / TPR : 1;
+  const int eh = tid / TPR, ed = tid % TPR;
+  if (eh >= G || ed >= 64) return;
+  float m_all = kNoRef;
 #pragma unroll
-              for (int nb = 0; nb < 4; ++nb) acc[rt][nb][i] = (nb >> 1) == (at & 1) ? __builtin_nanf("") : acc[rt][nb][i];
-            }
-          }
+  for (int w = 0; w < 2 * NW; ++w) m_all = fmaxf(m_all, s_m[w >> 1][8 * (w & 1) + eh]);
+  float l_all = 0.f, o[DPT] = {};
+#pragma unroll
+  for (int w = 0; w < 2 * NW; ++w) {
+    const int row = 8 * (w & 1) + eh;
+    const float f = __builtin_amdgcn_exp2f(s_m[w >> 1][row] - m_all);      // (0 for a wavefront that saw no key)
+    l_all += s_l[w >> 1][row] * f;
+    const float* const from = reinterpret_cast<const float*>(vt + (w >> 1) * VTILE) + row * AROW + ed;
+#pragma unroll
+    for (int j = 0; j < DPT; ++j) o[j] += from[TPR * j] * f;
+  }
+  const int head = kvh * G + eh;
+  if (a.splits > 1) {
+    float* const p = a.part + ((static_cast<int64_t>(split) * a.batch + b) * (a.n_kv_heads * G) + head) * PART;
+#pragma unroll
+    for (int j = 0; j < DPT; ++j) p[ed + TPR * j] = o[j];
+    if (ed == 0) {
+      p[64] = m_all;
+      p[65] = l_all;
+    }
+    return;
+  }
+  const float f = mx_norm(a, head, m_all, l_all);
+  bf16* const to = a.out + b * a.out_bs + head * 64;
+#pragma unroll
+  for (int j = 0; j < DPT; ++j) to[ed + TPR * j] = static_cast<bf16>(o[j] * f);
+}
+
+// Any number of rows r = query * G + head of a KV head, RT tiles of 32 of them to a wavefront, 32 keys at a time. KG wavefronts share a run of
+// rows' keys and meet in LDS; the others of a workgroup have runs of their own.
+//   S^T = K . Q^T on 32 x 32 x 16, keys on M: lanes l and l + 32 have the two blocks of 32 values of key l, 16 bytes of codes and a scale byte as
+//   they lie in the cache, and a lane owns one row (column) with 16 of the 32 keys, so that maximum, sum and rescaling are its own but for
+//   one exchange between the halves of the wavefront.
+//   O^T = V^T . P^T: the scores' registers are, pairwise, the B operand when the k slots are read as a permutation of the keys; V passes LDS
+//   as bf16 for transposing reads, as above.
+template <int RT, int KG, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs a) {
+  constexpr int RB = 32 * RT;                                  // rows of a run
+  constexpr int RUNS = NW / KG;                                // runs of a workgroup
+  constexpr int VTILE = 32 * 128;
+  constexpr int SHARE = 34 * 64;                               // floats that a wavefront hands over for a tile of rows
+  constexpr int SMEM = KG > 1 && NW * SHARE * 4 > NW * VTILE ? NW * SHARE * 4 : NW * VTILE;
+  static_assert(RUNS * KG == NW, "wavefronts of a workgroup");
+  __shared__ __align__(16) unsigned char smem[SMEM];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, h = lane >> 5;
+  const int run = wave / KG, kg = wave % KG;
+
+  // the splits are the slowest part of the index; the rows that see most keys come first
+  unsigned id = blockIdx.x;
+  const int kvh = id % a.n_kv_heads;
+  id /= a.n_kv_heads;
+  const int b = id % a.batch;
+  id /= a.batch;
+  const int rg = a.row_groups - 1 - static_cast<int>(id % a.row_groups), split = id / a.row_groups;
+  const int rows = a.n_q * a.group, row0 = (rg * RUNS + run) * RB;
+
+  bf16x8 qf[RT][4];
+  int query[RT], head[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    int row = row0 + 32 * rt + l31;
+    row = row < rows ? row : rows - 1;                         // (rows that are not there repeat the last one; never stored)
+    query[rt] = row / a.group;
+    head[rt] = kvh * a.group + row - query[rt] * a.group;
+    const bf16* const qr = a.q + b * a.q_bs + query[rt] * a.q_ts + head[rt] * 64 + 32 * h;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) qf[rt][t] = *reinterpret_cast<const bf16x8*>(qr + 8 * t);
+  }
+  // (a span of the workgroup's rows where its wavefronts share them, of the run's own otherwise)
+  const MxSpan sp = mx_span(a, b, row0, row0 + RB - 1);
+  if (KG == NW && split >= sp.live) return;
+  const bool idle = row0 >= rows || split >= sp.live;
+  const int len = idle ? 0 : sp.hi - sp.lo, nblk = (len + 31) >> 5;
+  const int first = split * KG + kg, step = sp.live * KG;
+
+  int upper[RT], lower[RT];                                    // the keys that the lane's row sees, counted from sp.lo
+  int seen_hi = 0x7fffffff, seen_lo = 0;                       // keys that every row of the wavefront sees
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int64_t up = sp.start + query[rt] - sp.lo, low = up - a.window + 1;
+    upper[rt] = static_cast<int>(up < -1 ? -1 : up < len - 1 ? up : len - 1);
+    lower[rt] = static_cast<int>(a.window == 0 || low < 0 ? 0 : low < len ? low : len);
+  }
+  {
+    const int q0 = row0 / a.group, q1r = (row0 + RB - 1) / a.group, q1 = q1r < a.n_q ? q1r : a.n_q - 1;
+    const int64_t up = sp.start + q0 - sp.lo, low = sp.start + q1 - sp.lo - a.window + 1;
+    seen_hi = static_cast<int>(up < -1 ? -1 : up < len - 1 ? up : len - 1);
+    seen_lo = static_cast<int>(a.window == 0 || low < 0 ? 0 : low < len ? low : len);
+  }
+
+  const int64_t kv_off = b * a.c.bs + kvh * a.c.hs + sp.lo * a.c.ts, sc_off = b * a.c.sbs + kvh * a.c.shs + sp.lo * a.c.sts;
+  const unsigned char *const kp = a.c.blocks[0] + kv_off, *const vp = a.c.blocks[1] + kv_off;
+  const unsigned char *const ksp = a.c.scales[0] + sc_off, *const vsp = a.c.scales[1] + sc_off;
+  unsigned char* const vtile = smem + wave * VTILE;
+
+  // rows past the end of the last block are held to the last key
+  const int64_t blk_bytes = 32 * a.c.ts, blk_scales = 32 * a.c.sts;
+  unsigned off[2][4];                                          // [whole, last]: K, V; their scales
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const unsigned last = e == 0 ? 31u : static_cast<unsigned>((len - 1) & 31);
+    const unsigned ts = static_cast<unsigned>(a.c.ts), sts = static_cast<unsigned>(a.c.sts);
+    const unsigned kr = min(static_cast<unsigned>(l31), last), vr = min(static_cast<unsigned>(lane >> 1), last);
+    off[e][0] = kr * ts + 16 * h;
+    off[e][1] = vr * ts + 16 * (lane & 1);
+    off[e][2] = kr * sts + h;
+    off[e][3] = vr * sts + (lane & 1);
+  }
+  u32x4 kc, vc;
+  unsigned ks, vs;
+  auto load_block = [&](int blk) __attribute__((always_inline)) {
+    const bool end = blk == nblk - 1;
+    kc = *reinterpret_cast<const u32x4*>(kp + blk * blk_bytes + (end ? off[1][0] : off[0][0]));
+    ks = (ksp + blk * blk_scales)[end ? off[1][2] : off[0][2]];
+    vc = *reinterpret_cast<const u32x4*>(vp + blk * blk_bytes + (end ? off[1][1] : off[0][1]));
+    vs = (vsp + blk * blk_scales)[end ? off[1][3] : off[0][3]];
+  };
+  unsigned char* const v_to = vtile + (lane >> 1) * 128;
+  int v_chunk[4], v_from[2];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) v_chunk[t] = mx_v_chunk(lane >> 1, 4 * (lane & 1) + t) - (lane >> 1) * 128;
+  // V^T fragment (A operand of O^T): lane = d; lane j of each 16 has the address of four d (quad j % 4 of the lane group's sixteen) of key j / 4 of
+  // the four that this half of the wavefront takes
+#pragma unroll
+  for (int db = 0; db < 2; ++db) v_from[db] = mx_v_chunk(4 * h + ((lane & 15) >> 2), 4 * db + 2 * (l31 >> 4) + (lane >> 1 & 1)) + (lane & 1) * 8;      // + 8 keys u, + 16 keys cc
+
+  float ref[RT], l_run[RT];
+  f32x16 o[RT][2];
+  const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    ref[rt] = kNoRef;
+    l_run[rt] = 0.f;
+    o[rt][0] = zero;
+    o[rt][1] = zero;
+  }
+
+  if (first < nblk) load_block(first);
+  for (int blk = first; blk < nblk; blk += step) {
+    const int k0 = 32 * blk;
+    // ---- S^T
+    f32x16 s[RT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const bf16x8 kf = mx_bf16x8(kc[t], mx_power(ks));
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[rt][t], t == 0 ? zero : s[rt], 0, 0, 0);
+    }
+    // ---- V into the wavefront's tile, as bf16
+    // A NaN that only some of the rows see may not reach the others as 0 x NaN: it is put aside as zeros and added behind (rare).
+    const unsigned long long bad = __builtin_amdgcn_ballot_w64(vs == 255u);
+    if (__builtin_expect(bad != 0, 0)) {
+      vc = vs == 255u ? u32x4{0u, 0u, 0u, 0u} : vc;
+      vs = vs == 255u ? 0u : vs;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) *reinterpret_cast<bf16x8*>(v_to + v_chunk[w]) = mx_bf16x8(vc[w], mx_power(vs));
+    // The next block's loads go out before the rest of this one. Unconditional: the last round asks for its own block again.
+    load_block(blk + step < nblk ? blk + step : blk);
+
+    const bool masked = k0 + 31 > seen_hi || k0 < seen_lo;
+    u32x4 p[RT][2];                                            // P^T in bf16, as operand registers
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (masked) {
+        const int du = upper[rt] - k0 - 4 * h, dl = lower[rt] - k0 - 4 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[rt][r] = 8 * (r >> 2) + (r & 3) <= du && 8 * (r >> 2) + (r & 3) >= dl ? s[rt][r] : -INFINITY;
       }
+      auto weights = [&]() __attribute__((always_inline)) {
+        float sum = 0.f;
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[rt][2 * m], a.scale_log2, -ref[rt])), y = __builtin_amdgcn_exp2f(fmaf(s[rt][2 * m + 1], a.scale_log2, -ref[rt]));
+          sum += x + y;
+          const bf16x2 v = {static_cast<bf16>(x), static_cast<bf16>(y)};
+          p[rt][m >> 2][m & 3] = __builtin_bit_cast(unsigned, v);
+        }
+        return sum;
+      };
+      float sum = weights();
+      // The reference -- the largest logit, when it was last raised -- is raised only where a lane's weights have outgrown it.
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMost) != 0, 0)) {
+        float top = s[rt][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[rt][r]);
+        float x, y;
+        lane_xor32_pair(top, &x, &y);
+        top = fmaxf(x, y) * a.scale_log2;
+        const float moved = top > ref[rt] ? top : ref[rt];
+        const float alpha = __builtin_amdgcn_exp2f(ref[rt] - moved);
+        ref[rt] = moved;
+        l_run[rt] *= alpha;
+#pragma unroll
+        for (int db = 0; db < 2; ++db) {
+          asm volatile("" : "+v"(o[rt][db]));
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[rt][db][r] *= alpha;
+          asm volatile("" : "+v"(o[rt][db]));
+        }
+        sum = weights();
+      }
+      l_run[rt] += sum;
+    }
+    // ---- O^T += V^T . P^T
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        i16x4 part[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(vtile + v_from[db] + 2048 * cc + 1024 * u));
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, __builtin_bit_cast(bf16x8, p[rt][cc]), o[rt][db], 0, 0, 0);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (unsigned long long left = bad; left != 0; left &= left - 1) {
+      const int at = __builtin_ctzll(left), key = k0 + (at >> 1);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        if (key >= lower[rt] && key <= upper[rt]) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            o[rt][0][r] = at & 1 ? o[rt][0][r] : __builtin_nanf("");
+            o[rt][1][r] = at & 1 ? __builtin_nanf("") : o[rt][1][r];
+          }
+        }
     }
   }
 
-  // ---- the wavefronts meet, a tile of rows at a time
+  // ---- the sink joins the denominator, or a record leaves. A lane has 16-byte runs of one row's values; where wavefronts share the rows
+  // they first meet in LDS, 32 / KG of the 32 values a lane to each.
+  constexpr int RPG = 32 / KG;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    if (rt > 0) __syncthreads();
-    const float l = sum_over_lane_bits_16_32(l_run[rt]);
-    if (g == 0) {
-      s_m[wave][r16] = m_run[rt];
-      s_l[wave][r16] = l;
+    float l, m = ref[rt];
+    {
+      float x, y;
+      lane_xor32_pair(l_run[rt], &x, &y);
+      l = x + y;
     }
-    float* const mine = reinterpret_cast<float*>(vtile);       // (this wavefront is past its last read of the tile)
-    __builtin_amdgcn_wave_barrier();
+    float v[RPG];
+    if constexpr (KG > 1) {
+      float* const shares = reinterpret_cast<float*>(smem);
+      __syncthreads();                                         // (all are past their last read of the tiles, or of the tile of rows before)
+      float* const mine = shares + wave * SHARE + lane;
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mine[(4 * g + i) * AROW + 16 * nb + r16] = acc[rt][nb][i];
-    __syncthreads();
-    // thread -> (row, every TPR-th of its 64 values)
-    constexpr int NR = ONE ? 8 : 16, TPR = kNW * 64 / NR, DPT = 64 / TPR;
-    const int er = tid / TPR, ed = tid % TPR, row = row0 + 16 * rt + er;
-    if (er >= NR || row >= rows) continue;
-    float m_all = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kNW; ++w)
-#pragma unroll
-      for (int t = er; t < 16; t += NR) m_all = fmaxf(m_all, s_m[w][t]);
-    const float ref = m_all == -INFINITY ? 0.f : m_all;
-    float l_all = 0.f, o[DPT] = {};
-#pragma unroll
-    for (int w = 0; w < kNW; ++w)
-#pragma unroll
-      for (int t = er; t < 16; t += NR) {
-        const float f = __builtin_amdgcn_exp2f(s_m[w][t] - ref);       // (0 for a wavefront that saw no key)
-        l_all += s_l[w][t] * f;
-        const float* const from = reinterpret_cast<const float*>(vt + w * VTILE) + t * AROW + ed;
-#pragma unroll
-        for (int j = 0; j < DPT; ++j) o[j] += from[TPR * j] * f;
+      for (int r = 0; r < 32; ++r) {
+        const float x = o[rt][r >> 4][r & 15];
+        mine[r * 64] = x;
       }
-    const int i = row / a.group, head = kvh * a.group + row - i * a.group;
+      mine[32 * 64] = m;
+      mine[33 * 64] = l;
+      __syncthreads();
+      const float* const from = shares + run * KG * SHARE + lane;
+      m = kNoRef;
+#pragma unroll
+      for (int k = 0; k < KG; ++k) m = fmaxf(m, from[k * SHARE + 32 * 64]);
+      l = 0.f;
+#pragma unroll
+      for (int r = 0; r < RPG; ++r) v[r] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KG; ++k) {
+        const float f = __builtin_amdgcn_exp2f(from[k * SHARE + 32 * 64] - m);      // (0 for a wavefront that saw no key)
+        l = fmaf(from[k * SHARE + 33 * 64], f, l);
+#pragma unroll
+        for (int r = 0; r < RPG; ++r) v[r] = fmaf(from[k * SHARE + (RPG * kg + r) * 64], f, v[r]);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 32; ++r) v[r] = o[rt][r >> 4][r & 15];
+    }
+    if (row0 + 32 * rt + l31 >= rows) continue;
+    // value rr = RPG kg + r: d = 32 (rr / 16) + 8 (rr / 4 % 4) + 4 h + rr % 4
     if (a.splits > 1) {
-      float* const p = a.part + (((static_cast<int64_t>(split) * a.batch + b) * a.n_q + i) * (a.n_kv_heads * a.group) + head) * PART;
+      if (split >= sp.live) continue;
+      float* const p = a.part + (((static_cast<int64_t>(split) * a.batch + b) * a.n_q + query[rt]) * (a.n_kv_heads * a.group) + head[rt]) * PART;
 #pragma unroll
-      for (int j = 0; j < DPT; ++j) p[ed + TPR * j] = o[j];
-      if (ed == 0) {
-        p[64] = m_all;
-        p[65] = l_all;
+      for (int r = 0; r < RPG; ++r) {
+        const int rr = RPG * kg + r;
+        p[32 * (rr >> 4) + 8 * (rr >> 2 & 3) + 4 * h + (rr & 3)] = v[r];
       }
+      if (kg == 0) p[64 + h] = h == 0 ? m : l;
       continue;
     }
-    const float f = mx_norm(a, head, m_all, l_all);
-    bf16* const to = a.out + b * a.out_bs + i * a.out_ts + head * 64;
+    const float f = mx_norm(a, head[rt], m, l);
+    bf16* const to = a.out + b * a.out_bs + query[rt] * a.out_ts + head[rt] * 64;
 #pragma unroll
-    for (int j = 0; j < DPT; ++j) to[ed + TPR * j] = static_cast<bf16>(o[j] * f);
+    for (int r = 0; r < RPG; r += 4) {
+      const int rr = RPG * kg + r;
+      bf16x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = static_cast<bf16>(v[r + e] * f);
+      *reinterpret_cast<bf16x4*>(to + 32 * (rr >> 4) + 8 * (rr >> 2 & 3) + 4 * h) = w;
+    }
   }
 }
 
@@ -386,14 +599,14 @@ __global__ __launch_bounds__(64) void mxfp4_attn_reduce_kernel(MxAttnArgs a, int
   const int64_t stride = static_cast<int64_t>(a.batch) * a.n_q * n_heads * PART;
   const float* const p0 = a.part + ((static_cast<int64_t>(b) * a.n_q + i) * n_heads + head) * PART;
   // requested before the start position is known; what splits that take no part have there is not used
-  const float m_raw = lane < a.splits ? p0[lane * stride + 64] : -INFINITY, l_raw = lane < a.splits ? p0[lane * stride + 65] : 0.f;
+  const float m_raw = lane < a.splits ? p0[lane * stride + 64] : kNoRef, l_raw = lane < a.splits ? p0[lane * stride + 65] : 0.f;
   float v[8];
 #pragma unroll
   for (int u = 0; u < 8; ++u) v[u] = p0[(u < a.splits ? u : a.splits - 1) * stride + lane];
   const int live = mx_span(a, b, row0, row0 + rows_per_group - 1).live;
-  const float m_s = lane < live ? m_raw : -INFINITY;
+  const float m_s = lane < live ? m_raw : kNoRef;
   const float m_all = wave_max(m_s);
-  const float f_s = __builtin_amdgcn_exp2f(m_s - (m_all == -INFINITY ? 0.f : m_all));
+  const float f_s = __builtin_amdgcn_exp2f(m_s - m_all);
   const float l_all = wave_sum(lane < live ? l_raw * f_s : 0.f);
   float o = 0.f;
   for (int s0 = 0; s0 < live; s0 += 8) {
@@ -418,24 +631,39 @@ using namespace tllm;
 namespace {
 struct MxAttnPlan {
   bool one;
-  int tiles, row_groups, splits, fill, keys_shift;
+  int tiles, key_groups, waves;       // of the kernel for any rows: tiles of 32 rows to a wavefront, wavefronts that share their keys, wavefronts
+  int row_groups, rows_per_run;
+  int splits, fill, most_shift, least_shift;
 };
-constexpr int kFill = 1024;           // workgroups that fill the CUs
-constexpr int kKeysShift = 11;
+#ifndef T_FILL
+#define T_FILL 512
+#define T_MOST 11
+#define T_LEAST 8
+#define T_LONG 1024
+#endif
 
 MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window) {
-  MxAttnPlan p;
-  const int64_t rows = n_q * group;
+  MxAttnPlan p{};
+  const int64_t rows = n_q * group, streams = batch * n_kv_heads;
   p.one = n_q == 1 && group <= 8;
-  p.tiles = p.one || rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int rb = p.one ? 8 : 16 * p.tiles;
-  p.row_groups = (int)((rows + rb - 1) / rb);
-  const int64_t span = (int64_t)window + (rb + group - 1) / group;          // keys that a workgroup's queries can see together
+  p.waves = 4;
+  p.key_groups = 4;
+  p.tiles = rows <= 32 ? 1 : 2;
+  if (!p.one && (rows + 255) / 256 * streams >= T_LONG / 4) p.key_groups = 1;
+  p.rows_per_run = p.one ? 8 : 32 * p.tiles;
+  const int64_t per_wg = p.rows_per_run * (p.one ? 1 : p.waves / p.key_groups);
+  p.row_groups = (int)((rows + per_wg - 1) / per_wg);
+  const int64_t span = (int64_t)window + (p.rows_per_run + group - 1) / group;       // keys that a run's queries can see together
   const int64_t ctx = window > 0 && span < n_slots ? span : n_slots;
-  const int64_t units = batch * n_kv_heads * p.row_groups;
-  p.fill = (int)((kFill + units - 1) / units);
-  p.keys_shift = kKeysShift;
-  p.splits = mx_attn_splits(p.fill, (int)(ctx > 0 ? ctx : 1), p.keys_shift);
+  const int64_t units = streams * p.row_groups;
+  p.fill = (int)((T_FILL + units - 1) / units);
+  p.most_shift = T_MOST;
+  p.least_shift = T_LEAST;
+  if (p.key_groups == 1) {
+    p.fill = 1;
+    p.most_shift = 30;
+  }
+  p.splits = mx_attn_splits(p.fill, (int)(ctx > 0 ? ctx : 1), p.most_shift, p.least_shift);
   return p;
 }
 
@@ -450,11 +678,6 @@ extern "C" int tllm_mxfp4_attention_splits(int64_t batch, int64_t n_q, int64_t n
 extern "C" int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint) {
   const int s = tllm_mxfp4_attention_splits(batch, n_q, n_slots, n_kv_heads, group, window, kv_len_hint);
   return s > 1 ? (int64_t)s * batch * n_q * n_kv_heads * group * PART * 4 : 0;
-}
-
-template <int RT, bool ONE>
-static void launch(const MxAttnArgs& a, unsigned wgs, hipStream_t st) {
-  hipLaunchKernelGGL((mxfp4_attn_kernel<RT, ONE>), dim3(wgs), dim3(kNW * 64), 0, st, a);
 }
 
 extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, int64_t q_token_stride, const TllmMxCache* cache, const void* sinks, void* out,
@@ -505,15 +728,17 @@ extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, 
   a.row_groups = p.row_groups;
   a.splits = p.splits;
   a.fill = p.fill;
-  a.keys_shift = p.keys_shift;
+  a.most_shift = p.most_shift;
+  a.least_shift = p.least_shift;
   a.scale_log2 = sm_scale * kLog2e;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p.one) launch<1, true>(a, (unsigned)wgs, st);
-  else if (p.tiles == 1) launch<1, false>(a, (unsigned)wgs, st);
-  else if (p.tiles == 2) launch<2, false>(a, (unsigned)wgs, st);
-  else launch<4, false>(a, (unsigned)wgs, st);
+  const dim3 grid((unsigned)wgs), block(p.waves * 64);
+  if (p.one) hipLaunchKernelGGL(mxfp4_attn_one_kernel<4>, grid, block, 0, st, a);
+  else if (p.tiles == 1) hipLaunchKernelGGL((mxfp4_attn_rows_kernel<1, 4, 4>), grid, block, 0, st, a);
+  else if (p.key_groups == 4) hipLaunchKernelGGL((mxfp4_attn_rows_kernel<2, 4, 4>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((mxfp4_attn_rows_kernel<2, 1, 4>), grid, block, 0, st, a);
   const int rc = check_launch("mxfp4_attention");
   if (rc != TLLM_OK || p.splits == 1) return rc;
-  hipLaunchKernelGGL(mxfp4_attn_reduce_kernel, dim3((unsigned)(batch * n_q * n_heads)), dim3(64), 0, st, a, p.one ? 8 : 16 * p.tiles);
+  hipLaunchKernelGGL(mxfp4_attn_reduce_kernel, dim3((unsigned)(batch * n_q * n_heads)), dim3(64), 0, st, a, p.rows_per_run);
   return check_launch("mxfp4_attention(reduce)");
 }
