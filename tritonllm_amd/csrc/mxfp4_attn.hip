@@ -21,28 +21,33 @@ struct MxAttnArgs {
   MxCache c;
   int batch, n_q, n_kv_heads, group, window;
   int row_groups;         // runs of rows (queries x heads of a KV head) that a workgroup takes
-  int splits, fill, most_shift, least_shift;
+  int splits, fill, most; // planned splits; what mx_attn_splits goes by
   float scale_log2;       // sm_scale * log2 e
 };
 
 namespace {
 constexpr int PART = 66;              // floats of a record in the workspace
+// Splits, one query of 8 heads, us. One workgroup walks up to 1024 keys alone (no second launch): 300 keys 4.9, split 6.7; 600 5.7, 6.7; 1000 6.4,
+// 6.8; 8 rows of 1024 6.5, 7.2; but 2000 9.0 and 6.8. A workgroup to a CU: 49 rows of up to 2048 11.9, with two 16.6; 32 of 4096 16.1, 19.2; one of
+// 32768 11.2, 13.2 -- until each has 4096 keys: 8 rows of 32768 28.6, with one of 8192 31.6 and two of 2048 30.4; 8 of 131072 96, 94 and 104. At
+// least 256 keys: one row of 4096 7.3, of 512 and more 7.6 - 9.0.
+constexpr int kUnsplit = 1024, kLeastShift = 8, kMostKeys = 4096, kFill = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoRef = -3.0e38f;    // no key has been seen: the reference (finite, so that a masked logit's weight is exp2(-inf); the first key's is infinite and raises it)
-constexpr float kMost = 256.f;        // a block's weights may sum to so much before the reference is raised
+constexpr float kMostSum = 256.f;       // a block's weights may sum to so much before the reference is raised
 }  // namespace
 
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
 typedef __attribute__((__vector_size__(8 * sizeof(short)))) short i16x8;
 
-// Context splits for `fill` workgroups a stream over `ctx` visible keys: enough to fill the CUs, beyond that about 2^most_shift keys each,
-// never less than 2^least_shift, at most 64. The host plans the launch with it from the size of the cache (or the caller's hint), the
-// kernels evaluate it again with the length that they read.
-__host__ __device__ inline int mx_attn_splits(int fill, int ctx, int most_shift, int least_shift) {
-  const int cap = ((ctx - 1) >> least_shift) + 1, by_work = ((ctx - 1) >> most_shift) + 1;
+// Context splits for `fill` workgroups a stream over `ctx` visible keys: one up to kUnsplit keys, then enough to fill the CUs, beyond that about
+// kMostKeys keys each, never less than kLeastKeys, at most 64. The host plans the launch with it from the size of the cache (or the
+// caller's hint), the kernels evaluate it again with the length that they read.
+__host__ __device__ inline int mx_attn_splits(int fill, int ctx, int most) {
+  const int cap = ((ctx - 1) >> kLeastShift) + 1, by_work = (ctx - 1) / most + 1;
   int s = fill > by_work ? fill : by_work;
   s = s < cap ? s : cap;
-  s = s > 1 ? s : 1;
+  s = s > 1 && ctx > kUnsplit ? s : 1;
   return s < 64 ? s : 64;
 }
 
@@ -63,7 +68,7 @@ __device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int b, int first_
   lo = lo < 0 ? 0 : lo < hi ? lo : hi;
   s.lo = static_cast<int>(lo);
   s.hi = static_cast<int>(hi);
-  const int live = mx_attn_splits(a.fill, hi > lo ? s.hi - s.lo : 1, a.most_shift, a.least_shift);
+  const int live = mx_attn_splits(a.fill, hi > lo ? s.hi - s.lo : 1, a.most);
   s.live = live < a.splits ? live : a.splits;
   return s;
 }
@@ -88,11 +93,30 @@ __device__ __forceinline__ int mx_v_chunk(int key, int chunk) { return key * 128
 // matrix instruction's sixteen columns, so that eight heads fill it.
 //   S^T = K . Q^T, keys on M, in two tiles of 16 x 2 keys: the k slots of the lane groups g = 0, 1 are a key's two blocks of 32 values, those of
 //   g = 2, 3 the key 32 places on; the columns 0 - 7 have Q in the former and zeros in the latter, the columns 8 - 15 the reverse.
-//   A lane loads 16 bytes of codes and their scale byte straight into that layout. A lane's scores are then four of a tile, all of use.
+//   A lane's scores are then four of a tile, all of use.
 //   O = P . V, the weights' registers being the A operand for the block's keys 0 - 31 in the rows 0 - 7 and for 32 - 63 in the rows 8 - 15: two
 //   accumulators, each of which is looked at in one half of its rows. V passes LDS as bf16, for transposing reads.
-template <int NW>
-__global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a) {
+// yes ? a : b for a condition that all lanes share, on a scalar mask in one instruction.
+__device__ __forceinline__ unsigned mx_choose(bool yes, unsigned a, unsigned b) {
+  unsigned x;
+  asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(x) : "s"(yes ? ~0u : 0u), "v"(a), "v"(b));
+  return x;
+}
+
+// DENSE: a head's scale bytes lie next to each other (two bytes from slot to slot).
+template <bool DENSE>
+__device__ __forceinline__ unsigned mx_scale_pair(const unsigned char* p, int64_t sts, int behind) {
+  typedef unsigned __attribute__((aligned(2))) u32_a2;
+  if constexpr (DENSE) {
+    return *reinterpret_cast<const u32_a2*>(p);
+  } else {
+    const unsigned char* const q = behind > 0 ? p + sts : p;   // (two single bytes each: a slot's may lie anywhere)
+    return p[0] | p[1] << 8 | q[0] << 16 | static_cast<unsigned>(q[1]) << 24;
+  }
+}
+
+template <bool DENSE, int NW>
+__global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a) {
   constexpr int VTILE = 64 * 128;
   constexpr int AROW = 64 + 1;                                 // accumulator row in LDS, floats
   __shared__ __align__(16) unsigned char vt[NW * VTILE];
@@ -120,49 +144,64 @@ __global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a
       qf[t] = __builtin_bit_cast(bf16x8, mine ? w : u32x4{0u, 0u, 0u, 0u});
     }
   }
-  const MxSpan sp = mx_span(a, b, 0, 0);
-  if (split >= sp.live) return;
-  const int len = sp.hi - sp.lo, nblk = (len + 63) >> 6;
-  const int first = split * NW + wave, step = sp.live * NW;     // the stream's wavefronts take its blocks in turn
+  // Without a window the keys begin at slot 0 and the wavefront's first block is known ahead of the start position, whose load takes as long as
+  // the block's own: it is asked for at once (and not looked at where the context turns out to be shorter).
+  int lo = 0;
+  if (a.window > 0) lo = min(mx_span(a, b, 0, 0).lo, a.c.n_slots - 1);      // (a slot of the cache, also where a window behind its end has none)
+  const int first = split * NW + wave;
+  const int nall = (a.c.n_slots - lo + 63) >> 6;                // blocks that the cache has from there on
 
-  const int64_t kv_off = b * a.c.bs + kvh * a.c.hs + sp.lo * a.c.ts, sc_off = b * a.c.sbs + kvh * a.c.shs + sp.lo * a.c.sts;
+  const int64_t kv_off = b * a.c.bs + kvh * a.c.hs + lo * a.c.ts, sc_off = b * a.c.sbs + kvh * a.c.shs + lo * a.c.sts;
   const unsigned char *const kp = a.c.blocks[0] + kv_off, *const vp = a.c.blocks[1] + kv_off;
   const unsigned char *const ksp = a.c.scales[0] + sc_off, *const vsp = a.c.scales[1] + sc_off;
   unsigned char* const vtile = vt + wave * VTILE;
 
-  // A lane's places in a block: of the two tiles of K, of the two halves of V. In the last block rows past the end are held to the last key,
-  // a visible one, so that no byte that the query does not see gets near the matrix cores.
+  // Loads: 32 keys' codes at a time, 16 bytes a lane as they lie in memory (a CU's cache serves four neighbouring lanes' 64 bytes in one access, and
+  // lanes whose pieces lie apart one by one); the scale bytes of 64 keys and 64 values in one load, two keys' to a lane. K's codes go
+  // through LDS into the operand's order, scale bytes from lane to lane.
+  // Behind the last slot of the cache rows are held to the last one (whose pair of keys ends with it).
   const int64_t blk_bytes = 64 * a.c.ts, blk_scales = 64 * a.c.sts;
-  unsigned off[2][8];                                          // [whole, last]: K, K + 16 rows, V, V + 32 rows; their scales
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const unsigned last = e == 0 ? 63u : static_cast<unsigned>((len - 1) & 63);
-    const unsigned ts = static_cast<unsigned>(a.c.ts), sts = static_cast<unsigned>(a.c.sts);
+  const int slots = a.c.n_slots - lo - 64 * (nall - 1);         // in the last one of them
+  const unsigned char* const sbase = (lane < 32 ? ksp : vsp) - 2;      // (two bytes ahead, so that offsets from it are positive)
+  unsigned off[2][2];                                          // [whole, last]: rows lane / 2 and 32 + lane / 2
+  unsigned soff[2];
+  const int pair = 2 * (lane & 31);
+  {
+    const unsigned ts = static_cast<unsigned>(a.c.ts);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const unsigned kr = min(16u * t + r16 + 32u * (g >> 1), last), vr = min(32u * t + (lane >> 1), last);
-      off[e][t] = kr * ts + 16 * (g & 1);
-      off[e][2 + t] = vr * ts + 16 * (lane & 1);
-      off[e][4 + t] = kr * sts + (g & 1);
-      off[e][6 + t] = vr * sts + (lane & 1);
+      const int r = 32 * t + (lane >> 1);
+      off[0][t] = static_cast<unsigned>(r) * ts + 16 * (lane & 1);
+      off[1][t] = static_cast<unsigned>(min(r, slots - 1)) * ts + 16 * (lane & 1);
     }
+    soff[0] = pair * static_cast<unsigned>(a.c.sts) + 2;
+    soff[1] = (DENSE ? min(pair, slots - 2) : min(pair, slots - 1)) * static_cast<int>(a.c.sts) + 2;
   }
-  u32x4 kc[2], vc[2];
-  unsigned ks[2], vs[2];
-  auto load_block = [&](int blk) __attribute__((always_inline)) {
-    const unsigned char *const kb = kp + blk * blk_bytes, *const vb = vp + blk * blk_bytes, *const ksb = ksp + blk * blk_scales, *const vsb = vsp + blk * blk_scales;
-    const bool end = blk == nblk - 1;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      kc[t] = *reinterpret_cast<const u32x4*>(kb + (end ? off[1][t] : off[0][t]));
-      ks[t] = ksb[end ? off[1][4 + t] : off[0][4 + t]];
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      vc[t] = *reinterpret_cast<const u32x4*>(vb + (end ? off[1][2 + t] : off[0][2 + t]));
-      vs[t] = vsb[end ? off[1][6 + t] : off[0][6 + t]];
-    }
+  const int pair_shift = DENSE && pair == slots - 1 ? 16 : 0;  // (in the last block)
+  struct Block {
+    u32x4 k[2], v[2];
+    unsigned s;
   };
+  auto load_block = [&](int at, Block& r) __attribute__((always_inline)) {
+    const int blk = at < nall ? at : nall - 1;                 // (a block that is not there: any)
+    const unsigned char *const kb = kp + blk * blk_bytes, *const vb = vp + blk * blk_bytes;
+    const bool end = blk == nall - 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const unsigned x = mx_choose(end, off[1][t], off[0][t]);
+      r.k[t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb + x));
+      r.v[t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vb + x));
+    }
+    r.s = mx_scale_pair<DENSE>(sbase + blk * blk_scales + mx_choose(end, soff[1], soff[0]), a.c.sts, end ? slots - 1 - pair : 1);
+  };
+  Block even, odd;
+  load_block(first, even);
+  __builtin_amdgcn_sched_barrier(0);                           // (in the loop's order, so that it can wait for the one and not the other)
+  const MxSpan sp = mx_span(a, b, 0, 0);
+  if (split >= sp.live) return;
+  const int len = sp.hi - sp.lo, nblk = (len + 63) >> 6, step = sp.live * NW;      // the stream's wavefronts take its blocks in turn
+  load_block(first + step, odd);
+  __builtin_amdgcn_sched_barrier(0);
   // where the lane's 64 bytes of V go, and where the transposing reads want them from: within 16 lanes, lane 4 r + c has the address of four d
   // (quad c of sixteen) of key r and gets one d (its own of the sixteen) of the four keys
   unsigned char* const v_to = vtile + (lane >> 1) * 128;
@@ -172,6 +211,12 @@ __global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) v_from[nb] = mx_v_chunk(4 * g + (r16 >> 2), 2 * nb + (r16 >> 1 & 1)) + (r16 & 1) * 8;
 
+  // K's codes in the operand's order: tile t, lane (key 16 t + r16 + 32 (g / 2), block g % 2). Scale bytes: a lane of the load has four, of two
+  // neighbouring slots; lanes 0 - 31 keys', 32 - 63 values'.
+  const int k_from = (r16 + 32 * (g >> 1)) * 32 + 16 * (g & 1);
+  const int k_lane = 4 * ((r16 + 32 * (g >> 1)) >> 1), k_shift = 16 * (r16 & 1) + 8 * (g & 1);
+  const int v_lane = 4 * (32 + (lane >> 2)), v_shift = 8 * (lane & 3);
+
   float ref = kNoRef, l_run = 0.f;                             // of column r16 (the sum: this lane's share of it)
   f32x4 acc[2][4];                                             // [half of the keys]; lane (d = 16 nb + r16, rows 4 g + i)
 #pragma unroll
@@ -179,8 +224,40 @@ __global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[h][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  if (first < nblk) load_block(first);
-  for (int blk = first; blk < nblk; blk += step) {
+  // A block's arithmetic; in its middle the block after the next is asked for (unconditionally: also one behind the last that is looked at).
+  auto process = [&](int blk, Block& r) __attribute__((always_inline)) {
+    const bool end = blk == nblk - 1;
+    // K's codes through LDS; the tile of V follows in the same place (a wavefront's LDS operations stay in order)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) *reinterpret_cast<u32x4*>(vtile + 1024 * t + 16 * lane) = r.k[t];
+    const unsigned pairs = blk == nall - 1 ? r.s >> pair_shift : r.s;
+    unsigned ks[2], vs[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      ks[t] = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(k_lane + 32 * t, static_cast<int>(pairs))) >> k_shift & 255u;
+      vs[t] = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(v_lane + 64 * t, static_cast<int>(pairs))) >> v_shift & 255u;
+    }
+    u32x4 kc[2], vc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      kc[t] = *reinterpret_cast<const u32x4*>(vtile + k_from + 512 * t);
+      vc[t] = r.v[t];
+    }
+    if (__builtin_expect(end, 0)) {                            // what lies behind the last key may be anything: zeros
+      const int left = len - 64 * blk;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const bool k_in = 16 * t + r16 + 32 * (g >> 1) < left, v_in = 32 * t + (lane >> 1) < left;
+        kc[t] = k_in ? kc[t] : u32x4{0u, 0u, 0u, 0u};
+        ks[t] = k_in ? ks[t] : 0u;
+        vc[t] = v_in ? vc[t] : u32x4{0u, 0u, 0u, 0u};
+        vs[t] = v_in ? vs[t] : 0u;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) *reinterpret_cast<bf16x8*>(v_to + 4096 * t + v_chunk[w]) = mx_bf16x8(vc[t][w], mx_power(vs[t]));
     f32x4 st[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -188,18 +265,13 @@ __global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a
 #pragma unroll
       for (int w = 0; w < 4; ++w) st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_bf16x8(kc[t][w], mx_power(ks[t])), qf[w], st[t], 0, 0, 0);
     }
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) *reinterpret_cast<bf16x8*>(v_to + 4096 * t + v_chunk[w]) = mx_bf16x8(vc[t][w], mx_power(vs[t]));
-    // The next block's loads go out before the rest of this one. Unconditional: the last round asks for its own block again.
-    load_block(blk + step < nblk ? blk + step : blk);
+    load_block(blk + 2 * step, r);
 
     // ---- weights: this lane has keys 16 t + 4 g + i of its half of the block
     float sc[8], p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) sc[j] = st[j >> 2][j & 3];
-    if (blk == nblk - 1) {
+    if (end) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) sc[j] = 64 * blk + 16 * (j >> 2) + 4 * g + (j & 3) + 32 * (r16 >> 3) < len ? sc[j] : -INFINITY;
     }
@@ -214,7 +286,7 @@ __global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a
     };
     float sum = weights();
     // The reference -- the largest logit, when it was last raised -- is raised only where a lane's weights have outgrown it.
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMost) != 0, 0)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMostSum) != 0, 0)) {
       float top = sc[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j]);
@@ -258,7 +330,13 @@ __global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a
       }
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  };
+  int blk = first;
+  for (; blk + step < nblk; blk += 2 * step) {
+    process(blk, even);
+    process(blk + step, odd);
   }
+  if (blk < nblk) process(blk, even);
 
   // ---- the wavefronts meet: sixteen columns of each, the heads over either half of the keys
   const float l = sum_over_lane_bits_16_32(l_run);
@@ -316,7 +394,7 @@ __global__ __launch_bounds__(NW * 64, 4) void mxfp4_attn_one_kernel(MxAttnArgs a
 //   one exchange between the halves of the wavefront.
 //   O^T = V^T . P^T: the scores' registers are, pairwise, the B operand when the k slots are read as a permutation of the keys; V passes LDS
 //   as bf16 for transposing reads, as above.
-template <int RT, int KG, int NW>
+template <bool DENSE, int RT, int KG, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs a) {
   constexpr int RB = 32 * RT;                                  // rows of a run
   constexpr int RUNS = NW / KG;                                // runs of a workgroup
@@ -378,28 +456,33 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   const unsigned char *const ksp = a.c.scales[0] + sc_off, *const vsp = a.c.scales[1] + sc_off;
   unsigned char* const vtile = smem + wave * VTILE;
 
-  // rows past the end of the last block are held to the last key
+  // Loads as above: 32 keys' codes, 16 bytes a lane as they lie in memory, and in one load the scale bytes of two neighbouring slots to a lane,
+  // keys' in lanes 0 - 15, values' in 16 - 31 (and the same in the other 32).
   const int64_t blk_bytes = 32 * a.c.ts, blk_scales = 32 * a.c.sts;
-  unsigned off[2][4];                                          // [whole, last]: K, V; their scales
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const unsigned last = e == 0 ? 31u : static_cast<unsigned>((len - 1) & 31);
-    const unsigned ts = static_cast<unsigned>(a.c.ts), sts = static_cast<unsigned>(a.c.sts);
-    const unsigned kr = min(static_cast<unsigned>(l31), last), vr = min(static_cast<unsigned>(lane >> 1), last);
-    off[e][0] = kr * ts + 16 * h;
-    off[e][1] = vr * ts + 16 * (lane & 1);
-    off[e][2] = kr * sts + h;
-    off[e][3] = vr * sts + (lane & 1);
-  }
-  u32x4 kc, vc;
-  unsigned ks, vs;
+  const int slots = a.c.n_slots - sp.lo - 32 * (nblk - 1);      // that the cache has from the last block's first key on
+  const unsigned char* const sbase = (lane & 16 ? vsp : ksp) - 2;
+  const int pair = 2 * (lane & 15);
+  unsigned off[2];                                             // [whole, last]
+  unsigned soff[2];
+  off[0] = static_cast<unsigned>(lane >> 1) * static_cast<unsigned>(a.c.ts) + 16 * (lane & 1);
+  off[1] = static_cast<unsigned>(min(lane >> 1, slots - 1)) * static_cast<unsigned>(a.c.ts) + 16 * (lane & 1);
+  soff[0] = pair * static_cast<unsigned>(a.c.sts) + 2;
+  soff[1] = (DENSE ? min(pair, slots - 2) : min(pair, slots - 1)) * static_cast<int>(a.c.sts) + 2;
+  const int pair_shift = DENSE && pair == slots - 1 ? 16 : 0;  // (in the last block)
+  struct Block {
+    u32x4 k, v;
+    unsigned s;
+  } r;
   auto load_block = [&](int blk) __attribute__((always_inline)) {
     const bool end = blk == nblk - 1;
-    kc = *reinterpret_cast<const u32x4*>(kp + blk * blk_bytes + (end ? off[1][0] : off[0][0]));
-    ks = (ksp + blk * blk_scales)[end ? off[1][2] : off[0][2]];
-    vc = *reinterpret_cast<const u32x4*>(vp + blk * blk_bytes + (end ? off[1][1] : off[0][1]));
-    vs = (vsp + blk * blk_scales)[end ? off[1][3] : off[0][3]];
+    const unsigned x = mx_choose(end, off[1], off[0]);
+    r.k = *reinterpret_cast<const u32x4*>(kp + blk * blk_bytes + x);
+    r.v = *reinterpret_cast<const u32x4*>(vp + blk * blk_bytes + x);
+    r.s = mx_scale_pair<DENSE>(sbase + blk * blk_scales + mx_choose(end, soff[1], soff[0]), a.c.sts, end ? slots - 1 - pair : 1);
   };
+  // K's codes pass LDS into the operand's order, lane (key l31, block h); the keys 16 - 31 have their blocks the other way round there, for the banks
+  const int k_to = 16 * (lane ^ (lane >> 5)), k_from = l31 * 32 + 16 * (h ^ (l31 >> 4));
+  const int k_lane = 4 * (l31 >> 1), k_shift = 16 * (l31 & 1) + 8 * h, v_lane = 4 * (16 + (lane >> 2)), v_shift = 8 * (lane & 3);
   unsigned char* const v_to = vtile + (lane >> 1) * 128;
   int v_chunk[4], v_from[2];
 #pragma unroll
@@ -423,6 +506,29 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   if (first < nblk) load_block(first);
   for (int blk = first; blk < nblk; blk += step) {
     const int k0 = 32 * blk;
+    const bool end = blk == nblk - 1;
+    // K's codes through LDS; the tile of V follows in the same place (a wavefront's LDS operations stay in order)
+    *reinterpret_cast<u32x4*>(vtile + k_to) = r.k;
+    const unsigned pairs = end ? r.s >> pair_shift : r.s;
+    const unsigned ks = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(k_lane, static_cast<int>(pairs))) >> k_shift & 255u;
+    unsigned vs = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(v_lane, static_cast<int>(pairs))) >> v_shift & 255u;
+    const u32x4 kc = *reinterpret_cast<const u32x4*>(vtile + k_from);
+    u32x4 vc = r.v;
+    // ---- V into the wavefront's tile, as bf16
+    // What lies behind the last key may be anything: zeros. A NaN that only some of the rows see may not reach the others as 0 x NaN: it is
+    // put aside as zeros and added behind (rare). (A key's NaN goes no further than its own scores.)
+    if (__builtin_expect(end, 0)) {
+      const bool in = k0 + (lane >> 1) < len;
+      vc = in ? vc : u32x4{0u, 0u, 0u, 0u};
+      vs = in ? vs : 0u;
+    }
+    const unsigned long long bad = __builtin_amdgcn_ballot_w64(vs == 255u);
+    if (__builtin_expect(bad != 0, 0)) {
+      vc = vs == 255u ? u32x4{0u, 0u, 0u, 0u} : vc;
+      vs = vs == 255u ? 0u : vs;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) *reinterpret_cast<bf16x8*>(v_to + v_chunk[w]) = mx_bf16x8(vc[w], mx_power(vs));
     // ---- S^T
     f32x16 s[RT];
 #pragma unroll
@@ -431,15 +537,6 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) s[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[rt][t], t == 0 ? zero : s[rt], 0, 0, 0);
     }
-    // ---- V into the wavefront's tile, as bf16
-    // A NaN that only some of the rows see may not reach the others as 0 x NaN: it is put aside as zeros and added behind (rare).
-    const unsigned long long bad = __builtin_amdgcn_ballot_w64(vs == 255u);
-    if (__builtin_expect(bad != 0, 0)) {
-      vc = vs == 255u ? u32x4{0u, 0u, 0u, 0u} : vc;
-      vs = vs == 255u ? 0u : vs;
-    }
-#pragma unroll
-    for (int w = 0; w < 4; ++w) *reinterpret_cast<bf16x8*>(v_to + v_chunk[w]) = mx_bf16x8(vc[w], mx_power(vs));
     // The next block's loads go out before the rest of this one. Unconditional: the last round asks for its own block again.
     load_block(blk + step < nblk ? blk + step : blk);
 
@@ -465,7 +562,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
       };
       float sum = weights();
       // The reference -- the largest logit, when it was last raised -- is raised only where a lane's weights have outgrown it.
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMost) != 0, 0)) {
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > kMostSum) != 0, 0)) {
         float top = s[rt][0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, s[rt][r]);
@@ -506,7 +603,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     for (unsigned long long left = bad; left != 0; left &= left - 1) {
-      const int at = __builtin_ctzll(left), key = k0 + (at >> 1);
+      const int at = __builtin_ctzll(left), key = k0 + (at >> 1);           // (one of the span's)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
         if (key >= lower[rt] && key <= upper[rt]) {
@@ -633,14 +730,8 @@ struct MxAttnPlan {
   bool one;
   int tiles, key_groups, waves;       // of the kernel for any rows: tiles of 32 rows to a wavefront, wavefronts that share their keys, wavefronts
   int row_groups, rows_per_run;
-  int splits, fill, most_shift, least_shift;
+  int splits, fill, most;
 };
-#ifndef T_FILL
-#define T_FILL 512
-#define T_MOST 11
-#define T_LEAST 8
-#define T_LONG 1024
-#endif
 
 MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window) {
   MxAttnPlan p{};
@@ -649,21 +740,20 @@ MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_he
   p.waves = 4;
   p.key_groups = 4;
   p.tiles = rows <= 32 ? 1 : 2;
-  if (!p.one && (rows + 255) / 256 * streams >= T_LONG / 4) p.key_groups = 1;
+  if (!p.one && (rows + 255) / 256 * streams >= 256) p.key_groups = 1;
   p.rows_per_run = p.one ? 8 : 32 * p.tiles;
   const int64_t per_wg = p.rows_per_run * (p.one ? 1 : p.waves / p.key_groups);
   p.row_groups = (int)((rows + per_wg - 1) / per_wg);
   const int64_t span = (int64_t)window + (p.rows_per_run + group - 1) / group;       // keys that a run's queries can see together
   const int64_t ctx = window > 0 && span < n_slots ? span : n_slots;
   const int64_t units = streams * p.row_groups;
-  p.fill = (int)((T_FILL + units - 1) / units);
-  p.most_shift = T_MOST;
-  p.least_shift = T_LEAST;
+  p.fill = (int)((kFill + units - 1) / units);
+  p.most = kMostKeys;
   if (p.key_groups == 1) {
     p.fill = 1;
-    p.most_shift = 30;
+    p.most = 1 << 30;
   }
-  p.splits = mx_attn_splits(p.fill, (int)(ctx > 0 ? ctx : 1), p.most_shift, p.least_shift);
+  p.splits = mx_attn_splits(p.fill, (int)(ctx > 0 ? ctx : 1), p.most);
   return p;
 }
 
@@ -678,6 +768,14 @@ extern "C" int tllm_mxfp4_attention_splits(int64_t batch, int64_t n_q, int64_t n
 extern "C" int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint) {
   const int s = tllm_mxfp4_attention_splits(batch, n_q, n_slots, n_kv_heads, group, window, kv_len_hint);
   return s > 1 ? (int64_t)s * batch * n_q * n_kv_heads * group * PART * 4 : 0;
+}
+
+template <bool DENSE>
+static void launch_attention(const MxAttnPlan& p, const MxAttnArgs& a, dim3 grid, dim3 block, hipStream_t st) {
+  if (p.one) hipLaunchKernelGGL((mxfp4_attn_one_kernel<DENSE, 4>), grid, block, 0, st, a);
+  else if (p.tiles == 1) hipLaunchKernelGGL((mxfp4_attn_rows_kernel<DENSE, 1, 4, 4>), grid, block, 0, st, a);
+  else if (p.key_groups == 4) hipLaunchKernelGGL((mxfp4_attn_rows_kernel<DENSE, 2, 4, 4>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((mxfp4_attn_rows_kernel<DENSE, 2, 1, 4>), grid, block, 0, st, a);
 }
 
 extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, int64_t q_token_stride, const TllmMxCache* cache, const void* sinks, void* out,
@@ -728,15 +826,12 @@ extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, 
   a.row_groups = p.row_groups;
   a.splits = p.splits;
   a.fill = p.fill;
-  a.most_shift = p.most_shift;
-  a.least_shift = p.least_shift;
+  a.most = p.most;
   a.scale_log2 = sm_scale * kLog2e;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)wgs), block(p.waves * 64);
-  if (p.one) hipLaunchKernelGGL(mxfp4_attn_one_kernel<4>, grid, block, 0, st, a);
-  else if (p.tiles == 1) hipLaunchKernelGGL((mxfp4_attn_rows_kernel<1, 4, 4>), grid, block, 0, st, a);
-  else if (p.key_groups == 4) hipLaunchKernelGGL((mxfp4_attn_rows_kernel<2, 4, 4>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((mxfp4_attn_rows_kernel<2, 1, 4>), grid, block, 0, st, a);
+  if (cache->scale_slot_stride == 2 && n_slots > 1) launch_attention<true>(p, a, grid, block, st);
+  else launch_attention<false>(p, a, grid, block, st);
   const int rc = check_launch("mxfp4_attention");
   if (rc != TLLM_OK || p.splits == 1) return rc;
   hipLaunchKernelGGL(mxfp4_attn_reduce_kernel, dim3((unsigned)(batch * n_q * n_heads)), dim3(64), 0, st, a, p.rows_per_run);
