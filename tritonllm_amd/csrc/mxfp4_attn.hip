@@ -408,13 +408,23 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   const int l31 = lane & 31, h = lane >> 5;
   const int run = wave / KG, kg = wave % KG;
 
-  // the splits are the slowest part of the index; the rows that see most keys come first
+  // the splits are the slowest part of the index; the rows that see most keys come first, and where the launch is two workgroups to a CU the
+  // second ones are taken in the opposite order, so that a CU with a long walk gets a short one next to it
   unsigned id = blockIdx.x;
   const int kvh = id % a.n_kv_heads;
   id /= a.n_kv_heads;
+  if constexpr (KG < NW) {
+    const unsigned per_round = 256 / (a.n_kv_heads < 256 ? a.n_kv_heads : 256), n = gridDim.x / a.n_kv_heads;
+    if (n <= 2 * per_round && id >= per_round) id = n + per_round - 1 - id;
+  }
   const int b = id % a.batch;
   id /= a.batch;
-  const int rg = a.row_groups - 1 - static_cast<int>(id % a.row_groups), split = id / a.row_groups;
+  int rg, split;
+  if constexpr (KG == NW) {
+    rg = a.row_groups - 1 - static_cast<int>(id % a.row_groups), split = id / a.row_groups;
+  } else {
+    rg = a.row_groups - 1 - static_cast<int>(id), split = 0;
+  }
   const int rows = a.n_q * a.group, row0 = (rg * RUNS + run) * RB;
 
   bf16x8 qf[RT][4];
@@ -472,8 +482,9 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   struct Block {
     u32x4 k, v;
     unsigned s;
-  } r;
-  auto load_block = [&](int blk) __attribute__((always_inline)) {
+  };
+  auto load_block = [&](int at, Block& r) __attribute__((always_inline)) {
+    const int blk = at < nblk ? at : nblk - 1;                 // (a block that is not there: the last one again)
     const bool end = blk == nblk - 1;
     const unsigned x = mx_choose(end, off[1], off[0]);
     r.k = *reinterpret_cast<const u32x4*>(kp + blk * blk_bytes + x);
@@ -503,8 +514,8 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     o[rt][1] = zero;
   }
 
-  if (first < nblk) load_block(first);
-  for (int blk = first; blk < nblk; blk += step) {
+  // A block's arithmetic; in its middle the block after the next is asked for.
+  auto process = [&](int blk, Block& r) __attribute__((always_inline)) {
     const int k0 = 32 * blk;
     const bool end = blk == nblk - 1;
     // K's codes through LDS; the tile of V follows in the same place (a wavefront's LDS operations stay in order)
@@ -537,15 +548,15 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) s[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[rt][t], t == 0 ? zero : s[rt], 0, 0, 0);
     }
-    // The next block's loads go out before the rest of this one. Unconditional: the last round asks for its own block again.
-    load_block(blk + step < nblk ? blk + step : blk);
+    load_block(blk + 2 * step, r);
 
     const bool masked = k0 + 31 > seen_hi || k0 < seen_lo;
     u32x4 p[RT][2];                                            // P^T in bf16, as operand registers
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      if (masked) {
-        const int du = upper[rt] - k0 - 4 * h, dl = lower[rt] - k0 - 4 * h;
+      if (__builtin_expect(masked, 0)) {
+        int du = upper[rt] - k0 - 4 * h, dl = lower[rt] - k0 - 4 * h;
+        asm volatile("" : "+v"(du), "+v"(dl));                 // (or the comparisons are made for every block)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[rt][r] = 8 * (r >> 2) + (r & 3) <= du && 8 * (r >> 2) + (r & 3) >= dl ? s[rt][r] : -INFINITY;
       }
@@ -614,6 +625,19 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
           }
         }
     }
+  };
+  if (first < nblk) {
+    Block even, odd;
+    load_block(first, even);
+    __builtin_amdgcn_sched_barrier(0);                         // (in the loop's order, so that it can wait for the one and not the other)
+    load_block(first + step, odd);
+    __builtin_amdgcn_sched_barrier(0);
+    int blk = first;
+    for (; blk + step < nblk; blk += 2 * step) {
+      process(blk, even);
+      process(blk + step, odd);
+    }
+    if (blk < nblk) process(blk, even);
   }
 
   // ---- the sink joins the denominator, or a record leaves. A lane has 16-byte runs of one row's values; where wavefronts share the rows
