@@ -3,12 +3,15 @@
 Tolerance of attention. Keys, values and queries are bf16 values, so their products are exact in fp32 and a logit, a sum of 64, is off by at most
 64 2^-23 sm_scale sum|q k|; its exponential's argument is rounded twice more, to 2^-23 of its magnitude, and the exponential itself to 2^-22.
 A weight is then rounded to bf16 (half a step, 2^-8 of it) ahead of the product with the values, whose fp32 sum over n keys is off by n 2^-23 of
-the sum of its magnitudes at most; the denominator is the fp32 sum. The result is rounded to bf16, 2^-8 of it. So with A = sum p|v| / Z
-  |got - want| <= 2^-8 |want| + (1 + 2^-8) A (2^-8 + 2 e + n 2^-23),   e = 64 2^-23 sm_scale max sum|q k| + 2^-22 (max |s| + 16)
-and 2^-133 more, twice the rounding of a bf16 value below the smallest normal one, for values of the smallest scales, and n 2^-126 max|v|: a
-weight below fp32's smallest normal number, 2^-126 of its row's largest, may be none at all (of logits hundreds apart: such a
-weight's value is lost, where the definition still has e^-90 of it; computed so in float64 the loss is what a call is off by)
-(the 2 e for numerator and denominator; 16 covers the running maximum, which lies up to 8 powers of two below the true one)."""
+the sum of its magnitudes at most. The denominator sums either the weights or what they were rounded to; in the latter case, with
+out = N / Z and roundings d_i, the quotient is off by sum w_i d_i (v_i - out) / Z, at most 2^-8 (A + |out|), A = sum p|v| / Z. The result
+is rounded to bf16, 2^-8 of it. So
+  |got - want| <= 2^-8 |want| + (1 + 2^-8) ((A + |want|) 2^-8 + A (2 e + n 2^-23)),   e = 64 2^-23 sm_scale max sum|q k| + 2^-22 (max |s| + 16)
+(the 2 e for numerator and denominator; 16 covers the running reference, which lies up to 8 powers of two below the largest logit or 7 above it)
+and 2^-133 more, twice the rounding of a bf16 value below the smallest normal one, for values of the smallest scales, and n 2^-119 max|v|: a
+weight whose fp32 value is below the smallest normal number, 2^-126, may be none at all, and with the reference 7 powers of two above the
+largest logit that is one of 2^-119 of its row's largest (of logits hundreds apart: such a weight's value is lost, where the definition still
+has e^-83 of it)."""
 import ctypes as C
 import itertools
 import math
@@ -89,7 +92,8 @@ def attention_ref(q, cache, sinks, scale, window, starts):
         want[row, i] = w @ vv / z[..., None]
         a = w @ vv.abs() / z[..., None]
         e = 64 * 2.0**-23 * mag.amax(-1) + 2.0**-22 * (s.abs().amax(-1) + 16)
-        tol[row, i] = 2.0**-8 * want[row, i].abs() + (1 + 2.0**-8) * a * (2.0**-8 + 2 * e + (hi - lo) * 2.0**-23)[..., None] + 2.0**-133 + (hi - lo) * 2.0**-126 * vv.abs().nan_to_num().amax()
+        tol[row, i] = (2.0**-8 * want[row, i].abs() + (1 + 2.0**-8) * ((a + want[row, i].abs()) * 2.0**-8 + a * (2 * e + (hi - lo) * 2.0**-23)[..., None]) + 2.0**-133
+                       + (hi - lo) * 2.0**-119 * vv.abs().nan_to_num().amax())
     return want.view(b, t, -1), tol.view(b, t, -1)
 
 

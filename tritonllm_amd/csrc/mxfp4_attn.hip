@@ -21,7 +21,7 @@ struct MxAttnArgs {
   MxCache c;
   int batch, n_q, n_kv_heads, group, window;
   int row_groups;         // runs of rows (queries x heads of a KV head) that a workgroup takes
-  int splits, fill, most; // planned splits; what mx_attn_splits goes by
+  int splits, fill;       // planned splits; workgroups a stream that fill the CUs
   float scale_log2;       // sm_scale * log2 e
 };
 
@@ -31,9 +31,12 @@ constexpr int PART = 66;              // floats of a record in the workspace
 // 6.8; 8 rows of 1024 6.5, 7.2; but 2000 9.0 and 6.8. A workgroup to a CU: 49 rows of up to 2048 11.9, with two 16.6; 32 of 4096 16.1, 19.2; one of
 // 32768 11.2, 13.2 -- until each has 4096 keys: 8 rows of 32768 28.6, with one of 8192 31.6 and two of 2048 30.4; 8 of 131072 96, 94 and 104. At
 // least 256 keys: one row of 4096 7.3, of 512 and more 7.6 - 9.0.
-constexpr int kUnsplit = 1024, kLeastShift = 8, kMostKeys = 4096, kFill = 256;
+constexpr int kUnsplit = 1024, kLeastShift = 8, kMostShift = 12, kFill = 256;
+constexpr int kManyWgs = 96;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoRef = -3.0e38f;    // no key has been seen: the reference (finite, so that a masked logit's weight is exp2(-inf); the first key's is infinite and raises it)
+constexpr float kLift = 7.f;          // ... or how far it lies above the largest logit that it was raised to
+constexpr int kShare = 34 * 64;       // floats that a wavefront hands over for a tile of 32 rows
 constexpr float kMostSum = 256.f;       // a block's weights may sum to so much before the reference is raised
 }  // namespace
 
@@ -41,10 +44,10 @@ typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
 typedef __attribute__((__vector_size__(8 * sizeof(short)))) short i16x8;
 
 // Context splits for `fill` workgroups a stream over `ctx` visible keys: one up to kUnsplit keys, then enough to fill the CUs, beyond that about
-// kMostKeys keys each, never less than kLeastKeys, at most 64. The host plans the launch with it from the size of the cache (or the
+// 2^kMostShift keys each, never less than 2^kLeastShift, at most 64. The host plans the launch with it from the size of the cache (or the
 // caller's hint), the kernels evaluate it again with the length that they read.
-__host__ __device__ inline int mx_attn_splits(int fill, int ctx, int most) {
-  const int cap = ((ctx - 1) >> kLeastShift) + 1, by_work = (ctx - 1) / most + 1;
+__host__ __device__ inline int mx_attn_splits(int fill, int ctx) {
+  const int cap = ((ctx - 1) >> kLeastShift) + 1, by_work = ((ctx - 1) >> kMostShift) + 1;
   int s = fill > by_work ? fill : by_work;
   s = s < cap ? s : cap;
   s = s > 1 && ctx > kUnsplit ? s : 1;
@@ -68,7 +71,7 @@ __device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int b, int first_
   lo = lo < 0 ? 0 : lo < hi ? lo : hi;
   s.lo = static_cast<int>(lo);
   s.hi = static_cast<int>(hi);
-  const int live = mx_attn_splits(a.fill, hi > lo ? s.hi - s.lo : 1, a.most);
+  const int live = mx_attn_splits(a.fill, hi > lo ? s.hi - s.lo : 1);
   s.live = live < a.splits ? live : a.splits;
   return s;
 }
@@ -88,6 +91,9 @@ __device__ __forceinline__ float mx_power(unsigned byte) { return __builtin_bit_
 // Where 16 bytes (eight values) of a V tile's row are in LDS: rows of 128 bytes, their chunks XORed so that the transposing reads (eight
 // rows x two chunks at a time) and the writes (eight rows x one chunk of either half) have every bank once.
 __device__ __forceinline__ int mx_v_chunk(int key, int chunk) { return key * 128 + ((chunk ^ ((key >> 1 & 3) << 1) ^ (chunk >> 2)) << 4); }
+
+// The same for tiles of 32 rows, whose transposing reads take four rows x four chunks at a time.
+__device__ __forceinline__ int mx_v_chunk4(int key, int chunk) { return key * 128 + ((chunk ^ ((key >> 1 & 1) << 2) ^ (key >> 2 & 1) ^ (chunk >> 2 << 1)) << 4); }
 
 // One query of up to eight heads. A wavefront takes 64 keys at a time: keys 0 - 31 and 32 - 63 of a block are dealt to the two halves of the
 // matrix instruction's sixteen columns, so that eight heads fill it.
@@ -387,45 +393,33 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
   for (int j = 0; j < DPT; ++j) to[ed + TPR * j] = static_cast<bf16>(o[j] * f);
 }
 
-// Any number of rows r = query * G + head of a KV head, RT tiles of 32 of them to a wavefront, 32 keys at a time. KG wavefronts share a run of
-// rows' keys and meet in LDS; the others of a workgroup have runs of their own.
+// RT tiles of 32 of the rows r = query * G + head of a KV head, 32 keys at a time. The KG wavefronts of a workgroup share the keys and meet in
+// LDS at the end.
 //   S^T = K . Q^T on 32 x 32 x 16, keys on M: lanes l and l + 32 have the two blocks of 32 values of key l, 16 bytes of codes and a scale byte as
 //   they lie in the cache, and a lane owns one row (column) with 16 of the 32 keys, so that maximum, sum and rescaling are its own but for
 //   one exchange between the halves of the wavefront.
 //   O^T = V^T . P^T: the scores' registers are, pairwise, the B operand when the k slots are read as a permutation of the keys; V passes LDS
 //   as bf16 for transposing reads, as above.
-template <bool DENSE, int RT, int KG, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs a) {
-  constexpr int RB = 32 * RT;                                  // rows of a run
-  constexpr int RUNS = NW / KG;                                // runs of a workgroup
+template <bool DENSE, int RT, int KG>
+__global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs a) {
+  constexpr int NW = KG, RB = 32 * RT;                         // wavefronts; rows
   constexpr int VTILE = 32 * 128;
-  constexpr int SHARE = 34 * 64;                               // floats that a wavefront hands over for a tile of rows
-  constexpr int SMEM = KG > 1 && NW * SHARE * 4 > NW * VTILE ? NW * SHARE * 4 : NW * VTILE;
-  static_assert(RUNS * KG == NW, "wavefronts of a workgroup");
-  __shared__ __align__(16) unsigned char smem[SMEM];
+  constexpr int SHARE = kShare;
+  static_assert(SHARE * 4 >= VTILE, "the shares are what needs most LDS");
+  extern __shared__ __align__(16) unsigned char smem[];        // NW shares
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
-  const int run = wave / KG, kg = wave % KG;
+  const int kg = wave;
 
-  // the splits are the slowest part of the index; the rows that see most keys come first, and where the launch is two workgroups to a CU the
-  // second ones are taken in the opposite order, so that a CU with a long walk gets a short one next to it
+  // the splits are the slowest part of the index: those that a context does not need are the last
   unsigned id = blockIdx.x;
   const int kvh = id % a.n_kv_heads;
   id /= a.n_kv_heads;
-  if constexpr (KG < NW) {
-    const unsigned per_round = 256 / (a.n_kv_heads < 256 ? a.n_kv_heads : 256), n = gridDim.x / a.n_kv_heads;
-    if (n <= 2 * per_round && id >= per_round) id = n + per_round - 1 - id;
-  }
   const int b = id % a.batch;
   id /= a.batch;
-  int rg, split;
-  if constexpr (KG == NW) {
-    rg = a.row_groups - 1 - static_cast<int>(id % a.row_groups), split = id / a.row_groups;
-  } else {
-    rg = a.row_groups - 1 - static_cast<int>(id), split = 0;
-  }
-  const int rows = a.n_q * a.group, row0 = (rg * RUNS + run) * RB;
+  const int rg = a.row_groups - 1 - static_cast<int>(id % a.row_groups), split = id / a.row_groups;
+  const int rows = a.n_q * a.group, row0 = rg * RB;
 
   bf16x8 qf[RT][4];
   int query[RT], head[RT];
@@ -439,11 +433,9 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
 #pragma unroll
     for (int t = 0; t < 4; ++t) qf[rt][t] = *reinterpret_cast<const bf16x8*>(qr + 8 * t);
   }
-  // (a span of the workgroup's rows where its wavefronts share them, of the run's own otherwise)
   const MxSpan sp = mx_span(a, b, row0, row0 + RB - 1);
-  if (KG == NW && split >= sp.live) return;
-  const bool idle = row0 >= rows || split >= sp.live;
-  const int len = idle ? 0 : sp.hi - sp.lo, nblk = (len + 31) >> 5;
+  if (split >= sp.live) return;
+  const int len = sp.hi - sp.lo, nblk = (len + 31) >> 5;
   const int first = split * KG + kg, step = sp.live * KG;
 
   int upper[RT], lower[RT];                                    // the keys that the lane's row sees, counted from sp.lo
@@ -497,11 +489,11 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   unsigned char* const v_to = vtile + (lane >> 1) * 128;
   int v_chunk[4], v_from[2];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) v_chunk[t] = mx_v_chunk(lane >> 1, 4 * (lane & 1) + t) - (lane >> 1) * 128;
+  for (int t = 0; t < 4; ++t) v_chunk[t] = mx_v_chunk4(lane >> 1, 4 * (lane & 1) + t) - (lane >> 1) * 128;
   // V^T fragment (A operand of O^T): lane = d; lane j of each 16 has the address of four d (quad j % 4 of the lane group's sixteen) of key j / 4 of
   // the four that this half of the wavefront takes
 #pragma unroll
-  for (int db = 0; db < 2; ++db) v_from[db] = mx_v_chunk(4 * h + ((lane & 15) >> 2), 4 * db + 2 * (l31 >> 4) + (lane >> 1 & 1)) + (lane & 1) * 8;      // + 8 keys u, + 16 keys cc
+  for (int db = 0; db < 2; ++db) v_from[db] = mx_v_chunk4(4 * h + ((lane & 15) >> 2), 4 * db + 2 * (l31 >> 4) + (lane >> 1 & 1)) + (lane & 1) * 8;      // + 8 keys u, + 16 keys cc
 
   float ref[RT], l_run[RT];
   f32x16 o[RT][2];
@@ -664,7 +656,7 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
       mine[32 * 64] = m;
       mine[33 * 64] = l;
       __syncthreads();
-      const float* const from = shares + run * KG * SHARE + lane;
+      const float* const from = shares + lane;
       m = kNoRef;
 #pragma unroll
       for (int k = 0; k < KG; ++k) m = fmaxf(m, from[k * SHARE + 32 * 64]);
@@ -685,7 +677,6 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     if (row0 + 32 * rt + l31 >= rows) continue;
     // value rr = RPG kg + r: d = 32 (rr / 16) + 8 (rr / 4 % 4) + 4 h + rr % 4
     if (a.splits > 1) {
-      if (split >= sp.live) continue;
       float* const p = a.part + (((static_cast<int64_t>(split) * a.batch + b) * a.n_q + query[rt]) * (a.n_kv_heads * a.group) + head[rt]) * PART;
 #pragma unroll
       for (int r = 0; r < RPG; ++r) {
@@ -704,6 +695,339 @@ __global__ __launch_bounds__(NW * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = static_cast<bf16>(v[r + e] * f);
       *reinterpret_cast<bf16x4*>(to + 32 * (rr >> 4) + 8 * (rr >> 2 & 3) + 4 * h) = w;
+    }
+  }
+}
+
+// Many rows: a workgroup's four wavefronts have 64 neighbouring rows each and walk the same keys, 64 at a time, which come to bf16 once for all
+// four of them: a thread has 16 bytes of codes of a unit, keys' in the first two wavefronts and values' in the others, and writes
+// their 32 values into one of three stages in LDS while the unit before is worked on. One barrier a unit.
+//   The matrix cores and the vector ALU work at the same time: with one tile's weights (32 keys x 32 rows) the next one's scores are issued in
+//   turn, and the products of the one before. Of block j (32 keys), S^T of tile 1, weights of tile 0 and P . V of block j - 1 in tile 1; then S^T of
+//   block j + 1 in tile 0, weights of tile 1 and P . V of tile 0. Operands of K and of V live from one such half to the next.
+__global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
+  constexpr int KTILE = 64 * 128, STAGE = 2 * KTILE;           // bytes: K [64 keys][64 values], then V
+  __shared__ __align__(16) unsigned char smem[3 * STAGE];
+  __shared__ __align__(8) unsigned s_any[3][2];                // whether a stage's values hold NaN, in its first and in its second 32 keys,
+  __shared__ unsigned long long s_bad[3][2];                   // and in which of the 32 x 2 pieces
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, h = lane >> 5;
+
+  // the rows that see most keys come first, and where the launch is two workgroups to a CU the second ones are taken in the opposite order, so
+  // that a CU with a long walk gets a short one next to it
+  unsigned id = blockIdx.x;
+  const int kvh = id % a.n_kv_heads;
+  id /= a.n_kv_heads;
+  {
+    const unsigned per_round = 256 / (a.n_kv_heads < 256 ? a.n_kv_heads : 256), n = gridDim.x / a.n_kv_heads;
+    if (n <= 2 * per_round && id >= per_round) id = n + per_round - 1 - id;
+  }
+  const int b = id % a.batch, rg = a.row_groups - 1 - static_cast<int>(id / a.batch);
+  const int rows = a.n_q * a.group, row0 = rg * 256 + wave * 64;
+
+  bf16x8 qf[2][4];
+  int query[2], head[2];
+#pragma unroll
+  for (int rt = 0; rt < 2; ++rt) {
+    int row = row0 + 32 * rt + l31;
+    row = row < rows ? row : rows - 1;                         // (rows that are not there repeat the last one; never stored)
+    query[rt] = row / a.group;
+    head[rt] = kvh * a.group + row - query[rt] * a.group;
+    const bf16* const qr = a.q + b * a.q_bs + query[rt] * a.q_ts + head[rt] * 64 + 32 * h;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) qf[rt][t] = *reinterpret_cast<const bf16x8*>(qr + 8 * t);
+  }
+  const MxSpan sp = mx_span(a, b, rg * 256, rg * 256 + 255);
+  const int len = sp.hi - sp.lo, units = (len + 63) >> 6;
+
+  int upper[2], lower[2];                                      // the keys that the lane's row sees, counted from sp.lo
+#pragma unroll
+  for (int rt = 0; rt < 2; ++rt) {
+    const int64_t up = sp.start + query[rt] - sp.lo, low = up - a.window + 1;
+    upper[rt] = static_cast<int>(up < -1 ? -1 : up < len - 1 ? up : len - 1);
+    lower[rt] = static_cast<int>(a.window == 0 || low < 0 ? 0 : low < len ? low : len);
+  }
+  int seen_hi, seen_lo, w_lo, w_hi;                            // keys that every row of the wavefront sees; units of which any row sees a key
+  {
+    const int last = rows - 1, r0 = row0 < last ? row0 : last, r1 = row0 + 63 < last ? row0 + 63 : last;
+    const int64_t up0 = sp.start + r0 / a.group - sp.lo, up1 = sp.start + r1 / a.group - sp.lo;
+    auto held = [&](int64_t x, int least, int most) { return static_cast<int>(x < least ? least : x < most ? x : most); };
+    seen_hi = held(up0, -1, len - 1);
+    seen_lo = a.window == 0 ? 0 : held(up1 - a.window + 1, 0, len);
+    w_hi = (held(up1, -1, len - 1) + 64) >> 6;
+    w_lo = a.window == 0 ? 0 : held(up0 - a.window + 1, 0, len) >> 6;
+    w_lo = w_lo < w_hi ? w_lo : w_hi;
+  }
+
+  // ---- the movers
+  const int kv = wave >> 1, piece = tid & 127;                 // 0: keys, 1: values; (key piece / 2, block piece % 2) of a unit
+  const unsigned char* const src = a.c.blocks[kv] + b * a.c.bs + kvh * a.c.hs + sp.lo * a.c.ts + 16 * (piece & 1);
+  const unsigned char* const ssrc = a.c.scales[kv] + b * a.c.sbs + kvh * a.c.shs + sp.lo * a.c.sts + (piece & 1);
+  const int64_t unit_bytes = 64 * a.c.ts, unit_scales = 64 * a.c.sts;
+  const unsigned off = (piece >> 1) * static_cast<unsigned>(a.c.ts), soff = (piece >> 1) * static_cast<unsigned>(a.c.sts);
+  const int at_end = min(piece >> 1, (len - 1) & 63);          // in the last unit rows behind the last key are held to it
+  const unsigned off_end = at_end * static_cast<unsigned>(a.c.ts), soff_end = at_end * static_cast<unsigned>(a.c.sts);
+  unsigned to[4];                                              // where the piece's four chunks of 16 bytes go
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int key = piece >> 1, c = 4 * (piece & 1) + t;
+    to[t] = kv == 0 ? key * 128 + ((c ^ (key >> 1 & 7)) << 4) : KTILE + mx_v_chunk4(key, c);
+  }
+  u32x4 raw;
+  unsigned raw_s;
+  auto load_unit = [&](int u) __attribute__((always_inline)) {
+    const int v = u < units ? u : units - 1;                   // (one that is not there: the last one again)
+    const bool end = v == units - 1;
+    raw = *reinterpret_cast<const u32x4*>(src + v * unit_bytes + mx_choose(end, off_end, off));
+    raw_s = (ssrc + v * unit_scales)[mx_choose(end, soff_end, soff)];
+  };
+  // What lies behind the last key of values is zeros in the tile (nothing there is seen; keys' scores are masked). A NaN that only some rows see
+  // may not reach the others as 0 x NaN: zeros in its place, and NaN in the rows that see it.
+  float power;
+  auto prepare = [&](int u, int stage) __attribute__((always_inline)) {   // the unit about to be written
+    if (kv != 0) {
+      const bool in = 64 * u + (piece >> 1) < len;
+      const unsigned long long bad = __builtin_amdgcn_ballot_w64(raw_s == 255u && in);
+      if (__builtin_expect(u >= units - 1 || bad != 0, 0)) {
+        const bool keep = in && raw_s != 255u;
+        raw = keep ? raw : u32x4{0u, 0u, 0u, 0u};
+        raw_s = keep ? raw_s : 0u;
+      }
+      if (lane == 0) {
+        s_any[stage][wave & 1] = bad != 0;
+        s_bad[stage][wave & 1] = bad;
+      }
+    }
+    power = mx_power(raw_s);
+  };
+  auto write_chunk = [&](int stage, int t) __attribute__((always_inline)) { *reinterpret_cast<bf16x8*>(smem + stage * STAGE + to[t]) = mx_bf16x8(raw[t], power); };
+  // In the middle of unit u: every wavefront has written its share of unit u + 1, and has read the last of unit u - 1, whose stage takes unit u + 2.
+  auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  auto after = [](int stage) { return stage == 2 ? 0 : stage + 1; };
+
+  // ---- operands
+  unsigned k_off[4], v_off[2];                                 // K: lane (key l31, block h), four chunks; V: transposing reads, as above
+#pragma unroll
+  for (int m = 0; m < 4; ++m) k_off[m] = l31 * 128 + (((4 * h + m) ^ (l31 >> 1 & 7)) << 4);
+#pragma unroll
+  for (int db = 0; db < 2; ++db) v_off[db] = KTILE + mx_v_chunk4(4 * h + ((lane & 15) >> 2), 4 * db + 2 * (l31 >> 4) + (lane >> 1 & 1)) + (lane & 1) * 8;      // + 8 keys u, + 16 keys cc
+  bf16x8 kf[4], vf[2][2];
+  auto load_k = [&](int stage, int half) __attribute__((always_inline)) {
+    const unsigned char* const t = smem + stage * STAGE + half * 4096;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) kf[m] = *reinterpret_cast<const bf16x8*>(t + k_off[m]);
+  };
+  auto load_v = [&](int stage, int half) __attribute__((always_inline)) {
+    const unsigned char* const t = smem + stage * STAGE + half * 4096;
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        i16x4 part[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(t + v_off[db] + 2048 * cc + 1024 * u));
+        vf[cc][db] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+  };
+
+  const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float ref[2] = {kNoRef, kNoRef};
+  f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  f32x16 o[2][2] = {{zero, zero}, {zero, zero}}, s[2];
+  u32x4 p[2][2];                                               // P^T in bf16, as operand registers
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      p[i][j] = u32x4{0u, 0u, 0u, 0u};
+      vf[i][j] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+    }
+  auto scores = [&](int rt, int m) __attribute__((always_inline)) { s[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m], qf[rt][m], m == 0 ? zero : s[rt], 0, 0, 0); };
+  auto product = [&](int rt, int m) __attribute__((always_inline)) {
+    o[rt][m & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[m >> 1][m & 1], __builtin_bit_cast(bf16x8, p[rt][m >> 1]), o[rt][m & 1], 0, 0, 0);
+  };
+  // weights in pairs; a pair is summed and rounded while the next one's exponentials are on their way
+  float e[2][2];
+  auto weigh = [&](int rt, int m) __attribute__((always_inline)) {
+    e[m & 1][0] = __builtin_amdgcn_exp2f(fmaf(s[rt][2 * m], a.scale_log2, -ref[rt]));
+    e[m & 1][1] = __builtin_amdgcn_exp2f(fmaf(s[rt][2 * m + 1], a.scale_log2, -ref[rt]));
+  };
+  auto keep = [&](int rt, int m) __attribute__((always_inline)) {
+    const bf16x2 v = {static_cast<bf16>(e[m & 1][0]), static_cast<bf16>(e[m & 1][1])};
+    p[rt][m >> 2][m & 3] = __builtin_bit_cast(unsigned, v);
+  };
+  // the rounded weights, as the products take them, summed on the matrix cores as well: ones times a lane's own four
+  const i16x4 ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80};
+  auto add_up = [&](int rt, int m) __attribute__((always_inline)) {
+    typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
+    const u32x2 four = {p[rt][m >> 1][2 * (m & 1)], p[rt][m >> 1][2 * (m & 1) + 1]};
+    sum[rt] = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_bit_cast(i16x4, four), sum[rt], 0, 0, 0);
+  };
+  auto mask = [&](int rt, int k0) __attribute__((always_inline)) {
+    int du = upper[rt] - k0 - 4 * h, dl = lower[rt] - k0 - 4 * h;
+    asm volatile("" : "+v"(du), "+v"(dl));                     // (or the comparisons are made for every block)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[rt][r] = 8 * (r >> 2) + (r & 3) <= du && 8 * (r >> 2) + (r & 3) >= dl ? s[rt][r] : -INFINITY;
+  };
+  // The reference lies kLift above the largest logit that it was raised to, and is raised only where a weight has reached 2 (or is no number): one
+  // OR over the rounded weights' bits tells.
+  auto settle = [&](int rt) __attribute__((always_inline)) {
+    unsigned bits = 0;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) bits |= p[rt][m >> 2][m & 3];
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64((bits & 0x40004000u) != 0) != 0, 0)) {
+      float top = s[rt][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[rt][r]);
+      float x, y;
+      lane_xor32_pair(top, &x, &y);
+      top = fmaf(fmaxf(x, y), a.scale_log2, kLift);
+      const float moved = top > ref[rt] ? top : ref[rt];
+      const float alpha = __builtin_amdgcn_exp2f(ref[rt] - moved);
+      ref[rt] = moved;
+      auto scale = [&](auto& v, int n) __attribute__((always_inline)) {
+        asm volatile("" : "+v"(v));
+#pragma unroll
+        for (int r = 0; r < n; ++r) v[r] *= alpha;
+        asm volatile("" : "+v"(v));
+      };
+      scale(sum[rt], 4);
+      scale(o[rt][0], 16);
+      scale(o[rt][1], 16);
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+        weigh(rt, m);
+        keep(rt, m);
+      }
+      asm volatile("" : "+v"(p[rt][0]), "+v"(p[rt][1]));
+    }
+  };
+  // A block, the first or the second of unit u in `stage`; the first writes the next unit on the way, the second meets the other wavefronts ahead.
+  // `any`: the unit's flags, asked for a unit ago.
+  typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
+  u32x2 any;
+  auto block = [&](int u, int stage, auto tag) __attribute__((always_inline)) {
+    constexpr int SECOND = decltype(tag)::value;
+    const int k0 = 64 * u + 32 * SECOND;
+    const unsigned mine = any[SECOND];
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(mine) != 0, 0)) {
+      for (unsigned long long left = s_bad[stage][SECOND]; left != 0; left &= left - 1) {
+        const int at = __builtin_ctzll(left), key = k0 + (at >> 1);
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+          if (key >= lower[rt] && key <= upper[rt]) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              o[rt][0][i] = at & 1 ? o[rt][0][i] : __builtin_nanf("");
+              o[rt][1][i] = at & 1 ? __builtin_nanf("") : o[rt][1][i];
+            }
+          }
+      }
+    }
+    const int next = after(stage);
+    if constexpr (SECOND) {
+      meet();
+      any = *reinterpret_cast<const u32x2*>(s_any[next]);
+    }
+    const bool masked = k0 + 31 > seen_hi || k0 < seen_lo;
+    if (__builtin_expect(masked, 0)) mask(0, k0);
+    if constexpr (!SECOND) prepare(u + 1, next);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      scores(1, m);
+      if constexpr (!SECOND) write_chunk(next, m);
+      weigh(0, m);
+      if (m > 0) keep(0, m - 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    load_k(SECOND ? next : stage, 1 - SECOND);                 // (the next block's, half a block ahead)
+    if constexpr (!SECOND) load_unit(u + 2);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 4; m < 8; ++m) {
+      product(1, m - 4);
+      add_up(1, m - 4);
+      weigh(0, m);
+      keep(0, m - 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    keep(0, 7);
+    load_v(stage, SECOND);
+    settle(0);
+    if (__builtin_expect(masked, 0)) mask(1, k0);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      scores(0, m);
+      weigh(1, m);
+      if (m > 0) keep(1, m - 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int m = 4; m < 8; ++m) {
+      product(0, m - 4);
+      add_up(0, m - 4);
+      weigh(1, m);
+      keep(1, m - 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    keep(1, 7);
+    settle(1);
+  };
+  auto move = [&](int u, int stage) __attribute__((always_inline)) {      // a unit that only other wavefronts look at
+    const int next = after(stage);
+    prepare(u + 1, next);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) write_chunk(next, t);
+    load_unit(u + 2);
+    meet();
+    any = *reinterpret_cast<const u32x2*>(s_any[next]);
+  };
+
+  if (units > 0) {
+    load_unit(0);
+    prepare(0, 0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) write_chunk(0, t);
+    load_unit(1);
+    meet();
+    any = *reinterpret_cast<const u32x2*>(s_any[0]);
+    int u = 0, stage = 0;
+    for (; u < w_lo; ++u, stage = after(stage)) move(u, stage);
+    if (w_lo < w_hi) {
+      load_k(stage, 0);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) scores(0, m);
+      for (; u < w_hi; ++u, stage = after(stage)) {
+        block(u, stage, std::integral_constant<int, 0>{});
+        block(u, stage, std::integral_constant<int, 1>{});
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        product(1, m);
+        add_up(1, m);
+      }
+    }
+    for (; u < units; ++u, stage = after(stage)) move(u, stage);
+  }
+
+  // ---- the sink joins the denominator; a lane has 8-byte runs of one row's values
+#pragma unroll
+  for (int rt = 0; rt < 2; ++rt) {
+    float x, y;
+    lane_xor32_pair(sum[rt][0], &x, &y);
+    if (row0 + 32 * rt + l31 >= rows) continue;
+    const float f = mx_norm(a, head[rt], ref[rt], x + y);
+    bf16* const out = a.out + b * a.out_bs + query[rt] * a.out_ts + head[rt] * 64 + 4 * h;
+#pragma unroll
+    for (int r = 0; r < 32; r += 4) {
+      bf16x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = o[rt][r >> 4][(r & 15) + e];
+        w[e] = static_cast<bf16>(v * f);
+      }
+      *reinterpret_cast<bf16x4*>(out + 32 * (r >> 4) + 8 * (r >> 2 & 3)) = w;
     }
   }
 }
@@ -751,33 +1075,40 @@ using namespace tllm;
 
 namespace {
 struct MxAttnPlan {
-  bool one;
-  int tiles, key_groups, waves;       // of the kernel for any rows: tiles of 32 rows to a wavefront, wavefronts that share their keys, wavefronts
-  int row_groups, rows_per_run;
-  int splits, fill, most;
+  bool one, many;                     // the kernel for one query, for many rows; otherwise the one for any
+  int tiles, waves;                   // of the latter: tiles of 32 rows; wavefronts of a workgroup
+  int row_groups, rows;               // runs of rows that workgroups take, rows in each
+  int splits, fill;
 };
 
+// Which kernel, by the runs of rows and of streams that there are (eight KV heads of eight query heads, us):
+//   many rows, from 385 runs of 256 on -- one prompt of 2048 51, in 64 rows a workgroup 56, 32 60; 4096 149, 173, 196; 2000 behind 2000 105, 121, 138 --
+//   and from 192 on where walks are short, up to 768 keys: 2 x 512 18.5, 19.4, 20.0; 4 x 256 13.4, 16.9, 16.8; 3 x 333 15.8, 17.7, 18.3;
+//   2 x 700 23.8, 27.1, 25.8; 32 x 32 10.3, 14.9, 14.7; 2048 with a window of 128 18.9, 32, 30. Below, a workgroup to a CU that walks alone is behind:
+//   1000 28.5, 22.7, 22.4; 1000 behind 2000 67, 56, 62; 1500 40, 37, 39; 512 18, 10.7, 11.9.
+//   32 rows shared out between eight wavefronts up to 256 runs of 32: 97 behind 1500 10.0, between four 11.6; 16 x 8 of 2000 11.5, 13.5; 64 behind
+//   8000 22.3, 26.9; with four from there on: 150 behind 1350 16.4, 13.4; 256 behind 2000 22, 18.2; 64 x 4 of 1000 16, 12.1.
+//   64 rows to a workgroup from 768 such runs on: 400 behind 1600 24, with 32 rows 26; 512 10.7, 11.9; 512 behind 4000 73, 80; but 256 behind 2000
+//   19.4, 18.2; 333 9.2, 7.5; 64 x 4 of 1000 16.2, 12.1.
+// Splits as far as they fill the CUs four times: 8 x 4 of 4096 (64 runs) 12.9, none 20.5; 8 x 8 of 2000 (128 runs) none 11.2, two 13.9; 4 x 16 of 3000
+// 14.3, 15.2; 97 behind 1500 (200) 10.0, two 20.4.
 MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window) {
   MxAttnPlan p{};
   const int64_t rows = n_q * group, streams = batch * n_kv_heads;
+  auto seen = [&](int64_t run) {                               // keys that the queries of a run of rows can see together
+    const int64_t span = (int64_t)window + (run + group - 1) / group;
+    return window > 0 && span < n_slots ? span : n_slots;
+  };
+  const int64_t wide = (rows + 255) / 256 * streams, narrow = (rows + 31) / 32 * streams;
   p.one = n_q == 1 && group <= 8;
-  p.waves = 4;
-  p.key_groups = 4;
-  p.tiles = rows <= 32 ? 1 : 2;
-  if (!p.one && (rows + 255) / 256 * streams >= 256) p.key_groups = 1;
-  p.rows_per_run = p.one ? 8 : 32 * p.tiles;
-  const int64_t per_wg = p.rows_per_run * (p.one ? 1 : p.waves / p.key_groups);
-  p.row_groups = (int)((rows + per_wg - 1) / per_wg);
-  const int64_t span = (int64_t)window + (p.rows_per_run + group - 1) / group;       // keys that a run's queries can see together
-  const int64_t ctx = window > 0 && span < n_slots ? span : n_slots;
+  p.many = !p.one && rows > 128 && (wide > 384 || (wide >= 192 && seen(256) <= 768));
+  p.tiles = narrow < 768 ? 1 : 2;
+  p.waves = narrow <= 256 ? 8 : 4;
+  p.rows = p.one ? 8 : p.many ? 256 : 32 * p.tiles;
+  p.row_groups = (int)((rows + p.rows - 1) / p.rows);
   const int64_t units = streams * p.row_groups;
-  p.fill = (int)((kFill + units - 1) / units);
-  p.most = kMostKeys;
-  if (p.key_groups == 1) {
-    p.fill = 1;
-    p.most = 1 << 30;
-  }
-  p.splits = mx_attn_splits(p.fill, (int)(ctx > 0 ? ctx : 1), p.most);
+  p.fill = p.one ? (int)((kFill + units - 1) / units) : kFill / units >= 4 ? (int)(kFill / units) : 1;
+  p.splits = p.many ? 1 : mx_attn_splits(p.fill, (int)seen(p.rows));
   return p;
 }
 
@@ -794,12 +1125,23 @@ extern "C" int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n
   return s > 1 ? (int64_t)s * batch * n_q * n_kv_heads * group * PART * 4 : 0;
 }
 
+template <bool DENSE, int RT, int KG>
+static int launch_rows(const MxAttnArgs& a, dim3 grid, hipStream_t st) {
+  constexpr int SMEM = KG * kShare * 4;
+  static std::atomic<uint64_t> done{0};
+  const hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(mxfp4_attn_rows_kernel<DENSE, RT, KG>), SMEM, done);
+  TLLM_REQUIRE(e == hipSuccess, TLLM_E_LAUNCH, "mxfp4_attention: cannot raise LDS limit: %s", hipGetErrorString(e));
+  hipLaunchKernelGGL((mxfp4_attn_rows_kernel<DENSE, RT, KG>), grid, dim3(KG * 64), SMEM, st, a);
+  return TLLM_OK;
+}
+
 template <bool DENSE>
-static void launch_attention(const MxAttnPlan& p, const MxAttnArgs& a, dim3 grid, dim3 block, hipStream_t st) {
-  if (p.one) hipLaunchKernelGGL((mxfp4_attn_one_kernel<DENSE, 4>), grid, block, 0, st, a);
-  else if (p.tiles == 1) hipLaunchKernelGGL((mxfp4_attn_rows_kernel<DENSE, 1, 4, 4>), grid, block, 0, st, a);
-  else if (p.key_groups == 4) hipLaunchKernelGGL((mxfp4_attn_rows_kernel<DENSE, 2, 4, 4>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((mxfp4_attn_rows_kernel<DENSE, 2, 1, 4>), grid, block, 0, st, a);
+static int launch_attention(const MxAttnPlan& p, const MxAttnArgs& a, dim3 grid, hipStream_t st) {
+  if (p.many) hipLaunchKernelGGL(mxfp4_attn_many_kernel, grid, dim3(256), 0, st, a);
+  else if (p.one) hipLaunchKernelGGL((mxfp4_attn_one_kernel<DENSE, 4>), grid, dim3(256), 0, st, a);
+  else if (p.waves == 8) return p.tiles == 1 ? launch_rows<DENSE, 1, 8>(a, grid, st) : launch_rows<DENSE, 2, 8>(a, grid, st);
+  else return p.tiles == 1 ? launch_rows<DENSE, 1, 4>(a, grid, st) : launch_rows<DENSE, 2, 4>(a, grid, st);
+  return TLLM_OK;
 }
 
 extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, int64_t q_token_stride, const TllmMxCache* cache, const void* sinks, void* out,
@@ -850,14 +1192,13 @@ extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, 
   a.row_groups = p.row_groups;
   a.splits = p.splits;
   a.fill = p.fill;
-  a.most = p.most;
   a.scale_log2 = sm_scale * kLog2e;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)wgs), block(p.waves * 64);
-  if (cache->scale_slot_stride == 2 && n_slots > 1) launch_attention<true>(p, a, grid, block, st);
-  else launch_attention<false>(p, a, grid, block, st);
-  const int rc = check_launch("mxfp4_attention");
+  const dim3 grid((unsigned)wgs);
+  int rc = cache->scale_slot_stride == 2 && n_slots > 1 ? launch_attention<true>(p, a, grid, st) : launch_attention<false>(p, a, grid, st);
+  if (rc != TLLM_OK) return rc;
+  rc = check_launch("mxfp4_attention");
   if (rc != TLLM_OK || p.splits == 1) return rc;
-  hipLaunchKernelGGL(mxfp4_attn_reduce_kernel, dim3((unsigned)(batch * n_q * n_heads)), dim3(64), 0, st, a, p.rows_per_run);
+  hipLaunchKernelGGL(mxfp4_attn_reduce_kernel, dim3((unsigned)(batch * n_q * n_heads)), dim3(64), 0, st, a, p.rows);
   return check_launch("mxfp4_attention(reduce)");
 }
