@@ -432,7 +432,9 @@ int tllm_mxfp4_cache_read_bf16(const TllmMxCache* cache, int64_t first, int64_t 
  * What a slot holds that a query does not see, NaN included, is nothing to it. start_q: device, int32 or int64. group up to 64,
  * sm_scale positive. kv_len_hint (0: none) plans the launch for that many visible keys instead of n_slots; results do not depend on it.
  * workspace: device memory of tllm_mxfp4_attention_workspace_bytes() for the same arguments, 4-byte aligned (may be 0 bytes). */
-int tllm_mxfp4_attention_splits(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint);
+/* Diagnostic: the workgroup that it takes, rows (queries x heads of a KV head) << 16 | wavefronts << 8 | the workgroups that share a run of
+ * rows' keys. Rows: 8 for one query of up to eight heads, 32 or 64, 256 where there are many. */
+int tllm_mxfp4_attention_shape(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint);
 int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window,
                                              int64_t kv_len_hint);
 int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, int64_t q_token_stride, const TllmMxCache* cache, const void* sinks,

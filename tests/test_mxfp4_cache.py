@@ -297,6 +297,38 @@ def test_prompts_of_any_group(heads, group):
         attention_case(2, t, heads, group, t, [0, -3], window=60)
 
 
+def shape(batch, t, slots, heads, group, window=0, hint=0):
+    """rows of a run, wavefronts, splits"""
+    x = _lib.lib().tllm_mxfp4_attention_shape(batch, t, slots, heads, group, window, hint)
+    return x >> 16, x >> 8 & 255, x & 255
+
+
+def test_shapes():
+    """Which kernel serves which sizes, and how many workgroups share the keys."""
+    assert shape(1, 1, 300, 8, 8) == (8, 4, 1) and shape(1, 1, 4096, 8, 8, hint=300) == (8, 4, 1)
+    assert shape(8, 1, 4096, 8, 8) == (8, 4, 4) and shape(8, 1, 32768, 8, 8) == (8, 4, 8) and shape(49, 1, 2048, 8, 8) == (8, 4, 1)
+    assert shape(1, 1, 1 << 29, 1, 1) == (8, 4, 64)
+    assert shape(1, 1, 300, 8, 9) == (32, 8, 1) and shape(8, 4, 4096, 8, 8) == (32, 8, 4) and shape(1, 97, 1597, 8, 8) == (32, 8, 1)
+    assert shape(1, 256, 2256, 8, 8) == (32, 4, 1) and shape(1, 512, 512, 8, 8) == (64, 4, 1)
+    assert shape(1, 2048, 2048, 8, 8) == (256, 4, 1) and shape(3, 333, 333, 8, 8) == (256, 4, 1) and shape(1, 2048, 10**6, 8, 8, window=128) == (256, 4, 1)
+
+
+# (batch, tokens, KV heads, heads of each, slots, run of rows)
+KERNELS = [(2, 3, 2, 8, 1500, 32), (24, 6, 8, 8, 90, 32), (30, 7, 8, 8, 70, 32), (50, 16, 8, 8, 60, 64), (24, 40, 8, 8, 120, 256), (16, 150, 16, 1, 200, 0), (64, 3, 4, 60, 50, 0),
+           (7, 300, 5, 5, 333, 256), (30, 70, 8, 4, 70, 256), (100, 40, 1, 16, 77, 0)]
+
+
+@gpu
+@pytest.mark.parametrize("batch,t,heads,group,slots,run", KERNELS)
+def test_several_tokens_of_each_kernel(batch, t, heads, group, slots, run):
+    if run:
+        assert shape(batch, t, slots, heads, group)[0] == run
+    g = torch.Generator().manual_seed(batch)
+    starts = [int(i) for i in torch.randint(-2, max(slots - t, 1), (batch,), generator=g)]
+    attention_case(batch, t, heads, group, slots, starts, sinks=False)
+    attention_case(batch, t, heads, group, slots, starts[0] % 20, window=slots // 3, layout="slots", ints=torch.int32)
+
+
 @gpu
 @pytest.mark.parametrize("t", [1, 3, 20, 200])
 def test_attention_past_the_end_and_before_the_beginning(t):
@@ -325,17 +357,18 @@ def test_attention_of_smallest_and_largest_scales(t):
 
 
 @gpu
-@pytest.mark.parametrize("t,group", [(1, 8), (1, 16), (4, 8), (33, 4), (200, 8)])
-def test_what_is_not_seen_does_not_matter(t, group):
-    """Slots of NaN and of the largest values outside what the queries see."""
+@pytest.mark.parametrize("t,group,heads,pairs", [(1, 8, 2, 1), (1, 16, 2, 1), (4, 8, 2, 1), (33, 4, 2, 1), (200, 8, 2, 1), (100, 4, 8, 8), (100, 4, 8, 32)])
+def test_what_is_not_seen_does_not_matter(t, group, heads, pairs):
+    """Slots of NaN, of the largest values and of infinite ones outside what the queries see."""
     g = torch.Generator().manual_seed(t)
     for start, window in ((0, 0), (40, 0), (40, 16), (45, 7)):
-        cache = make_cache(g, 2, 300, 2)
-        q = torch.randn(2, t, 2, group, 64, generator=g).bfloat16().cuda()
-        at = torch.tensor([start, start + 3]).cuda()
+        cache = make_cache(g, 2 * pairs, 300, heads)
+        q = torch.randn(2 * pairs, t, heads, group, 64, generator=g).bfloat16().cuda()
+        at = torch.tensor([start, start + 3] * pairs).cuda()
         first = T.mxfp4_attention(q, cache, None, 0.125, window, at)
-        for byte in (255, 252):
-            for b, s in enumerate((start, start + 3)):
+        assert first.isfinite().all()
+        for byte in (255, 254, 252):
+            for b, s in enumerate((start, start + 3) * pairs):
                 cache.k_scales[b, s + t :] = byte
                 cache.v_scales[b, s + t :] = byte
                 if window:
@@ -358,6 +391,24 @@ def test_nan_reaches_who_sees_it(t, group):
                 q = torch.randn(1, t, 2, group, 64, generator=g).bfloat16()
                 want, tol = attention_ref(q, cpu(cache), None, 0.125, window, [64])
                 check(T.mxfp4_attention(q.cuda(), cache, None, 0.125, window, torch.tensor([64]).cuda()), want, tol, f"{t} queries, window {window}, NaN at {where}")
+
+
+@gpu
+@pytest.mark.parametrize("batch,t,group,run", [(24, 40, 8, 256), (50, 16, 8, 64), (30, 7, 8, 32)])
+def test_nan_in_a_batch_of_each_kernel(batch, t, group, run):
+    assert shape(batch, t, 150, 8, group)[0] == run
+    for window in (0, 25):
+        g = torch.Generator().manual_seed(run)
+        cache = make_cache(g, batch, 150, 8)
+        for b in range(batch):                                 # somewhere in each row: a block of keys, of values, of both, of neither
+            for what in (1, 3):
+                if int(torch.randint(0, 3, (), generator=g)):
+                    cache[what][b, int(torch.randint(0, 110, (), generator=g)), int(torch.randint(0, 8, (), generator=g)), int(torch.randint(0, 2, (), generator=g))] = 255
+        q = torch.randn(batch, t, 8, group, 64, generator=g).bfloat16()
+        starts = [int(i) for i in torch.randint(0, 110 - t, (batch,), generator=g)]
+        want, tol = attention_ref(q, cpu(cache), None, 0.125, window, starts)
+        assert want.isnan().any() and not want.isnan().all()
+        check(T.mxfp4_attention(q.cuda(), cache, None, 0.125, window, torch.tensor(starts).cuda()), want, tol, f"runs of {run}, window {window}")
 
 
 @gpu
@@ -614,7 +665,7 @@ def test_entry_points_refuse_what_they_cannot_do():
     assert attend(n_q=0) == 0 and attend(cache=descriptor(batch=0)) == 0
     need = lib.tllm_mxfp4_attention_workspace_bytes(2, 1, 100000, 2, 8, 0, 0)
     assert need > 0 and attend(cache=descriptor(n_slots=100000), work=p, size=need - 1) == -1 and "workspace" in said()
-    assert lib.tllm_mxfp4_attention_workspace_bytes(2, 1, 100000, 2, 8, 0, 100) < need and lib.tllm_mxfp4_attention_splits(0, 1, 10, 1, 1, 0, 0) == 0
+    assert lib.tllm_mxfp4_attention_workspace_bytes(2, 1, 100000, 2, 8, 0, 100) < need and lib.tllm_mxfp4_attention_shape(0, 1, 10, 1, 1, 0, 0) == 0
 
 
 def test_ops_refuse_cpu_tensors():

@@ -95,7 +95,7 @@ SIGNATURES = {
     "tllm_moe_mlp2_bf16": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i64, _i64, _vp]),
     "tllm_mxfp4_cache_write": (_i32, [C.POINTER(TllmMxCache), _vp, _vp, _i32, C.POINTER(_i64), C.POINTER(_i64), _i64, _vp, _i32, _i32, _vp, _i32, _i32, _vp]),
     "tllm_mxfp4_cache_read_bf16": (_i32, [C.POINTER(TllmMxCache), _i64, _i64, _vp, _vp, _vp]),
-    "tllm_mxfp4_attention_splits": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32, _i64]),
+    "tllm_mxfp4_attention_shape": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32, _i64]),
     "tllm_mxfp4_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i64]),
     "tllm_mxfp4_attention_bf16": (_i32, [_vp, _i64, _i64, C.POINTER(TllmMxCache), _vp, _vp, _i64, _i64, _i64, _i32, _f32, _i32, _vp, _i32, _i32, _i64, _vp,
                                          _i64, _vp]),

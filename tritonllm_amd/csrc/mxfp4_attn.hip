@@ -1115,13 +1115,14 @@ MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_he
 int64_t mx_attn_ctx(int64_t n_slots, int64_t hint) { return hint > 0 && hint < n_slots ? hint : n_slots; }
 }  // namespace
 
-extern "C" int tllm_mxfp4_attention_splits(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint) {
-  if (batch < 1 || n_q < 1 || n_slots < 1 || n_kv_heads < 1 || group < 1 || window < 0) return 0;
-  return mx_attn_plan(batch, n_q, mx_attn_ctx(n_slots, kv_len_hint), n_kv_heads, group, window).splits;
+extern "C" int tllm_mxfp4_attention_shape(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint) {
+  if (batch < 1 || n_q < 1 || n_slots < 1 || n_kv_heads < 1 || group < 1 || window < 0 || kv_len_hint < 0) return 0;
+  const MxAttnPlan p = mx_attn_plan(batch, n_q, mx_attn_ctx(n_slots, kv_len_hint), n_kv_heads, group, window);
+  return p.rows << 16 | (p.one || p.many ? 4 : p.waves) << 8 | p.splits;
 }
 
 extern "C" int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint) {
-  const int s = tllm_mxfp4_attention_splits(batch, n_q, n_slots, n_kv_heads, group, window, kv_len_hint);
+  const int s = tllm_mxfp4_attention_shape(batch, n_q, n_slots, n_kv_heads, group, window, kv_len_hint) & 0xff;
   return s > 1 ? (int64_t)s * batch * n_q * n_kv_heads * group * PART * 4 : 0;
 }
 
