@@ -32,7 +32,6 @@ constexpr int PART = 66;              // floats of a record in the workspace
 // 32768 11.2, 13.2 -- until each has 4096 keys: 8 rows of 32768 28.6, with one of 8192 31.6 and two of 2048 30.4; 8 of 131072 96, 94 and 104. At
 // least 256 keys: one row of 4096 7.3, of 512 and more 7.6 - 9.0.
 constexpr int kUnsplit = 1024, kLeastShift = 8, kMostShift = 12, kFill = 256;
-constexpr int kManyWgs = 96;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoRef = -3.0e38f;    // no key has been seen: the reference (finite, so that a masked logit's weight is exp2(-inf); the first key's is infinite and raises it)
 constexpr float kLift = 7.f;          // ... or how far it lies above the largest logit that it was raised to
@@ -699,20 +698,25 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   }
 }
 
-// Many rows: a workgroup's four wavefronts have 64 neighbouring rows each and walk the same keys, 64 at a time, which come to bf16 once for all
-// four of them: a thread has 16 bytes of codes of a unit, keys' in the first two wavefronts and values' in the others, and writes
-// their 32 values into one of three stages in LDS while the unit before is worked on. One barrier a unit.
+// Many rows: a workgroup's wavefronts have 64 neighbouring rows each, RUNS of them walk the same keys, and these come to bf16 once for all of
+// them: a thread has 16 bytes of codes of a unit of 16 RUNS keys, and writes their 32 values into one of three stages in LDS while the
+// units before are worked on. One barrier a unit. Four runs, or two with two groups of wavefronts that take the units in turn and meet at the end.
 //   The matrix cores and the vector ALU work at the same time: with one tile's weights (32 keys x 32 rows) the next one's scores are issued in
 //   turn, and the products of the one before. Of block j (32 keys), S^T of tile 1, weights of tile 0 and P . V of block j - 1 in tile 1; then S^T of
 //   block j + 1 in tile 0, weights of tile 1 and P . V of tile 0. Operands of K and of V live from one such half to the next.
+template <int RUNS>
 __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
-  constexpr int KTILE = 64 * 128, STAGE = 2 * KTILE;           // bytes: K [64 keys][64 values], then V
-  __shared__ __align__(16) unsigned char smem[3 * STAGE];
-  __shared__ __align__(8) unsigned s_any[3][2];                // whether a stage's values hold NaN, in its first and in its second 32 keys,
-  __shared__ unsigned long long s_bad[3][2];                   // and in which of the 32 x 2 pieces
+  static_assert(RUNS == 4 || RUNS == 2, "runs of a workgroup");
+  constexpr int KG = 4 / RUNS, UNIT = 16 * RUNS, HALVES = UNIT / 32, RB = 64 * RUNS;
+  constexpr int KTILE = UNIT * 128, STAGE = 2 * KTILE;         // bytes: K [UNIT keys][64 values], then V
+  __shared__ __align__(16) unsigned char smem[KG * 3 * STAGE];
+  __shared__ __align__(8) unsigned s_any[KG][3][2];            // whether a stage's values hold NaN, by 32 keys,
+  __shared__ unsigned long long s_bad[KG][3][2];               // and in which of the 32 x 2 pieces
+  static_assert(KG == 1 || RUNS * 2 * kShare * 4 <= KG * 3 * STAGE, "the shares fit the stages");
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
+  const int run = wave % RUNS, kg = wave / RUNS;
 
   // the rows that see most keys come first, and where the launch is two workgroups to a CU the second ones are taken in the opposite order, so
   // that a CU with a long walk gets a short one next to it
@@ -724,7 +728,7 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
     if (n <= 2 * per_round && id >= per_round) id = n + per_round - 1 - id;
   }
   const int b = id % a.batch, rg = a.row_groups - 1 - static_cast<int>(id / a.batch);
-  const int rows = a.n_q * a.group, row0 = rg * 256 + wave * 64;
+  const int rows = a.n_q * a.group, row0 = rg * RB + run * 64;
 
   bf16x8 qf[2][4];
   int query[2], head[2];
@@ -738,8 +742,10 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) qf[rt][t] = *reinterpret_cast<const bf16x8*>(qr + 8 * t);
   }
-  const MxSpan sp = mx_span(a, b, rg * 256, rg * 256 + 255);
-  const int len = sp.hi - sp.lo, units = (len + 63) >> 6;
+  const MxSpan sp = mx_span(a, b, rg * RB, rg * RB + RB - 1);
+  const int len = sp.hi - sp.lo, all = (len + UNIT - 1) / UNIT;
+  const int units = (all + KG - 1) / KG;                       // of each group: the wavefronts meet as often in all of them
+  auto key_of = [&](int u) { return UNIT * (KG * u + kg); };   // a unit's first key
 
   int upper[2], lower[2];                                      // the keys that the lane's row sees, counted from sp.lo
 #pragma unroll
@@ -755,18 +761,19 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
     auto held = [&](int64_t x, int least, int most) { return static_cast<int>(x < least ? least : x < most ? x : most); };
     seen_hi = held(up0, -1, len - 1);
     seen_lo = a.window == 0 ? 0 : held(up1 - a.window + 1, 0, len);
-    w_hi = (held(up1, -1, len - 1) + 64) >> 6;
-    w_lo = a.window == 0 ? 0 : held(up0 - a.window + 1, 0, len) >> 6;
+    const int n_hi = (held(up1, -1, len - 1) + UNIT) / UNIT, n_lo = a.window == 0 ? 0 : held(up0 - a.window + 1, 0, len) / UNIT;
+    w_hi = (n_hi - kg + KG - 1) / KG;                          // (n_hi >= 0, kg < KG)
+    w_lo = (n_lo - kg + KG - 1) / KG;
     w_lo = w_lo < w_hi ? w_lo : w_hi;
   }
 
   // ---- the movers
-  const int kv = wave >> 1, piece = tid & 127;                 // 0: keys, 1: values; (key piece / 2, block piece % 2) of a unit
+  const int kv = run / (RUNS / 2), piece = tid & (UNIT * 2 - 1);      // 0: keys, 1: values; (key piece / 2, block piece % 2) of a unit
   const unsigned char* const src = a.c.blocks[kv] + b * a.c.bs + kvh * a.c.hs + sp.lo * a.c.ts + 16 * (piece & 1);
   const unsigned char* const ssrc = a.c.scales[kv] + b * a.c.sbs + kvh * a.c.shs + sp.lo * a.c.sts + (piece & 1);
-  const int64_t unit_bytes = 64 * a.c.ts, unit_scales = 64 * a.c.sts;
+  const int64_t unit_bytes = UNIT * a.c.ts, unit_scales = UNIT * a.c.sts;
   const unsigned off = (piece >> 1) * static_cast<unsigned>(a.c.ts), soff = (piece >> 1) * static_cast<unsigned>(a.c.sts);
-  const int at_end = min(piece >> 1, (len - 1) & 63);          // in the last unit rows behind the last key are held to it
+  const int at_end = min(piece >> 1, (len - 1) & (UNIT - 1));  // in the last unit rows behind the last key are held to it
   const unsigned off_end = at_end * static_cast<unsigned>(a.c.ts), soff_end = at_end * static_cast<unsigned>(a.c.sts);
   unsigned to[4];                                              // where the piece's four chunks of 16 bytes go
 #pragma unroll
@@ -777,8 +784,8 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
   u32x4 raw;
   unsigned raw_s;
   auto load_unit = [&](int u) __attribute__((always_inline)) {
-    const int v = u < units ? u : units - 1;                   // (one that is not there: the last one again)
-    const bool end = v == units - 1;
+    const int v = min(KG * u + kg, all - 1);                   // (one that is not there: the last one again)
+    const bool end = v == all - 1;
     raw = *reinterpret_cast<const u32x4*>(src + v * unit_bytes + mx_choose(end, off_end, off));
     raw_s = (ssrc + v * unit_scales)[mx_choose(end, soff_end, soff)];
   };
@@ -787,22 +794,24 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
   float power;
   auto prepare = [&](int u, int stage) __attribute__((always_inline)) {   // the unit about to be written
     if (kv != 0) {
-      const bool in = 64 * u + (piece >> 1) < len;
+      const bool in = key_of(u) + (piece >> 1) < len;
       const unsigned long long bad = __builtin_amdgcn_ballot_w64(raw_s == 255u && in);
-      if (__builtin_expect(u >= units - 1 || bad != 0, 0)) {
+      if (__builtin_expect(key_of(u) + UNIT > len || bad != 0, 0)) {
         const bool keep = in && raw_s != 255u;
         raw = keep ? raw : u32x4{0u, 0u, 0u, 0u};
         raw_s = keep ? raw_s : 0u;
       }
       if (lane == 0) {
-        s_any[stage][wave & 1] = bad != 0;
-        s_bad[stage][wave & 1] = bad;
+        s_any[kg][stage][run % HALVES] = bad != 0;
+        s_bad[kg][stage][run % HALVES] = bad;
       }
     }
     power = mx_power(raw_s);
   };
-  auto write_chunk = [&](int stage, int t) __attribute__((always_inline)) { *reinterpret_cast<bf16x8*>(smem + stage * STAGE + to[t]) = mx_bf16x8(raw[t], power); };
-  // In the middle of unit u: every wavefront has written its share of unit u + 1, and has read the last of unit u - 1, whose stage takes unit u + 2.
+  unsigned char* const ring = smem + kg * 3 * STAGE;
+  auto write_chunk = [&](int stage, int t) __attribute__((always_inline)) { *reinterpret_cast<bf16x8*>(ring + stage * STAGE + to[t]) = mx_bf16x8(raw[t], power); };
+  // Ahead of the last block of unit u: every wavefront has written its share of unit u + 1, and has read the last of unit u - 1, whose stage takes
+  // unit u + 2.
   auto meet = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   auto after = [](int stage) { return stage == 2 ? 0 : stage + 1; };
 
@@ -814,12 +823,12 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
   for (int db = 0; db < 2; ++db) v_off[db] = KTILE + mx_v_chunk4(4 * h + ((lane & 15) >> 2), 4 * db + 2 * (l31 >> 4) + (lane >> 1 & 1)) + (lane & 1) * 8;      // + 8 keys u, + 16 keys cc
   bf16x8 kf[4], vf[2][2];
   auto load_k = [&](int stage, int half) __attribute__((always_inline)) {
-    const unsigned char* const t = smem + stage * STAGE + half * 4096;
+    const unsigned char* const t = ring + stage * STAGE + half * 4096;
 #pragma unroll
     for (int m = 0; m < 4; ++m) kf[m] = *reinterpret_cast<const bf16x8*>(t + k_off[m]);
   };
   auto load_v = [&](int stage, int half) __attribute__((always_inline)) {
-    const unsigned char* const t = smem + stage * STAGE + half * 4096;
+    const unsigned char* const t = ring + stage * STAGE + half * 4096;
 #pragma unroll
     for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
@@ -903,16 +912,18 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
       asm volatile("" : "+v"(p[rt][0]), "+v"(p[rt][1]));
     }
   };
-  // A block, the first or the second of unit u in `stage`; the first writes the next unit on the way, the second meets the other wavefronts ahead.
-  // `any`: the unit's flags, asked for a unit ago.
+  // A block, `half` of unit u in `stage`. The last of a unit meets the other wavefronts ahead; a unit is written on the way of the first one -- of two
+  // blocks' units the next one, of one block's the one after it. `any`: the unit's flags, asked for a unit ago.
   typedef __attribute__((__vector_size__(2 * sizeof(unsigned)))) unsigned u32x2;
   u32x2 any;
   auto block = [&](int u, int stage, auto tag) __attribute__((always_inline)) {
-    constexpr int SECOND = decltype(tag)::value;
-    const int k0 = 64 * u + 32 * SECOND;
-    const unsigned mine = any[SECOND];
+    constexpr int half = decltype(tag)::value;
+    constexpr bool FIRST = half == 0, LAST = half == HALVES - 1;
+    constexpr int AHEAD = 3 - HALVES;
+    const int k0 = key_of(u) + 32 * half;
+    const unsigned mine = any[half];
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(mine) != 0, 0)) {
-      for (unsigned long long left = s_bad[stage][SECOND]; left != 0; left &= left - 1) {
+      for (unsigned long long left = s_bad[kg][stage][half]; left != 0; left &= left - 1) {
         const int at = __builtin_ctzll(left), key = k0 + (at >> 1);
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt)
@@ -925,24 +936,24 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
           }
       }
     }
-    const int next = after(stage);
-    if constexpr (SECOND) {
+    const int next = after(stage), to_stage = AHEAD == 1 ? next : after(next);
+    if constexpr (LAST) {
       meet();
-      any = *reinterpret_cast<const u32x2*>(s_any[next]);
+      any = *reinterpret_cast<const u32x2*>(s_any[kg][next]);
     }
     const bool masked = k0 + 31 > seen_hi || k0 < seen_lo;
     if (__builtin_expect(masked, 0)) mask(0, k0);
-    if constexpr (!SECOND) prepare(u + 1, next);
+    if constexpr (FIRST) prepare(u + AHEAD, to_stage);
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       scores(1, m);
-      if constexpr (!SECOND) write_chunk(next, m);
+      if constexpr (FIRST) write_chunk(to_stage, m);
       weigh(0, m);
       if (m > 0) keep(0, m - 1);
       __builtin_amdgcn_sched_barrier(0);
     }
-    load_k(SECOND ? next : stage, 1 - SECOND);                 // (the next block's, half a block ahead)
-    if constexpr (!SECOND) load_unit(u + 2);
+    load_k(LAST ? next : stage, LAST ? 0 : half + 1);          // (the next block's, half a block ahead)
+    if constexpr (FIRST) load_unit(u + AHEAD + 1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 4; m < 8; ++m) {
@@ -953,7 +964,7 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     }
     keep(0, 7);
-    load_v(stage, SECOND);
+    load_v(stage, half);
     settle(0);
     if (__builtin_expect(masked, 0)) mask(1, k0);
 #pragma unroll
@@ -974,24 +985,27 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
     keep(1, 7);
     settle(1);
   };
+  constexpr int AHEAD = 3 - HALVES;
+  auto write_unit = [&](int u, int stage) __attribute__((always_inline)) {
+    prepare(u, stage);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) write_chunk(stage, t);
+    load_unit(u + 1);
+  };
   auto move = [&](int u, int stage) __attribute__((always_inline)) {      // a unit that only other wavefronts look at
     const int next = after(stage);
-    prepare(u + 1, next);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) write_chunk(next, t);
-    load_unit(u + 2);
+    if constexpr (AHEAD == 1) write_unit(u + 1, next);
     meet();
-    any = *reinterpret_cast<const u32x2*>(s_any[next]);
+    any = *reinterpret_cast<const u32x2*>(s_any[kg][next]);
+    if constexpr (AHEAD == 2) write_unit(u + 2, after(next));
   };
 
   if (units > 0) {
     load_unit(0);
-    prepare(0, 0);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) write_chunk(0, t);
-    load_unit(1);
+    write_unit(0, 0);
+    if constexpr (AHEAD == 2) write_unit(1, 1);
     meet();
-    any = *reinterpret_cast<const u32x2*>(s_any[0]);
+    any = *reinterpret_cast<const u32x2*>(s_any[kg][0]);
     int u = 0, stage = 0;
     for (; u < w_lo; ++u, stage = after(stage)) move(u, stage);
     if (w_lo < w_hi) {
@@ -1000,7 +1014,7 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
       for (int m = 0; m < 4; ++m) scores(0, m);
       for (; u < w_hi; ++u, stage = after(stage)) {
         block(u, stage, std::integral_constant<int, 0>{});
-        block(u, stage, std::integral_constant<int, 1>{});
+        if constexpr (HALVES == 2) block(u, stage, std::integral_constant<int, 1>{});
       }
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
@@ -1011,13 +1025,49 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
     for (; u < units; ++u, stage = after(stage)) move(u, stage);
   }
 
-  // ---- the sink joins the denominator; a lane has 8-byte runs of one row's values
+  // ---- the second group hands its shares over
+  float l[2];
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) {
     float x, y;
     lane_xor32_pair(sum[rt][0], &x, &y);
+    l[rt] = x + y;
+  }
+  if constexpr (KG == 2) {
+    float* const shares = reinterpret_cast<float*>(smem) + run * 2 * kShare + lane;
+    __syncthreads();                                           // (all are past their last read of the stages)
+    if (kg == 1) {
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+          const float v = o[rt][r >> 4][r & 15];
+          shares[rt * kShare + r * 64] = v;
+        }
+        shares[rt * kShare + 32 * 64] = ref[rt];
+        shares[rt * kShare + 33 * 64] = l[rt];
+      }
+    }
+    __syncthreads();
+    if (kg == 1) return;
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+      const float* const from = shares + rt * kShare;
+      const float m = fmaxf(ref[rt], from[32 * 64]), f0 = __builtin_amdgcn_exp2f(ref[rt] - m), f1 = __builtin_amdgcn_exp2f(from[32 * 64] - m);
+      ref[rt] = m;
+      l[rt] = l[rt] * f0 + from[33 * 64] * f1;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        const float v = o[rt][r >> 4][r & 15];
+        o[rt][r >> 4][r & 15] = v * f0 + from[r * 64] * f1;
+      }
+    }
+  }
+  // ---- the sink joins the denominator; a lane has 8-byte runs of one row's values
+#pragma unroll
+  for (int rt = 0; rt < 2; ++rt) {
     if (row0 + 32 * rt + l31 >= rows) continue;
-    const float f = mx_norm(a, head[rt], ref[rt], x + y);
+    const float f = mx_norm(a, head[rt], ref[rt], l[rt]);
     bf16* const out = a.out + b * a.out_bs + query[rt] * a.out_ts + head[rt] * 64 + 4 * h;
 #pragma unroll
     for (int r = 0; r < 32; r += 4) {
@@ -1082,10 +1132,13 @@ struct MxAttnPlan {
 };
 
 // Which kernel, by the runs of rows and of streams that there are (eight KV heads of eight query heads, us):
-//   many rows, from 385 runs of 256 on -- one prompt of 2048 51, in 64 rows a workgroup 56, 32 60; 4096 149, 173, 196; 2000 behind 2000 105, 121, 138 --
-//   and from 192 on where walks are short, up to 768 keys: 2 x 512 18.5, 19.4, 20.0; 4 x 256 13.4, 16.9, 16.8; 3 x 333 15.8, 17.7, 18.3;
-//   2 x 700 23.8, 27.1, 25.8; 32 x 32 10.3, 14.9, 14.7; 2048 with a window of 128 18.9, 32, 30. Below, a workgroup to a CU that walks alone is behind:
-//   1000 28.5, 22.7, 22.4; 1000 behind 2000 67, 56, 62; 1500 40, 37, 39; 512 18, 10.7, 11.9.
+//   many rows, 256 to a workgroup, from 385 runs of 256 on -- one prompt of 2048 51, in 64 rows a workgroup 57, 32 64; 4096 149, 173, 196; 2000 behind
+//   2000 105, 121, 138 -- and from 513 runs of 128 on where walks are short, up to 768 keys: 2 x 700 23.9, 27.2, 26.4; 2048 with a window of 128 19, 32,
+//   31. Between, two workgroups to a CU do not come out even: 1200 33, 28.7, 29.2; 1200 behind 2800 106, 91, 103; 1500 40, 37, 41.
+//   128 to a workgroup where that is one or two workgroups to a CU, 321 to 512: 1000 behind 8000 167, in 256 rows a workgroup 187, 64 214; 800 behind
+//   4000 85, 102, 114; 700 behind 4000 84, 101, 103; 1000 22.1, 28.4, 22.4; 2 x 512 16, 18.6, 18.9; 4 x 256 12.8, 13.5, 16.8; 3 x 333 13.8, 15.9, 17.3;
+//   8 x 128 behind 2000 48.8, 51.2, 51; a short prompt is behind (700 17.8, in 32 rows 15.3), as are all with fewer workgroups than that: 512 13.9,
+//   18, in 64 rows 10.9; 600 16.6, 20, 16.6; 1100 behind 1000 (576) 52, 53, 47.6.
 //   32 rows shared out between eight wavefronts up to 256 runs of 32: 97 behind 1500 10.0, between four 11.6; 16 x 8 of 2000 11.5, 13.5; 64 behind
 //   8000 22.3, 26.9; with four from there on: 150 behind 1350 16.4, 13.4; 256 behind 2000 22, 18.2; 64 x 4 of 1000 16, 12.1.
 //   64 rows to a workgroup from 768 such runs on: 400 behind 1600 24, with 32 rows 26; 512 10.7, 11.9; 512 behind 4000 73, 80; but 256 behind 2000
@@ -1099,12 +1152,12 @@ MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_he
     const int64_t span = (int64_t)window + (run + group - 1) / group;
     return window > 0 && span < n_slots ? span : n_slots;
   };
-  const int64_t wide = (rows + 255) / 256 * streams, narrow = (rows + 31) / 32 * streams;
+  const int64_t wide = (rows + 255) / 256 * streams, half = (rows + 127) / 128 * streams, narrow = (rows + 31) / 32 * streams;
   p.one = n_q == 1 && group <= 8;
-  p.many = !p.one && rows > 128 && (wide > 384 || (wide >= 192 && seen(256) <= 768));
+  p.many = !p.one && rows > 128 && (wide > 384 || (half > 320 && half <= 512) || (half > 512 && seen(256) <= 768));
   p.tiles = narrow < 768 ? 1 : 2;
   p.waves = narrow <= 256 ? 8 : 4;
-  p.rows = p.one ? 8 : p.many ? 256 : 32 * p.tiles;
+  p.rows = p.one ? 8 : p.many ? (half > 512 ? 256 : 128) : 32 * p.tiles;
   p.row_groups = (int)((rows + p.rows - 1) / p.rows);
   const int64_t units = streams * p.row_groups;
   p.fill = p.one ? (int)((kFill + units - 1) / units) : kFill / units >= 4 ? (int)(kFill / units) : 1;
@@ -1138,9 +1191,12 @@ static int launch_rows(const MxAttnArgs& a, dim3 grid, hipStream_t st) {
 
 template <bool DENSE>
 static int launch_attention(const MxAttnPlan& p, const MxAttnArgs& a, dim3 grid, hipStream_t st) {
-  if (p.many) hipLaunchKernelGGL(mxfp4_attn_many_kernel, grid, dim3(256), 0, st, a);
+  if (p.many) {
+    if (p.rows == 256) hipLaunchKernelGGL(mxfp4_attn_many_kernel<4>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(mxfp4_attn_many_kernel<2>, grid, dim3(256), 0, st, a);
+  }
   else if (p.one) hipLaunchKernelGGL((mxfp4_attn_one_kernel<DENSE, 4>), grid, dim3(256), 0, st, a);
-  else if (p.waves == 8) return p.tiles == 1 ? launch_rows<DENSE, 1, 8>(a, grid, st) : launch_rows<DENSE, 2, 8>(a, grid, st);
+  else if (p.waves == 8) return launch_rows<DENSE, 1, 8>(a, grid, st);
   else return p.tiles == 1 ? launch_rows<DENSE, 1, 4>(a, grid, st) : launch_rows<DENSE, 2, 4>(a, grid, st);
   return TLLM_OK;
 }
