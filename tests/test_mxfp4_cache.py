@@ -478,6 +478,25 @@ def test_queries_from_strides(t):
 
 
 @gpu
+@pytest.mark.parametrize("t", [1, 4, 200])
+def test_scales_at_odd_addresses(t):
+    g = torch.Generator().manual_seed(13)
+    cache = make_cache(g, 2, 90, 2)
+
+    def odd(s):
+        s = s.transpose(1, 2)
+        return torch.empty(s.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view(s.shape).copy_(s).transpose(1, 2)
+
+    cache = cache._replace(k_scales=odd(cache.k_scales), v_scales=odd(cache.v_scales))
+    k, v = torch.randn(2, 2, 2, 64, generator=g).bfloat16().cuda(), torch.randn(2, 2, 2, 64, generator=g).bfloat16().cuda()
+    T.mxfp4_cache_write(cache, k, v, torch.tensor([11, 40]).cuda())
+    assert same_values(T.mxfp4_cache_read(cache)[0], values(*cpu(cache)[:2]))
+    q = torch.randn(2, t, 2, 8, 64, generator=g).bfloat16()
+    want, tol = attention_ref(q, cpu(cache), None, 0.125, 0, [89, 44])
+    check(T.mxfp4_attention(q.cuda(), cache, None, 0.125, 0, torch.tensor([89, 44]).cuda(), 2**70), want, tol)
+
+
+@gpu
 def test_slots_beyond_32_bits():
     """Slots 16 MB apart: 300 of them span 5 GB, and the offsets of a cache's end pass 32 bits."""
     n, far = 300, 2**24 - 16
@@ -665,6 +684,7 @@ def test_entry_points_refuse_what_they_cannot_do():
     need = lib.tllm_mxfp4_attention_workspace_bytes(2, 1, 100000, 2, 8, 0, 0)
     assert need > 0 and attend(cache=descriptor(n_slots=100000), work=p, size=need - 1) == -1 and "workspace" in said()
     assert lib.tllm_mxfp4_attention_workspace_bytes(2, 1, 100000, 2, 8, 0, 100) < need and lib.tllm_mxfp4_attention_shape(0, 1, 10, 1, 1, 0, 0) == 0
+    assert lib.tllm_mxfp4_attention_shape(1, 1, 2**30, 1, 1, 0, 0) == 0 and lib.tllm_mxfp4_attention_workspace_bytes(1, 2**24, 10, 1, 1, 0, 0) == 0
 
 
 def test_ops_refuse_cpu_tensors():
@@ -706,8 +726,9 @@ def test_ops_refuse_wrong_types_and_shapes():
     for scale in (0.0, -1.0, math.nan, math.inf):
         with pytest.raises(RuntimeError, match="sm_scale"):
             T.mxfp4_attention(q, cache, sinks, scale, 0, at)
-    with pytest.raises(RuntimeError, match="window"):
-        T.mxfp4_attention(q, cache, sinks, 1.0, -1, at)
+    for window in (-1, -(2**32) + 5):
+        with pytest.raises(RuntimeError, match="window"):
+            T.mxfp4_attention(q, cache, sinks, 1.0, window, at)
     with pytest.raises(RuntimeError, match="query heads"):
         T.mxfp4_attention(q.repeat(1, 1, 1, 20, 1), cache, None, 1.0, 0, at)
     with pytest.raises(NotImplementedError):

@@ -33,10 +33,12 @@ constexpr int PART = 66;              // floats of a record in the workspace
 // least 256 keys: one row of 4096 7.3, of 512 and more 7.6 - 9.0.
 constexpr int kUnsplit = 1024, kLeastShift = 8, kMostShift = 12, kFill = 256;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoRef = -3.0e38f;    // no key has been seen: the reference (finite, so that a masked logit's weight is exp2(-inf); the first key's is infinite and raises it)
-constexpr float kLift = 7.f;          // ... or how far it lies above the largest logit that it was raised to
+// Weights are exp2(logit - reference). The reference of one query and of a few rows is the largest logit that it was raised to, and stays there
+// until a lane's weights of a block sum to more than kMostSum; that of many rows lies kLift above it, and stays until a weight reaches 2.
+constexpr float kNoRef = -3.0e38f;    // no key has been seen (finite, so that a masked logit's weight is exp2(-inf); the first key's is infinite and raises it)
+constexpr float kLift = 7.f;
+constexpr float kMostSum = 256.f;
 constexpr int kShare = 34 * 64;       // floats that a wavefront hands over for a tile of 32 rows
-constexpr float kMostSum = 256.f;       // a block's weights may sum to so much before the reference is raised
 }  // namespace
 
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
@@ -94,13 +96,6 @@ __device__ __forceinline__ int mx_v_chunk(int key, int chunk) { return key * 128
 // The same for tiles of 32 rows, whose transposing reads take four rows x four chunks at a time.
 __device__ __forceinline__ int mx_v_chunk4(int key, int chunk) { return key * 128 + ((chunk ^ ((key >> 1 & 1) << 2) ^ (key >> 2 & 1) ^ (chunk >> 2 << 1)) << 4); }
 
-// One query of up to eight heads. A wavefront takes 64 keys at a time: keys 0 - 31 and 32 - 63 of a block are dealt to the two halves of the
-// matrix instruction's sixteen columns, so that eight heads fill it.
-//   S^T = K . Q^T, keys on M, in two tiles of 16 x 2 keys: the k slots of the lane groups g = 0, 1 are a key's two blocks of 32 values, those of
-//   g = 2, 3 the key 32 places on; the columns 0 - 7 have Q in the former and zeros in the latter, the columns 8 - 15 the reverse.
-//   A lane's scores are then four of a tile, all of use.
-//   O = P . V, the weights' registers being the A operand for the block's keys 0 - 31 in the rows 0 - 7 and for 32 - 63 in the rows 8 - 15: two
-//   accumulators, each of which is looked at in one half of its rows. V passes LDS as bf16, for transposing reads.
 // yes ? a : b for a condition that all lanes share, on a scalar mask in one instruction.
 __device__ __forceinline__ unsigned mx_choose(bool yes, unsigned a, unsigned b) {
   unsigned x;
@@ -108,7 +103,7 @@ __device__ __forceinline__ unsigned mx_choose(bool yes, unsigned a, unsigned b) 
   return x;
 }
 
-// DENSE: a head's scale bytes lie next to each other (two bytes from slot to slot).
+// The scale bytes of two neighbouring slots. DENSE: a head's lie next to each other (two bytes from slot to slot, at even addresses).
 template <bool DENSE>
 __device__ __forceinline__ unsigned mx_scale_pair(const unsigned char* p, int64_t sts, int behind) {
   typedef unsigned __attribute__((aligned(2))) u32_a2;
@@ -120,6 +115,13 @@ __device__ __forceinline__ unsigned mx_scale_pair(const unsigned char* p, int64_
   }
 }
 
+// One query of up to eight heads. A wavefront takes 64 keys at a time: keys 0 - 31 and 32 - 63 of a block are dealt to the two halves of the
+// matrix instruction's sixteen columns, so that eight heads fill it.
+//   S^T = K . Q^T, keys on M, in two tiles of 16 x 2 keys: the k slots of the lane groups g = 0, 1 are a key's two blocks of 32 values, those of
+//   g = 2, 3 the key 32 places on; the columns 0 - 7 have Q in the former and zeros in the latter, the columns 8 - 15 the reverse.
+//   A lane's scores are then four of a tile, all of use.
+//   O = P . V, the weights' registers being the A operand for the block's keys 0 - 31 in the rows 0 - 7 and for 32 - 63 in the rows 8 - 15: two
+//   accumulators, each of which is looked at in one half of its rows. V passes LDS as bf16, for transposing reads.
 template <bool DENSE, int NW>
 __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a) {
   constexpr int VTILE = 64 * 128;
@@ -1169,7 +1171,9 @@ int64_t mx_attn_ctx(int64_t n_slots, int64_t hint) { return hint > 0 && hint < n
 }  // namespace
 
 extern "C" int tllm_mxfp4_attention_shape(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint) {
-  if (batch < 1 || n_q < 1 || n_slots < 1 || n_kv_heads < 1 || group < 1 || window < 0 || kv_len_hint < 0) return 0;
+  if (batch < 1 || batch > 65535 || n_q < 1 || n_q >= (1ll << 24) || n_slots < 1 || n_slots >= (1ll << 30) || n_kv_heads < 1 || n_kv_heads > 65535 || group < 1 ||
+      group > 64 || window < 0 || kv_len_hint < 0)
+    return 0;
   const MxAttnPlan p = mx_attn_plan(batch, n_q, mx_attn_ctx(n_slots, kv_len_hint), n_kv_heads, group, window);
   return p.rows << 16 | (p.one || p.many ? 4 : p.waves) << 8 | p.splits;
 }
@@ -1252,7 +1256,8 @@ extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, 
   a.scale_log2 = sm_scale * kLog2e;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)wgs);
-  int rc = cache->scale_slot_stride == 2 && n_slots > 1 ? launch_attention<true>(p, a, grid, st) : launch_attention<false>(p, a, grid, st);
+  const uintptr_t scales_at = reinterpret_cast<uintptr_t>(cache->k_scales) | reinterpret_cast<uintptr_t>(cache->v_scales) | static_cast<uintptr_t>(cache->scale_batch_stride | cache->scale_head_stride);
+  int rc = cache->scale_slot_stride == 2 && n_slots > 1 && scales_at % 2 == 0 ? launch_attention<true>(p, a, grid, st) : launch_attention<false>(p, a, grid, st);
   if (rc != TLLM_OK) return rc;
   rc = check_launch("mxfp4_attention");
   if (rc != TLLM_OK || p.splits == 1) return rc;

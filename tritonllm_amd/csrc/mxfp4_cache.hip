@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void mxfp4_cache_write_kernel(MxWriteArgs a) {
   Eight<T> e;
   e.load(a.x[kv] + b * a.xs_batch[kv] + h * a.xs_head[kv] + (t * a.xs_token[kv] + c * 8u * static_cast<unsigned>(sizeof(T))));
   // slots outside the cache and tokens behind the sequence's end are left as they are: the tokens from .. to - 1 are written
-  const int64_t far = 1ll << 40;                                       // (beyond any slot and any token; sums of it stay within 64 bits)
+  const int64_t far = 1ll << 36;                                       // (beyond any slot and any token; its bytes stay within 64 bits)
   auto held = [&](int64_t x) { return x < -far ? -far : x > far ? far : x; };
   const int64_t slot0 = held(mx_row_int(a.offset, a.offset_is_i64, b * a.offset_stride)) + a.first;      // of the launch's first token
   int64_t to = a.cache.n_slots - slot0;

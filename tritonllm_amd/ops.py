@@ -1137,7 +1137,7 @@ def mxfp4_attention(q: torch.Tensor, cache: Mxfp4Cache, sinks: torch.Tensor | No
     ``start_q`` (int32 or int64, read on the device) has one element or one per row: query ``i`` of row ``b`` sits at position ``start_q[b] + i``
     and sees the slots up to there (``bandwidth`` of them, if given). A query that sees none gives zeros; what it does not see, NaN
     included, is nothing to it. Any number of queries: drafts to verify, a chat's next turn, a prompt. ``kv_len_hint`` (the most keys that
-    a query sees, as far as the host knows) plans the launch; the result never depends on it."""
+    a query sees, as far as the host knows) plans the launch; it may be wrong, and changes no more than the order of sums."""
     done = host().mxfp4_attention(q, *cache, sinks, sm_scale, bandwidth, start_q, kv_len_hint)
     if done is not None:
         return done
@@ -1153,8 +1153,8 @@ def mxfp4_attention(q: torch.Tensor, cache: Mxfp4Cache, sinks: torch.Tensor | No
     sinks = sinks if sinks is None else sinks.contiguous()
     ok = q.stride(4) == 1 and q.stride(3) == 64 and q.stride(2) == 64 * repeat_kv and q.stride(1) % 8 == 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
     q = q if ok else _aligned(q)
-    window = min(int(bandwidth), 2**31 - 1) if bandwidth else 0
-    hint = 0 if kv_len_hint is None else max(int(kv_len_hint), 1)
+    window = max(min(int(bandwidth), 2**31 - 1), -1) if bandwidth else 0
+    hint = 0 if kv_len_hint is None else max(min(int(kv_len_hint), 2**31 - 1), 1)
     o = torch.empty((bs, n_ctx, n_heads * 64), dtype=_BF16, device=q.device)
     if o.numel():
         need = lib().tllm_mxfp4_attention_workspace_bytes(bs, n_ctx, desc.n_slots, n_kv_heads, repeat_kv, window, hint)
