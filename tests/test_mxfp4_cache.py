@@ -309,7 +309,8 @@ def test_shapes():
     assert shape(8, 1, 4096, 8, 8) == (8, 4, 4) and shape(8, 1, 32768, 8, 8) == (8, 4, 8) and shape(49, 1, 2048, 8, 8) == (8, 4, 1)
     assert shape(1, 1, 1 << 29, 1, 1) == (8, 4, 64)
     assert shape(1, 1, 300, 8, 9) == (32, 8, 1) and shape(8, 4, 4096, 8, 8) == (32, 8, 4) and shape(1, 97, 1597, 8, 8) == (32, 8, 1)
-    assert shape(1, 256, 2256, 8, 8) == (32, 4, 1) and shape(1, 512, 512, 8, 8) == (64, 4, 1)
+    assert shape(1, 256, 2256, 8, 8) == (32, 4, 1) and shape(1, 512, 512, 8, 8) == (64, 4, 1) and shape(1, 512, 8192, 8, 8) == (64, 4, 1)
+    assert shape(1, 64, 4096, 8, 8) == (32, 8, 1) and shape(1, 64, 8192, 8, 8) == (32, 8, 2) and shape(2, 72, 11011, 4, 4) == (32, 8, 3)
     assert shape(1, 2048, 2048, 8, 8) == (256, 4, 1) and shape(3, 333, 333, 8, 8) == (128, 4, 1) and shape(1, 1000, 9000, 8, 8) == (128, 4, 1) and shape(1, 2048, 10**6, 8, 8, window=128) == (256, 4, 1)
 
 

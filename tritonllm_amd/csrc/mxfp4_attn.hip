@@ -21,17 +21,18 @@ struct MxAttnArgs {
   MxCache c;
   int batch, n_q, n_kv_heads, group, window;
   int row_groups;         // runs of rows (queries x heads of a KV head) that a workgroup takes
-  int splits, fill;       // planned splits; workgroups a stream that fill the CUs
+  int splits, fill, one;  // planned splits; workgroups a stream that fill the CUs; whether this is the kernel for one query
   float scale_log2;       // sm_scale * log2 e
 };
 
 namespace {
 constexpr int PART = 66;              // floats of a record in the workspace
-// Splits, one query of 8 heads, us. One workgroup walks up to 1024 keys alone (no second launch): 300 keys 4.9, split 6.7; 600 5.7, 6.7; 1000 6.4,
-// 6.8; 8 rows of 1024 6.5, 7.2; but 2000 9.0 and 6.8. A workgroup to a CU: 49 rows of up to 2048 11.9, with two 16.6; 32 of 4096 16.1, 19.2; one of
-// 32768 11.2, 13.2 -- until each has 4096 keys: 8 rows of 32768 28.6, with one of 8192 31.6 and two of 2048 30.4; 8 of 131072 96, 94 and 104. At
-// least 256 keys: one row of 4096 7.3, of 512 and more 7.6 - 9.0.
-constexpr int kUnsplit = 1024, kLeastShift = 8, kMostShift = 12, kFill = 256;
+// Splits, one query of 8 heads, us. One workgroup walks up to kUnsplit keys alone (no second launch): 300 keys 4.9, split 6.7; 600 5.7, 6.7; 1000 6.4,
+// 6.8; 8 rows of 1024 6.4, 7.9; but 2000 9.0 and 6.8. A workgroup to a CU: 49 rows of up to 2048 11.9, with two 17.2; 32 of 4096 16.1, 19.2; one of
+// 32768 11.2, 13.2 -- until each has 2^kMostShift keys: 8 rows of 32768 28.6, with one of 8192 31.6 and two of 2048 30.4; 8 of 131072 96, 94 and 104.
+// At least 2^kLeastShift keys: one row of 4096 7.3, of 512 and more 7.6 - 9.0. (Eight wavefronts instead of four, with as many splits or half: 300
+// keys 5.4, 8 rows of 4096 10.5 and 11.7 against 10.1, 32 of 2048 10.5 against 10.2.)
+constexpr int kUnsplit = 1024, kLeastShift = 8, kMostShift = 12, kFill = 256, kDeep = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are exp2(logit - reference). The reference of one query and of a few rows is the largest logit that it was raised to, and stays there
 // until a lane's weights of a block sum to more than kMostSum; that of many rows lies kLift above it, and stays until a weight reaches 2.
@@ -44,12 +45,12 @@ constexpr int kShare = 34 * 64;       // floats that a wavefront hands over for 
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short i16x4;
 typedef __attribute__((__vector_size__(8 * sizeof(short)))) short i16x8;
 
-// Context splits for `fill` workgroups a stream over `ctx` visible keys: one up to kUnsplit keys, then enough to fill the CUs, beyond that about
-// 2^kMostShift keys each, never less than 2^kLeastShift, at most 64. The host plans the launch with it from the size of the cache (or the
-// caller's hint), the kernels evaluate it again with the length that they read.
-__host__ __device__ inline int mx_attn_splits(int fill, int ctx) {
+// Context splits over `ctx` visible keys where `fill` workgroups a stream (or a run of rows) fill the CUs, by the rules above and at the plan below;
+// at most 64. The host plans the launch with it from the size of the cache (or the caller's hint), the kernels evaluate it again with
+// the length that they read.
+__host__ __device__ inline int mx_attn_splits(bool one, int fill, int ctx) {
   const int cap = ((ctx - 1) >> kLeastShift) + 1, by_work = ((ctx - 1) >> kMostShift) + 1;
-  int s = fill > by_work ? fill : by_work;
+  int s = one ? (fill > by_work ? fill : by_work) : fill >= 4 || ctx > kDeep ? fill : 1;
   s = s < cap ? s : cap;
   s = s > 1 && ctx > kUnsplit ? s : 1;
   return s < 64 ? s : 64;
@@ -72,7 +73,7 @@ __device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int b, int first_
   lo = lo < 0 ? 0 : lo < hi ? lo : hi;
   s.lo = static_cast<int>(lo);
   s.hi = static_cast<int>(hi);
-  const int live = mx_attn_splits(a.fill, hi > lo ? s.hi - s.lo : 1);
+  const int live = mx_attn_splits(a.one != 0, a.fill, hi > lo ? s.hi - s.lo : 1);
   s.live = live < a.splits ? live : a.splits;
   return s;
 }
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
     for (int j = 0; j < DPT; ++j) o[j] += from[TPR * j] * f;
   }
   const int head = kvh * G + eh;
-  if (a.splits > 1) {
+  if (sp.live > 1) {
     float* const p = a.part + ((static_cast<int64_t>(split) * a.batch + b) * (a.n_kv_heads * G) + head) * PART;
 #pragma unroll
     for (int j = 0; j < DPT; ++j) p[ed + TPR * j] = o[j];
@@ -677,7 +678,7 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     }
     if (row0 + 32 * rt + l31 >= rows) continue;
     // value rr = RPG kg + r: d = 32 (rr / 16) + 8 (rr / 4 % 4) + 4 h + rr % 4
-    if (a.splits > 1) {
+    if (sp.live > 1) {
       float* const p = a.part + (((static_cast<int64_t>(split) * a.batch + b) * a.n_q + query[rt]) * (a.n_kv_heads * a.group) + head[rt]) * PART;
 #pragma unroll
       for (int r = 0; r < RPG; ++r) {
@@ -1101,6 +1102,7 @@ __global__ __launch_bounds__(64) void mxfp4_attn_reduce_kernel(MxAttnArgs a, int
 #pragma unroll
   for (int u = 0; u < 8; ++u) v[u] = p0[(u < a.splits ? u : a.splits - 1) * stride + lane];
   const int live = mx_span(a, b, row0, row0 + rows_per_group - 1).live;
+  if (live == 1) return;                                       // (whoever walked the keys alone has stored the answer)
   const float m_s = lane < live ? m_raw : kNoRef;
   const float m_all = wave_max(m_s);
   const float f_s = __builtin_amdgcn_exp2f(m_s - m_all);
@@ -1133,20 +1135,21 @@ struct MxAttnPlan {
   int splits, fill;
 };
 
-// Which kernel, by the runs of rows and of streams that there are (eight KV heads of eight query heads, us):
-//   many rows, 256 to a workgroup, from 385 runs of 256 on -- one prompt of 2048 51, in 64 rows a workgroup 57, 32 64; 4096 149, 173, 196; 2000 behind
-//   2000 105, 121, 138 -- and from 513 runs of 128 on where walks are short, up to 768 keys: 2 x 700 23.9, 27.2, 26.4; 2048 with a window of 128 19, 32,
-//   31. Between, two workgroups to a CU do not come out even: 1200 33, 28.7, 29.2; 1200 behind 2800 106, 91, 103; 1500 40, 37, 41.
-//   128 to a workgroup where that is one or two workgroups to a CU, 321 to 512: 1000 behind 8000 167, in 256 rows a workgroup 187, 64 214; 800 behind
-//   4000 85, 102, 114; 700 behind 4000 84, 101, 103; 1000 22.1, 28.4, 22.4; 2 x 512 16, 18.6, 18.9; 4 x 256 12.8, 13.5, 16.8; 3 x 333 13.8, 15.9, 17.3;
-//   8 x 128 behind 2000 48.8, 51.2, 51; a short prompt is behind (700 17.8, in 32 rows 15.3), as are all with fewer workgroups than that: 512 13.9,
-//   18, in 64 rows 10.9; 600 16.6, 20, 16.6; 1100 behind 1000 (576) 52, 53, 47.6.
-//   32 rows shared out between eight wavefronts up to 256 runs of 32: 97 behind 1500 10.0, between four 11.6; 16 x 8 of 2000 11.5, 13.5; 64 behind
-//   8000 22.3, 26.9; with four from there on: 150 behind 1350 16.4, 13.4; 256 behind 2000 22, 18.2; 64 x 4 of 1000 16, 12.1.
-//   64 rows to a workgroup from 768 such runs on: 400 behind 1600 24, with 32 rows 26; 512 10.7, 11.9; 512 behind 4000 73, 80; but 256 behind 2000
-//   19.4, 18.2; 333 9.2, 7.5; 64 x 4 of 1000 16.2, 12.1.
-// Splits as far as they fill the CUs four times: 8 x 4 of 4096 (64 runs) 12.9, none 20.5; 8 x 8 of 2000 (128 runs) none 11.2, two 13.9; 4 x 16 of 3000
-// 14.3, 15.2; 97 behind 1500 (200) 10.0, two 20.4.
+// Which kernel, by the runs of rows and of streams that there are (eight KV heads of eight query heads, us; "n behind m": n queries behind m tokens):
+//   Many rows, 256 to a workgroup, from 385 runs of 256 on -- one prompt of 2048 51.9, in 128 rows a workgroup 55.7, 64 56.7, 32 62.5; 4096 158, 174, 183,
+//   213 -- and from 513 runs of 128 on where walks are short, up to 768 keys: 2 x 700 24.3, 26.2, 27.6, 27.2; 2048 with a window of 128 19, 25, 32, 31.
+//   Between, two workgroups to a CU do not come out even: 1200 33.7, 25.7, 28.8, 29; 1200 behind 6800 223, 213, 178, 202; 1500 behind 2500 104, 104, 102,
+//   116.
+//   128 to a workgroup from 385 to 512 runs of them, one or two workgroups to a CU: 2 x 512 15.8, in 256 rows 18.8, 64 18.8, 32 18.9; 4 x 256 13.0,
+//   13.6, 17.0, 17.2; 3 x 333 13.9, 16.0, 17.5, 17.8; 8 x 128 behind 2000 47.6, 51.4, 49.8, 56; 1000 behind 8000 162, 188, 165, 188; 800 behind 4000
+//   85.4, 103, 86.8, 89; but 700 behind 4000 (352) 84, 101, 70, 77, and 512 behind 4000 64, 96, 48, 56.
+//   32 rows shared out between eight wavefronts up to 256 runs of 32: 97 behind 1500 10.0, between four 11.7; 97 behind 8000 31, 39; 64 behind 8000
+//   24.2, 26.9; with four from there on: 150 behind 1350 17.3, 13.8; 256 behind 2000 22, 18.2; 64 x 4 of 1000 16.1, 12.5.
+//   64 rows to a workgroup from 768 such runs on: 512 behind 4000 48, with 32 rows 56; 700 behind 4000 70, 77; 512 10.7, 11.9; a little behind on
+//   700 17.8, 15.7; but 350 behind 4000 44.6, 40; 333 9.2, 7.8; 64 x 4 of 1000 16.4, 12.5.
+// Workgroups that share rows' keys, as many as there are CUs for, up to kDeep keys only if that is four: 8 x 4 of 4096 (64 runs) 12.5, none 16.8;
+// 64 behind 8000 (128) two 22.2, none 28.9; 72 x 2 of 11000 in four heads of four (72) three 22.3, none 36; but 8 x 8 of 2000 (128) two 13.9, none
+// 11.2; 97 behind 8000 (200) two 38, none 28.7; 512 behind 4000 in 64 rows (512) two 67, none 48.
 MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window) {
   MxAttnPlan p{};
   const int64_t rows = n_q * group, streams = batch * n_kv_heads;
@@ -1156,14 +1159,14 @@ MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_he
   };
   const int64_t wide = (rows + 255) / 256 * streams, half = (rows + 127) / 128 * streams, narrow = (rows + 31) / 32 * streams;
   p.one = n_q == 1 && group <= 8;
-  p.many = !p.one && rows > 128 && (wide > 384 || (half > 320 && half <= 512) || (half > 512 && seen(256) <= 768));
+  p.many = !p.one && rows > 128 && (wide > 384 || (half > 384 && half <= 512) || (half > 512 && seen(256) <= 768));
   p.tiles = narrow < 768 ? 1 : 2;
   p.waves = narrow <= 256 ? 8 : 4;
   p.rows = p.one ? 8 : p.many ? (half > 512 ? 256 : 128) : 32 * p.tiles;
   p.row_groups = (int)((rows + p.rows - 1) / p.rows);
   const int64_t units = streams * p.row_groups;
-  p.fill = p.one ? (int)((kFill + units - 1) / units) : kFill / units >= 4 ? (int)(kFill / units) : 1;
-  p.splits = p.many ? 1 : mx_attn_splits(p.fill, (int)seen(p.rows));
+  p.fill = p.one ? (int)((kFill + units - 1) / units) : kFill / units > 0 ? (int)(kFill / units) : 1;
+  p.splits = p.many ? 1 : mx_attn_splits(p.one, p.fill, (int)seen(p.rows));
   return p;
 }
 
@@ -1253,6 +1256,7 @@ extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, 
   a.row_groups = p.row_groups;
   a.splits = p.splits;
   a.fill = p.fill;
+  a.one = p.one;
   a.scale_log2 = sm_scale * kLog2e;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)wgs);
