@@ -23,6 +23,7 @@ struct MxAttnArgs {
   int row_groups;         // runs of rows (queries x heads of a KV head) that a workgroup takes
   int splits, fill, one;  // planned splits; workgroups a stream that fill the CUs; whether this is the kernel for one query
   float scale_log2;       // sm_scale * log2 e
+  MxDiv by_group, by_heads, by_batch, by_row_groups, by_n_q;      // the latter two for the kernels that need them
 };
 
 namespace {
@@ -56,17 +57,18 @@ __host__ __device__ inline int mx_attn_splits(bool one, int fill, int ctx) {
   return s < 64 ? s : 64;
 }
 
-// The keys lo .. hi-1 that any of the rows first .. last of batch row b sees, and the number of splits that take part.
+// The keys lo .. hi-1 that any of the rows first .. last of a batch row that starts at `start` sees, and the number of splits that take part.
 struct MxSpan {
   int64_t start;
   int lo, hi, live;
 };
-__device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int b, int first_row, int last_row) {
+__device__ __forceinline__ int64_t mx_start(const MxAttnArgs& a, int b) { return mx_row_int(a.start_q, a.start_is_i64, static_cast<int64_t>(b) * a.start_stride); }
+__device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int64_t start, int first_row, int last_row) {
   MxSpan s;
-  s.start = mx_row_int(a.start_q, a.start_is_i64, static_cast<int64_t>(b) * a.start_stride);
+  s.start = start;
   const int64_t far = 1ll << 40;                               // (beyond any slot; sums of it stay within 64 bits)
   s.start = s.start < -far ? -far : s.start > far ? far : s.start;
-  const int q0 = a.n_q == 1 ? 0 : first_row / a.group, q1 = a.n_q == 1 ? 0 : last_row / a.group;
+  const int q0 = a.n_q == 1 ? 0 : a.by_group(first_row), q1 = a.n_q == 1 ? 0 : a.by_group(last_row);
   int64_t hi = s.start + (q1 < a.n_q ? q1 : a.n_q - 1) + 1;
   hi = hi < 0 ? 0 : hi < a.c.n_slots ? hi : a.c.n_slots;
   int64_t lo = a.window > 0 ? s.start + q0 - a.window + 1 : 0;
@@ -78,10 +80,17 @@ __device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int b, int first_
   return s;
 }
 
+// A head's sink: asked for at a kernel's beginning (its latency would stand at the end), without a branch that would wait for it, and looked at
+// at the end, as an exponent of two.
+__device__ __forceinline__ bf16 mx_sink(const MxAttnArgs& a, int head) {
+  const bf16* const p = a.sinks ? a.sinks : a.q;
+  return p[a.sinks ? head : 0];
+}
+
 // What the weighted sum of a row's values is multiplied with: the sink joins the denominator. Nothing at all to attend to -- no key and a
 // sink of -infinity -- gives zeros.
-__device__ __forceinline__ float mx_norm(const MxAttnArgs& a, int head, float m, float l) {
-  const float sink = a.sinks ? static_cast<float>(a.sinks[head]) * kLog2e : 0.f;
+__device__ __forceinline__ float mx_norm(const MxAttnArgs& a, bf16 sink_of, float m, float l) {
+  const float sink = a.sinks ? static_cast<float>(sink_of) * kLog2e : 0.f;
   const float top = fmaxf(m, sink);
   const float f = __builtin_amdgcn_exp2f(m - top);
   const float z = l * f + __builtin_amdgcn_exp2f(sink - top);
@@ -135,10 +144,8 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
   const int r16 = lane & 15, g = lane >> 4;
 
   // the splits are the slowest part of the index: those that a context does not need are the last
-  unsigned id = blockIdx.x;
-  const int kvh = id % a.n_kv_heads;
-  id /= a.n_kv_heads;
-  const int b = id % a.batch, split = id / a.batch;
+  const int id = a.by_heads(blockIdx.x), kvh = blockIdx.x - id * a.n_kv_heads;
+  const int split = a.by_batch(id), b = id - split * a.batch;
   const int G = a.group;
 
   bf16x8 qf[4];
@@ -155,8 +162,11 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
   // Without a window the keys begin at slot 0 and the wavefront's first block is known ahead of the start position, whose load takes as long as
   // the block's own: it is asked for at once (and not looked at where the context turns out to be shorter).
   int lo = 0;
-  if (a.window > 0) lo = min(mx_span(a, b, 0, 0).lo, a.c.n_slots - 1);      // (a slot of the cache, also where a window behind its end has none)
+  if (a.window > 0) lo = min(mx_span(a, mx_start(a, b), 0, 0).lo, a.c.n_slots - 1);      // (a slot of the cache, also where a window behind its end has none)
   const int first = split * NW + wave;
+  constexpr int TPR = NW * 64 / 8, DPT = 64 / TPR > 0 ? 64 / TPR : 1;      // at the end: thread -> (head, every TPR-th of its 64 values)
+  const int eh = tid / TPR, ed = tid % TPR;
+  const bf16 sink = mx_sink(a, kvh * G + (eh < G ? eh : G - 1));
   const int nall = (a.c.n_slots - lo + 63) >> 6;                // blocks that the cache has from there on
 
   const int64_t kv_off = b * a.c.bs + kvh * a.c.hs + lo * a.c.ts, sc_off = b * a.c.sbs + kvh * a.c.shs + lo * a.c.sts;
@@ -205,7 +215,7 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
   Block even, odd;
   load_block(first, even);
   __builtin_amdgcn_sched_barrier(0);                           // (in the loop's order, so that it can wait for the one and not the other)
-  const MxSpan sp = mx_span(a, b, 0, 0);
+  const MxSpan sp = mx_span(a, mx_start(a, b), 0, 0);
   if (split >= sp.live) return;
   const int len = sp.hi - sp.lo, nblk = (len + 63) >> 6, step = sp.live * NW;      // the stream's wavefronts take its blocks in turn
   load_block(first + step, odd);
@@ -361,9 +371,6 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
       mine[(4 * g + i) * AROW + 16 * nb + r16] = g < 2 ? x : y;
     }
   __syncthreads();
-  // thread -> (head, every TPR-th of its 64 values)
-  constexpr int TPR = NW * 64 / 8, DPT = 64 / TPR > 0 ? 64 / TPR : 1;
-  const int eh = tid / TPR, ed = tid % TPR;
   if (eh >= G || ed >= 64) return;
   float m_all = kNoRef;
 #pragma unroll
@@ -389,7 +396,7 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
     }
     return;
   }
-  const float f = mx_norm(a, head, m_all, l_all);
+  const float f = mx_norm(a, sink, m_all, l_all);
   bf16* const to = a.out + b * a.out_bs + head * 64;
 #pragma unroll
   for (int j = 0; j < DPT; ++j) to[ed + TPR * j] = static_cast<bf16>(o[j] * f);
@@ -415,47 +422,33 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   const int kg = wave;
 
   // the splits are the slowest part of the index: those that a context does not need are the last
-  unsigned id = blockIdx.x;
-  const int kvh = id % a.n_kv_heads;
-  id /= a.n_kv_heads;
-  const int b = id % a.batch;
-  id /= a.batch;
-  const int rg = a.row_groups - 1 - static_cast<int>(id % a.row_groups), split = id / a.row_groups;
+  const int i0 = a.by_heads(blockIdx.x), kvh = blockIdx.x - i0 * a.n_kv_heads;
+  const int i1 = a.by_batch(i0), b = i0 - i1 * a.batch;
+  const int split = a.by_row_groups(i1), rg = a.row_groups - 1 - (i1 - split * a.row_groups);
   const int rows = a.n_q * a.group, row0 = rg * RB;
 
   bf16x8 qf[RT][4];
   int query[RT], head[RT];
+  bf16 sink[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     int row = row0 + 32 * rt + l31;
     row = row < rows ? row : rows - 1;                         // (rows that are not there repeat the last one; never stored)
-    query[rt] = row / a.group;
+    query[rt] = a.by_group(row);
     head[rt] = kvh * a.group + row - query[rt] * a.group;
+    sink[rt] = mx_sink(a, head[rt]);
     const bf16* const qr = a.q + b * a.q_bs + query[rt] * a.q_ts + head[rt] * 64 + 32 * h;
 #pragma unroll
     for (int t = 0; t < 4; ++t) qf[rt][t] = *reinterpret_cast<const bf16x8*>(qr + 8 * t);
   }
-  const MxSpan sp = mx_span(a, b, row0, row0 + RB - 1);
-  if (split >= sp.live) return;
-  const int len = sp.hi - sp.lo, nblk = (len + 31) >> 5;
-  const int first = split * KG + kg, step = sp.live * KG;
 
-  int upper[RT], lower[RT];                                    // the keys that the lane's row sees, counted from sp.lo
-  int seen_hi = 0x7fffffff, seen_lo = 0;                       // keys that every row of the wavefront sees
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int64_t up = sp.start + query[rt] - sp.lo, low = up - a.window + 1;
-    upper[rt] = static_cast<int>(up < -1 ? -1 : up < len - 1 ? up : len - 1);
-    lower[rt] = static_cast<int>(a.window == 0 || low < 0 ? 0 : low < len ? low : len);
-  }
-  {
-    const int q0 = row0 / a.group, q1r = (row0 + RB - 1) / a.group, q1 = q1r < a.n_q ? q1r : a.n_q - 1;
-    const int64_t up = sp.start + q0 - sp.lo, low = sp.start + q1 - sp.lo - a.window + 1;
-    seen_hi = static_cast<int>(up < -1 ? -1 : up < len - 1 ? up : len - 1);
-    seen_lo = static_cast<int>(a.window == 0 || low < 0 ? 0 : low < len ? low : len);
-  }
+  // Without a window the keys begin at slot 0, and the first block is asked for ahead of the start position (whose load takes as long as its own).
+  int lo = 0;
+  if (a.window > 0) lo = min(mx_span(a, mx_start(a, b), row0, row0 + RB - 1).lo, a.c.n_slots - 1);
+  const int first = split * KG + kg;
+  const int nall = (a.c.n_slots - lo + 31) >> 5;                // blocks that the cache has from there on
 
-  const int64_t kv_off = b * a.c.bs + kvh * a.c.hs + sp.lo * a.c.ts, sc_off = b * a.c.sbs + kvh * a.c.shs + sp.lo * a.c.sts;
+  const int64_t kv_off = b * a.c.bs + kvh * a.c.hs + lo * a.c.ts, sc_off = b * a.c.sbs + kvh * a.c.shs + lo * a.c.sts;
   const unsigned char *const kp = a.c.blocks[0] + kv_off, *const vp = a.c.blocks[1] + kv_off;
   const unsigned char *const ksp = a.c.scales[0] + sc_off, *const vsp = a.c.scales[1] + sc_off;
   unsigned char* const vtile = smem + wave * VTILE;
@@ -463,7 +456,7 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   // Loads as above: 32 keys' codes, 16 bytes a lane as they lie in memory, and in one load the scale bytes of two neighbouring slots to a lane,
   // keys' in lanes 0 - 15, values' in 16 - 31 (and the same in the other 32).
   const int64_t blk_bytes = 32 * a.c.ts, blk_scales = 32 * a.c.sts;
-  const int slots = a.c.n_slots - sp.lo - 32 * (nblk - 1);      // that the cache has from the last block's first key on
+  const int slots = a.c.n_slots - lo - 32 * (nall - 1);         // in the last one of them
   const unsigned char* const sbase = (lane & 16 ? vsp : ksp) - 2;
   const int pair = 2 * (lane & 15);
   unsigned off[2];                                             // [whole, last]
@@ -478,13 +471,37 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     unsigned s;
   };
   auto load_block = [&](int at, Block& r) __attribute__((always_inline)) {
-    const int blk = at < nblk ? at : nblk - 1;                 // (a block that is not there: the last one again)
-    const bool end = blk == nblk - 1;
+    const int blk = at < nall ? at : nall - 1;                 // (a block that is not there: any)
+    const bool end = blk == nall - 1;
     const unsigned x = mx_choose(end, off[1], off[0]);
     r.k = *reinterpret_cast<const u32x4*>(kp + blk * blk_bytes + x);
     r.v = *reinterpret_cast<const u32x4*>(vp + blk * blk_bytes + x);
     r.s = mx_scale_pair<DENSE>(sbase + blk * blk_scales + mx_choose(end, soff[1], soff[0]), a.c.sts, end ? slots - 1 - pair : 1);
   };
+  Block even, odd;
+  load_block(first, even);
+  __builtin_amdgcn_sched_barrier(0);                           // (in the loop's order, so that it can wait for the one and not the other)
+  const MxSpan sp = mx_span(a, mx_start(a, b), row0, row0 + RB - 1);
+  if (split >= sp.live) return;
+  const int len = sp.hi - sp.lo, nblk = (len + 31) >> 5, step = sp.live * KG;
+  load_block(first + step, odd);
+  __builtin_amdgcn_sched_barrier(0);
+
+  int upper[RT], lower[RT];                                    // the keys that the lane's row sees, counted from sp.lo
+  int seen_hi = 0x7fffffff, seen_lo = 0;                       // keys that every row of the wavefront sees
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int64_t up = sp.start + query[rt] - sp.lo, low = up - a.window + 1;
+    upper[rt] = static_cast<int>(up < -1 ? -1 : up < len - 1 ? up : len - 1);
+    lower[rt] = static_cast<int>(a.window == 0 || low < 0 ? 0 : low < len ? low : len);
+  }
+  {
+    const int q0 = a.by_group(row0), q1r = a.by_group(row0 + RB - 1), q1 = q1r < a.n_q ? q1r : a.n_q - 1;
+    const int64_t up = sp.start + q0 - sp.lo, low = sp.start + q1 - sp.lo - a.window + 1;
+    seen_hi = static_cast<int>(up < -1 ? -1 : up < len - 1 ? up : len - 1);
+    seen_lo = static_cast<int>(a.window == 0 || low < 0 ? 0 : low < len ? low : len);
+  }
+
   // K's codes pass LDS into the operand's order, lane (key l31, block h); the keys 16 - 31 have their blocks the other way round there, for the banks
   const int k_to = 16 * (lane ^ (lane >> 5)), k_from = l31 * 32 + 16 * (h ^ (l31 >> 4));
   const int k_lane = 4 * (l31 >> 1), k_shift = 16 * (l31 & 1) + 8 * h, v_lane = 4 * (16 + (lane >> 2)), v_shift = 8 * (lane & 3);
@@ -514,7 +531,7 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     const bool end = blk == nblk - 1;
     // K's codes through LDS; the tile of V follows in the same place (a wavefront's LDS operations stay in order)
     *reinterpret_cast<u32x4*>(vtile + k_to) = r.k;
-    const unsigned pairs = end ? r.s >> pair_shift : r.s;
+    const unsigned pairs = blk == nall - 1 ? r.s >> pair_shift : r.s;
     const unsigned ks = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(k_lane, static_cast<int>(pairs))) >> k_shift & 255u;
     unsigned vs = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(v_lane, static_cast<int>(pairs))) >> v_shift & 255u;
     const u32x4 kc = *reinterpret_cast<const u32x4*>(vtile + k_from);
@@ -621,11 +638,6 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     }
   };
   if (first < nblk) {
-    Block even, odd;
-    load_block(first, even);
-    __builtin_amdgcn_sched_barrier(0);                         // (in the loop's order, so that it can wait for the one and not the other)
-    load_block(first + step, odd);
-    __builtin_amdgcn_sched_barrier(0);
     int blk = first;
     for (; blk + step < nblk; blk += 2 * step) {
       process(blk, even);
@@ -688,7 +700,7 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
       if (kg == 0) p[64 + h] = h == 0 ? m : l;
       continue;
     }
-    const float f = mx_norm(a, head[rt], m, l);
+    const float f = mx_norm(a, sink[rt], m, l);
     bf16* const to = a.out + b * a.out_bs + query[rt] * a.out_ts + head[rt] * 64;
 #pragma unroll
     for (int r = 0; r < RPG; r += 4) {
@@ -707,10 +719,10 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
 //   The matrix cores and the vector ALU work at the same time: with one tile's weights (32 keys x 32 rows) the next one's scores are issued in
 //   turn, and the products of the one before. Of block j (32 keys), S^T of tile 1, weights of tile 0 and P . V of block j - 1 in tile 1; then S^T of
 //   block j + 1 in tile 0, weights of tile 1 and P . V of tile 0. Operands of K and of V live from one such half to the next.
-template <int RUNS>
-__global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
+template <int RUNS, int KG>
+__global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
   static_assert(RUNS == 4 || RUNS == 2, "runs of a workgroup");
-  constexpr int KG = 4 / RUNS, UNIT = 16 * RUNS, HALVES = UNIT / 32, RB = 64 * RUNS;
+  constexpr int UNIT = 16 * RUNS, HALVES = UNIT / 32, RB = 64 * RUNS;
   constexpr int KTILE = UNIT * 128, STAGE = 2 * KTILE;         // bytes: K [UNIT keys][64 values], then V
   __shared__ __align__(16) unsigned char smem[KG * 3 * STAGE];
   __shared__ __align__(8) unsigned s_any[KG][3][2];            // whether a stage's values hold NaN, by 32 keys,
@@ -723,29 +735,71 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
 
   // the rows that see most keys come first, and where the launch is two workgroups to a CU the second ones are taken in the opposite order, so
   // that a CU with a long walk gets a short one next to it
-  unsigned id = blockIdx.x;
-  const int kvh = id % a.n_kv_heads;
-  id /= a.n_kv_heads;
+  unsigned id = a.by_heads(blockIdx.x);
+  const int kvh = blockIdx.x - id * a.n_kv_heads;
   {
-    const unsigned per_round = 256 / (a.n_kv_heads < 256 ? a.n_kv_heads : 256), n = gridDim.x / a.n_kv_heads;
-    if (n <= 2 * per_round && id >= per_round) id = n + per_round - 1 - id;
+    const unsigned per_round = a.n_kv_heads < 256 ? a.by_heads(256) : 1, n = a.by_heads(gridDim.x);
+    if (RUNS * KG == 4 && n <= 2 * per_round && id >= per_round) id = n + per_round - 1 - id;
   }
-  const int b = id % a.batch, rg = a.row_groups - 1 - static_cast<int>(id / a.batch);
+  const int i1 = a.by_batch(id), b = id - i1 * a.batch, rg = a.row_groups - 1 - i1;
   const int rows = a.n_q * a.group, row0 = rg * RB + run * 64;
 
-  bf16x8 qf[2][4];
-  int query[2], head[2];
+  // Without a window the keys begin at slot 0, and the first unit is asked for ahead of the start position (whose load takes as long as its own).
+  int lo = 0;
+  if (a.window > 0) lo = min(mx_span(a, mx_start(a, b), rg * RB, rg * RB + RB - 1).lo, a.c.n_slots - 1);
+  const int nall = (a.c.n_slots - lo + UNIT - 1) / UNIT;       // units that the cache has from there on
+  // ---- the movers
+  const int kv = run / (RUNS / 2), piece = tid & (UNIT * 2 - 1);      // 0: keys, 1: values; (key piece / 2, block piece % 2) of a unit
+  const unsigned char* const src = a.c.blocks[kv] + b * a.c.bs + kvh * a.c.hs + lo * a.c.ts + 16 * (piece & 1);
+  const unsigned char* const ssrc = a.c.scales[kv] + b * a.c.sbs + kvh * a.c.shs + lo * a.c.sts + (piece & 1);
+  const int64_t unit_bytes = UNIT * a.c.ts, unit_scales = UNIT * a.c.sts;
+  const unsigned off = (piece >> 1) * static_cast<unsigned>(a.c.ts), soff = (piece >> 1) * static_cast<unsigned>(a.c.sts);
+  const int at_end = min(piece >> 1, (a.c.n_slots - lo - 1) & (UNIT - 1));      // behind the last slot of the cache rows are held to it
+  const unsigned off_end = at_end * static_cast<unsigned>(a.c.ts), soff_end = at_end * static_cast<unsigned>(a.c.sts);
+  unsigned to[4];                                              // where the piece's four chunks of 16 bytes go
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int key = piece >> 1, c = 4 * (piece & 1) + t;
+    to[t] = kv == 0 ? key * 128 + ((c ^ (key >> 1 & 7)) << 4) : KTILE + mx_v_chunk4(key, c);
+  }
+  u32x4 raw;
+  unsigned raw_s;
+  auto load_unit = [&](int u) __attribute__((always_inline)) {
+    const int v = min(KG * u + kg, nall - 1);                  // (one that is not there: any)
+    const bool end = v == nall - 1;
+    raw = *reinterpret_cast<const u32x4*>(src + v * unit_bytes + mx_choose(end, off_end, off));
+    raw_s = (ssrc + v * unit_scales)[mx_choose(end, soff_end, soff)];
+  };
+  load_unit(0);
+  __builtin_amdgcn_sched_barrier(0);
+
+  int query[2];
+  bf16 sink[2];
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) {
     int row = row0 + 32 * rt + l31;
     row = row < rows ? row : rows - 1;                         // (rows that are not there repeat the last one; never stored)
-    query[rt] = row / a.group;
-    head[rt] = kvh * a.group + row - query[rt] * a.group;
-    const bf16* const qr = a.q + b * a.q_bs + query[rt] * a.q_ts + head[rt] * 64 + 32 * h;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) qf[rt][t] = *reinterpret_cast<const bf16x8*>(qr + 8 * t);
+    query[rt] = a.by_group(row);
+    sink[rt] = mx_sink(a, kvh * a.group + row - query[rt] * a.group);
   }
-  const MxSpan sp = mx_span(a, b, rg * RB, rg * RB + RB - 1);
+  // Q and the outputs pass LDS, for whole rows of 128 bytes from and to memory (a lane's own pieces of them are 64 accesses an instruction): eight
+  // rows at a time, lane / 8 of them, 16 bytes lane % 8; in LDS the pieces of a row are XORed with its number.
+  const int last_row = rows - 1, q_first = a.by_group(row0 < last_row ? row0 : last_row);
+  auto place = [&](int j, int* q_of, int* h_of) __attribute__((always_inline)) {     // row 8 j + lane / 8's query and head
+    const int row = row0 + 8 * j + (lane >> 3), x = (row < rows ? row : last_row) - q_first * a.group;
+    const int qx = a.by_group(x);
+    *q_of = q_first + qx;
+    *h_of = kvh * a.group + x - qx * a.group;
+  };
+  bf16x8 qf[2][4];
+  u32x4 q_raw[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    int qq, hh;
+    place(j, &qq, &hh);
+    q_raw[j] = *reinterpret_cast<const u32x4*>(a.q + b * a.q_bs + qq * a.q_ts + hh * 64 + 8 * (lane & 7));
+  }
+  const MxSpan sp = mx_span(a, mx_start(a, b), rg * RB, rg * RB + RB - 1);
   const int len = sp.hi - sp.lo, all = (len + UNIT - 1) / UNIT;
   const int units = (all + KG - 1) / KG;                       // of each group: the wavefronts meet as often in all of them
   auto key_of = [&](int u) { return UNIT * (KG * u + kg); };   // a unit's first key
@@ -760,7 +814,7 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
   int seen_hi, seen_lo, w_lo, w_hi;                            // keys that every row of the wavefront sees; units of which any row sees a key
   {
     const int last = rows - 1, r0 = row0 < last ? row0 : last, r1 = row0 + 63 < last ? row0 + 63 : last;
-    const int64_t up0 = sp.start + r0 / a.group - sp.lo, up1 = sp.start + r1 / a.group - sp.lo;
+    const int64_t up0 = sp.start + a.by_group(r0) - sp.lo, up1 = sp.start + a.by_group(r1) - sp.lo;
     auto held = [&](int64_t x, int least, int most) { return static_cast<int>(x < least ? least : x < most ? x : most); };
     seen_hi = held(up0, -1, len - 1);
     seen_lo = a.window == 0 ? 0 : held(up1 - a.window + 1, 0, len);
@@ -770,28 +824,6 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
     w_lo = w_lo < w_hi ? w_lo : w_hi;
   }
 
-  // ---- the movers
-  const int kv = run / (RUNS / 2), piece = tid & (UNIT * 2 - 1);      // 0: keys, 1: values; (key piece / 2, block piece % 2) of a unit
-  const unsigned char* const src = a.c.blocks[kv] + b * a.c.bs + kvh * a.c.hs + sp.lo * a.c.ts + 16 * (piece & 1);
-  const unsigned char* const ssrc = a.c.scales[kv] + b * a.c.sbs + kvh * a.c.shs + sp.lo * a.c.sts + (piece & 1);
-  const int64_t unit_bytes = UNIT * a.c.ts, unit_scales = UNIT * a.c.sts;
-  const unsigned off = (piece >> 1) * static_cast<unsigned>(a.c.ts), soff = (piece >> 1) * static_cast<unsigned>(a.c.sts);
-  const int at_end = min(piece >> 1, (len - 1) & (UNIT - 1));  // in the last unit rows behind the last key are held to it
-  const unsigned off_end = at_end * static_cast<unsigned>(a.c.ts), soff_end = at_end * static_cast<unsigned>(a.c.sts);
-  unsigned to[4];                                              // where the piece's four chunks of 16 bytes go
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int key = piece >> 1, c = 4 * (piece & 1) + t;
-    to[t] = kv == 0 ? key * 128 + ((c ^ (key >> 1 & 7)) << 4) : KTILE + mx_v_chunk4(key, c);
-  }
-  u32x4 raw;
-  unsigned raw_s;
-  auto load_unit = [&](int u) __attribute__((always_inline)) {
-    const int v = min(KG * u + kg, all - 1);                   // (one that is not there: the last one again)
-    const bool end = v == all - 1;
-    raw = *reinterpret_cast<const u32x4*>(src + v * unit_bytes + mx_choose(end, off_end, off));
-    raw_s = (ssrc + v * unit_scales)[mx_choose(end, soff_end, soff)];
-  };
   // What lies behind the last key of values is zeros in the tile (nothing there is seen; keys' scores are masked). A NaN that only some rows see
   // may not reach the others as 0 x NaN: zeros in its place, and NaN in the rows that see it.
   float power;
@@ -1003,8 +1035,16 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
     if constexpr (AHEAD == 2) write_unit(u + 2, after(next));
   };
 
+  unsigned char* const q_lds = smem + wave * 8192;
+  static_assert(RUNS * KG * 8192 <= KG * 3 * STAGE, "Q fits the stages");
+#pragma unroll
+  for (int j = 0; j < 8; ++j) *reinterpret_cast<u32x4*>(q_lds + 1024 * j + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4)) = q_raw[j];
+#pragma unroll
+  for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) qf[rt][m] = *reinterpret_cast<const bf16x8*>(q_lds + (32 * rt + l31) * 128 + (((4 * h + m) ^ (l31 & 7)) << 4));
+  __syncthreads();
   if (units > 0) {
-    load_unit(0);
     write_unit(0, 0);
     if constexpr (AHEAD == 2) write_unit(1, 1);
     meet();
@@ -1067,11 +1107,11 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
     }
   }
   // ---- the sink joins the denominator; a lane has 8-byte runs of one row's values
+  unsigned char* const o_lds = KG == 2 ? smem + run * (2 * kShare * 4) : smem + wave * 8192;      // (of two groups, the shares just read)
+  if constexpr (KG == 1) __syncthreads();                      // (all are past their last read of the stages)
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) {
-    if (row0 + 32 * rt + l31 >= rows) continue;
-    const float f = mx_norm(a, head[rt], ref[rt], l[rt]);
-    bf16* const out = a.out + b * a.out_bs + query[rt] * a.out_ts + head[rt] * 64 + 4 * h;
+    const float f = mx_norm(a, sink[rt], ref[rt], l[rt]);
 #pragma unroll
     for (int r = 0; r < 32; r += 4) {
       bf16x4 w;
@@ -1080,8 +1120,15 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
         const float v = o[rt][r >> 4][(r & 15) + e];
         w[e] = static_cast<bf16>(v * f);
       }
-      *reinterpret_cast<bf16x4*>(out + 32 * (r >> 4) + 8 * (r >> 2 & 3)) = w;
+      *reinterpret_cast<bf16x4*>(o_lds + (32 * rt + l31) * 128 + ((r >> 2 ^ (l31 & 7)) << 4) + 8 * h) = w;
     }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(o_lds + 1024 * j + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4));
+    int qq, hh;
+    place(j, &qq, &hh);
+    if (row0 + 8 * j + (lane >> 3) < rows) *reinterpret_cast<u32x4*>(a.out + b * a.out_bs + qq * a.out_ts + hh * 64 + 8 * (lane & 7)) = w;
   }
 }
 
@@ -1089,11 +1136,9 @@ __global__ __launch_bounds__(256, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
 __global__ __launch_bounds__(64) void mxfp4_attn_reduce_kernel(MxAttnArgs a, int rows_per_group) {
   const int lane = threadIdx.x;
   const int n_heads = a.n_kv_heads * a.group;
-  unsigned id = blockIdx.x;
-  const int head = id % n_heads;
-  id /= n_heads;
-  const int i = id % a.n_q, b = id / a.n_q;
-  const int kvh = head / a.group, row = i * a.group + head - kvh * a.group, row0 = row / rows_per_group * rows_per_group;
+  const int i0 = a.by_group(blockIdx.x), i1 = a.by_heads(i0), kvh = i0 - i1 * a.n_kv_heads;      // (the block is ((batch row, query), head))
+  const int head = blockIdx.x - i1 * n_heads, b = a.by_n_q(i1), i = i1 - b * a.n_q;
+  const int row = i * a.group + head - kvh * a.group, row0 = row & -rows_per_group;      // (a power of two)
   const int64_t stride = static_cast<int64_t>(a.batch) * a.n_q * n_heads * PART;
   const float* const p0 = a.part + ((static_cast<int64_t>(b) * a.n_q + i) * n_heads + head) * PART;
   // requested before the start position is known; what splits that take no part have there is not used
@@ -1101,7 +1146,8 @@ __global__ __launch_bounds__(64) void mxfp4_attn_reduce_kernel(MxAttnArgs a, int
   float v[8];
 #pragma unroll
   for (int u = 0; u < 8; ++u) v[u] = p0[(u < a.splits ? u : a.splits - 1) * stride + lane];
-  const int live = mx_span(a, b, row0, row0 + rows_per_group - 1).live;
+  const bf16 sink = mx_sink(a, head);
+  const int live = mx_span(a, mx_start(a, b), row0, row0 + rows_per_group - 1).live;
   if (live == 1) return;                                       // (whoever walked the keys alone has stored the answer)
   const float m_s = lane < live ? m_raw : kNoRef;
   const float m_all = wave_max(m_s);
@@ -1119,7 +1165,7 @@ __global__ __launch_bounds__(64) void mxfp4_attn_reduce_kernel(MxAttnArgs a, int
       o += s0 + u < live ? v[u] * f : 0.f;
     }
   }
-  const float f = mx_norm(a, head, m_all, l_all);
+  const float f = mx_norm(a, sink, m_all, l_all);
   a.out[b * a.out_bs + i * a.out_ts + static_cast<int64_t>(head) * 64 + lane] = static_cast<bf16>(o * f);
 }
 
@@ -1161,7 +1207,7 @@ MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_he
   p.one = n_q == 1 && group <= 8;
   p.many = !p.one && rows > 128 && (wide > 384 || (half > 384 && half <= 512) || (half > 512 && seen(256) <= 768));
   p.tiles = narrow < 768 ? 1 : 2;
-  p.waves = narrow <= 256 ? 8 : 4;
+  p.waves = !p.one && !p.many && narrow <= 256 ? 8 : 4;
   p.rows = p.one ? 8 : p.many ? (half > 512 ? 256 : 128) : 32 * p.tiles;
   p.row_groups = (int)((rows + p.rows - 1) / p.rows);
   const int64_t units = streams * p.row_groups;
@@ -1178,7 +1224,7 @@ extern "C" int tllm_mxfp4_attention_shape(int64_t batch, int64_t n_q, int64_t n_
       group > 64 || window < 0 || kv_len_hint < 0)
     return 0;
   const MxAttnPlan p = mx_attn_plan(batch, n_q, mx_attn_ctx(n_slots, kv_len_hint), n_kv_heads, group, window);
-  return p.rows << 16 | (p.one || p.many ? 4 : p.waves) << 8 | p.splits;
+  return p.rows << 16 | p.waves << 8 | p.splits;
 }
 
 extern "C" int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window, int64_t kv_len_hint) {
@@ -1199,8 +1245,9 @@ static int launch_rows(const MxAttnArgs& a, dim3 grid, hipStream_t st) {
 template <bool DENSE>
 static int launch_attention(const MxAttnPlan& p, const MxAttnArgs& a, dim3 grid, hipStream_t st) {
   if (p.many) {
-    if (p.rows == 256) hipLaunchKernelGGL(mxfp4_attn_many_kernel<4>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(mxfp4_attn_many_kernel<2>, grid, dim3(256), 0, st, a);
+    if (p.waves == 8) hipLaunchKernelGGL((mxfp4_attn_many_kernel<4, 2>), grid, dim3(512), 0, st, a);
+    else if (p.rows == 256) hipLaunchKernelGGL((mxfp4_attn_many_kernel<4, 1>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mxfp4_attn_many_kernel<2, 2>), grid, dim3(256), 0, st, a);
   }
   else if (p.one) hipLaunchKernelGGL((mxfp4_attn_one_kernel<DENSE, 4>), grid, dim3(256), 0, st, a);
   else if (p.waves == 8) return launch_rows<DENSE, 1, 8>(a, grid, st);
@@ -1258,6 +1305,11 @@ extern "C" int tllm_mxfp4_attention_bf16(const void* q, int64_t q_batch_stride, 
   a.fill = p.fill;
   a.one = p.one;
   a.scale_log2 = sm_scale * kLog2e;
+  a.by_group = mx_div((unsigned)group);
+  a.by_heads = mx_div((unsigned)n_kv_heads);
+  a.by_batch = mx_div((unsigned)batch);
+  a.by_row_groups = mx_div((unsigned)p.row_groups);
+  a.by_n_q = mx_div((unsigned)n_q);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)wgs);
   const uintptr_t scales_at = reinterpret_cast<uintptr_t>(cache->k_scales) | reinterpret_cast<uintptr_t>(cache->v_scales) | static_cast<uintptr_t>(cache->scale_batch_stride | cache->scale_head_stride);
