@@ -311,7 +311,7 @@ def test_shapes():
     assert shape(1, 1, 300, 8, 9) == (32, 8, 1) and shape(8, 4, 4096, 8, 8) == (32, 8, 4) and shape(1, 97, 1597, 8, 8) == (32, 8, 1)
     assert shape(1, 256, 2256, 8, 8) == (32, 4, 1) and shape(1, 512, 512, 8, 8) == (64, 4, 1) and shape(1, 512, 8192, 8, 8) == (64, 4, 1)
     assert shape(1, 64, 4096, 8, 8) == (32, 8, 1) and shape(1, 64, 8192, 8, 8) == (32, 8, 2) and shape(2, 72, 11011, 4, 4) == (32, 8, 3)
-    assert shape(1, 2048, 2048, 8, 8) == (256, 4, 1) and shape(3, 333, 333, 8, 8) == (128, 4, 1) and shape(1, 1000, 9000, 8, 8) == (128, 4, 1) and shape(1, 2048, 10**6, 8, 8, window=128) == (256, 4, 1)
+    assert shape(1, 2048, 2048, 8, 8) == (256, 8, 1) and shape(1, 2048, 8192, 8, 8) == (256, 4, 1) and shape(1, 2048, 8192, 8, 8, hint=2048) == (256, 8, 1) and shape(3, 333, 333, 8, 8) == (128, 4, 1) and shape(1, 1000, 9000, 8, 8) == (128, 4, 1) and shape(1, 2048, 10**6, 8, 8, window=128) == (256, 4, 1)
 
 
 # (batch, tokens, KV heads, heads of each, slots, run of rows)
@@ -327,6 +327,22 @@ def test_several_tokens_of_each_kernel(batch, t, heads, group, slots, run):
     starts = [int(i) for i in torch.randint(-2, max(slots - t, 1), (batch,), generator=g)]
     attention_case(batch, t, heads, group, slots, starts, sinks=False)
     attention_case(batch, t, heads, group, slots, starts[0] % 20, window=slots // 3, layout="slots", ints=torch.int32)
+
+
+@gpu
+@pytest.mark.parametrize("batch,heads,group,starts,nan", [(1, 16, 5, [0], False), (1, 10, 8, [9], True), (3, 8, 4, [0, -40, 700], True)])
+def test_one_long_prompt(batch, heads, group, starts, nan):
+    t, slots = 1030, 1100
+    assert shape(batch, t, slots, heads, group) == (256, 8, 1)
+    g = torch.Generator().manual_seed(heads)
+    cache = make_cache(g, batch, slots, heads)
+    if nan:                                                    # keys and values of a few places, in either group of wavefronts' shares
+        for b, what, at in itertools.product(range(batch), (1, 3), (500, 575, 950)):
+            cache[what][b, at + 7 * b, 3, what // 2] = 255
+    q = torch.randn(batch, t, heads, group, 64, generator=g).bfloat16()
+    want, tol = attention_ref(q, cpu(cache), None, 0.125, 0, starts)
+    assert not nan or (want.isnan().any() and not want.isnan().all())
+    check(T.mxfp4_attention(q.cuda(), cache, None, 0.125, 0, torch.tensor(starts).cuda()), want, tol, f"prompts at {starts}")
 
 
 @gpu

@@ -1068,7 +1068,6 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
     for (; u < units; ++u, stage = after(stage)) move(u, stage);
   }
 
-  // ---- the second group hands its shares over
   float l[2];
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) {
@@ -1076,41 +1075,9 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
     lane_xor32_pair(sum[rt][0], &x, &y);
     l[rt] = x + y;
   }
-  if constexpr (KG == 2) {
-    float* const shares = reinterpret_cast<float*>(smem) + run * 2 * kShare + lane;
-    __syncthreads();                                           // (all are past their last read of the stages)
-    if (kg == 1) {
-#pragma unroll
-      for (int rt = 0; rt < 2; ++rt) {
-#pragma unroll
-        for (int r = 0; r < 32; ++r) {
-          const float v = o[rt][r >> 4][r & 15];
-          shares[rt * kShare + r * 64] = v;
-        }
-        shares[rt * kShare + 32 * 64] = ref[rt];
-        shares[rt * kShare + 33 * 64] = l[rt];
-      }
-    }
-    __syncthreads();
-    if (kg == 1) return;
-#pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-      const float* const from = shares + rt * kShare;
-      const float m = fmaxf(ref[rt], from[32 * 64]), f0 = __builtin_amdgcn_exp2f(ref[rt] - m), f1 = __builtin_amdgcn_exp2f(from[32 * 64] - m);
-      ref[rt] = m;
-      l[rt] = l[rt] * f0 + from[33 * 64] * f1;
-#pragma unroll
-      for (int r = 0; r < 32; ++r) {
-        const float v = o[rt][r >> 4][r & 15];
-        o[rt][r >> 4][r & 15] = v * f0 + from[r * 64] * f1;
-      }
-    }
-  }
-  // ---- the sink joins the denominator; a lane has 8-byte runs of one row's values
-  unsigned char* const o_lds = KG == 2 ? smem + run * (2 * kShare * 4) : smem + wave * 8192;      // (of two groups, the shares just read)
-  if constexpr (KG == 1) __syncthreads();                      // (all are past their last read of the stages)
-#pragma unroll
-  for (int rt = 0; rt < 2; ++rt) {
+  // A tile's end: the sink joins the denominator; a lane has 8-byte runs of one row's values, which leave through 4 KB of LDS of the wavefront's own.
+  auto lay = [&](auto tag, unsigned char* lds) __attribute__((always_inline)) {
+    constexpr int rt = decltype(tag)::value;
     const float f = mx_norm(a, sink[rt], ref[rt], l[rt]);
 #pragma unroll
     for (int r = 0; r < 32; r += 4) {
@@ -1120,15 +1087,66 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
         const float v = o[rt][r >> 4][(r & 15) + e];
         w[e] = static_cast<bf16>(v * f);
       }
-      *reinterpret_cast<bf16x4*>(o_lds + (32 * rt + l31) * 128 + ((r >> 2 ^ (l31 & 7)) << 4) + 8 * h) = w;
+      *reinterpret_cast<bf16x4*>(lds + l31 * 128 + ((r >> 2 ^ (l31 & 7)) << 4) + 8 * h) = w;
     }
-  }
+  };
+  auto leave = [&](auto tag, const unsigned char* lds) __attribute__((always_inline)) {
+    constexpr int rt = decltype(tag)::value;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(o_lds + 1024 * j + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4));
-    int qq, hh;
-    place(j, &qq, &hh);
-    if (row0 + 8 * j + (lane >> 3) < rows) *reinterpret_cast<u32x4*>(a.out + b * a.out_bs + qq * a.out_ts + hh * 64 + 8 * (lane & 7)) = w;
+    for (int j = 0; j < 4; ++j) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(lds + 1024 * j + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4));
+      int qq, hh;
+      place(4 * rt + j, &qq, &hh);
+      if (row0 + 32 * rt + 8 * j + (lane >> 3) < rows) *reinterpret_cast<u32x4*>(a.out + b * a.out_bs + qq * a.out_ts + hh * 64 + 8 * (lane & 7)) = w;
+    }
+  };
+  typedef std::integral_constant<int, 0> first_tile;
+  typedef std::integral_constant<int, 1> second_tile;
+  __syncthreads();                                             // (all are past their last read of the stages)
+  if constexpr (KG == 2) {
+    // each group hands one tile over and finishes the other
+    auto share = [&](int rt) { return reinterpret_cast<float*>(smem) + (run * 2 + rt) * kShare; };
+    auto give = [&](auto tag) __attribute__((always_inline)) {
+      constexpr int rt = decltype(tag)::value;
+      float* const to = share(rt);
+#pragma unroll
+      for (int r = 0; r < 32; r += 4) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = o[rt][r >> 4][(r & 15) + e];
+        *reinterpret_cast<f32x4*>(to + 64 * r + 4 * lane) = v;
+      }
+      to[32 * 64 + lane] = ref[rt];
+      to[33 * 64 + lane] = l[rt];
+    };
+    auto take = [&](auto tag) __attribute__((always_inline)) {
+      constexpr int rt = decltype(tag)::value;
+      const float* const from = share(rt);
+      const float other = from[32 * 64 + lane], m = fmaxf(ref[rt], other);
+      const float f0 = __builtin_amdgcn_exp2f(ref[rt] - m), f1 = __builtin_amdgcn_exp2f(other - m);
+      ref[rt] = m;
+      l[rt] = l[rt] * f0 + from[33 * 64 + lane] * f1;
+#pragma unroll
+      for (int r = 0; r < 32; r += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(from + 64 * r + 4 * lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[rt][r >> 4][(r & 15) + e] = o[rt][r >> 4][(r & 15) + e] * f0 + v[e] * f1;
+      }
+      unsigned char* const lds = reinterpret_cast<unsigned char*>(share(rt));      // (read by this wavefront alone)
+      lay(tag, lds);
+      leave(tag, lds);
+    };
+    if (kg == 0) give(second_tile{});
+    else give(first_tile{});
+    __syncthreads();
+    if (kg == 0) take(first_tile{});
+    else take(second_tile{});
+  } else {
+    unsigned char* const lds = smem + wave * 8192;
+    lay(first_tile{}, lds);
+    lay(second_tile{}, lds + 4096);
+    leave(first_tile{}, lds);
+    leave(second_tile{}, lds + 4096);
   }
 }
 
@@ -1186,6 +1204,10 @@ struct MxAttnPlan {
 //   213 -- and from 513 runs of 128 on where walks are short, up to 768 keys: 2 x 700 24.3, 26.2, 27.6, 27.2; 2048 with a window of 128 19, 25, 32, 31.
 //   Between, two workgroups to a CU do not come out even: 1200 33.7, 25.7, 28.8, 29; 1200 behind 6800 223, 213, 178, 202; 1500 behind 2500 104, 104, 102,
 //   116.
+//   Of those, 321 to 512 runs of 256 of prompts (walks up to twice as long as there are queries, and longer than 1024): two groups of wavefronts that
+//   take the keys in turn, one workgroup to a CU after the other. Otherwise the longest walks' workgroups, which alone have a CU's matrix cores
+//   at 0.7 of their rate, are what the launch takes: 2048 48.4, without 51.5; 1800 42.7, 45.6; 1500 32.8, 39.0, in 64 rows 35.3; 1300 28.7, 34.6, 30.6;
+//   but 1200 26.8, 32.3, 27.5; 2 x 978 32.5, 30.5; 4 x 500 24.9, 20.6; 2048 behind 2048 113.5, 111.9.
 //   128 to a workgroup from 385 to 512 runs of them, one or two workgroups to a CU: 2 x 512 15.8, in 256 rows 18.8, 64 18.8, 32 18.9; 4 x 256 13.0,
 //   13.6, 17.0, 17.2; 3 x 333 13.9, 16.0, 17.5, 17.8; 8 x 128 behind 2000 47.6, 51.4, 49.8, 56; 1000 behind 8000 162, 188, 165, 188; 800 behind 4000
 //   85.4, 103, 86.8, 89; but 700 behind 4000 (352) 84, 101, 70, 77, and 512 behind 4000 64, 96, 48, 56.
@@ -1205,9 +1227,10 @@ MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_he
   };
   const int64_t wide = (rows + 255) / 256 * streams, half = (rows + 127) / 128 * streams, narrow = (rows + 31) / 32 * streams;
   p.one = n_q == 1 && group <= 8;
-  p.many = !p.one && rows > 128 && (wide > 384 || (half > 384 && half <= 512) || (half > 512 && seen(256) <= 768));
+  const bool unlike = wide > 320 && wide <= 512 && window == 0 && n_slots > 1024 && n_slots <= 2 * n_q;
+  p.many = !p.one && rows > 128 && (unlike || wide > 384 || (half > 384 && half <= 512) || (half > 512 && seen(256) <= 768));
   p.tiles = narrow < 768 ? 1 : 2;
-  p.waves = !p.one && !p.many && narrow <= 256 ? 8 : 4;
+  p.waves = !p.one && (p.many ? unlike : narrow <= 256) ? 8 : 4;
   p.rows = p.one ? 8 : p.many ? (half > 512 ? 256 : 128) : 32 * p.tiles;
   p.row_groups = (int)((rows + p.rows - 1) / p.rows);
   const int64_t units = streams * p.row_groups;
