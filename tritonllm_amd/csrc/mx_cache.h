@@ -15,8 +15,11 @@ struct MxCache {
 // Host: what a caller describes, checked.
 int mx_cache_of(const TllmMxCache* c, const char* what, MxCache* out);
 
-// (without a branch, whose join would wait for the value)
 __device__ __forceinline__ int64_t mx_row_int(const void* p, int is_i64, int64_t i) {
+  return is_i64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int*>(p)[i]);
+}
+// The same without a branch, whose join would wait for the value (the write waits for it anyway: 21.0 us with, 21.9 without for 8 x 4096 tokens).
+__device__ __forceinline__ int64_t mx_row_int_ahead(const void* p, int is_i64, int64_t i) {
   const int64_t two = is_i64 != 0;
   const int* const w = static_cast<const int*>(p) + (i << two);
   const int lo = w[0], hi = w[two];

@@ -62,7 +62,7 @@ struct MxSpan {
   int64_t start;
   int lo, hi, live;
 };
-__device__ __forceinline__ int64_t mx_start(const MxAttnArgs& a, int b) { return mx_row_int(a.start_q, a.start_is_i64, static_cast<int64_t>(b) * a.start_stride); }
+__device__ __forceinline__ int64_t mx_start(const MxAttnArgs& a, int b) { return mx_row_int_ahead(a.start_q, a.start_is_i64, static_cast<int64_t>(b) * a.start_stride); }
 __device__ __forceinline__ MxSpan mx_span(const MxAttnArgs& a, int64_t start, int first_row, int last_row) {
   MxSpan s;
   s.start = start;
@@ -132,6 +132,9 @@ __device__ __forceinline__ unsigned mx_scale_pair(const unsigned char* p, int64_
 //   A lane's scores are then four of a tile, all of use.
 //   O = P . V, the weights' registers being the A operand for the block's keys 0 - 31 in the rows 0 - 7 and for 32 - 63 in the rows 8 - 15: two
 //   accumulators, each of which is looked at in one half of its rows. V passes LDS as bf16, for transposing reads.
+// Bound by the cache's bytes where contexts are long -- 8 rows of 32768 keys 28.4 us (143 MB, 5.0 TB/s, the joining launch among them), of 131072 96
+// (5.9 TB/s; loads of this pattern alone 6.8) --, else by a chain of latencies: 300 keys of one row 4.8 us, 8 rows of 4096 9.9, 2.2 of which are
+// the second launch.
 template <bool DENSE, int NW>
 __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a) {
   constexpr int VTILE = 64 * 128;
@@ -409,6 +412,9 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
 //   one exchange between the halves of the wavefront.
 //   O^T = V^T . P^T: the scores' registers are, pairwise, the B operand when the k slots are read as a permutation of the keys; V passes LDS
 //   as bf16 for transposing reads, as above.
+// Bound by the vector ALU (a wavefront converts its keys and values for its own rows alone, an exponential for each weight) beside the matrix cores
+// where there is enough to do -- 512 queries behind 4000 tokens 48 us, 34 GFLOP: 0.7 PFLOP/s --, else by latencies as above: four drafts to each of 8
+// rows of 4096 12.2 us, 97 behind 1500 9.6.
 template <bool DENSE, int RT, int KG>
 __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs a) {
   constexpr int NW = KG, RB = 32 * RT;                         // wavefronts; rows
@@ -719,6 +725,8 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
 //   The matrix cores and the vector ALU work at the same time: with one tile's weights (32 keys x 32 rows) the next one's scores are issued in
 //   turn, and the products of the one before. Of block j (32 keys), S^T of tile 1, weights of tile 0 and P . V of block j - 1 in tile 1; then S^T of
 //   block j + 1 in tile 0, weights of tile 1 and P . V of tile 0. Operands of K and of V live from one such half to the next.
+// Bound by what the two units take together at the clock that the power limit leaves (1.8 - 1.9 GHz): a prompt of 8192 514 - 546 us (550 GFLOP: 1.0 -
+// 1.07 PFLOP/s; 431 with the LDS traffic left out); of 2048 48.4 (0.7), of which a workgroup's beginning and end are 4 each.
 template <int RUNS, int KG>
 __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
   static_assert(RUNS == 4 || RUNS == 2, "runs of a workgroup");
@@ -1150,7 +1158,8 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
   }
 }
 
-// A wavefront per (batch row, query, head): the splits' records and the sink. Lane s has the (max, sum) of split s.
+// A wavefront per (batch row, query, head): the splits' records and the sink. Lane s has the (max, sum) of split s. Two reads' latency and a launch:
+// 2.2 us as traced, for 512 heads of four splits.
 __global__ __launch_bounds__(64) void mxfp4_attn_reduce_kernel(MxAttnArgs a, int rows_per_group) {
   const int lane = threadIdx.x;
   const int n_heads = a.n_kv_heads * a.group;
