@@ -133,7 +133,7 @@ __device__ __forceinline__ unsigned mx_scale_pair(const unsigned char* p, int64_
 //   O = P . V, the weights' registers being the A operand for the block's keys 0 - 31 in the rows 0 - 7 and for 32 - 63 in the rows 8 - 15: two
 //   accumulators, each of which is looked at in one half of its rows. V passes LDS as bf16, for transposing reads.
 // Bound by the cache's bytes where contexts are long -- 8 rows of 32768 keys 28.4 us (143 MB, 5.0 TB/s, the joining launch among them), of 131072 96
-// (5.9 TB/s; loads of this pattern alone 6.8) --, else by a chain of latencies: 300 keys of one row 4.8 us, 8 rows of 4096 9.9, 2.2 of which are
+// (5.9 TB/s; loads of this pattern alone 6.8) --, else by a chain of latencies: 300 keys of one row 4.7 us, 8 rows of 4096 9.7, 2.2 of which are
 // the second launch.
 template <bool DENSE, int NW>
 __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a) {
@@ -286,6 +286,23 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
 #pragma unroll
       for (int w = 0; w < 4; ++w) st[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_bf16x8(kc[t][w], mx_power(ks[t])), qf[w], st[t], 0, 0, 0);
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    // half of V on its way while the weights are made (8 rows of 4096 9.9 -> 9.7 us, 49 of up to 2048 11.9 -> 11.6; all of it takes the registers of a
+    // third wavefront)
+    bf16x8 vf[2][4];
+    auto read_v = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb) {
+        i16x4 part[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(vtile + v_from[nb] + 4096 * h + 2048 * u));
+        vf[h][nb] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    };
+    read_v(0);
     load_block(blk + 2 * step, r);
 
     // ---- weights: this lane has keys 16 t + 4 g + i of its half of the block
@@ -335,20 +352,11 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
     bf16x8 pa;                                                 // A operand of P . V: k slot j <-> key 4 g + j (j < 4), 16 + 4 g + j - 4 of the half
 #pragma unroll
     for (int j = 0; j < 8; ++j) pa[j] = static_cast<bf16>(p[j]);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    read_v(1);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int nb = 0; nb < 4; ++nb) {
-        i16x4 part[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(vtile + v_from[nb] + 4096 * h + 2048 * u));
-        acc[h][nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa, __builtin_bit_cast(bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7)),
-                                                             acc[h][nb], 0, 0, 0);
-      }
+      for (int nb = 0; nb < 4; ++nb) acc[h][nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa, vf[h][nb], acc[h][nb], 0, 0, 0);
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
   };

@@ -1115,13 +1115,13 @@ def mxfp4_cache_write(cache: Mxfp4Cache, k: torch.Tensor, v: torch.Tensor, offse
 def mxfp4_cache_read(cache: Mxfp4Cache, first: int = 0, tokens: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Slots ``first`` to ``first + tokens`` (``None``: to the end) as ``(k, v)``, bf16 ``[batch, tokens, n_kv_heads, head_dim]``, exactly; a scale
     byte of 255 gives NaN."""
-    n_ctx = cache[0].shape[1]
     if tokens is None:
-        tokens = n_ctx - first
+        tokens = cache[0].shape[1] - first
     done = host().mxfp4_cache_read(*cache, first, tokens)
     if done is not None:
         return done
     desc = _mx_cache_desc(cache)
+    n_ctx = desc.n_slots
     _require(0 <= first <= n_ctx and 0 <= tokens <= n_ctx - first, f"mxfp4_cache_read: slots {first} to {first + tokens} of {n_ctx}")
     k, v = (torch.empty((desc.batch, tokens, desc.n_kv_heads, desc.head_dim), dtype=_BF16, device=cache[0].device) for _ in range(2))
     if k.numel():
