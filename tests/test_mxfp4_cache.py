@@ -530,6 +530,13 @@ def test_slots_beyond_32_bits():
         q = torch.randn(1, t, 1, 8, 64, generator=g).bfloat16()
         want, tol = attention_ref(q, [kb, ks, vb, vs], None, 0.125, 0, [n - t])
         check(T.mxfp4_attention(q.cuda(), cache, None, 0.125, 0, torch.tensor([n - t]).cuda()), want, tol)
+    q = torch.randn(1, 64, 1, 8, 64, generator=g).bfloat16()
+    want, tol = attention_ref(q, [kb, ks, vb, vs], None, 0.125, 0, [n - 64])
+    for batch, run in ((100, 128), (140, 256)):                     # the same for many rows, all over the one cache
+        assert shape(batch, 64, n, 1, 8)[0] == run
+        got = T.mxfp4_attention(q.cuda().expand(batch, 64, 1, 8, 64), T.Mxfp4Cache(*(x.expand(batch, *x.shape[1:]) for x in cache)), None, 0.125, 0, torch.tensor([n - 64]).cuda())
+        check(got[:1], want, tol)
+        assert torch.equal(got, got[:1].expand_as(got))
     del buffer
     torch.cuda.empty_cache()
 
