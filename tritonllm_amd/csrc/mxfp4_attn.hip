@@ -1227,11 +1227,13 @@ struct MxAttnPlan {
 //   but 1200 26.8, 32.3, 27.5; 2 x 978 32.5, 30.5; 4 x 500 24.9, 20.6; 2048 behind 2048 113.5, 111.9.
 //   128 to a workgroup from 385 to 512 runs of them, one or two workgroups to a CU: 2 x 512 15.8, in 256 rows 18.8, 64 18.8, 32 18.9; 4 x 256 13.0,
 //   13.6, 17.0, 17.2; 3 x 333 13.9, 16.0, 17.5, 17.8; 8 x 128 behind 2000 47.6, 51.4, 49.8, 56; 1000 behind 8000 162, 188, 165, 188; 800 behind 4000
-//   85.4, 103, 86.8, 89; but 700 behind 4000 (352) 84, 101, 70, 77, and 512 behind 4000 64, 96, 48, 56.
+//   85.4, 103, 86.8, 89; but 700 behind 4000 (352) 84, 101, 70, 77, and 512 behind 4000 64, 96, 48, 56. To 640 for prompts: 1200 24.5, 31.7, 27.6, 27.5;
+//   1100 23.1, 30.2, 25.5, 24.4 (behind 1000 52, 53, 47.6, 50).
 //   32 rows shared out between eight wavefronts up to 256 runs of 32: 97 behind 1500 10.0, between four 11.7; 97 behind 8000 31, 39; 64 behind 8000
 //   24.2, 26.9; with four from there on: 150 behind 1350 17.3, 13.8; 256 behind 2000 22, 18.2; 64 x 4 of 1000 16.1, 12.5.
-//   64 rows to a workgroup from 768 such runs on: 512 behind 4000 48, with 32 rows 56; 700 behind 4000 70, 77; 512 10.7, 11.9; a little behind on
-//   700 17.8, 15.7; but 350 behind 4000 44.6, 40; 333 9.2, 7.8; 64 x 4 of 1000 16.4, 12.5.
+//   64 rows to a workgroup from 768 such runs on: 512 behind 4000 48, with 32 rows 56; 700 behind 4000 70, 77; 512 9.9, 11.4; but 350 behind 4000 44.6,
+//   40; 333 9.2, 7.8; 64 x 4 of 1000 16.4, 12.5; not where that is a little more than two workgroups to a CU: 600 15.2, 12.9; 600 behind 4000 68, 65.5;
+//   prompts of 700 16.8, 14.3, of 800 18.1, 17.2.
 // Workgroups that share rows' keys, as many as there are CUs for, up to kDeep keys only if that is four: 8 x 4 of 4096 (64 runs) 12.5, none 16.8;
 // 64 behind 8000 (128) two 22.2, none 28.9; 72 x 2 of 11000 in four heads of four (72) three 22.3, none 36; but 8 x 8 of 2000 (128) two 13.9, none
 // 11.2; 97 behind 8000 (200) two 38, none 28.7; 512 behind 4000 in 64 rows (512) two 67, none 48.
@@ -1244,11 +1246,12 @@ MxAttnPlan mx_attn_plan(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_he
   };
   const int64_t wide = (rows + 255) / 256 * streams, half = (rows + 127) / 128 * streams, narrow = (rows + 31) / 32 * streams;
   p.one = n_q == 1 && group <= 8;
-  const bool unlike = wide > 320 && wide <= 512 && window == 0 && n_slots > 1024 && n_slots <= 2 * n_q;
-  p.many = !p.one && rows > 128 && (unlike || wide > 384 || (half > 384 && half <= 512) || (half > 512 && seen(256) <= 768));
-  p.tiles = narrow < 768 ? 1 : 2;
+  const bool prompt = window == 0 && n_slots <= 2 * n_q, unlike = prompt && n_slots > 1024 && wide > 320 && wide <= 512;
+  const bool halves = !unlike && half > 384 && half <= (prompt && n_slots > 768 ? 640 : 512);
+  p.many = !p.one && rows > 128 && (unlike || halves || wide > 384 || (half > 512 && seen(256) <= 768));
+  p.tiles = narrow < 768 || (narrow > 1024 && narrow <= (prompt ? 1600 : 1300)) ? 1 : 2;
   p.waves = !p.one && (p.many ? unlike : narrow <= 256) ? 8 : 4;
-  p.rows = p.one ? 8 : p.many ? (half > 512 ? 256 : 128) : 32 * p.tiles;
+  p.rows = p.one ? 8 : p.many ? (halves ? 128 : 256) : 32 * p.tiles;
   p.row_groups = (int)((rows + p.rows - 1) / p.rows);
   const int64_t units = streams * p.row_groups;
   p.fill = p.one ? (int)((kFill + units - 1) / units) : kFill / units > 0 ? (int)(kFill / units) : 1;
