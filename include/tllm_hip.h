@@ -429,9 +429,9 @@ int tllm_mxfp4_cache_read_bf16(const TllmMxCache* cache, int64_t first, int64_t 
  * without start_q_per_row) and sees the slots n <= position, n < n_slots and, when window > 0, n > position - window; otherwise
  * as tllm_attention_prefill_bf16. q [batch, n_q, n_kv_heads * group, 64] bf16 with batch / token strides in elements, out
  * [batch, n_q, n_kv_heads * group * 64] likewise; sinks bf16 [n_kv_heads * group] or NULL (logit 0). A row that sees nothing gives zeros.
- * What a slot holds that a query does not see, NaN included, is nothing to it; seen, a scale byte of 255 is NaN, and values that
- * tllm_mxfp4_cache_read_bf16 reads as infinite (which the quantisation never writes) give NaN or an infinite result. start_q: device, int32
- * or int64. group up to 64, sm_scale positive. kv_len_hint (0: none) plans the launch for that many visible keys instead of n_slots; any hint
+ * What a slot holds that a query does not see, NaN and infinities included, is nothing to it; seen, a scale byte of 255 is NaN, and what
+ * tllm_mxfp4_cache_read_bf16 reads as infinite (which the quantisation never writes) is infinite: a value gives an infinite result or NaN, a key
+ * NaN, or no weight where its logit is -infinity. start_q: device, int32 or int64. group up to 64, sm_scale positive. kv_len_hint (0: none) plans the launch for that many visible keys instead of n_slots; any hint
  * is right, results differ by the order of sums alone.
  * workspace: device memory of tllm_mxfp4_attention_workspace_bytes() for the same arguments, 4-byte aligned (may be 0 bytes). */
 int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window,

@@ -428,6 +428,64 @@ def test_nan_in_a_batch_of_each_kernel(batch, t, group, run):
 
 
 @gpu
+@pytest.mark.parametrize("batch,t,heads,group,slots,run", [(1, 4, 2, 8, 100, (32, 8)), (2, 33, 2, 4, 120, (32, 8)), (30, 7, 8, 8, 70, (32, 4)), (50, 16, 8, 8, 60, (64, 4)), (100, 40, 1, 16, 77, (128, 4)),
+                                                           (24, 40, 8, 8, 120, (256, 4)), (1, 1030, 10, 8, 1100, (256, 8))])
+def test_infinite_values_reach_who_sees_them(batch, t, heads, group, slots, run):
+    """One slot of each row whose 32 values of one half of one head read as infinite in every other place (2^128 and more of scale bytes 253 and
+    254), and as large finite ones or as zeros between. Queries ahead of the slot, or past it with a window, have the answer without it; those
+    that see it have nothing finite in the infinite places, with the sign of the infinity unless it is NaN, and the definition's answer in all others."""
+    assert shape(batch, t, slots, heads, group)[:2] == run
+    g = torch.Generator().manual_seed(batch + t)
+    plain = make_cache(g, batch, slots, heads)
+    q = torch.randn(batch, t, heads, group, 64, generator=g).bfloat16()
+    start = 9
+    cases = [(0, start + t // 2, 253, 3), (0, start + t - 1, 254, 1), (12, start + t // 2, 253, 0), (12, start - 5, 254, 0), (0, start - 5, 253, 1)]
+    for window, slot, byte, finite in cases if t < 1000 else cases[::2]:
+        half, head = slot % 2, t % heads
+        codes = torch.tensor([7, finite, 14, finite + 8] * 8, dtype=torch.uint8)      # 6 and -4: infinite; between them the code `finite`, of either sign
+        infinite = torch.tensor([True, False] * 16)
+        cache, without, between = ([x.clone() for x in plain] for _ in range(3))
+        for c, kept, power in ((cache, codes, byte), (without, 0 * codes, 0), (between, torch.where(infinite, 0, codes), byte)):
+            c[0][:, slot, head] = 0                                 # a key of zeros: its weight is about 1 at most, and the finite values' sums stay finite
+            c[2][:, slot, head, half] = (kept[0::2] | kept[1::2] << 4).cuda()
+            c[3][:, slot, head, half] = power
+        got = T.mxfp4_attention(q.cuda(), T.Mxfp4Cache(*cache), None, 0.125, window, torch.tensor([start]).cuda())
+        want, tol = (x.view(batch, t, heads, group, 64) for x in attention_ref(q, cpu(without), None, 0.125, window, [start] * batch))
+        with_between = [x.view(batch, t, heads, group, 64) for x in attention_ref(q, cpu(between), None, 0.125, window, [start] * batch)]
+        at = start + torch.arange(t)
+        sees = (slot <= at) & (slot > at - window if window else slot >= 0)
+        assert sees.any() and (window or slot < start or not sees.all())
+        got = got.cpu().double().view(batch, t, heads, group, 64).clone()
+        piece = got[:, sees, head, :, 32 * half : 32 * half + 32]
+        assert not piece[..., infinite].isfinite().any()
+        sign = torch.tensor([1.0, -1.0] * 8, dtype=torch.float64)   # (of the infinite places)
+        assert (piece[..., infinite].isnan() | (piece[..., infinite] == sign * math.inf)).all()
+        for x, y in zip((want, tol), with_between):                 # the finite values of the piece: the bound of their own sums, for their own columns alone
+            x[:, sees, head, :, 32 * half : 32 * half + 32] = y[:, sees, head, :, 32 * half : 32 * half + 32]
+        columns = torch.arange(32 * half, 32 * half + 32)[infinite]
+        for x in (got, want, tol):
+            x[:, sees.nonzero()[:, None], head, :, columns[None, :]] = 0
+        check(got.reshape(batch, t, -1), want.reshape(batch, t, -1), tol.reshape(batch, t, -1), f"byte {byte} at {slot}, window {window}, {finite} between")
+
+
+@gpu
+@pytest.mark.parametrize("batch,t,heads,group,slots", [(1, 4, 2, 8, 100), (50, 16, 8, 8, 60), (100, 40, 1, 16, 77), (24, 40, 8, 8, 120)])
+def test_infinite_keys_are_nothing_to_who_does_not_see_them(batch, t, heads, group, slots):
+    g = torch.Generator().manual_seed(batch + t)
+    plain = make_cache(g, batch, slots, heads)
+    q = torch.randn(batch, t, heads, group, 64, generator=g).bfloat16()
+    for window, slot, byte in ((0, 9 + t // 2, 254), (12, 9 + t // 2, 253), (12, 7, 254)):
+        cache = [x.clone() for x in plain]
+        cache[1][:, slot] = byte
+        got = T.mxfp4_attention(q.cuda(), T.Mxfp4Cache(*cache), None, 0.125, window, torch.tensor([9]).cuda())
+        want, tol = attention_ref(q, cpu(plain), None, 0.125, window, [9] * batch)
+        at = 9 + torch.arange(t)
+        other = (slot > at) | (slot <= at - window if window else slot < 0)
+        if other.any():
+            check(got[:, other], want[:, other], tol[:, other], f"byte {byte} at {slot}, window {window}")
+
+
+@gpu
 def test_nan_and_infinite_queries_stay_with_their_row():
     g = torch.Generator().manual_seed(4)
     for t, group in ((1, 8), (5, 4), (200, 4)):

@@ -5,7 +5,8 @@
 //   out[i, h]  = sum_n exp(s - m) v[n, kv(h)] / (sum_n exp(s - m) + exp(sink[h] - m)),    m = max(sink[h], max_n s)
 //
 // with k and v the values that the cache's codes and scale bytes stand for, exactly (an e2m1 value times a power of two is a bf16 value).
-// A scale byte of 255 makes its 32 values NaN, for the queries that see the slot and for no other.
+// A scale byte of 255 makes its 32 values NaN, and values of 2^128 and more (scale bytes 253 and 254) are infinite in bf16: for the queries that see
+// the slot, and for no other.
 #include "mx_cache.h"
 
 namespace tllm {
@@ -98,6 +99,43 @@ __device__ __forceinline__ float mx_norm(const MxAttnArgs& a, bf16 sink_of, floa
 }
 
 __device__ __forceinline__ float mx_power(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// Values that are no number in bf16 -- NaN of scale byte 255, infinities of 254 (2 x 2^127 and more) and 253 (4 and 6 x 2^126) -- may not stand in a tile of
+// V that several rows share: to a row that does not see the key they would be 0 x NaN or 0 x infinity. kFinite bytes have none.
+constexpr unsigned kFinite = 252;
+// Which of a dword's eight codes they are, in the low bit of each nibble; `byte` is beyond kFinite.
+__device__ __forceinline__ unsigned mx_not_finite(unsigned codes, unsigned byte) {
+  const unsigned two = codes >> 2, four = codes >> 2 & codes >> 1;      // (codes of a magnitude of 2 and more, of 4 and more)
+  return 0x11111111u & (byte == 255u ? ~0u : byte == 254u ? two : four);
+}
+// Sixteen bytes of codes without them, and the scale byte for what stays.
+__device__ __forceinline__ void mx_set_aside(u32x4* codes, unsigned* byte) {
+  if (*byte <= kFinite) return;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) (*codes)[w] &= ~(15u * mx_not_finite((*codes)[w], *byte));
+  *byte = *byte == 255u ? 0u : *byte;
+}
+// What was set aside of the 32 values at `from`, for a row that sees them: its lane's sixteen, 8 (r / 4) + 4 h + r % 4. A weight above zero times an
+// infinity is the infinity. The codes come once more from memory, so that no register waits for this, and by scalar loads: behind vector loads here
+// the kernels would wait for the block that is on its way.
+__device__ __forceinline__ void mx_add_aside(f32x16* o, const unsigned char* from, unsigned byte, int h) {
+  const auto codes = (const __attribute__((address_space(4))) unsigned*)from;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const unsigned x = codes[w] >> 16 * h, aside = mx_not_finite(x, byte);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const unsigned bits = byte == 255u ? 0x7fc00000u : 0x7f800000u | (x >> 4 * r & 8u) << 28;
+      (*o)[4 * w + r] += aside >> 4 * r & 1u ? __builtin_bit_cast(float, bits) : 0.f;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+// Pieces (bits) with values that are set aside, and which of them have scale bytes of 255 and of 254.
+struct MxAside {
+  unsigned long long any, nan, large;
+  __device__ __forceinline__ unsigned byte(int at) const { return nan >> at & 1 ? 255u : large >> at & 1 ? 254u : 253u; }
+};
 
 // Where 16 bytes (eight values) of a V tile's row are in LDS: rows of 128 bytes, their chunks XORed so that the transposing reads (eight
 // rows x two chunks at a time) and the writes (eight rows x one chunk of either half) have every bank once.
@@ -551,17 +589,18 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     const u32x4 kc = *reinterpret_cast<const u32x4*>(vtile + k_from);
     u32x4 vc = r.v;
     // ---- V into the wavefront's tile, as bf16
-    // What lies behind the last key may be anything: zeros. A NaN that only some of the rows see may not reach the others as 0 x NaN: it is
-    // put aside as zeros and added behind (rare). (A key's NaN goes no further than its own scores.)
+    // What lies behind the last key may be anything: zeros. What only some of the rows may see is set aside as zeros and added behind (rare). (A
+    // key's NaN or infinity goes no further than its own scores.)
     if (__builtin_expect(end, 0)) {
       const bool in = k0 + (lane >> 1) < len;
       vc = in ? vc : u32x4{0u, 0u, 0u, 0u};
       vs = in ? vs : 0u;
     }
-    const unsigned long long bad = __builtin_amdgcn_ballot_w64(vs == 255u);
-    if (__builtin_expect(bad != 0, 0)) {
-      vc = vs == 255u ? u32x4{0u, 0u, 0u, 0u} : vc;
-      vs = vs == 255u ? 0u : vs;
+    MxAside aside{__builtin_amdgcn_ballot_w64(vs > kFinite), 0, 0};
+    if (__builtin_expect(aside.any != 0, 0)) {
+      aside.nan = __builtin_amdgcn_ballot_w64(vs == 255u);
+      aside.large = __builtin_amdgcn_ballot_w64(vs == 254u);
+      mx_set_aside(&vc, &vs);
     }
 #pragma unroll
     for (int w = 0; w < 4; ++w) *reinterpret_cast<bf16x8*>(v_to + v_chunk[w]) = mx_bf16x8(vc[w], mx_power(vs));
@@ -638,17 +677,18 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
       }
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    for (unsigned long long left = bad; left != 0; left &= left - 1) {
-      const int at = __builtin_ctzll(left), key = k0 + (at >> 1);           // (one of the span's)
+    if (__builtin_expect(aside.any != 0, 0)) {
+      for (unsigned long long left = aside.any; left != 0; left &= left - 1) {
+        const int at = __builtin_ctzll(left), key = k0 + (at >> 1);         // (one of the span's)
+        const unsigned char* const from = vp + key * a.c.ts + 16 * (at & 1);
+        const unsigned byte = aside.byte(at);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        if (key >= lower[rt] && key <= upper[rt]) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            o[rt][0][r] = at & 1 ? o[rt][0][r] : __builtin_nanf("");
-            o[rt][1][r] = at & 1 ? __builtin_nanf("") : o[rt][1][r];
+        for (int rt = 0; rt < RT; ++rt)
+          if (key >= lower[rt] && key <= upper[rt]) {
+            if (at & 1) mx_add_aside(&o[rt][1], from, byte, h);
+            else mx_add_aside(&o[rt][0], from, byte, h);
           }
-        }
+      }
     }
   };
   if (first < nblk) {
@@ -741,8 +781,8 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
   constexpr int UNIT = 16 * RUNS, HALVES = UNIT / 32, RB = 64 * RUNS;
   constexpr int KTILE = UNIT * 128, STAGE = 2 * KTILE;         // bytes: K [UNIT keys][64 values], then V
   __shared__ __align__(16) unsigned char smem[KG * 3 * STAGE];
-  __shared__ __align__(8) unsigned s_any[KG][3][2];            // whether a stage's values hold NaN, by 32 keys,
-  __shared__ unsigned long long s_bad[KG][3][2];               // and in which of the 32 x 2 pieces
+  __shared__ __align__(8) unsigned s_any[KG][3][2];            // whether a stage's values hold NaN or infinities, by 32 keys,
+  __shared__ MxAside s_aside[KG][3][2];                        // and (where they do) in which of the 32 x 2 pieces
   static_assert(KG == 1 || RUNS * 2 * kShare * 4 <= KG * 3 * STAGE, "the shares fit the stages");
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -840,21 +880,20 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
     w_lo = w_lo < w_hi ? w_lo : w_hi;
   }
 
-  // What lies behind the last key of values is zeros in the tile (nothing there is seen; keys' scores are masked). A NaN that only some rows see
-  // may not reach the others as 0 x NaN: zeros in its place, and NaN in the rows that see it.
+  // What lies behind the last key of values is zeros in the tile (nothing there is seen; keys' scores are masked). What only some rows may see is
+  // set aside as zeros, and added to the rows that see it.
   float power;
   auto prepare = [&](int u, int stage) __attribute__((always_inline)) {   // the unit about to be written
     if (kv != 0) {
       const bool in = key_of(u) + (piece >> 1) < len;
-      const unsigned long long bad = __builtin_amdgcn_ballot_w64(raw_s == 255u && in);
+      const unsigned long long bad = __builtin_amdgcn_ballot_w64(raw_s > kFinite && in);
+      if (lane == 0) s_any[kg][stage][run % HALVES] = bad != 0;
       if (__builtin_expect(key_of(u) + UNIT > len || bad != 0, 0)) {
-        const bool keep = in && raw_s != 255u;
-        raw = keep ? raw : u32x4{0u, 0u, 0u, 0u};
-        raw_s = keep ? raw_s : 0u;
-      }
-      if (lane == 0) {
-        s_any[kg][stage][run % HALVES] = bad != 0;
-        s_bad[kg][stage][run % HALVES] = bad;
+        const MxAside pieces{bad, __builtin_amdgcn_ballot_w64(raw_s == 255u && in), __builtin_amdgcn_ballot_w64(raw_s == 254u && in)};
+        if (lane == 0) s_aside[kg][stage][run % HALVES] = pieces;
+        raw = in ? raw : u32x4{0u, 0u, 0u, 0u};
+        raw_s = in ? raw_s : 0u;
+        mx_set_aside(&raw, &raw_s);
       }
     }
     power = mx_power(raw_s);
@@ -973,20 +1012,7 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
     constexpr int AHEAD = 3 - HALVES;
     const int k0 = key_of(u) + 32 * half;
     const unsigned mine = any[half];
-    if (__builtin_expect(__builtin_amdgcn_readfirstlane(mine) != 0, 0)) {
-      for (unsigned long long left = s_bad[kg][stage][half]; left != 0; left &= left - 1) {
-        const int at = __builtin_ctzll(left), key = k0 + (at >> 1);
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
-          if (key >= lower[rt] && key <= upper[rt]) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              o[rt][0][i] = at & 1 ? o[rt][0][i] : __builtin_nanf("");
-              o[rt][1][i] = at & 1 ? __builtin_nanf("") : o[rt][1][i];
-            }
-          }
-      }
-    }
+    const unsigned aside = __builtin_amdgcn_readfirstlane(mine);
     const int next = after(stage), to_stage = AHEAD == 1 ? next : after(next);
     if constexpr (LAST) {
       meet();
@@ -1035,6 +1061,22 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
     }
     keep(1, 7);
     settle(1);
+    // (behind both tiles' products of the keys ahead, at the references that the tiles have now)
+    if (__builtin_expect(aside != 0, 0)) {
+      auto scalar = [](unsigned long long x) { return static_cast<unsigned long long>(__builtin_amdgcn_readfirstlane(static_cast<unsigned>(x >> 32))) << 32 | static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<unsigned>(x))); };
+      const MxAside pieces{scalar(s_aside[kg][stage][half].any), scalar(s_aside[kg][stage][half].nan), scalar(s_aside[kg][stage][half].large)};
+      for (unsigned long long left = pieces.any; left != 0; left &= left - 1) {
+        const int at = __builtin_ctzll(left), key = k0 + (at >> 1);
+        const unsigned char* const from = a.c.blocks[1] + b * a.c.bs + kvh * a.c.hs + (lo + key) * a.c.ts + 16 * (at & 1);
+        const unsigned byte = pieces.byte(at);
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+          if (key >= lower[rt] && key <= upper[rt]) {
+            if (at & 1) mx_add_aside(&o[rt][1], from, byte, h);
+            else mx_add_aside(&o[rt][0], from, byte, h);
+          }
+      }
+    }
   };
   constexpr int AHEAD = 3 - HALVES;
   auto write_unit = [&](int u, int stage) __attribute__((always_inline)) {
