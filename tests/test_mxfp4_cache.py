@@ -267,6 +267,35 @@ def test_one_token_of_long_caches(slots, start, hint):
 
 
 @gpu
+@pytest.mark.parametrize("window", [1025, 1100, 2500, 5000])
+@pytest.mark.parametrize("batch,t,heads,group,slots", [(3, 1, 2, 8, 9000), (3, 1, 2, 4, 4000), (3, 1, 2, 12, 9000), (3, 4, 2, 8, 9000), (3, 64, 1, 8, 4001)])
+def test_windows_that_workgroups_share(batch, t, heads, group, slots, window):
+    """Windows long enough for several workgroups to a stream: rows with all of theirs, with less than is shared out, and with windows that reach past
+    either end of the cache."""
+    assert shape(batch, t, slots, heads, group, window)[2] > 1
+    for layout, starts, sinks in (("heads", [slots - t, 700, 1150], True), ("slots", [slots + window // 3, 3001, window], False), ("apart", [slots + window - 2, 2 * window // 3, -t], True)):
+        attention_case(batch, t, heads, group, slots, starts, window=window, layout=layout, sinks=sinks)
+
+
+@gpu
+@pytest.mark.parametrize("t,group,window", [(1, 8, 1100), (1, 8, 0), (1, 12, 2500), (4, 8, 1101), (4, 8, 0), (32, 8, 1100), (32, 8, 0)])
+def test_nan_in_walks_that_workgroups_share(t, group, window):
+    """Keys and values of NaN just inside and just outside what the first and the last query of a row see, and in the middle."""
+    slots, starts = 5000, [4901, 3000, 1177]
+    assert shape(3, t, slots, 2, group, window)[2] > 1
+    g = torch.Generator().manual_seed(t + window)
+    cache = make_cache(g, 3, slots, 2)
+    q = torch.randn(3, t, 2, group, 64, generator=g).bfloat16()
+    inside = lambda start: start - window + 1 if window else 0
+    for row, what, head, half, at in ((0, 3, 0, 1, inside(starts[0])), (0, 3, 1, 0, inside(starts[0]) - 1 if window else starts[0] + t), (0, 1, 1, 0, starts[0] + t - 1), (1, 1, 0, 0, inside(starts[1])),
+                                      (1, 3, 1, 1, starts[1]), (1, 3, 1, 0, starts[1] + t), (2, 3, 0, 1, starts[2] - 600), (2, 1, 1, 0, starts[2] + t)):
+        cache[what][row, at, head, half] = 255
+    want, tol = attention_ref(q, cpu(cache), None, 0.125, window, starts)
+    assert want.isnan().any() and not want.isnan().all()
+    check(T.mxfp4_attention(q.cuda(), cache, None, 0.125, window, torch.tensor(starts).cuda()), want, tol, f"{t} queries, window {window}")
+
+
+@gpu
 @pytest.mark.parametrize("t", [2, 3, 4, 5, 8, 9, 16, 17, 31, 33, 70])
 @pytest.mark.parametrize("heads,group", [(2, 8), (1, 1), (2, 3), (1, 16), (1, 20)])
 def test_several_tokens(t, heads, group):
