@@ -431,8 +431,9 @@ int tllm_mxfp4_cache_read_bf16(const TllmMxCache* cache, int64_t first, int64_t 
  * [batch, n_q, n_kv_heads * group * 64] likewise; sinks bf16 [n_kv_heads * group] or NULL (logit 0). A row that sees nothing gives zeros.
  * What a slot holds that a query does not see, NaN and infinities included, is nothing to it; seen, a scale byte of 255 is NaN, and what
  * tllm_mxfp4_cache_read_bf16 reads as infinite (which the quantisation never writes) is infinite: a value gives an infinite result or NaN, a key
- * NaN, or no weight where its logit is -infinity. start_q: device, int32 or int64. group up to 64, sm_scale positive. kv_len_hint (0: none) plans the launch for that many visible keys instead of n_slots; any hint
- * is right, results differ by the order of sums alone.
+ * NaN, or no weight where its logit is -infinity. start_q: device, int32 or int64. group up to 64, sm_scale positive. kv_len_hint (0: none) plans the launch for that many visible keys instead of n_slots: how many
+ * workgroups share a row's keys, and which kernel it is. Any hint is right: results differ within the rounding that all of them have (weights
+ * rounded to bf16 at unlike references, sums in another order, a denominator of weights or of what they were rounded to).
  * workspace: device memory of tllm_mxfp4_attention_workspace_bytes() for the same arguments, 4-byte aligned (may be 0 bytes). */
 int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window,
                                              int64_t kv_len_hint);

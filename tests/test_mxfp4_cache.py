@@ -374,6 +374,31 @@ def test_one_long_prompt(batch, heads, group, starts, nan):
     check(T.mxfp4_attention(q.cuda(), cache, None, 0.125, 0, torch.tensor(starts).cuda()), want, tol, f"prompts at {starts}")
 
 
+# (batch, tokens, KV heads, heads of each, slots, most keys, {hint: run of rows, wavefronts, splits})
+HINTS = [(3, 1, 2, 8, 9000, 4000, {1: (8, 4, 1), 1100: (8, 4, 5), 4000: (8, 4, 16), 10**6: (8, 4, 36)}),
+         (8, 4, 2, 8, 4096, 1500, {1: (32, 8, 1), 700: (32, 8, 1), 1500: (32, 8, 6), 10**6: (32, 8, 16)}),
+         (3, 32, 2, 8, 5000, 3000, {1: (32, 8, 1), 3000: (32, 8, 5), 10**6: (32, 8, 5)}),
+         (24, 40, 8, 8, 1500, 120, {1: (256, 4, 1), 120: (256, 4, 1), 10**6: (64, 4, 1)}),
+         (50, 16, 8, 8, 600, 60, {1: (32, 4, 1), 60: (64, 4, 1), 10**6: (64, 4, 1)}),
+         (1, 1030, 10, 8, 4096, 1030, {1: (256, 4, 1), 1030: (256, 8, 1), 10**6: (64, 4, 1)})]
+
+
+@gpu
+@pytest.mark.parametrize("batch,t,heads,group,slots,keys,plans", HINTS)
+def test_hints_that_change_the_plan(batch, t, heads, group, slots, keys, plans):
+    """Hints far below, at and far above the keys that there are: another kernel, another number of splits, an answer within the same bound."""
+    g = torch.Generator().manual_seed(slots + t)
+    cache = make_cache(g, batch, slots, heads)
+    q = (2 * torch.randn(batch, t, heads, group, 64, generator=g)).bfloat16()
+    sinks = torch.randn(heads * group, generator=g).bfloat16()
+    starts = [keys - t] + [int(i) for i in torch.randint(0, keys - t + 1, (batch - 1,), generator=g)]
+    n = max(starts) + t
+    want, tol = attention_ref(q, [x[:, :n] for x in cpu(cache)], sinks, 0.125, 0, starts)
+    for hint, plan in (*plans.items(), (None, plans[10**6])):
+        assert shape(batch, t, slots, heads, group, hint=hint or 0) == plan
+        check(T.mxfp4_attention(q.cuda(), cache, sinks.cuda(), 0.125, 0, torch.tensor(starts).cuda(), hint), want, tol, f"hint {hint}, plan {plan}")
+
+
 @gpu
 @pytest.mark.parametrize("t", [1, 3, 20, 200])
 def test_attention_past_the_end_and_before_the_beginning(t):

@@ -1137,7 +1137,8 @@ def mxfp4_attention(q: torch.Tensor, cache: Mxfp4Cache, sinks: torch.Tensor | No
     ``start_q`` (int32 or int64, read on the device) has one element or one per row: query ``i`` of row ``b`` sits at position ``start_q[b] + i``
     and sees the slots up to there (``bandwidth`` of them, if given). A query that sees none gives zeros; what it does not see, NaN
     included, is nothing to it. Any number of queries: drafts to verify, a chat's next turn, a prompt. ``kv_len_hint`` (the most keys that
-    a query sees, as far as the host knows) plans the launch; it may be wrong, and changes no more than the order of sums."""
+    a query sees, as far as the host knows) plans the launch: which kernel, and how many workgroups share keys. It may be wrong, and changes
+    results by no more than the kernels' own rounding."""
     done = host().mxfp4_attention(q, *cache, sinks, sm_scale, bandwidth, start_q, kv_len_hint)
     if done is not None:
         return done
