@@ -873,3 +873,15 @@ def test_ops_refuse_wrong_types_and_shapes():
         T.mxfp4_attention_decode(q.expand(2, 2, 3, 4, 64), cache, None, 1.0, 0, at)
     with pytest.raises(RuntimeError, match="GPU"):
         T.mxfp4_attention(q, cache, sinks.cpu(), 1.0, 0, at)
+
+
+@gpu
+def test_more_heads_and_values_than_32_bits_count():
+    """Numbers of heads and of blocks that are 8 and 2 beyond a power of two: refused, not taken for 8 heads of 64."""
+    cache = T.Mxfp4Cache(*(t[:, :, :1].expand(1, 4, 2**32 + 8, *t.shape[3:]) for t in T.mxfp4_cache(1, 4, 1)))
+    blocks, scales = torch.empty(1, 1, 1, 2**27 + 2, 16, dtype=torch.uint8, device="cuda"), torch.empty(1, 1, 1, 2**27 + 2, dtype=torch.uint8, device="cuda")
+    for bad, what in ((cache, "heads"), (T.Mxfp4Cache(blocks, scales, blocks, scales), "head_dim")):
+        with pytest.raises(AssertionError, match=what):
+            T.mxfp4_cache_read(bad)
+    del blocks, scales, bad
+    torch.cuda.empty_cache()

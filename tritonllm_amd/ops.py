@@ -1069,6 +1069,7 @@ def _mx_cache_desc(cache, *others: torch.Tensor) -> TllmMxCache:
     _require(kb.stride()[3:] == (16, 1) or (groups == 1 and kb.stride(4) == 1), "a cache's blocks must be dense inside a head")
     _require(groups == 1 or ks.stride(3) == 1, "a cache's scales must be dense inside a head")
     _require(vb.stride() == kb.stride() and vs.stride() == ks.stride(), "a cache's keys and values must have the same strides")
+    _require(max(kb.shape[2], 32 * groups) < 2**31, f"a cache of {kb.shape[2]} heads of head_dim {32 * groups}")      # (32-bit fields)
     return TllmMxCache(kb.data_ptr(), ks.data_ptr(), vb.data_ptr(), vs.data_ptr(), kb.stride(0), kb.stride(1), kb.stride(2), ks.stride(0), ks.stride(1),
                        ks.stride(2), kb.shape[0], kb.shape[1], kb.shape[2], 32 * groups)
 
