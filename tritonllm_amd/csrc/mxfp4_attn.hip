@@ -173,8 +173,9 @@ __device__ __forceinline__ unsigned mx_scale_pair(const unsigned char* p, int64_
 // Bound by the cache's bytes where contexts are long -- 8 rows of 32768 keys 28.4 us (143 MB, 5.0 TB/s, the joining launch among them), of 131072 96
 // (5.9 TB/s; loads of this pattern alone 6.8) --, else by a chain of latencies: 300 keys of one row 4.7 us, 8 rows of 4096 9.7, 2.2 of which are
 // the second launch.
-template <bool DENSE, int NW>
-__global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a) {
+template <bool DENSE>
+__global__ __launch_bounds__(256, 3) void mxfp4_attn_one_kernel(MxAttnArgs a) {
+  constexpr int NW = 4;                                        // wavefronts
   constexpr int VTILE = 64 * 128;
   constexpr int AROW = 64 + 1;                                 // accumulator row in LDS, floats
   __shared__ __align__(16) unsigned char vt[NW * VTILE];
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
   int lo = 0;
   if (a.window > 0) lo = min(mx_span(a, mx_start(a, b), 0, 0).lo, a.c.n_slots - 1);      // (a slot of the cache, also where a window behind its end has none)
   const int first = split * NW + wave;
-  constexpr int TPR = NW * 64 / 8, DPT = 64 / TPR > 0 ? 64 / TPR : 1;      // at the end: thread -> (head, every TPR-th of its 64 values)
+  constexpr int TPR = NW * 64 / 8, DPT = 64 / TPR;             // at the end: thread -> (head, every TPR-th of its 64 values)
   const int eh = tid / TPR, ed = tid % TPR;
   const bf16 sink = mx_sink(a, kvh * G + (eh < G ? eh : G - 1));
   const int nall = (a.c.n_slots - lo + 63) >> 6;                // blocks that the cache has from there on
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
       mine[(4 * g + i) * AROW + 16 * nb + r16] = g < 2 ? x : y;
     }
   __syncthreads();
-  if (eh >= G || ed >= 64) return;
+  if (eh >= G) return;
   float m_all = kNoRef;
 #pragma unroll
   for (int w = 0; w < 2 * NW; ++w) m_all = fmaxf(m_all, s_m[w >> 1][8 * (w & 1) + eh]);
@@ -463,15 +464,13 @@ __global__ __launch_bounds__(NW * 64, 3) void mxfp4_attn_one_kernel(MxAttnArgs a
 // rows of 4096 12.2 us, 97 behind 1500 9.6.
 template <bool DENSE, int RT, int KG>
 __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs a) {
-  constexpr int NW = KG, RB = 32 * RT;                         // wavefronts; rows
+  constexpr int RB = 32 * RT;                                  // rows
   constexpr int VTILE = 32 * 128;
-  constexpr int SHARE = kShare;
-  static_assert(SHARE * 4 >= VTILE, "the shares are what needs most LDS");
-  extern __shared__ __align__(16) unsigned char smem[];        // NW shares
+  static_assert(kShare * 4 >= VTILE, "the shares are what needs most LDS");
+  extern __shared__ __align__(16) unsigned char smem[];        // KG shares
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
-  const int kg = wave;
 
   // the splits are the slowest part of the index: those that a context does not need are the last
   const int i0 = a.by_heads(blockIdx.x), kvh = blockIdx.x - i0 * a.n_kv_heads;
@@ -497,7 +496,7 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   // Without a window the keys begin at slot 0, and the first block is asked for ahead of the start position (whose load takes as long as its own).
   int lo = 0;
   if (a.window > 0) lo = min(mx_span(a, mx_start(a, b), row0, row0 + RB - 1).lo, a.c.n_slots - 1);
-  const int first = split * KG + kg;
+  const int first = split * KG + wave;
   const int nall = (a.c.n_slots - lo + 31) >> 5;                // blocks that the cache has from there on
 
   const int64_t kv_off = b * a.c.bs + kvh * a.c.hs + lo * a.c.ts, sc_off = b * a.c.sbs + kvh * a.c.shs + lo * a.c.sts;
@@ -540,7 +539,7 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
   __builtin_amdgcn_sched_barrier(0);
 
   int upper[RT], lower[RT];                                    // the keys that the lane's row sees, counted from sp.lo
-  int seen_hi = 0x7fffffff, seen_lo = 0;                       // keys that every row of the wavefront sees
+  int seen_hi, seen_lo;                                        // keys that every row of the wavefront sees
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int64_t up = sp.start + query[rt] - sp.lo, low = up - a.window + 1;
@@ -700,8 +699,8 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
     if (blk < nblk) process(blk, even);
   }
 
-  // ---- the sink joins the denominator, or a record leaves. A lane has 16-byte runs of one row's values; where wavefronts share the rows
-  // they first meet in LDS, 32 / KG of the 32 values a lane to each.
+  // ---- the sink joins the denominator, or a record leaves. A lane has 16-byte runs of one row's values; the wavefronts,
+  // which share the rows, meet in LDS: 32 / KG of the 32 values a lane to each.
   constexpr int RPG = 32 / KG;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -712,53 +711,48 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
       l = x + y;
     }
     float v[RPG];
-    if constexpr (KG > 1) {
-      float* const shares = reinterpret_cast<float*>(smem);
-      __syncthreads();                                         // (all are past their last read of the tiles, or of the tile of rows before)
-      float* const mine = shares + wave * SHARE + lane;
+    float* const shares = reinterpret_cast<float*>(smem);
+    __syncthreads();                                         // (all are past their last read of the tiles, or of the tile of rows before)
+    float* const mine = shares + wave * kShare + lane;
 #pragma unroll
-      for (int r = 0; r < 32; ++r) {
-        const float x = o[rt][r >> 4][r & 15];
-        mine[r * 64] = x;
-      }
-      mine[32 * 64] = m;
-      mine[33 * 64] = l;
-      __syncthreads();
-      const float* const from = shares + lane;
-      m = kNoRef;
+    for (int r = 0; r < 32; ++r) {
+      const float x = o[rt][r >> 4][r & 15];
+      mine[r * 64] = x;
+    }
+    mine[32 * 64] = m;
+    mine[33 * 64] = l;
+    __syncthreads();
+    const float* const from = shares + lane;
+    m = kNoRef;
 #pragma unroll
-      for (int k = 0; k < KG; ++k) m = fmaxf(m, from[k * SHARE + 32 * 64]);
-      l = 0.f;
+    for (int k = 0; k < KG; ++k) m = fmaxf(m, from[k * kShare + 32 * 64]);
+    l = 0.f;
 #pragma unroll
-      for (int r = 0; r < RPG; ++r) v[r] = 0.f;
+    for (int r = 0; r < RPG; ++r) v[r] = 0.f;
 #pragma unroll
-      for (int k = 0; k < KG; ++k) {
-        const float f = __builtin_amdgcn_exp2f(from[k * SHARE + 32 * 64] - m);      // (0 for a wavefront that saw no key)
-        l = fmaf(from[k * SHARE + 33 * 64], f, l);
+    for (int k = 0; k < KG; ++k) {
+      const float f = __builtin_amdgcn_exp2f(from[k * kShare + 32 * 64] - m);      // (0 for a wavefront that saw no key)
+      l = fmaf(from[k * kShare + 33 * 64], f, l);
 #pragma unroll
-        for (int r = 0; r < RPG; ++r) v[r] = fmaf(from[k * SHARE + (RPG * kg + r) * 64], f, v[r]);
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 32; ++r) v[r] = o[rt][r >> 4][r & 15];
+      for (int r = 0; r < RPG; ++r) v[r] = fmaf(from[k * kShare + (RPG * wave + r) * 64], f, v[r]);
     }
     if (row0 + 32 * rt + l31 >= rows) continue;
-    // value rr = RPG kg + r: d = 32 (rr / 16) + 8 (rr / 4 % 4) + 4 h + rr % 4
+    // value rr = RPG wave + r: d = 32 (rr / 16) + 8 (rr / 4 % 4) + 4 h + rr % 4
     if (sp.live > 1) {
       float* const p = a.part + (((static_cast<int64_t>(split) * a.batch + b) * a.n_q + query[rt]) * (a.n_kv_heads * a.group) + head[rt]) * PART;
 #pragma unroll
       for (int r = 0; r < RPG; ++r) {
-        const int rr = RPG * kg + r;
+        const int rr = RPG * wave + r;
         p[32 * (rr >> 4) + 8 * (rr >> 2 & 3) + 4 * h + (rr & 3)] = v[r];
       }
-      if (kg == 0) p[64 + h] = h == 0 ? m : l;
+      if (wave == 0) p[64 + h] = h == 0 ? m : l;
       continue;
     }
     const float f = mx_norm(a, sink[rt], m, l);
     bf16* const to = a.out + b * a.out_bs + query[rt] * a.out_ts + head[rt] * 64;
 #pragma unroll
     for (int r = 0; r < RPG; r += 4) {
-      const int rr = RPG * kg + r;
+      const int rr = RPG * wave + r;
       bf16x4 w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = static_cast<bf16>(v[r + e] * f);
@@ -1334,7 +1328,7 @@ static int launch_attention(const MxAttnPlan& p, const MxAttnArgs& a, dim3 grid,
     else if (p.rows == 256) hipLaunchKernelGGL((mxfp4_attn_many_kernel<4, 1>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((mxfp4_attn_many_kernel<2, 2>), grid, dim3(256), 0, st, a);
   }
-  else if (p.one) hipLaunchKernelGGL((mxfp4_attn_one_kernel<DENSE, 4>), grid, dim3(256), 0, st, a);
+  else if (p.one) hipLaunchKernelGGL((mxfp4_attn_one_kernel<DENSE>), grid, dim3(256), 0, st, a);
   else if (p.waves == 8) return launch_rows<DENSE, 1, 8>(a, grid, st);
   else return p.tiles == 1 ? launch_rows<DENSE, 1, 4>(a, grid, st) : launch_rows<DENSE, 2, 4>(a, grid, st);
   return TLLM_OK;
