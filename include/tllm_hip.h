@@ -404,7 +404,7 @@ int tllm_moe_mlp2_bf16(const void* h, int64_t h_row_stride, const int32_t* order
  * values; the last two dimensions of the codes and the last of the scales are dense, the others have strides in bytes, the same for keys
  * and values: those of the codes multiples of 16, none negative, those between slots below 2^24. Device pointers, codes 16-byte aligned.
  * Attention reads fastest where a head's slots are neighbours (slot_stride = head_dim / 2). batch and n_kv_heads up to 65535,
- * n_slots below 2^30, head_dim a multiple of 32 up to 1024 (attention: 64). */
+ * n_slots below 2^30, head_dim a multiple of 32 up to 1024 (attention: 64, and at least one slot). */
 typedef struct TllmMxCache {
   void *k_blocks, *k_scales, *v_blocks, *v_scales;
   int64_t batch_stride, slot_stride, head_stride;
@@ -431,9 +431,11 @@ int tllm_mxfp4_cache_read_bf16(const TllmMxCache* cache, int64_t first, int64_t 
  * [batch, n_q, n_kv_heads * group * 64] likewise; sinks bf16 [n_kv_heads * group] or NULL (logit 0). A row that sees nothing gives zeros.
  * What a slot holds that a query does not see, NaN and infinities included, is nothing to it; seen, a scale byte of 255 is NaN, and what
  * tllm_mxfp4_cache_read_bf16 reads as infinite (which the quantisation never writes) is infinite: a value gives an infinite result or NaN, a key
- * NaN, or no weight where its logit is -infinity. start_q: device, int32 or int64. group up to 64, sm_scale positive. kv_len_hint (0: none) plans the launch for that many visible keys instead of n_slots: how many
- * workgroups share a row's keys, and which kernel it is. Any hint is right: results differ within the rounding that all of them have (weights
- * rounded to bf16 at unlike references, sums in another order, a denominator of weights or of what they were rounded to).
+ * NaN, or no weight where its logit is -infinity. Weighted values are summed in fp32 ahead of the division by the weights' sum: values beyond
+ * 2^120 / (the keys seen) may give an infinite result or NaN.
+ * start_q: device, int32 or int64. group up to 64, sm_scale positive. kv_len_hint (0: none) plans the launch for that many visible keys instead
+ * of n_slots: how many workgroups share a row's keys, and which kernel it is. Any hint is right: results differ within the rounding that
+ * all of them have (weights rounded to bf16 at unlike references, sums in another order, a denominator of weights or of what they were rounded to).
  * workspace: device memory of tllm_mxfp4_attention_workspace_bytes() for the same arguments, 4-byte aligned (may be 0 bytes). */
 int64_t tllm_mxfp4_attention_workspace_bytes(int64_t batch, int64_t n_q, int64_t n_slots, int n_kv_heads, int group, int window,
                                              int64_t kv_len_hint);

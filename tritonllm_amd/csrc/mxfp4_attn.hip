@@ -7,6 +7,10 @@
 // with k and v the values that the cache's codes and scale bytes stand for, exactly (an e2m1 value times a power of two is a bf16 value).
 // A scale byte of 255 makes its 32 values NaN, and values of 2^128 and more (scale bytes 253 and 254) are infinite in bf16: for the queries that see
 // the slot, and for no other.
+// Logits, sums, references and denominators are fp32. The weights are rounded to bf16 ahead of the second product, whose matrix instruction takes
+// them so (at most 2^-8 of a weight, as in the kernels over a bf16 cache: results are 1.9e-3 - 2.1e-3 from the definition, of which 1.6e-3 - 1.7e-3 is
+// the result's own rounding). Where many rows share a tile the denominator sums what they were rounded to, on the matrix cores; else the fp32 ones.
+// Weighted values are summed ahead of the division, at weights of up to 2^8: values beyond 2^120 / (the keys seen) may pass fp32's range.
 #include "mx_cache.h"
 
 namespace tllm {
@@ -29,7 +33,7 @@ struct MxAttnArgs {
 
 namespace {
 constexpr int PART = 66;              // floats of a record in the workspace
-// Splits, one query of 8 heads, us. One workgroup walks up to kUnsplit keys alone (no second launch): 300 keys 4.9, split 6.7; 600 5.7, 6.7; 1000 6.4,
+// Splits, one query of 8 heads, us (a line's figures are of one sweep in graphs; between boxes they differ by up to 5 %). One workgroup walks up to kUnsplit keys alone (no second launch): 300 keys 4.9, split 6.7; 600 5.7, 6.7; 1000 6.4,
 // 6.8; 8 rows of 1024 6.4, 7.9; but 2000 9.0 and 6.8. A workgroup to a CU: 49 rows of up to 2048 11.9, with two 17.2; 32 of 4096 16.1, 19.2; one of
 // 32768 11.2, 13.2 -- until each has 2^kMostShift keys: 8 rows of 32768 28.6, with one of 8192 31.6 and two of 2048 30.4; 8 of 131072 96, 94 and 104.
 // At least 2^kLeastShift keys: one row of 4096 7.3, of 512 and more 7.6 - 9.0. (Eight wavefronts instead of four, with as many splits or half: 300
@@ -170,9 +174,9 @@ __device__ __forceinline__ unsigned mx_scale_pair(const unsigned char* p, int64_
 //   A lane's scores are then four of a tile, all of use.
 //   O = P . V, the weights' registers being the A operand for the block's keys 0 - 31 in the rows 0 - 7 and for 32 - 63 in the rows 8 - 15: two
 //   accumulators, each of which is looked at in one half of its rows. V passes LDS as bf16, for transposing reads.
-// Bound by the cache's bytes where contexts are long -- 8 rows of 32768 keys 28.4 us (143 MB, 5.0 TB/s, the joining launch among them), of 131072 96
-// (5.9 TB/s; loads of this pattern alone 6.8) --, else by a chain of latencies: 300 keys of one row 4.7 us, 8 rows of 4096 9.7, 2.2 of which are
-// the second launch.
+// Bound by the cache's bytes where contexts are long -- in a graph, 8 rows of 32768 keys 28.2 us (143 MB, 5.1 TB/s, the joining launch among them), of
+// 131072 96 - 98 (5.9 TB/s; loads of this pattern alone 6.8) --, else by a chain of latencies: 300 keys of one row planned for 300 4.7 us, 8 rows of
+// 4096 9.7, about 2 of which are the second launch, a window of 128 keys 4.2 (the start position comes ahead of the first keys there).
 template <bool DENSE>
 __global__ __launch_bounds__(256, 3) void mxfp4_attn_one_kernel(MxAttnArgs a) {
   constexpr int NW = 4;                                        // wavefronts
@@ -460,8 +464,8 @@ __global__ __launch_bounds__(256, 3) void mxfp4_attn_one_kernel(MxAttnArgs a) {
 //   O^T = V^T . P^T: the scores' registers are, pairwise, the B operand when the k slots are read as a permutation of the keys; V passes LDS
 //   as bf16 for transposing reads, as above.
 // Bound by the vector ALU (a wavefront converts its keys and values for its own rows alone, an exponential for each weight) beside the matrix cores
-// where there is enough to do -- 512 queries behind 4000 tokens 48 us, 34 GFLOP: 0.7 PFLOP/s --, else by latencies as above: four drafts to each of 8
-// rows of 4096 12.2 us, 97 behind 1500 9.6.
+// where there is enough to do -- 512 queries behind 4000 tokens 48 - 49 us, 36 GFLOP: 0.7 PFLOP/s --, else by latencies as above: four drafts to each of
+// 8 rows of 4096 12.4 us, 97 behind 1500 9.7, one query of sixteen heads a KV head 8 x 4096 11.5 (all in graphs).
 template <bool DENSE, int RT, int KG>
 __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs a) {
   constexpr int RB = 32 * RT;                                  // rows
@@ -767,8 +771,8 @@ __global__ __launch_bounds__(KG * 64, 2) void mxfp4_attn_rows_kernel(MxAttnArgs 
 //   The matrix cores and the vector ALU work at the same time: with one tile's weights (32 keys x 32 rows) the next one's scores are issued in
 //   turn, and the products of the one before. Of block j (32 keys), S^T of tile 1, weights of tile 0 and P . V of block j - 1 in tile 1; then S^T of
 //   block j + 1 in tile 0, weights of tile 1 and P . V of tile 0. Operands of K and of V live from one such half to the next.
-// Bound by what the two units take together at the clock that the power limit leaves (1.8 - 1.9 GHz): a prompt of 8192 514 - 546 us (550 GFLOP: 1.0 -
-// 1.07 PFLOP/s; 431 with the LDS traffic left out); of 2048 48.4 (0.7), of which a workgroup's beginning and end are 4 each.
+// Bound by what the two units take together at the clock that the power limit leaves (1.8 - 1.9 GHz): a prompt of 8192 513 - 536 us (550 GFLOP: 1.0 -
+// 1.07 PFLOP/s; 431 with the LDS traffic left out); of 2048 47.5 - 48.8 (0.7), of which a workgroup's beginning and end are 4 each.
 template <int RUNS, int KG>
 __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAttnArgs a) {
   static_assert(RUNS == 4 || RUNS == 2, "runs of a workgroup");
@@ -1203,7 +1207,7 @@ __global__ __launch_bounds__(RUNS * KG * 64, 2) void mxfp4_attn_many_kernel(MxAt
 }
 
 // A wavefront per (batch row, query, head): the splits' records and the sink. Lane s has the (max, sum) of split s. Two reads' latency and a launch:
-// 2.2 us as traced, for 512 heads of four splits.
+// for 512 heads of four splits 2.8 us as traced (1.9 at least), and a graph is 1.8 longer with it than a call that is not split (8 rows of 1000).
 __global__ __launch_bounds__(64) void mxfp4_attn_reduce_kernel(MxAttnArgs a, int rows_per_group) {
   const int lane = threadIdx.x;
   const int n_heads = a.n_kv_heads * a.group;
@@ -1252,7 +1256,8 @@ struct MxAttnPlan {
   int splits, fill;
 };
 
-// Which kernel, by the runs of rows and of streams that there are (eight KV heads of eight query heads, us; "n behind m": n queries behind m tokens):
+// Which kernel, by the runs of rows and of streams that there are (eight KV heads of eight query heads, us; "n behind m": n queries behind m tokens;
+// the figures of one sweep compare kernels with each other, and some of those they name have become faster since, or serve other sizes now):
 //   Many rows, 256 to a workgroup, from 385 runs of 256 on -- one prompt of 2048 51.9, in 128 rows a workgroup 55.7, 64 56.7, 32 62.5; 4096 158, 174, 183,
 //   213 -- and from 513 runs of 128 on where walks are short, up to 768 keys: 2 x 700 24.3, 26.2, 27.6, 27.2; 2048 with a window of 128 19, 25, 32, 31.
 //   Between, two workgroups to a CU do not come out even: 1200 33.7, 25.7, 28.8, 29; 1200 behind 6800 223, 213, 178, 202; 1500 behind 2500 104, 104, 102,
@@ -1264,7 +1269,8 @@ struct MxAttnPlan {
 //   128 to a workgroup from 385 to 512 runs of them, one or two workgroups to a CU: 2 x 512 15.8, in 256 rows 18.8, 64 18.8, 32 18.9; 4 x 256 13.0,
 //   13.6, 17.0, 17.2; 3 x 333 13.9, 16.0, 17.5, 17.8; 8 x 128 behind 2000 47.6, 51.4, 49.8, 56; 1000 behind 8000 162, 188, 165, 188; 800 behind 4000
 //   85.4, 103, 86.8, 89; but 700 behind 4000 (352) 84, 101, 70, 77, and 512 behind 4000 64, 96, 48, 56. To 640 for prompts: 1200 24.5, 31.7, 27.6, 27.5;
-//   1100 23.1, 30.2, 25.5, 24.4 (behind 1000 52, 53, 47.6, 50).
+//   1100 23.1, 30.2, 25.5, 24.4 (behind 1000 52, 53, 47.6, 50). (Not the best where walks are shortest or longest: 16 x 64 10.2, in 256 rows 8.8; 1000
+//   behind 8000 164, in 256 rows with two groups of wavefronts 151.)
 //   32 rows shared out between eight wavefronts up to 256 runs of 32: 97 behind 1500 10.0, between four 11.7; 97 behind 8000 31, 39; 64 behind 8000
 //   24.2, 26.9; with four from there on: 150 behind 1350 17.3, 13.8; 256 behind 2000 22, 18.2; 64 x 4 of 1000 16.1, 12.5.
 //   64 rows to a workgroup from 768 such runs on: 512 behind 4000 48, with 32 rows 56; 700 behind 4000 70, 77; 512 9.9, 11.4; but 350 behind 4000 44.6,

@@ -7,8 +7,9 @@
 //
 // A thread takes eight values (reading many, four times eight). A workgroup stays with one head: eight neighbours have a whole line of k or v
 // (64 values of bf16), a wavefront 256 neighbouring bytes of the head's codes.
-// Bound by the bytes: 8 rows of 4096 tokens of eight heads written in 21.0 us (85 MB, 4.05 TB/s; a large copy reaches 4.7), read in 15.5 (5.5); 8192
-// tokens 7.3 and 4.8; one token of eight rows 2.4 and 2.4, a launch.
+// Bound by the bytes, in a graph over several caches and outputs in turn: 8 rows of 4096 tokens of eight heads written in 21.0 us (85 MB, 4.05 TB/s; a
+// large copy reaches 4.8), read in 15.5 (5.5; 13.1 into outputs that the chip's caches still hold); 8192 tokens 7.2 and 4.8; one token of eight rows 2.5
+// and 2.6, a launch.
 #include "mx_cache.h"
 #include "mx_quantize.h"
 
@@ -129,7 +130,7 @@ MxPlace place_of(int eights) { return MxPlace{(unsigned)eights, (eights & (eight
 // most, 32 bits hold; rows that keep a grid below 2^32 threads.
 template <class F>
 int in_launches(int64_t batch, int64_t tokens, int heads, int eights, int per_thread, int64_t stride, F f) {
-  int64_t most = (1ll << 23) / eights;                         // (65535 workgroups of 256 at least)
+  int64_t most = (1ll << 23) / eights;                         // (at most 32768 workgroups of 256, of the 65535 that a grid's second dimension takes)
   const int64_t fits = (1ll << 22) / heads * 256 / eights;     // (heads are up to 65535: one token at least)
   most = most < fits ? most : fits;
   if (stride > 0 && most > (1ll << 31) / stride) most = (1ll << 31) / stride > 0 ? (1ll << 31) / stride : 1;
