@@ -523,6 +523,46 @@ def test_infinite_values_reach_who_sees_them(batch, t, heads, group, slots, run)
 
 
 @gpu
+@pytest.mark.parametrize("batch,t,heads,group,slots,window", [(2, 1, 2, 8, 90, 0), (2, 1, 2, 16, 90, 30), (2, 5, 2, 8, 100, 0), (1, 33, 1, 12, 120, 20), (30, 7, 8, 8, 70, 0), (50, 16, 8, 8, 60, 12), (100, 40, 1, 16, 77, 0),
+                                                              (24, 40, 8, 8, 120, 0), (24, 40, 8, 8, 120, 25), (1, 70, 2, 8, 3000, 0)])
+def test_nan_and_infinities_together(batch, t, heads, group, slots, window):
+    """Several pieces of NaN and of infinities in each row, some of them neighbours: a query has NaN where it sees NaN, nothing finite where it sees an
+    infinity, and the definition's answer everywhere else."""
+    g = torch.Generator().manual_seed(slots + t + window)
+    pick = lambda n: int(torch.randint(0, n, (), generator=g))
+    start = slots - t if slots > 1000 else 9
+    plain = make_cache(g, batch, slots, heads)
+    q = torch.randn(batch, t, heads, group, 64, generator=g).bfloat16()
+    at = start + torch.arange(t)
+    cache, without = [x.cpu().clone() for x in plain], [x.cpu().clone() for x in plain]
+    for b in range(batch):
+        first = max(0, start + t - 40) if slots > 1000 else 0
+        places = {(first + pick(start + t + 3 - first), pick(heads), pick(2)) for _ in range(3)}
+        n, h, half = next(iter(places))
+        places |= {(n + 1, h, half), (n, h, 1 - half)}              # (its neighbours)
+        for n, h, half in sorted(places):
+            n = min(n, slots - 1)
+            byte = (253, 254, 255)[pick(3)]
+            which = torch.rand(32, generator=g) < 0.3
+            codes = torch.where(which, torch.tensor((7, 14, 15, 6))[torch.randint(0, 4, (32,), generator=g)], 0).to(torch.uint8)
+            cache[2][b, n, h, half], cache[3][b, n, h, half] = codes[0::2] | codes[1::2] << 4, byte
+            without[2][b, n, h, half], without[3][b, n, h, half] = 0, 0
+    v = values(cache[2], cache[3])                                  # [batch, slots, heads, 64]
+    key = torch.arange(slots)
+    sees = (key <= at[:, None]) & (key > at[:, None] - window if window else key >= 0)
+    nan = torch.einsum("tn,bnhd->bthd", sees.float(), v.isnan().float()) > 0
+    infinite = torch.einsum("tn,bnhd->bthd", sees.float(), (v.abs() >= 2.0**128).float()) > 0
+    got = T.mxfp4_attention(q.cuda(), T.Mxfp4Cache(*(x.transpose(1, 2).contiguous().cuda().transpose(1, 2) for x in cache)), None, 0.125, window, torch.tensor([start]).cuda())
+    want, tol = attention_ref(q, without, None, 0.125, window, [start] * batch)
+    wide = lambda x: x[:, :, :, None].expand(batch, t, heads, group, 64).reshape(batch, t, -1)
+    got = got.cpu().double()
+    assert got[wide(nan)].isnan().all() and not got[wide(infinite)].isfinite().any()
+    for x in (got, want, tol):
+        x[wide(nan | infinite)] = 0
+    check(got, want, tol, f"{t} queries, window {window}")
+
+
+@gpu
 @pytest.mark.parametrize("batch,t,heads,group,slots", [(1, 4, 2, 8, 100), (50, 16, 8, 8, 60), (100, 40, 1, 16, 77), (24, 40, 8, 8, 120)])
 def test_infinite_keys_are_nothing_to_who_does_not_see_them(batch, t, heads, group, slots):
     g = torch.Generator().manual_seed(batch + t)

@@ -33,11 +33,12 @@ struct MxAttnArgs {
 
 namespace {
 constexpr int PART = 66;              // floats of a record in the workspace
-// Splits, one query of 8 heads, us (a line's figures are of one sweep in graphs; between boxes they differ by up to 5 %). One workgroup walks up to kUnsplit keys alone (no second launch): 300 keys 4.9, split 6.7; 600 5.7, 6.7; 1000 6.4,
-// 6.8; 8 rows of 1024 6.4, 7.9; but 2000 9.0 and 6.8. A workgroup to a CU: 49 rows of up to 2048 11.9, with two 17.2; 32 of 4096 16.1, 19.2; one of
-// 32768 11.2, 13.2 -- until each has 2^kMostShift keys: 8 rows of 32768 28.6, with one of 8192 31.6 and two of 2048 30.4; 8 of 131072 96, 94 and 104.
-// At least 2^kLeastShift keys: one row of 4096 7.3, of 512 and more 7.6 - 9.0. (Eight wavefronts instead of four, with as many splits or half: 300
-// keys 5.4, 8 rows of 4096 10.5 and 11.7 against 10.1, 32 of 2048 10.5 against 10.2.)
+// Splits, one query of 8 heads, us (a line's figures are of one sweep in graphs; from one machine to another they differ by up to 5 %). One workgroup
+// walks up to kUnsplit keys alone (no second launch): 300 keys 4.9, split 6.7; 600 5.7, 6.7; 1000 6.4, 6.8; 8 rows of 1024 6.4, 7.9; but 2000 9.0 and
+// 6.8. A workgroup to a CU: 49 rows of up to 2048 11.9, with two 17.2; 32 of 4096 16.1, 19.2; one of 32768 11.2, 13.2 -- until each has 2^kMostShift
+// keys: 8 rows of 32768 28.6, with one of 8192 31.6 and two of 2048 30.4; 8 of 131072 96, 94 and 104. At least 2^kLeastShift keys: one row of 4096
+// 7.3, of 512 and more 7.6 - 9.0. (Eight wavefronts instead of four, with as many splits or half: 300 keys 5.4, 8 rows of 4096 10.5 and 11.7 against
+// 10.1, 32 of 2048 10.5 against 10.2.)
 constexpr int kUnsplit = 1024, kLeastShift = 8, kMostShift = 12, kFill = 256, kDeep = 4096;
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are exp2(logit - reference). The reference of one query and of a few rows is the largest logit that it was raised to, and stays there

@@ -134,7 +134,7 @@ struct ScaleRaw {
 
 // One 256-lane workgroup per row; VPT = 16-byte vectors per thread. The few-row case is all latency, so every load --
 // the row and the scale -- goes out before anything waits (left at its use, behind the barrier, the scale's load would
-// add a memory round trip to the chain: 2.36 -> 2.28 us at 8 rows, 2.43 -> 2.34 at 32, same box).
+// add a memory round trip to the chain: 2.36 -> 2.28 us at 8 rows, 2.43 -> 2.34 at 32, same machine).
 template <int VPT, bool kScaleBf16, bool GATHER>
 __global__ __launch_bounds__(256) void rmsnorm_block_kernel(const bf16x8* x, const void* __restrict__ scale,
                                                             bf16x8* out, int nvec, float hidden_f, float eps, GatherSrc g) {
